@@ -153,6 +153,21 @@ _SIGNATURES = {
 
 EXPORTED = tuple(_SIGNATURES)
 
+# the entry points of include/ossm_lm.h
+_LM_SIGNATURES = {
+    "ossm_lm_abi_version": (ctypes.c_int, []),
+    "ossm_mixer_step": (ctypes.c_int, [ctypes.c_int, _vp, _c_int64] + [_vp] * 12 + [_c_int64] * 6 + [_vp]),
+    "ossm_mixer_prompt": (ctypes.c_int, [ctypes.c_int, _vp, _c_int64] + [_vp] * 14 + [_c_int64] * 7 + [_vp]),
+    "ossm_control_logits": (
+        ctypes.c_int,
+        [ctypes.c_int, _vp, _c_int64, _vp, _c_int64, _vp, _c_int64, _c_int64, _vp, _vp, _fp, ctypes.c_float, _fp,
+         ctypes.c_float, _fp, ctypes.c_float, _vp, _fp, _c_int64, _c_int64, _vp, _c_int64, _c_int64, _c_int64, _vp]),
+}
+
+LM_EXPORTED = tuple(_LM_SIGNATURES)
+# the dtype argument of the language-model entry points
+LM_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -165,7 +180,7 @@ def load() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m ossm_amd.build` "
                 "(the HIP path has no fallback)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in _SIGNATURES.items():
+        for name, (res, args) in (*_SIGNATURES.items(), *_LM_SIGNATURES.items()):
             fn = getattr(lib, name, None)
             if fn is None:
                 continue

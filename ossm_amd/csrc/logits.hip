@@ -1,0 +1,200 @@
+// Penalties for repeated tokens, biases and a grammar's mask on a model's logits, in
+// one pass over them (ossm_control_logits):
+//
+//   l = logits[v];  v seen in the history: l = l > 0 ? l / rep : l rep
+//   l -= freq c + pres (c > 0)   c: v's count in the part after the prompt
+//   l += bias of v;  l = -inf where the mask forbids v
+//
+// A workgroup takes a row's block of kBlock vocabulary entries: it counts the row's
+// history and marks its biases for that block in LDS, then streams the block.
+// Integer LDS atomics only (counts, a mark, the highest bias index), so the result does not
+// depend on their order.  Every block of a row reads the row's history again (from
+// L2: a few kB against the block's logits).
+//
+// Vectors of 16 bytes are aligned to the row's address, whatever its offset (a
+// vocabulary of odd size puts every row at another one); the row's ends take single
+// elements.
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+#include <string>
+
+#include "../../include/ossm_lm.h"
+#include "lm_types.hpp"
+#include "runtime.hpp"
+
+namespace ossm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 8192;               // vocabulary entries of a workgroup
+constexpr uint32_t kSeen = 0x80000000u;    // of an entry's word: seen at all; below: its count
+
+template <class E>
+struct Logits {
+  const E* in;
+  E* out;
+  const int32_t* history;
+  const int32_t* lengths;
+  const int32_t* prompts;
+  const float* rep;
+  const float* pres;
+  const float* freq;
+  const int32_t* bias_ids;
+  const float* bias;
+  const int32_t* allowed;
+  long long ld_in, ld_out, ld_h, ld_b, ld_a;
+  float rep_all, pres_all, freq_all;
+  int V, H, n_bias, n_blocks;
+};
+
+template <class E, int W>
+struct alignas(W * sizeof(E)) Pack {
+  E v[W];
+};
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
+  constexpr int W = 16 / static_cast<int>(sizeof(E));
+  extern __shared__ uint32_t s_word[];  // [kBlock] counts, then [kBlock] bias indices + 1 where there are biases
+  uint32_t* s_bias = s_word + kBlock;
+  const int row = static_cast<int>(blockIdx.x / g.n_blocks);
+  const int blk = static_cast<int>(blockIdx.x % g.n_blocks);
+  const int tid = threadIdx.x;
+  const E* in = g.in + row * g.ld_in;
+  E* out = g.out + row * g.ld_out;
+  // entry v of the row is entry v + shift of its 16-byte vectors
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(E) % W);
+  const bool same = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(E) % W) == shift;
+  const int v0 = blk * kBlock - shift;  // the block's first entry, before the row's start in its first block
+  const int n = min(kBlock, g.V - v0);
+
+  const int words = g.n_bias > 0 ? 2 * kBlock : kBlock;
+  for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  const int len = g.lengths != nullptr ? min(max(g.lengths[row], 0), g.H) : g.H;
+  const int first = g.prompts != nullptr ? min(max(g.prompts[row], 0), g.H) : 0;
+  const int32_t* hist = g.history + row * g.ld_h;
+  for (int i = tid; i < len; i += kThreads) {
+    const int id = hist[i];
+    if (id < 0 || id >= g.V) continue;
+    const int at = id - v0;
+    if (at < 0 || at >= n) continue;
+    if (i >= first) atomicAdd(&s_word[at], 1u);
+    else atomicOr(&s_word[at], kSeen);
+  }
+  for (int i = tid; i < g.n_bias; i += kThreads) {
+    const int id = g.bias_ids[row * g.ld_b + i];
+    if (id < 0 || id >= g.V) continue;
+    const int at = id - v0;
+    if (at >= 0 && at < n) atomicMax(&s_bias[at], static_cast<uint32_t>(i + 1));
+  }
+  __syncthreads();
+
+  const float rep = g.rep != nullptr ? g.rep[row] : g.rep_all;
+  const float pres = g.pres != nullptr ? g.pres[row] : g.pres_all;
+  const float freq = g.freq != nullptr ? g.freq[row] : g.freq_all;
+  const int32_t* allowed = g.allowed != nullptr ? g.allowed + row * g.ld_a : nullptr;
+  const float* bias = g.bias + row * g.ld_b;
+  const auto control = [&](float l, int at) {
+    const uint32_t w = s_word[at];
+    if (w != 0) {
+      l = l > 0.f ? l / rep : l * rep;
+      const uint32_t c = w & ~kSeen;
+      if (c != 0) l -= freq * static_cast<float>(c) + pres;
+    }
+    if (g.n_bias > 0) {
+      const uint32_t b = s_bias[at];
+      if (b != 0) l += bias[b - 1];
+    }
+    return l;
+  };
+  const float kNone = -__builtin_inff();
+  for (int i = tid * W; i < n; i += kThreads * W) {
+    const int v = v0 + i;
+    // bits of entries v .. v + W - 1 (of which those in the row count)
+    uint32_t bits = 0xffffffffu;
+    if (allowed != nullptr) {
+      const int lo = max(v, 0), hi = min(v + W, g.V) - 1;
+      const uint64_t pair = static_cast<uint32_t>(allowed[lo >> 5]) |
+                            (static_cast<uint64_t>(static_cast<uint32_t>(allowed[hi >> 5])) << 32);
+      // entry e's bit: word (e >> 5) - (lo >> 5) of the pair
+      bits = 0;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const int e = v + k;
+        if (e >= lo && e <= hi)
+          bits |= static_cast<uint32_t>(pair >> ((((e >> 5) != (lo >> 5)) ? 32 : 0) + (e & 31)) & 1u) << k;
+      }
+    }
+    if (same && v >= 0 && i + W <= n) {
+      Pack<E, W> p = *reinterpret_cast<const Pack<E, W>*>(in + v);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float l = control(to_f(p.v[k]), i + k);
+        p.v[k] = from_f<E>((bits >> k) & 1 ? l : kNone);
+      }
+      *reinterpret_cast<Pack<E, W>*>(out + v) = p;
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (v + k >= 0 && i + k < n) {
+          const float l = control(to_f(in[v + k]), i + k);
+          out[v + k] = from_f<E>((bits >> k) & 1 ? l : kNone);
+        }
+    }
+  }
+}
+
+template <class E>
+int run(Logits<E> g, int64_t rows, hipStream_t st) {
+  constexpr int W = 16 / static_cast<int>(sizeof(E));
+  g.n_blocks = (g.V + W - 1 + kBlock - 1) / kBlock;  // the shift may need one more
+  if (rows * g.n_blocks > INT_MAX)
+    return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
+  const size_t lds = (g.n_bias > 0 ? 2 : 1) * kBlock * sizeof(uint32_t);
+  hipLaunchKernelGGL(control_logits_kernel<E>, dim3(static_cast<unsigned>(rows * g.n_blocks)), dim3(kThreads), lds, st, g);
+  return launch_check("control_logits_kernel");
+}
+
+}  // namespace
+}  // namespace ossm
+
+using namespace ossm;
+
+extern "C" {
+
+int ossm_control_logits(int dtype, const void* logits, int64_t ld_logits, void* out, int64_t ld_out,
+                        const int32_t* history, int64_t ld_history, int64_t history_len,
+                        const int32_t* lengths, const int32_t* prompt_lengths, const float* repetition,
+                        float repetition_all, const float* presence, float presence_all,
+                        const float* frequency, float frequency_all, const int32_t* bias_ids,
+                        const float* bias_values, int64_t ld_bias, int64_t n_bias, const int32_t* allowed,
+                        int64_t ld_allowed, int64_t rows, int64_t vocab, ossm_stream_t stream_v) {
+  clear_error();
+  if (dtype != OSSM_F32 && dtype != OSSM_BF16)
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, "control_logits: unknown dtype");
+  if (rows < 0 || vocab < 0 || history_len < 0 || n_bias < 0)
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, "control_logits: negative size");
+  if (vocab > INT_MAX / 2 || history_len > INT_MAX / 2 || n_bias > INT_MAX / 2)
+    return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
+  if (rows == 0 || vocab == 0) return OSSM_OK;
+  if (!logits || !out || (history_len > 0 && !history) || (n_bias > 0 && (!bias_ids || !bias_values)))
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, "control_logits: null pointer");
+  if (rows > 1 && ld_out < vocab)
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, "control_logits: row stride of the output below the vocabulary");
+  hipStream_t st = static_cast<hipStream_t>(stream_v);
+  const auto go = [&](auto e) {
+    using E = decltype(e);
+    return run(Logits<E>{static_cast<const E*>(logits), static_cast<E*>(out), history, lengths, prompt_lengths,
+                         repetition, presence, frequency, bias_ids, bias_values, allowed, ld_logits, ld_out,
+                         ld_history, ld_bias, ld_allowed, repetition_all, presence_all, frequency_all,
+                         static_cast<int>(vocab), static_cast<int>(history_len), static_cast<int>(n_bias), 0},
+               rows, st);
+  };
+  return dtype == OSSM_BF16 ? go(bf16_t{}) : go(0.f);
+}
+
+}  // extern "C"
