@@ -94,6 +94,30 @@ int ossm_control_logits(int dtype, const void* logits, int64_t ld_logits, void* 
                         const float* bias_values, int64_t ld_bias, int64_t n_bias, const int32_t* allowed,
                         int64_t ld_allowed, int64_t rows, int64_t vocab, ossm_stream_t stream);
 
+enum { OSSM_ACT_SILU = 0, OSSM_ACT_GELU = 1, OSSM_ACT_GELU_TANH = 2, OSSM_ACT_SIGMOID = 3, OSSM_ACT_RELU = 4 };
+
+/*
+ * The gated projection of a feed-forward block:
+ *   a = x w_gate^T + b_gate,  b = x w_up^T + b_up,  y = act(a) b
+ * x E [rows, d_in], w_* E [d_out, d_in] with row strides ld_* (up to 2^20), b_* E
+ * [d_out] or null, y E [rows, d_out] dense.  a, b: f32 [rows, d_out] dense, written for the
+ * backward, or both null.
+ *
+ * ossm_gated_backward: with grad_y E [rows, d_out] (row stride ld_grad) and the
+ * forward's a and b, the gradients of x, of the weights and of the biases, all dense E;
+ * a null gradient is not computed.  float32 products take three bf16 terms of
+ * each operand (24 bits); in bfloat16 the gradients of a and b are rounded to
+ * bfloat16 before their products.
+ */
+int ossm_gated_forward(int dtype, const void* x, int64_t ld_x, const void* w_gate, int64_t ld_gate, const void* w_up,
+                       int64_t ld_up, const void* b_gate, const void* b_up, int activation, void* y, float* a, float* b,
+                       int64_t rows, int64_t d_in, int64_t d_out, ossm_stream_t stream);
+
+int ossm_gated_backward(int dtype, const void* grad_y, int64_t ld_grad, const void* x, int64_t ld_x, const void* w_gate,
+                        int64_t ld_gate, const void* w_up, int64_t ld_up, int activation, const float* a, const float* b,
+                        void* grad_x, void* grad_w_gate, void* grad_w_up, void* grad_b_gate, void* grad_b_up,
+                        int64_t rows, int64_t d_in, int64_t d_out, ossm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

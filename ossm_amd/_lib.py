@@ -158,6 +158,13 @@ _LM_SIGNATURES = {
     "ossm_lm_abi_version": (ctypes.c_int, []),
     "ossm_mixer_step": (ctypes.c_int, [ctypes.c_int, _vp, _c_int64] + [_vp] * 12 + [_c_int64] * 6 + [_vp]),
     "ossm_mixer_prompt": (ctypes.c_int, [ctypes.c_int, _vp, _c_int64] + [_vp] * 14 + [_c_int64] * 7 + [_vp]),
+    "ossm_gated_forward": (
+        ctypes.c_int,
+        [ctypes.c_int, _vp, _c_int64, _vp, _c_int64, _vp, _c_int64, _vp, _vp, ctypes.c_int, _vp, _vp, _vp] + [_c_int64] * 3
+        + [_vp]),
+    "ossm_gated_backward": (
+        ctypes.c_int,
+        [ctypes.c_int] + [_vp, _c_int64] * 4 + [ctypes.c_int] + [_vp] * 7 + [_c_int64] * 3 + [_vp]),
     "ossm_control_logits": (
         ctypes.c_int,
         [ctypes.c_int, _vp, _c_int64, _vp, _c_int64, _vp, _c_int64, _c_int64, _vp, _vp, _fp, ctypes.c_float, _fp,

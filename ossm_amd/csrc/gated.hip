@@ -1,0 +1,723 @@
+// The gated projection of a feed-forward block, forward and backward:
+//
+//   a = x Wg^T + bg,  b = x Wu^T + bu,  y = act(a) b
+//   da = dy b act'(a),  db = dy act(a)
+//   dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x,  dbg = sum da,  dbu = sum db
+//
+// for row-major x [T, D], Wg, Wu [F, D], y [T, F].  One product kernel serves all of
+// it: C(m, n) = sum_k A(m, k) B(n, k) of bf16 operands that lie either along k ("row":
+// x and the weights in the forward, da and db in dx) or across it ("col": the weights in
+// dx, both operands of dW).  Tiles go from memory straight into LDS, two buffers deep;
+// operands across k are transposed by the LDS's transposing reads on their way to
+// the matrix cores.  In the forward a tile's columns are half gate, half up rows of the
+// same outputs, so that each wave holds a and b of an output in the same registers and
+// the activation and product are its epilogue; training stores a and b (in float32) beside y,
+// which the backward's elementwise kernel turns into da and db.
+//
+// float32: operands are split into three bf16 planes, x = x0 + x1 + x2, and the
+// six products of order up to 2 are further stretches of k (split_mfma.hpp has the
+// error).  A value that is not finite is held as (x, 0, 0), which makes NaN of sums
+// where inf is due, so a wave whose sums are not all finite forms them again on the fp32
+// matrix instruction from the planes' sums.
+//
+// bfloat16: da and db are rounded to bf16 between the elementwise kernel and the products
+// (relative 2^-9, random; gradients then are 0.0024 off, where an exact sum rounded to
+// bf16 is 0.0017 off); sums are float32 throughout, and so are the stored a and b: in
+// bf16 they left 0.0031.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <initializer_list>
+#include <string>
+
+#include "../../include/ossm_lm.h"
+#include "lm_types.hpp"
+#include "runtime.hpp"
+#include "scan_device.hpp"
+#include "split_mfma.hpp"
+
+namespace ossm {
+namespace {
+
+constexpr int kTk = 64;           // k of a tile
+constexpr int kOutside = 0x7ffffff0;  // a buffer offset past every range: the load gives zeros
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// ---- activations -------------------------------------------------------------
+struct ActGrad {
+  float f, d;  // act(a), act'(a)
+};
+
+__device__ __forceinline__ ActGrad activate(int act, float a) {
+  switch (act) {
+    case OSSM_ACT_SILU: {
+      const float s = sigmoid_f(a);
+      return {a * s, s * (1.f + a * (1.f - s))};
+    }
+    case OSSM_ACT_SIGMOID: {
+      const float s = sigmoid_f(a);
+      return {s, s * (1.f - s)};
+    }
+    case OSSM_ACT_RELU: return {a > 0.f ? a : (a != a ? a : 0.f), a <= 0.f ? 0.f : 1.f};
+    case OSSM_ACT_GELU: {
+      const float cdf = 0.5f * (1.f + erff(a * 0.70710678118654752f));
+      return {a * cdf, cdf + a * __expf(-0.5f * a * a) * 0.39894228040143268f};
+    }
+    default: {  // gelu, tanh form
+      const float c = 0.79788456080286536f, k = 0.044715f;
+      const float e = __expf(2.f * c * (a + k * a * a * a));
+      const float t = 1.f - 2.f / (e + 1.f);
+      return {0.5f * a * (1.f + t), 0.5f * (1.f + t) + 0.5f * a * (1.f - t * t) * c * (1.f + 3.f * k * a * a)};
+    }
+  }
+}
+
+// ---- the product -------------------------------------------------------------
+// Plane s of part p starts at p[part] + s * plane.  Row: element (i, k) at i ld + k; col:
+// at k ld + i.  ld and every start are multiples of 8 elements (16 bytes).
+struct Operand {
+  const uint16_t* p[2];
+  long long plane, ld;
+};
+
+template <class E>
+struct Product {
+  Operand a, b;
+  int M, N, K;       // K: of one part
+  int parts, combos; // stretches of k: parts x (1, or 6 products of planes)
+  int tiles_m, tiles_n, splits, per_split;  // per_split: k tiles of one split
+  // outputs
+  E* c[2];           // plain: rows below `half` to c[0], from it on to c[1] (less half); gated: y in c[0]
+  long long ldc;
+  int half, half_rows;  // rows of each half that exist
+  float* part;       // splits > 1: [splits][M][N]
+  const E* bias[2];  // gated
+  float* save[2];    // gated: a, b or null
+  int act;
+};
+
+// products of planes, smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+__device__ __forceinline__ int plane_a(int combo) { return (0x001012 >> (4 * combo)) & 3; }
+__device__ __forceinline__ int plane_b(int combo) { return (0x010210 >> (4 * combo)) & 3; }
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+// One operand's tile of R rows (of m or n) and kTk k, from element (i0, k0), into LDS.  An LDS
+// row is 64 k (row) or R columns (col) of 16-byte chunks; chunk c sits at c ^ (i % 8)
+// (row) or c ^ 4 (k % 4) (col), which spreads the fragments' reads over the banks.
+template <bool COL, int R, int THREADS>
+__device__ __forceinline__ void load_tile(uint16_t* lds, const uint16_t* p, long long ld, int i0, int rows, int k0,
+                                          int K) {
+  const int tid = static_cast<int>(threadIdx.x), w = wave_id();
+  constexpr int kRounds = R * (kTk / 8) / THREADS;
+  if constexpr (!COL) {
+    const int n = min(rows - i0, R);  // may be <= 0: every chunk is outside
+    const uint16_t* base = p + (n > 0 ? static_cast<long long>(i0) * ld + k0 : 0);
+    const int bytes = n > 0 ? static_cast<int>(((n - 1) * ld + ((K - k0 + 7) & ~7)) * 2) : 0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, bytes, 0x00027000);
+    const int c = (tid & 7) ^ ((tid >> 3) & 7);
+    const bool in = k0 + c * 8 < K;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int r = (tid >> 3) + i * (THREADS / 8);
+      const int off = in && r < n ? static_cast<int>(r * ld * 2) + c * 16 : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * THREADS + w * kWave) * 8), 16, off, 0, 0, 0);
+    }
+  } else {
+    constexpr int kChunks = R / 8;
+    const int n = min(K - k0, kTk), cols = rows - i0;
+    const uint16_t* base = p + (cols > 0 ? static_cast<long long>(k0) * ld + i0 : 0);
+    const int bytes = cols > 0 ? static_cast<int>(((n - 1) * ld + ((min(cols, R) + 7) & ~7)) * 2) : 0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, bytes, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int q = i * THREADS + tid, k = q / kChunks, c = (q % kChunks) ^ (4 * (k & 3));
+      const int off = k < n && c * 8 < cols ? static_cast<int>(k * ld * 2) + c * 16 : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * THREADS + w * kWave) * 8), 16, off, 0, 0, 0);
+    }
+  }
+}
+
+// The wave's fragment of 32 rows from i0 at k step kk (16 k) of a tile in LDS: lane l
+// holds row l % 32 at k = 8 (l / 32) .. + 7.
+template <bool COL, int R>
+__device__ __forceinline__ bf16x8 load_frag(const uint16_t* lds, int i0, int kk) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  if constexpr (!COL) {
+    const int r = i0 + (lane & 31), c = kk * 2 + (lane >> 5);
+    return *reinterpret_cast<const bf16x8*>(lds + r * kTk + ((c ^ (r & 7)) * 8));
+  } else {
+    // a group of 16 lanes reads 4 k of 16 columns, transposed: lane i gets column i
+    const int g = lane >> 4, i16 = lane & 15, kr = i16 >> 2;
+    const int k = kk * 16 + (g >> 1) * 8 + kr, col = i0 + (g & 1) * 16 + (i16 & 3) * 4;
+    const uint16_t* q = lds + k * R + (((col >> 3) ^ (4 * kr)) * 8) + (col & 7);
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)q);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(q + 4 * R));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// Element (i, k) of an operand as its planes' sum (0 outside).
+template <bool COL>
+__device__ __forceinline__ float element(const Operand& o, int part, int i, int rows, int k, int K) {
+  if (i >= rows || k >= K) return 0.f;
+  const uint16_t* p = o.p[part] + (COL ? static_cast<long long>(k) * o.ld + i : static_cast<long long>(i) * o.ld + k);
+  return (to_f(bf16_t{p[2 * o.plane]}) + to_f(bf16_t{p[o.plane]})) + to_f(bf16_t{p[0]});
+}
+
+// Workgroup tile: WM x WN waves of FM x FN fragments of 32 x 32.  GATED: the tile's
+// columns are 32-column pairs, gate and up rows of the same outputs (N counts outputs).
+template <class E, bool ACOL, bool BCOL, bool GATED, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> g) {
+  constexpr int THREADS = WM * WN * kWave, TM = WM * FM * 32, TN = WN * FN * 32;
+  constexpr int NOUT = GATED ? TN / 2 : TN;  // output columns of a tile
+  static_assert(!GATED || (FN == 2 && !BCOL), "a wave holds 32 gate and 32 up columns");
+  extern __shared__ __align__(16) uint16_t s_tiles[];  // two buffers of (A, B)
+  constexpr int kA = TM * kTk, kBuf = (TM + TN) * kTk;
+  const int w = wave_id(), wm = w / WN, wn = w % WN;
+
+  // consecutive ids share an XCD; bands of 8 tile rows keep their operands in its L2
+  const int total = static_cast<int>(gridDim.x), per = total / 8, bid = static_cast<int>(blockIdx.x);
+  int id = bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int split = id / tiles;
+  id -= split * tiles;
+  const int band = id / (8 * g.tiles_n), first = band * 8, in_band = min(8, g.tiles_m - first);
+  const int m0 = (first + (id - band * 8 * g.tiles_n) % in_band) * TM;
+  const int n0 = (id - band * 8 * g.tiles_n) / in_band * NOUT;
+
+  const int k_tiles = (g.K + kTk - 1) / kTk;
+  const int kt0 = split * g.per_split, kt1 = min(kt0 + g.per_split, k_tiles);
+  const int steps = (kt1 - kt0) * g.parts * g.combos;
+
+  const auto load = [&](int step, int buf) {
+    const int seg = step / (kt1 - kt0), k0 = (kt0 + step % (kt1 - kt0)) * kTk;
+    const int combo = seg / g.parts, part = seg % g.parts;
+    uint16_t* s = s_tiles + buf * kBuf;
+    const long long pa = (g.combos > 1 ? plane_a(combo) : 0) * g.a.plane, pb = (g.combos > 1 ? plane_b(combo) : 0) * g.b.plane;
+    load_tile<ACOL, TM, THREADS>(s, g.a.p[part] + pa, g.a.ld, m0, g.M, k0, g.K);
+    if constexpr (GATED) {
+      load_tile<BCOL, TN / 2, THREADS>(s + kA, g.b.p[0] + pb, g.b.ld, n0, g.N, k0, g.K);
+      load_tile<BCOL, TN / 2, THREADS>(s + kA + TN / 2 * kTk, g.b.p[1] + pb, g.b.ld, n0, g.N, k0, g.K);
+    } else {
+      load_tile<BCOL, TN, THREADS>(s + kA, g.b.p[part] + pb, g.b.ld, n0, g.N, k0, g.K);
+    }
+  };
+
+  floatx16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  if (steps > 0) load(0, 0);
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the tile has arrived
+    __syncthreads();  // everyone's has, and everyone is done with the other buffer
+    if (step + 1 < steps) load(step + 1, (step + 1) & 1);
+    const uint16_t* sa = s_tiles + (step & 1) * kBuf;
+    const uint16_t* sb = sa + kA;
+#pragma unroll
+    for (int kk = 0; kk < kTk / 16; ++kk) {
+      bf16x8 fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = load_frag<ACOL, TM>(sa, wm * FM * 32 + i * 32, kk);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        fb[j] = load_frag<BCOL, TN>(sb, GATED ? j * (TN / 2) + wn * 32 : wn * FN * 32 + j * 32, kk);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_bf16(fa[i], fb[j], acc[i][j]);
+    }
+  }
+
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
+  if constexpr (sizeof(E) == 4) {
+    bool again = false;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) again = again || any_nonfinite(acc[i]);
+    if (again) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+      const int k_end = min(kt1 * kTk, g.K);
+      for (int part = 0; part < g.parts; ++part)
+#pragma unroll 1
+        for (int k = kt0 * kTk; k < k_end; k += 2) {
+          float va[FM], vb[FN];
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+            va[i] = element<ACOL>(g.a, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            vb[j] = GATED ? element<BCOL>(g.b, j, n0 + wn * 32 + l32, g.N, k + half, k_end)
+                          : element<BCOL>(g.b, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(va[i], vb[j], acc[i][j]);
+        }
+    }
+  }
+
+  // register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
+  if constexpr (GATED) {
+    const int n = n0 + wn * 32 + l32;
+    const bool in = n < g.N;
+    const float bg = in && g.bias[0] != nullptr ? to_f(g.bias[0][n]) : 0.f;
+    const float bu = in && g.bias[1] != nullptr ? to_f(g.bias[1][n]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = m0 + wm * FM * 32 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        const float a = acc[i][0][r] + bg, b = acc[i][1][r] + bu;
+        if (in && m < g.M) {
+          const long long at = m * g.ldc + n;
+          g.c[0][at] = from_f<E>(activate(g.act, a).f * b);
+          if (g.save[0] != nullptr) {
+            g.save[0][at] = a;
+            g.save[1][at] = b;
+          }
+        }
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = m0 + wm * FM * 32 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (m >= g.M) continue;
+        const int second = m >= g.half ? 1 : 0, row = m - second * g.half;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int n = n0 + wn * FN * 32 + j * 32 + l32;
+          if (n >= g.N) continue;
+          if (g.splits > 1) g.part[(static_cast<size_t>(split) * g.M + m) * g.N + n] = acc[i][j][r];
+          else if (row < g.half_rows && g.c[second] != nullptr) g.c[second][row * g.ldc + n] = from_f<E>(acc[i][j][r]);
+        }
+      }
+  }
+}
+
+// The splits' sums, in order.
+template <class E>
+__global__ __launch_bounds__(256) void product_sum_kernel(Product<E> g) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, n = static_cast<long long>(g.M) * g.N;
+  if (i >= n) return;
+  const int m = static_cast<int>(i / g.N), col = static_cast<int>(i % g.N);
+  const int second = m >= g.half ? 1 : 0, row = m - second * g.half;
+  if (row >= g.half_rows || g.c[second] == nullptr) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < g.splits; ++k) s += g.part[k * n + i];
+  g.c[second][row * g.ldc + col] = from_f<E>(s);
+}
+
+// ---- operands as bf16 planes ---------------------------------------------------
+// x as the nearest bf16s of it and of what they leave; what is not finite as (x, 0, 0).
+__device__ __forceinline__ void split3(float x, uint16_t (&t)[3]) {
+  t[0] = from_f<bf16_t>(x).bits;
+  t[1] = t[2] = 0;
+  if (!(fabsf(x) <= 3.4028234663852886e38f)) return;
+  if ((t[0] & 0x7fff) == 0x7f80) t[0] -= 1;  // rounded past the largest bf16
+  const float r = x - to_f(bf16_t{t[0]});
+  t[1] = from_f<bf16_t>(r).bits;
+  t[2] = from_f<bf16_t>(r - to_f(bf16_t{t[1]})).bits;
+}
+
+__device__ __forceinline__ void put8(uint16_t* dst, const uint16_t (&v)[8]) {
+  u32x4 q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = v[2 * i] | (static_cast<uint32_t>(v[2 * i + 1]) << 16);
+  *reinterpret_cast<u32x4*>(dst) = q;
+}
+
+// rows of C elements as 1 (bf16) or 3 (float32) planes of rows of Cp, zeros from C on
+template <class E>
+__global__ __launch_bounds__(256) void pack_kernel(const E* __restrict__ src, long long ld, uint16_t* __restrict__ dst,
+                                                   long long plane, long long rows, int C, int Cp) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const int chunks = Cp / 8;
+  if (i >= rows * chunks) return;
+  const long long r = i / chunks;
+  const int c = static_cast<int>(i % chunks) * 8;
+  const E* s = src + r * ld + c;
+  uint16_t t[3][8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint16_t v[3] = {0, 0, 0};
+    if (c + k < C) {
+      if constexpr (sizeof(E) == 4) split3(s[k], v);
+      else v[0] = s[k].bits;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) t[j][k] = v[j];
+  }
+#pragma unroll
+  for (int j = 0; j < (sizeof(E) == 4 ? 3 : 1); ++j) put8(dst + j * plane + r * Cp + c, t[j]);
+}
+
+// ---- da, db ----------------------------------------------------------------------
+constexpr int kRowsPer = 16;  // rows of a thread
+
+// da and db side by side, [T][2 Fp] (1 or 3 planes), zeros from F on, and each thread's
+// sums over its rows for the biases' gradients (in float32, before any rounding).
+template <class E>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go, long long ld_go, const float* __restrict__ a,
+                                                        const float* __restrict__ b, uint16_t* __restrict__ dab,
+                                                        long long plane, float* __restrict__ sums, int T, int F, int Fp,
+                                                        int act) {
+  const int groups = Fp / 8;
+  const long long gid = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const int rb = static_cast<int>(gid / groups), f0 = static_cast<int>(gid % groups) * 8;
+  if (rb * kRowsPer >= T) return;
+  float sa[8], sb[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sa[i] = sb[i] = 0.f;
+  for (int r = rb * kRowsPer; r < min(T, (rb + 1) * kRowsPer); ++r) {
+    uint16_t ta[3][8], tb[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint16_t va[3] = {0, 0, 0}, vb[3] = {0, 0, 0};
+      if (f0 + i < F) {
+        const long long at = static_cast<long long>(r) * F + f0 + i;
+        const ActGrad d = activate(act, a[at]);
+        const float g = to_f(go[r * ld_go + f0 + i]);
+        const float ga = g * b[at] * d.d, gb = g * d.f;
+        sa[i] += ga;
+        sb[i] += gb;
+        if constexpr (sizeof(E) == 4) {
+          split3(ga, va);
+          split3(gb, vb);
+        } else {
+          va[0] = from_f<bf16_t>(ga).bits;
+          vb[0] = from_f<bf16_t>(gb).bits;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 3; ++j) { ta[j][i] = va[j]; tb[j][i] = vb[j]; }
+    }
+#pragma unroll
+    for (int j = 0; j < (sizeof(E) == 4 ? 3 : 1); ++j) {
+      uint16_t* dst = dab + j * plane + static_cast<long long>(r) * 2 * Fp + f0;
+      put8(dst, ta[j]);
+      put8(dst + Fp, tb[j]);
+    }
+  }
+  if (sums != nullptr) {
+    float* dst = sums + static_cast<long long>(rb) * 2 * Fp + f0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { dst[i] = sa[i]; dst[Fp + i] = sb[i]; }
+  }
+}
+
+// Column sums of [rows][2 Fp] in a fixed order: 64 columns, 4 lanes of rows each.
+template <class E>
+__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int rows, int F, int Fp, E* ga,
+                                                        E* gb) {
+  __shared__ float s_p[4][kWave];
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), w = wave_id();
+  const int c = static_cast<int>(blockIdx.x) * kWave + lane;
+  float s = 0.f;
+  if (c < 2 * Fp)
+#pragma unroll 8
+    for (int r = w; r < rows; r += 4) s += sums[static_cast<long long>(r) * 2 * Fp + c];
+  s_p[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || c >= 2 * Fp) return;
+  s = ((s_p[0][lane] + s_p[1][lane]) + s_p[2][lane]) + s_p[3][lane];
+  E* out = c < Fp ? ga : gb;
+  const int f = c < Fp ? c : c - Fp;
+  if (f < F && out != nullptr) out[f] = from_f<E>(s);
+}
+
+// ---- host ------------------------------------------------------------------------
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Row-major matrices of one shape (one, or the gate's and the up weights) as the two
+// parts of an operand: themselves where every row can be read in place, else planes in
+// the workspace.
+template <class E>
+struct Source {
+  const E* src[2];
+  int64_t ld[2], rows, cols;
+  int n;
+  bool direct() const {
+    bool ok = sizeof(E) == 2 && cols % 8 == 0;
+    for (int i = 0; i < n; ++i) ok = ok && aligned16(src[i]) && ld[i] % 8 == 0 && ld[i] == ld[0];
+    return ok;
+  }
+  int64_t plane() const { return up8(rows * up8(cols)); }
+  int64_t elems() const { return direct() ? 0 : n * plane() * (sizeof(E) == 4 ? 3 : 1); }  // of bf16
+};
+
+template <class E>
+int pack(const Source<E>& m, uint16_t* ws, Operand* o, hipStream_t st) {
+  if (m.direct()) {
+    for (int i = 0; i < m.n; ++i) o->p[i] = reinterpret_cast<const uint16_t*>(m.src[i]);
+    o->ld = m.ld[0];
+    o->plane = 0;
+    return OSSM_OK;
+  }
+  const int64_t cp = up8(m.cols), chunks = m.rows * (cp / 8);
+  if (chunks == 0) return OSSM_OK;  // nothing is read
+  o->ld = cp;
+  o->plane = m.plane();
+  for (int i = 0; i < m.n; ++i) {
+    uint16_t* dst = ws + i * (m.elems() / m.n);
+    o->p[i] = dst;
+    hipLaunchKernelGGL(pack_kernel<E>, dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, st, m.src[i], m.ld[i],
+                       dst, o->plane, m.rows, static_cast<int>(m.cols), static_cast<int>(cp));
+    if (int rc = launch_check("pack_kernel")) return rc;
+  }
+  return OSSM_OK;
+}
+
+template <class E, bool ACOL, bool BCOL, bool GATED, int WM, int WN, int FM, int FN>
+int launch_tiled(Product<E> g, hipStream_t st) {
+  constexpr int TM = WM * FM * 32, TN = WN * FN * 32;
+  constexpr int lds = 2 * (TM + TN) * kTk * 2;
+  g.tiles_m = (g.M + TM - 1) / TM;
+  g.tiles_n = (g.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
+  const int64_t grid = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
+  if (grid > INT_MAX) return set_error(OSSM_ERR_UNSUPPORTED, "gated: size exceeds launch limits");
+  auto kern = product_kernel<E, ACOL, BCOL, GATED, WM, WN, FM, FN>;
+  if (int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+                         "hipFuncSetAttribute"))
+    return rc;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * kWave), lds, st, g);
+  if (int rc = launch_check("product_kernel")) return rc;
+  if (g.splits > 1) {
+    const int64_t n = static_cast<int64_t>(g.M) * g.N;
+    hipLaunchKernelGGL(product_sum_kernel<E>, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, g);
+    return launch_check("product_sum_kernel");
+  }
+  return OSSM_OK;
+}
+
+int64_t tiles(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
+
+// How many ways the k of an [M, N] product of `k_tiles` tiles is split: towards two
+// workgroups a CU, none with fewer than 8 tiles.
+int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t cus) {
+  const int64_t t = std::max<int64_t>(1, tiles(m, n, 128, 128));  // an input without columns has none
+  return static_cast<int>(std::max<int64_t>(1, std::min(2 * cus / t, k_tiles / 8)));
+}
+
+template <class E, bool ACOL, bool BCOL, bool GATED>
+int launch_product(Product<E> g, int64_t cus, hipStream_t st) {
+  const int k_tiles = std::max(1, (g.K + kTk - 1) / kTk);
+  g.per_split = (k_tiles + g.splits - 1) / g.splits;
+  g.splits = (k_tiles + g.per_split - 1) / g.per_split;
+  if (g.splits == 1 && tiles(g.M, g.N, 256, GATED ? 128 : 256) >= cus)
+    return launch_tiled<E, ACOL, BCOL, GATED, 2, 4, 4, 2>(g, st);
+  return launch_tiled<E, ACOL, BCOL, GATED, 2, 2, 2, 2>(g, st);
+}
+
+constexpr int kCombos(size_t e) { return e == 4 ? 6 : 1; }
+
+int check_gated(const char* what, int dtype, int act, int64_t T, int64_t D, int64_t F, std::initializer_list<int64_t> d_strides) {
+  const std::string w(what);
+  if (dtype != OSSM_F32 && dtype != OSSM_BF16) return set_error(OSSM_ERR_INVALID_ARGUMENT, w + ": unknown dtype");
+  if (act < 0 || act > OSSM_ACT_RELU) return set_error(OSSM_ERR_INVALID_ARGUMENT, w + ": unknown activation");
+  if (T < 0 || D < 0 || F < 0) return set_error(OSSM_ERR_INVALID_ARGUMENT, w + ": negative size");
+  for (int64_t ld : d_strides) {
+    if (ld < D) return set_error(OSSM_ERR_INVALID_ARGUMENT, w + ": a row stride is below the row");
+    if (ld > (1 << 20)) return set_error(OSSM_ERR_UNSUPPORTED, w + ": row strides up to 2^20");
+  }
+  if (T > (1 << 26) || D > (1 << 20) || F > (1 << 19) || T * std::max(D, F) > (int64_t(1) << 40))
+    return set_error(OSSM_ERR_UNSUPPORTED, w + ": size exceeds launch limits");
+  return OSSM_OK;
+}
+
+template <class E>
+struct Gated {
+  const E* x;
+  const E* w[2];
+  const E* bias[2];
+  int64_t ld_x, ld_w[2], T, D, F;
+  int act;
+  Source<E> rows() const { return {{x, nullptr}, {ld_x, 0}, T, D, 1}; }
+  Source<E> weights() const { return {{w[0], w[1]}, {ld_w[0], ld_w[1]}, F, D, 2}; }
+};
+
+template <class E>
+int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipStream_t st) {
+  const Source<E> px = p.rows(), pw = p.weights();
+  void* ws = nullptr;
+  if (px.elems() + pw.elems() > 0)
+    if (int rc = acquire_workspace(call, static_cast<size_t>(px.elems() + pw.elems()) * 2, &ws)) return rc;
+  Product<E> g{};
+  uint16_t* q = static_cast<uint16_t*>(ws);
+  if (int rc = pack(px, q, &g.a, st)) return rc;
+  if (int rc = pack(pw, q + px.elems(), &g.b, st)) return rc;
+  g.M = static_cast<int>(p.T);
+  g.N = static_cast<int>(p.F);
+  g.K = static_cast<int>(p.D);
+  g.parts = g.splits = 1;
+  g.combos = kCombos(sizeof(E));
+  g.c[0] = y;
+  g.ldc = p.F;
+  for (int i = 0; i < 2; ++i) g.bias[i] = p.bias[i];
+  g.save[0] = a;
+  g.save[1] = b;
+  g.act = p.act;
+  return launch_product<E, false, false, true>(g, std::max(1, device_cu_count(call.device())), st);
+}
+
+template <class E>
+int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, const float* b, E* gx, E* const gw[2], E* const gb[2],
+             StreamCall& call, hipStream_t st) {
+  const Source<E> px = p.rows(), pw = p.weights();
+  const int64_t Fp = up8(p.F), planes = sizeof(E) == 4 ? 3 : 1;
+  const int64_t dab_plane = p.T * 2 * Fp, rbs = (p.T + kRowsPer - 1) / kRowsPer;
+  const int64_t cus = std::max(1, device_cu_count(call.device()));
+  const bool want_w = gw[0] != nullptr || gw[1] != nullptr, want_b = gb[0] != nullptr || gb[1] != nullptr;
+  const int sx = choose_splits(p.T, p.D, (p.F + kTk - 1) / kTk, cus);
+  const int sw = choose_splits(2 * Fp, p.D, (p.T + kTk - 1) / kTk, cus);
+  const int64_t part = std::max<int64_t>(gx != nullptr && sx > 1 ? sx * p.T * p.D : 0, want_w && sw > 1 ? sw * 2 * Fp * p.D : 0);
+  // bytes; every start a multiple of 16
+  size_t at = 0;
+  const auto take = [&](int64_t bytes) { const size_t o = at; at += static_cast<size_t>((bytes + 255) / 256 * 256); return o; };
+  const size_t o_dab = take(dab_plane * planes * 2), o_x = take(want_w ? px.elems() * 2 : 0);
+  const size_t o_w = take(gx != nullptr ? pw.elems() * 2 : 0), o_part = take(part * 4);
+  const size_t o_sums = take(want_b ? rbs * 2 * Fp * 4 : 0);
+  void* ws = nullptr;
+  if (int rc = acquire_workspace(call, at, &ws)) return rc;
+  char* base = static_cast<char*>(ws);
+  uint16_t* dab = reinterpret_cast<uint16_t*>(base + o_dab);
+  float* sums = want_b ? reinterpret_cast<float*>(base + o_sums) : nullptr;
+  const int T = static_cast<int>(p.T), F = static_cast<int>(p.F), D = static_cast<int>(p.D), fp = static_cast<int>(Fp);
+  hipLaunchKernelGGL(gate_grad_kernel<E>, dim3(static_cast<unsigned>((rbs * (Fp / 8) + 255) / 256)), dim3(256), 0, st, go,
+                     ld_go, a, b, dab, static_cast<long long>(dab_plane), sums, T, F, fp, p.act);
+  if (int rc = launch_check("gate_grad_kernel")) return rc;
+  if (want_b) {
+    hipLaunchKernelGGL(bias_grad_kernel<E>, dim3(static_cast<unsigned>((2 * Fp + kWave - 1) / kWave)), dim3(256), 0, st,
+                       static_cast<const float*>(sums), static_cast<int>(rbs), F, fp, gb[0], gb[1]);
+    if (int rc = launch_check("bias_grad_kernel")) return rc;
+  }
+  Product<E> g{};
+  g.combos = kCombos(sizeof(E));
+  g.part = reinterpret_cast<float*>(base + o_part);
+  g.a.p[0] = dab;
+  g.a.p[1] = dab + Fp;
+  g.a.plane = dab_plane;
+  g.a.ld = 2 * Fp;
+  g.N = D;
+  g.ldc = p.D;
+  if (gx != nullptr) {
+    if (int rc = pack(pw, reinterpret_cast<uint16_t*>(base + o_w), &g.b, st)) return rc;
+    g.M = T;
+    g.K = F;
+    g.parts = 2;
+    g.splits = sx;
+    g.half = g.half_rows = T;
+    g.c[0] = gx;
+    if (int rc = launch_product<E, false, true, false>(g, cus, st)) return rc;
+  }
+  if (want_w) {
+    if (int rc = pack(px, reinterpret_cast<uint16_t*>(base + o_x), &g.b, st)) return rc;
+    g.M = 2 * fp;
+    g.K = T;
+    g.parts = 1;
+    g.splits = sw;
+    g.half = fp;
+    g.half_rows = F;
+    g.c[0] = gw[0];
+    g.c[1] = gw[1];
+    if (int rc = launch_product<E, true, true, false>(g, cus, st)) return rc;
+  }
+  return OSSM_OK;
+}
+
+__global__ __launch_bounds__(256) void gated_zero_kernel(uint16_t* p, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+int zero(void* p, int64_t bytes, hipStream_t st) {
+  if (p == nullptr || bytes == 0) return OSSM_OK;
+  const int64_t n = bytes / 2;
+  hipLaunchKernelGGL(gated_zero_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, static_cast<uint16_t*>(p), n);
+  return launch_check("gated_zero_kernel");
+}
+
+}  // namespace
+}  // namespace ossm
+
+using namespace ossm;
+
+extern "C" {
+
+int ossm_gated_forward(int dtype, const void* x, int64_t ld_x, const void* w_gate, int64_t ld_gate, const void* w_up,
+                       int64_t ld_up, const void* b_gate, const void* b_up, int activation, void* y, float* a, float* b,
+                       int64_t rows, int64_t d_in, int64_t d_out, ossm_stream_t stream_v) {
+  clear_error();
+  const char* what = "gated_forward";
+  if (int rc = check_gated(what, dtype, activation, rows, d_in, d_out, {ld_x, ld_gate, ld_up})) return rc;
+  if (rows == 0 || d_out == 0) return OSSM_OK;
+  if (!y || (d_in > 0 && (!x || !w_gate || !w_up)) || (a == nullptr) != (b == nullptr))
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": null pointer");
+  hipStream_t st = static_cast<hipStream_t>(stream_v);
+  StreamCall call(st);
+  if (call.status()) return call.status();
+  const auto run = [&](auto e) {
+    using E = decltype(e);
+    const auto in = [](const void* q) { return static_cast<const E*>(q); };
+    const Gated<E> p{in(x), {in(w_gate), in(w_up)}, {in(b_gate), in(b_up)}, ld_x, {ld_gate, ld_up}, rows, d_in, d_out, activation};
+    return forward(p, static_cast<E*>(y), a, b, call, st);
+  };
+  return dtype == OSSM_BF16 ? run(bf16_t{}) : run(0.f);
+}
+
+int ossm_gated_backward(int dtype, const void* grad_y, int64_t ld_grad, const void* x, int64_t ld_x, const void* w_gate,
+                        int64_t ld_gate, const void* w_up, int64_t ld_up, int activation, const float* a, const float* b,
+                        void* grad_x, void* grad_w_gate, void* grad_w_up, void* grad_b_gate, void* grad_b_up,
+                        int64_t rows, int64_t d_in, int64_t d_out, ossm_stream_t stream_v) {
+  clear_error();
+  const char* what = "gated_backward";
+  if (int rc = check_gated(what, dtype, activation, rows, d_in, d_out, {ld_x, ld_gate, ld_up})) return rc;
+  if (rows > 0 && ld_grad < d_out)
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": a row stride is below the row");
+  hipStream_t st = static_cast<hipStream_t>(stream_v);
+  const int64_t e = dtype == OSSM_BF16 ? 2 : 4;
+  if (rows == 0 || d_out == 0 || d_in == 0) {
+    if (int rc = zero(grad_x, rows * d_in * e, st)) return rc;
+    if (int rc = zero(grad_w_gate, d_out * d_in * e, st)) return rc;
+    if (int rc = zero(grad_w_up, d_out * d_in * e, st)) return rc;
+    if (rows == 0 || d_out == 0) {
+      if (int rc = zero(grad_b_gate, d_out * e, st)) return rc;
+      return zero(grad_b_up, d_out * e, st);
+    }
+    grad_x = grad_w_gate = grad_w_up = nullptr;
+  }
+  if (!grad_y || !a || !b || (d_in > 0 && (!x || !w_gate || !w_up)))
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": null pointer");
+  StreamCall call(st);
+  if (call.status()) return call.status();
+  const auto run = [&](auto t) {
+    using E = decltype(t);
+    const auto in = [](const void* q) { return static_cast<const E*>(q); };
+    const auto out = [](void* q) { return static_cast<E*>(q); };
+    const Gated<E> p{in(x), {in(w_gate), in(w_up)}, {nullptr, nullptr}, ld_x, {ld_gate, ld_up}, rows, d_in, d_out, activation};
+    E* const gw[2] = {out(grad_w_gate), out(grad_w_up)};
+    E* const gb[2] = {out(grad_b_gate), out(grad_b_up)};
+    return backward(p, in(grad_y), ld_grad, a, b, out(grad_x), gw, gb, call, st);
+  };
+  return dtype == OSSM_BF16 ? run(bf16_t{}) : run(0.f);
+}
+
+}  // extern "C"

@@ -98,3 +98,28 @@ def test_pack_allowed():
         assert w.dtype == torch.int32 and w.shape == (3, (V + 31) // 32)
         for i in range(3):
             assert [(int(w[i, v // 32]) >> (v % 32)) & 1 for v in range(V)] == m[i].int().tolist()
+
+
+@pytest.mark.parametrize("name", ["ossm_gated_forward", "ossm_gated_backward"])
+def test_gated_entry_points_check_before_any_hip_call(name):
+    ld = {"ld_x": 8, "ld_gate": 8, "ld_up": 8, "ld_grad": 8}
+    assert _call(name, dtype=9) == (1, f"{name[5:]}: unknown dtype")
+    assert _call(name, activation=5)[0] == 1 and _call(name, activation=-1)[0] == 1
+    assert _call(name, rows=-1)[0] == 1 and _call(name, d_in=2)[0] == 1
+    assert _call(name, ld_x=2**21)[0] == 3 and _call(name, **ld, d_out=2**20)[0] == 3
+    for p in ("x", "w_gate", "w_up", "b" if name.endswith("forward") else "a"):
+        assert _call(name, **ld, **{p: None}) == (1, f"{name[5:]}: null pointer")
+    if name.endswith("backward"):
+        assert _call(name, ld_grad=0)[0] == 1
+
+
+def test_gated_refuses_host_tensors_and_unknown_activations():
+    from ossm_amd.gated import GatedFeedForward, gated_linear
+
+    z = torch.zeros(2, 8)
+    with pytest.raises(RuntimeError, match="one dtype on one GPU"):
+        gated_linear(z, z, z)
+    with pytest.raises(ValueError, match="activation"):
+        gated_linear(z, z, z, activation="tanh")
+    with pytest.raises(ValueError, match="activation"):
+        GatedFeedForward(8, 8, activation="tanh")
