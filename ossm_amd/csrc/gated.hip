@@ -17,8 +17,8 @@
 // float32: operands are split into three bf16 planes, x = x0 + x1 + x2, and the
 // six products of order up to 2 are further stretches of k (split_mfma.hpp has the
 // error).  A value that is not finite is held as (x, 0, 0), which makes NaN of sums
-// where inf is due, so a wave whose sums are not all finite forms them again on the fp32
-// matrix instruction from the planes' sums.
+// where inf is due, so sums that are not finite are formed again on the fp32 matrix
+// instruction from the planes' sums.
 //
 // bfloat16: da and db are rounded to bf16 between the elementwise kernel and the products
 // (relative 2^-9, random; gradients then are 0.0024 off, where an exact sum rounded to
@@ -32,6 +32,7 @@
 #include <cstdint>
 #include <initializer_list>
 #include <string>
+#include <type_traits>
 
 #include "../../include/ossm_lm.h"
 #include "lm_types.hpp"
@@ -52,8 +53,9 @@ struct ActGrad {
   float f, d;  // act(a), act'(a)
 };
 
-__device__ __forceinline__ ActGrad activate(int act, float a) {
-  switch (act) {
+template <int ACT>
+__device__ __forceinline__ ActGrad activate(float a) {
+  switch (ACT) {
     case OSSM_ACT_SILU: {
       const float s = sigmoid_f(a);
       return {a * s, s * (1.f + a * (1.f - s))};
@@ -73,6 +75,16 @@ __device__ __forceinline__ ActGrad activate(int act, float a) {
       const float t = 1.f - 2.f / (e + 1.f);
       return {0.5f * a * (1.f + t), 0.5f * (1.f + t) + 0.5f * a * (1.f - t * t) * c * (1.f + 3.f * k * a * a)};
     }
+  }
+}
+
+__device__ __forceinline__ float activation_of(int act, float a) {
+  switch (act) {
+    case OSSM_ACT_SILU: return activate<OSSM_ACT_SILU>(a).f;
+    case OSSM_ACT_SIGMOID: return activate<OSSM_ACT_SIGMOID>(a).f;
+    case OSSM_ACT_RELU: return activate<OSSM_ACT_RELU>(a).f;
+    case OSSM_ACT_GELU: return activate<OSSM_ACT_GELU>(a).f;
+    default: return activate<OSSM_ACT_GELU_TANH>(a).f;
   }
 }
 
@@ -241,34 +253,28 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
 
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
   if constexpr (sizeof(E) == 4) {
-    bool again = false;
+    // the elements of a fragment that are not finite
+    const int k_end = min(kt1 * kTk, g.K);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) again = again || any_nonfinite(acc[i]);
-    if (again) {
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-      const int k_end = min(kt1 * kTk, g.K);
-      for (int part = 0; part < g.parts; ++part)
+      for (int j = 0; j < FN; ++j) {
+        const floatx16 one[1] = {acc[i][j]};
+        if (any_nonfinite(one)) {
+          floatx16 c = {};
+          for (int part = 0; part < g.parts; ++part)
 #pragma unroll 1
-        for (int k = kt0 * kTk; k < k_end; k += 2) {
-          float va[FM], vb[FN];
+            for (int k = kt0 * kTk; k < k_end; k += 2) {
+              const float va = element<ACOL>(g.a, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
+              const float vb = GATED ? element<BCOL>(g.b, j, n0 + wn * 32 + l32, g.N, k + half, k_end)
+                                     : element<BCOL>(g.b, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
+              c = mfma32(va, vb, c);
+            }
 #pragma unroll
-          for (int i = 0; i < FM; ++i)
-            va[i] = element<ACOL>(g.a, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            vb[j] = GATED ? element<BCOL>(g.b, j, n0 + wn * 32 + l32, g.N, k + half, k_end)
-                          : element<BCOL>(g.b, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(va[i], vb[j], acc[i][j]);
+          for (int r = 0; r < 16; ++r)
+            acc[i][j][r] = fabsf(acc[i][j][r]) <= 3.4028234663852886e38f ? acc[i][j][r] : c[r];
         }
-    }
+      }
   }
 
   // register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
@@ -285,7 +291,7 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
         const float a = acc[i][0][r] + bg, b = acc[i][1][r] + bu;
         if (in && m < g.M) {
           const long long at = m * g.ldc + n;
-          g.c[0][at] = from_f<E>(activate(g.act, a).f * b);
+          g.c[0][at] = from_f<E>(activation_of(g.act, a) * b);
           if (g.save[0] != nullptr) {
             g.save[0][at] = a;
             g.save[1][at] = b;
@@ -372,13 +378,29 @@ __global__ __launch_bounds__(256) void pack_kernel(const E* __restrict__ src, lo
 // ---- da, db ----------------------------------------------------------------------
 constexpr int kRowsPer = 16;  // rows of a thread
 
+__device__ __forceinline__ void read8(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void read8(const bf16_t* p, float (&v)[8]) {
+  const u32x4 q = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(q[i]);
+    v[2 * i + 1] = bf16_hi(q[i]);
+  }
+}
+
 // da and db side by side, [T][2 Fp] (1 or 3 planes), zeros from F on, and each thread's
-// sums over its rows for the biases' gradients (in float32, before any rounding).
-template <class E>
-__global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go, long long ld_go, const float* __restrict__ a,
-                                                        const float* __restrict__ b, uint16_t* __restrict__ dab,
-                                                        long long plane, float* __restrict__ sums, int T, int F, int Fp,
-                                                        int act) {
+// sums over its rows for the biases' gradients (in float32, before any rounding).  Bound by
+// memory: 12 bytes read and 4 written an element in bf16.  VEC: F and every row are
+// multiples of 16 bytes, and a thread's eight columns move in vectors.
+template <class E, int ACT, bool VEC>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go, long long ld_go,
+                                                        const float* __restrict__ a, const float* __restrict__ b,
+                                                        uint16_t* __restrict__ dab, long long plane,
+                                                        float* __restrict__ sums, int T, int F, int Fp) {
   const int groups = Fp / 8;
   const long long gid = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   const int rb = static_cast<int>(gid / groups), f0 = static_cast<int>(gid % groups) * 8;
@@ -386,25 +408,38 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go
   float sa[8], sb[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sa[i] = sb[i] = 0.f;
+#pragma unroll 2
   for (int r = rb * kRowsPer; r < min(T, (rb + 1) * kRowsPer); ++r) {
+    const long long at = static_cast<long long>(r) * F + f0;
+    const E* g = go + r * ld_go + f0;
+    float xa[8], xb[8], xg[8];
+    if constexpr (VEC) {
+      read8(a + at, xa);
+      read8(b + at, xb);
+      read8(g, xg);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = f0 + i < F;
+        xa[i] = in ? a[at + i] : 0.f;
+        xb[i] = in ? b[at + i] : 0.f;
+        xg[i] = in ? to_f(g[i]) : 0.f;  // da = db = 0
+      }
+    }
     uint16_t ta[3][8], tb[3][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      const ActGrad d = activate<ACT>(xa[i]);
+      const float ga = xg[i] * xb[i] * d.d, gb = xg[i] * d.f;
+      sa[i] += ga;
+      sb[i] += gb;
       uint16_t va[3] = {0, 0, 0}, vb[3] = {0, 0, 0};
-      if (f0 + i < F) {
-        const long long at = static_cast<long long>(r) * F + f0 + i;
-        const ActGrad d = activate(act, a[at]);
-        const float g = to_f(go[r * ld_go + f0 + i]);
-        const float ga = g * b[at] * d.d, gb = g * d.f;
-        sa[i] += ga;
-        sb[i] += gb;
-        if constexpr (sizeof(E) == 4) {
-          split3(ga, va);
-          split3(gb, vb);
-        } else {
-          va[0] = from_f<bf16_t>(ga).bits;
-          vb[0] = from_f<bf16_t>(gb).bits;
-        }
+      if constexpr (sizeof(E) == 4) {
+        split3(ga, va);
+        split3(gb, vb);
+      } else {
+        va[0] = from_f<bf16_t>(ga).bits;
+        vb[0] = from_f<bf16_t>(gb).bits;
       }
 #pragma unroll
       for (int j = 0; j < 3; ++j) { ta[j][i] = va[j]; tb[j][i] = vb[j]; }
@@ -601,9 +636,24 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   uint16_t* dab = reinterpret_cast<uint16_t*>(base + o_dab);
   float* sums = want_b ? reinterpret_cast<float*>(base + o_sums) : nullptr;
   const int T = static_cast<int>(p.T), F = static_cast<int>(p.F), D = static_cast<int>(p.D), fp = static_cast<int>(Fp);
-  hipLaunchKernelGGL(gate_grad_kernel<E>, dim3(static_cast<unsigned>((rbs * (Fp / 8) + 255) / 256)), dim3(256), 0, st, go,
-                     ld_go, a, b, dab, static_cast<long long>(dab_plane), sums, T, F, fp, p.act);
-  if (int rc = launch_check("gate_grad_kernel")) return rc;
+  const bool vec = F % 8 == 0 && aligned16(go) && aligned16(a) && aligned16(b) && ld_go * static_cast<int64_t>(sizeof(E)) % 16 == 0;
+  const auto grads = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    auto kern = vec ? gate_grad_kernel<E, ACT, true> : gate_grad_kernel<E, ACT, false>;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((rbs * (Fp / 8) + 255) / 256)), dim3(256), 0, st, go, ld_go, a, b, dab,
+                       static_cast<long long>(dab_plane), sums, T, F, fp);
+    return launch_check("gate_grad_kernel");
+  };
+  const auto by_act = [&] {
+    switch (p.act) {
+      case OSSM_ACT_SILU: return grads(std::integral_constant<int, OSSM_ACT_SILU>{});
+      case OSSM_ACT_GELU: return grads(std::integral_constant<int, OSSM_ACT_GELU>{});
+      case OSSM_ACT_GELU_TANH: return grads(std::integral_constant<int, OSSM_ACT_GELU_TANH>{});
+      case OSSM_ACT_SIGMOID: return grads(std::integral_constant<int, OSSM_ACT_SIGMOID>{});
+      default: return grads(std::integral_constant<int, OSSM_ACT_RELU>{});
+    }
+  };
+  if (int rc = by_act()) return rc;
   if (want_b) {
     hipLaunchKernelGGL(bias_grad_kernel<E>, dim3(static_cast<unsigned>((2 * Fp + kWave - 1) / kWave)), dim3(256), 0, st,
                        static_cast<const float*>(sums), static_cast<int>(rbs), F, fp, gb[0], gb[1]);

@@ -7,7 +7,7 @@
 //
 // A workgroup takes a row's block of kBlock vocabulary entries: it counts the row's
 // history and marks its biases for that block in LDS, then streams the block.
-// Integer LDS atomics only (counts, a mark, the highest bias index), so the result does not
+// Integer LDS atomics only (the highest bias index, a mark, counts), so the result does not
 // depend on their order.  Every block of a row reads the row's history again (from
 // L2: a few kB against the block's logits).
 //
@@ -29,8 +29,18 @@ namespace ossm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlock = 8192;               // vocabulary entries of a workgroup
-constexpr uint32_t kSeen = 0x80000000u;    // of an entry's word: seen at all; below: its count
+constexpr int kBlock = 8192;  // vocabulary entries of a workgroup
+constexpr int kAhead = 8;     // history loads in flight a thread
+
+// An entry's word in LDS.  Narrow: bias index + 1 in the upper half, set first (the
+// largest wins), then the mark of one seen at all and the count; it serves
+// histories below 2^15 tokens and up to 2^16 - 1 biases with one word an entry (32 KB:
+// five workgroups a CU).  Wide: the mark and the count in a word, biases in a second.
+template <bool WIDE>
+struct Words {
+  static constexpr uint32_t kSeen = WIDE ? 0x80000000u : 0x8000u;
+  static constexpr uint32_t kCount = kSeen - 1;
+};
 
 template <class E>
 struct Logits {
@@ -55,11 +65,12 @@ struct alignas(W * sizeof(E)) Pack {
   E v[W];
 };
 
-template <class E>
+template <class E, bool WIDE>
 __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   constexpr int W = 16 / static_cast<int>(sizeof(E));
-  extern __shared__ uint32_t s_word[];  // [kBlock] counts, then [kBlock] bias indices + 1 where there are biases
-  uint32_t* s_bias = s_word + kBlock;
+  constexpr uint32_t kSeen = Words<WIDE>::kSeen, kCount = Words<WIDE>::kCount;
+  extern __shared__ uint32_t s_word[];
+  uint32_t* s_bias = WIDE ? s_word + kBlock : s_word;
   const int row = static_cast<int>(blockIdx.x / g.n_blocks);
   const int blk = static_cast<int>(blockIdx.x % g.n_blocks);
   const int tid = threadIdx.x;
@@ -70,26 +81,32 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   const bool same = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(E) % W) == shift;
   const int v0 = blk * kBlock - shift;  // the block's first entry, before the row's start in its first block
   const int n = min(kBlock, g.V - v0);
+  const int lo = max(v0, 0), span = max(v0 + n - lo, 0);  // the entries that exist
 
-  const int words = g.n_bias > 0 ? 2 * kBlock : kBlock;
+  const int words = WIDE ? 2 * kBlock : kBlock;
   for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
+  for (int i = tid; i < g.n_bias; i += kThreads) {
+    const int id = g.bias_ids[row * g.ld_b + i];
+    if (static_cast<unsigned>(id - lo) < static_cast<unsigned>(span))
+      atomicMax(&s_bias[id - v0], static_cast<uint32_t>(i + 1) << (WIDE ? 0 : 16));
+  }
+  if (!WIDE && g.n_bias > 0) __syncthreads();
   const int len = g.lengths != nullptr ? min(max(g.lengths[row], 0), g.H) : g.H;
   const int first = g.prompts != nullptr ? min(max(g.prompts[row], 0), g.H) : 0;
   const int32_t* hist = g.history + row * g.ld_h;
-  for (int i = tid; i < len; i += kThreads) {
-    const int id = hist[i];
-    if (id < 0 || id >= g.V) continue;
-    const int at = id - v0;
-    if (at < 0 || at >= n) continue;
-    if (i >= first) atomicAdd(&s_word[at], 1u);
-    else atomicOr(&s_word[at], kSeen);
-  }
-  for (int i = tid; i < g.n_bias; i += kThreads) {
-    const int id = g.bias_ids[row * g.ld_b + i];
-    if (id < 0 || id >= g.V) continue;
-    const int at = id - v0;
-    if (at >= 0 && at < n) atomicMax(&s_bias[at], static_cast<uint32_t>(i + 1));
+  for (int i0 = tid; i0 < len; i0 += kThreads * kAhead) {
+    int id[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) id[k] = i0 + k * kThreads < len ? hist[i0 + k * kThreads] : -1;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      // an id below zero is far outside as an unsigned number, and lo >= 0
+      if (id[k] >= 0 && static_cast<unsigned>(id[k] - lo) < static_cast<unsigned>(span)) {
+        if (i0 + k * kThreads >= first) atomicAdd(&s_word[id[k] - v0], 1u);
+        else atomicOr(&s_word[id[k] - v0], kSeen);
+      }
+    }
   }
   __syncthreads();
 
@@ -100,15 +117,13 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   const float* bias = g.bias + row * g.ld_b;
   const auto control = [&](float l, int at) {
     const uint32_t w = s_word[at];
-    if (w != 0) {
+    if (w & (kSeen | kCount)) {
       l = l > 0.f ? l / rep : l * rep;
-      const uint32_t c = w & ~kSeen;
+      const uint32_t c = w & kCount;
       if (c != 0) l -= freq * static_cast<float>(c) + pres;
     }
-    if (g.n_bias > 0) {
-      const uint32_t b = s_bias[at];
-      if (b != 0) l += bias[b - 1];
-    }
+    const uint32_t b = WIDE ? s_bias[at] : w >> 16;
+    if (b != 0) l += bias[b - 1];
     return l;
   };
   const float kNone = -__builtin_inff();
@@ -154,8 +169,10 @@ int run(Logits<E> g, int64_t rows, hipStream_t st) {
   g.n_blocks = (g.V + W - 1 + kBlock - 1) / kBlock;  // the shift may need one more
   if (rows * g.n_blocks > INT_MAX)
     return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
-  const size_t lds = (g.n_bias > 0 ? 2 : 1) * kBlock * sizeof(uint32_t);
-  hipLaunchKernelGGL(control_logits_kernel<E>, dim3(static_cast<unsigned>(rows * g.n_blocks)), dim3(kThreads), lds, st, g);
+  const bool wide = g.H >= (1 << 15) || g.n_bias >= (1 << 16);
+  const size_t lds = (wide ? 2 : 1) * kBlock * sizeof(uint32_t);
+  hipLaunchKernelGGL(wide ? (control_logits_kernel<E, true>) : (control_logits_kernel<E, false>),
+                     dim3(static_cast<unsigned>(rows * g.n_blocks)), dim3(kThreads), lds, st, g);
   return launch_check("control_logits_kernel");
 }
 

@@ -9,16 +9,18 @@
 // All of it in float32 whatever E is: u, p, dt and h are never rounded to E (h is an
 // output in float32, and a u rounded to bf16 would leave 2^-9 in it).
 //
-// A token's launches: mixer_proj_kernel (conv, its state's update, x_proj over a block
-// of channels) and mixer_token_kernel (the blocks' sums, dt, the state's update, the
+// A token's launches: token_proj_kernel (conv, its state's update, x_proj over a block
+// of channels) and token_scan_kernel (the blocks' sums, dt, the state's update, the
 // gate).  x_proj sums over all channels, so two launches is the least.
 //
 // A prompt batch is one row of packed tokens cut into chunks of equal length,
 // whatever the prompts' lengths (the host never reads the offsets): a prompt's
 // first token resets the recurrence, so a chunk may hold many prompts or a
-// piece of one.  mixer_scan_kernel<summary> finds what each chunk leaves to a zero
+// piece of one.  prompt_proj_kernel (conv and x_proj) and prompt_dt_kernel (dt_proj) put both
+// projections on the matrix cores, u and p as three bf16 terms (split_mfma.hpp has
+// the error).  mixer_scan_kernel<summary> finds what each chunk leaves to a zero
 // carry and the sum of its dt (the decay over the chunk is exp(A sum dt)),
-// mixer_carry_kernel folds the chunks in order, mixer_scan_kernel<output> walks the
+// the carry kernels fold the chunks in order, mixer_scan_kernel<output> walks the
 // chunks again from their carries.  One chunk needs the last only.
 
 #include <hip/hip_runtime.h>
@@ -32,6 +34,7 @@
 #include "lm_types.hpp"
 #include "runtime.hpp"
 #include "scan_device.hpp"
+#include "split_mfma.hpp"
 
 namespace ossm {
 namespace {
@@ -60,17 +63,19 @@ struct Mixer {
   const int32_t* offsets;  // null for single tokens
   const uint8_t* resume;
   E* y;
-  float* part;   // [n_blocks][rows][Nc]: x_proj's sums over blocks of channels
+  float* part;   // [n_blocks][rows][Nc]: x_proj's sums over blocks (splits) of the channels
   float* u;      // tokens: [rows][Di]
   float* bc;     // prompts: [rows][2][Npad], B and C, zero from N on
   float* dt;     // prompts: [rows][Di]
   float* local;  // prompts: [n_chunks][N][Di], a chunk's end from a zero carry
   float* carry;  // prompts: [n_chunks][N][Di], the state before a chunk
   float* sum_dt; // prompts: [n_chunks][Di], negative where a prompt starts in the chunk
+  float* group_local;  // the same of groups of chunks: [n_groups][N][Di], [n_groups][Di]
+  float* group_dt;
   float* init;   // prompts: [n_seqs][N][Di] copies of the resumed states, or null
   float* y_sum;  // prompts with N past a block of states: [rows][Di]
   long long ld;
-  int rows, n_seqs, n_slots, Di, N, R, K, Nc, Npad, n_blocks, chunk, n_chunks;
+  int rows, n_seqs, n_slots, Di, N, R, K, Nc, Npad, n_blocks, chunk, n_chunks, group, n_groups;
 };
 
 // Where sequence i starts, in range whatever the offsets hold.
@@ -135,62 +140,55 @@ __device__ __forceinline__ void load8(const bf16_t* p, int n, bool vec, float (&
   }
 }
 
-// conv + SiLU of RB rows over a block of channels, and x_proj's partial sums over it.
-// Each wave takes kSub of the channels and all Nc outputs, 64 at a time, one per lane;
-// the waves' sums meet in LDS in a fixed order.
-template <class E, int RB, bool PROMPT>
-__global__ __launch_bounds__(kProjThreads) void mixer_proj_kernel(Mixer<E> g, bool vec) {
+// conv + SiLU of RB tokens over a block of channels, the conv's new state, and x_proj's
+// partial sums over the block.  Each wave takes kSub of the channels and all Nc outputs, 64 at
+// a time, one per lane; the waves' sums meet in LDS in a fixed order.  KT >= K taps.
+template <class E, int RB, int KT>
+__global__ __launch_bounds__(kProjThreads) void token_proj_kernel(Mixer<E> g, bool vec) {
   __shared__ float s_u[RB][kProjBlock];
   __shared__ float s_sum[kProjWaves][RB][kWave];
-  __shared__ int s_start[RB], s_slot[RB];
   const int blk = static_cast<int>(blockIdx.x % g.n_blocks);
   const int r0 = static_cast<int>(blockIdx.x / g.n_blocks) * RB;
   const int c0 = blk * kProjBlock;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = wave_id();
-  if (tid < RB) {
-    const int r = r0 + tid;
-    int start = INT_MAX, slot = -1;  // INT_MAX: padding
-    if (r < g.rows) {
-      if constexpr (PROMPT) {
-        const int s = seq_of(g, r);
-        if (s >= 0 && r < offset_of(g, s + 1)) { start = offset_of(g, s); slot = start_slot(g, s); }
-      } else {
-        start = r;
-        slot = start_slot(g, r);
-      }
-    }
-    s_start[tid] = start;
-    s_slot[tid] = slot;
+  const int skip_taps = KT - g.K;
+  // every row's inputs are loaded before the first is used (a thread's rows are
+  // kProjThreads / kProjBlock apart)
+  constexpr int kRows = (RB * kProjBlock + kProjThreads - 1) / kProjThreads;
+  const int c = tid % kProjBlock, d = min(c0 + c, g.Di - 1);
+  float x[kRows][KT], wt[KT];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = min(r0 + tid / kProjBlock + i * (kProjThreads / kProjBlock), g.rows - 1);
+    const int slot = start_slot(g, r);
+#pragma unroll
+    for (int k = 0; k < KT - 1; ++k)
+      x[i][k] = k >= skip_taps && slot >= 0
+                    ? to_f(g.conv_state[(static_cast<size_t>(slot) * (g.K - 1) + k - skip_taps) * g.Di + d]) : 0.f;
+    x[i][KT - 1] = to_f(g.xz[static_cast<size_t>(r) * g.ld + d]);
   }
-  __syncthreads();
-  for (int i = tid; i < RB * kProjBlock; i += kProjThreads) {
-    const int rr = i / kProjBlock, c = i % kProjBlock, r = r0 + rr, d = c0 + c;
+#pragma unroll
+  for (int k = 0; k < KT; ++k) wt[k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d) * g.K + k - skip_taps]) : 0.f;
+  const float cb = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int rr = tid / kProjBlock + i * (kProjThreads / kProjBlock), r = r0 + rr;
+    if (rr >= RB) break;
     float u = 0.f;
-    if (d < g.Di && s_start[rr] != INT_MAX) {
-      float p = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
-      if constexpr (PROMPT) {
-        for (int k = 0; k < g.K; ++k)
-          p = fmaf(to_f(g.conv_w[static_cast<size_t>(d) * g.K + k]),
-                   conv_input(g, r - g.K + 1 + k, s_start[rr], s_slot[rr], d), p);
-        u = silu_f(p);
-      } else {
-        float x[kMaxConv];
+    if (r < g.rows && c0 + c < g.Di) {
+      float p = cb;
 #pragma unroll
-        for (int k = 0; k < kMaxConv; ++k)
-          if (k < g.K) {
-            x[k] = conv_input(g, r - g.K + 1 + k, r, s_slot[rr], d);
-            p = fmaf(to_f(g.conv_w[static_cast<size_t>(d) * g.K + k]), x[k], p);
-          }
-        u = silu_f(p);
-        const int out = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
-        if (in_pool(g, out)) {
+      for (int k = 0; k < KT; ++k)
+        if (k >= skip_taps) p = fmaf(wt[k], x[i][k], p);
+      u = silu_f(p);
+      const int out = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
+      if (in_pool(g, out)) {
 #pragma unroll
-          for (int k = 1; k < kMaxConv; ++k)
-            if (k < g.K)
-              g.conv_state[(static_cast<size_t>(out) * (g.K - 1) + k - 1) * g.Di + d] = from_f<E>(x[k]);
-        }
-        g.u[static_cast<size_t>(r) * g.Di + d] = u;
+        for (int k = 1; k < KT; ++k)
+          if (k > skip_taps)
+            g.conv_state[(static_cast<size_t>(out) * (g.K - 1) + k - 1 - skip_taps) * g.Di + d] = from_f<E>(x[i][k]);
       }
+      g.u[static_cast<size_t>(r) * g.Di + d] = u;
     }
     s_u[rr][c] = u;
   }
@@ -202,14 +200,14 @@ __global__ __launch_bounds__(kProjThreads) void mixer_proj_kernel(Mixer<E> g, bo
     for (int rr = 0; rr < RB; ++rr) acc[rr] = 0.f;
 #pragma unroll
     for (int q = 0; q < kSub; q += 8) {
-      const int c = w * kSub + q;
-      float wt[8];
-      const int left = g.Di - (c0 + c);
-      load8(g.x_proj + static_cast<size_t>(j) * g.Di + (left > 0 ? c0 + c : 0), left, vec, wt);
+      const int c8 = w * kSub + q;
+      float v[8];
+      const int left = g.Di - (c0 + c8);
+      load8(g.x_proj + static_cast<size_t>(j) * g.Di + (left > 0 ? c0 + c8 : 0), left, vec, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int rr = 0; rr < RB; ++rr) acc[rr] = fmaf(wt[i], s_u[rr][c + i], acc[rr]);
+        for (int rr = 0; rr < RB; ++rr) acc[rr] = fmaf(v[i], s_u[rr][c8 + i], acc[rr]);
     }
 #pragma unroll
     for (int rr = 0; rr < RB; ++rr) s_sum[w][rr][lane] = acc[rr];
@@ -217,35 +215,57 @@ __global__ __launch_bounds__(kProjThreads) void mixer_proj_kernel(Mixer<E> g, bo
     for (int i = tid; i < RB * kWave; i += kProjThreads) {
       const int rr = i / kWave, l = i % kWave;
       if (r0 + rr < g.rows && j0 + l < g.Nc) {
-        float s = s_sum[0][rr][l];
+        float t = s_sum[0][rr][l];
 #pragma unroll
-        for (int v = 1; v < kProjWaves; ++v) s += s_sum[v][rr][l];
-        g.part[(static_cast<size_t>(blk) * g.rows + r0 + rr) * g.Nc + j0 + l] = s;
+        for (int v = 1; v < kProjWaves; ++v) t += s_sum[v][rr][l];
+        g.part[(static_cast<size_t>(blk) * g.rows + r0 + rr) * g.Nc + j0 + l] = t;
       }
     }
     __syncthreads();
   }
 }
 
-// s_p[RB][Nc] = the rows' projections, from the blocks' partial sums.
-template <int RB, class E>
-__device__ __forceinline__ void sum_proj(const Mixer<E>& g, int r0, float* s_p) {
+// Column j of row r's projection, from the blocks' partial sums.
+template <class E>
+__device__ __forceinline__ float proj_of(const Mixer<E>& g, int r, int j) {
   const size_t step = static_cast<size_t>(g.rows) * g.Nc;
-  for (int i = threadIdx.x; i < RB * g.Nc; i += blockDim.x) {
-    const int r = r0 + i / g.Nc;
-    float s = 0.f;
-    if (r < g.rows) {
-      const float* p = g.part + static_cast<size_t>(r) * g.Nc + i % g.Nc;
+  const float* p = g.part + static_cast<size_t>(r) * g.Nc + j;
+  float s = 0.f;
 #pragma unroll 8
-      for (int b = 0; b < g.n_blocks; ++b) s += p[b * step];
-    }
-    s_p[i] = s;
-  }
+  for (int b = 0; b < g.n_blocks; ++b) s += p[b * step];
+  return s;
 }
 
-// dt of RB rows at channel d from their projections in LDS.
-template <int RB, class E>
-__device__ __forceinline__ void dt_of(const Mixer<E>& g, const float* s_p, int d, bool vec, float (&dt)[RB]) {
+// One token: a thread per channel, RB rows.  The first 16 states of all rows are asked
+// for before the projections are summed: the states' traffic is what bounds a large
+// batch, and this keeps 16 RB loads a thread in flight.
+template <class E, int RB>
+__global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, bool vec) {
+  extern __shared__ float s_p[];  // [RB][Nc]
+  const int r0 = static_cast<int>(blockIdx.y) * RB;
+  const int d_own = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x), d = min(d_own, g.Di - 1);
+  constexpr int NB = 16;
+  int in[RB], to[RB];
+  float h[RB][NB], u[RB], z[RB], a2[NB];
+#pragma unroll
+  for (int rr = 0; rr < RB; ++rr) {
+    const int r = min(r0 + rr, g.rows - 1);
+    in[rr] = start_slot(g, r);
+    to[rr] = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
+    const float* src = g.ssm + (static_cast<size_t>(max(in[rr], 0)) * g.N) * g.Di + d;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) h[rr][i] = in[rr] >= 0 && i < g.N ? src[static_cast<size_t>(i) * g.Di] : 0.f;
+    u[rr] = g.u[static_cast<size_t>(r) * g.Di + d];
+    z[rr] = to_f(g.xz[static_cast<size_t>(r) * g.ld + g.Di + d]);
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i) a2[i] = i < g.N ? g.a_log[static_cast<size_t>(d) * g.N + i] : 0.f;
+  for (int i = threadIdx.x; i < RB * g.Nc; i += blockDim.x) {
+    const int r = r0 + i / g.Nc;
+    s_p[i] = r < g.rows ? proj_of(g, r, i % g.Nc) : 0.f;
+  }
+  __syncthreads();
+  float dt[RB];
   const float bias = g.dt_bias[d];
 #pragma unroll
   for (int rr = 0; rr < RB; ++rr) dt[rr] = bias;
@@ -254,91 +274,353 @@ __device__ __forceinline__ void dt_of(const Mixer<E>& g, const float* s_p, int d
     load8(g.dt_proj + static_cast<size_t>(d) * g.R + q, g.R - q, vec, wt);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int k = min(q + i, g.Nc - 1);  // past R the weight is zero; what it meets is finite or replaced
+      const int k = min(q + i, g.Nc - 1);
 #pragma unroll
-      for (int rr = 0; rr < RB; ++rr) {
-        const float p = s_p[rr * g.Nc + k];
-        dt[rr] = q + i < g.R ? fmaf(wt[i], p, dt[rr]) : dt[rr];
-      }
+      for (int rr = 0; rr < RB; ++rr) dt[rr] = q + i < g.R ? fmaf(wt[i], s_p[rr * g.Nc + k], dt[rr]) : dt[rr];
     }
   }
-#pragma unroll
-  for (int rr = 0; rr < RB; ++rr) dt[rr] = softplus_f(dt[rr]);
-}
-
-// One token: a thread per channel, RB rows one after another.
-template <class E, int RB>
-__global__ __launch_bounds__(256) void mixer_token_kernel(Mixer<E> g, bool vec) {
-  extern __shared__ float s_p[];  // [RB][Nc]
-  const int r0 = static_cast<int>(blockIdx.y) * RB;
-  sum_proj<RB>(g, r0, s_p);
-  __syncthreads();
-  const int d = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
-  if (d >= g.Di) return;
-  float dt[RB];
-  dt_of<RB>(g, s_p, d, vec, dt);
+  if (d_own >= g.Di) return;
   const float skip = g.skip != nullptr ? g.skip[d] : 0.f;
+  float y[RB], du[RB];
 #pragma unroll
   for (int rr = 0; rr < RB; ++rr) {
-    const int r = r0 + rr;
-    if (r >= g.rows) break;
-    const int in = start_slot(g, r);
-    const int to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
-    const bool keep = in_pool(g, to);
-    E* out = g.y + static_cast<size_t>(r) * g.Di + d;
-    if (in < 0 && !keep) { *out = from_f<E>(0.f); continue; }
-    const float u = g.u[static_cast<size_t>(r) * g.Di + d];
-    const float z = to_f(g.xz[static_cast<size_t>(r) * g.ld + g.Di + d]);
-    const float* B = s_p + rr * g.Nc + g.R;
-    const float* C = B + g.N;
-    const float* hi = g.ssm + (static_cast<size_t>(in < 0 ? 0 : in) * g.N) * g.Di + d;
-    float* ho = g.ssm + (static_cast<size_t>(keep ? to : 0) * g.N) * g.Di + d;
-    const float du = dt[rr] * u;
-    float y = skip * u;
-    for (int n0 = 0; n0 < g.N; n0 += 16) {
-      float h[16], a[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int n = min(n0 + i, g.N - 1);
-        h[i] = in >= 0 ? hi[static_cast<size_t>(n) * g.Di] : 0.f;
-        a[i] = g.a_log[static_cast<size_t>(d) * g.N + n];
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (n0 + i >= g.N) break;
-        const float decay = __builtin_amdgcn_exp2f(-expf(a[i]) * kLog2e * dt[rr]);
-        const float v = fmaf(decay, h[i], du * B[n0 + i]);
-        y = fmaf(C[n0 + i], v, y);
-        if (keep) ho[static_cast<size_t>(n0 + i) * g.Di] = v;
-      }
-    }
-    *out = from_f<E>(y * silu_f(z));
+    dt[rr] = softplus_f(dt[rr]);
+    du[rr] = dt[rr] * u[rr];
+    y[rr] = skip * u[rr];
   }
-}
-
-// Prompts: B, C and dt of every token, from x_proj's partial sums.
-template <class E, int RB>
-__global__ __launch_bounds__(256) void mixer_dt_kernel(Mixer<E> g, bool vec) {
-  extern __shared__ float s_p[];  // [RB][Nc]
-  const int nb = (g.Di + 255) / 256;
-  const int r0 = static_cast<int>(blockIdx.x / nb) * RB, cb = static_cast<int>(blockIdx.x % nb);
-  sum_proj<RB>(g, r0, s_p);
-  __syncthreads();
-  if (cb == 0) {
-    for (int i = threadIdx.x; i < RB * 2 * g.Npad; i += blockDim.x) {
-      const int rr = i / (2 * g.Npad), k = i % (2 * g.Npad), half = k / g.Npad, n = k % g.Npad;
-      if (r0 + rr < g.rows)
-        g.bc[static_cast<size_t>(r0 + rr) * 2 * g.Npad + k] =
-            n < g.N ? s_p[rr * g.Nc + g.R + half * g.N + n] : 0.f;
+  for (int n0 = 0; n0 < g.N; n0 += NB) {
+    if (n0 > 0) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) a2[i] = n0 + i < g.N ? g.a_log[static_cast<size_t>(d) * g.N + n0 + i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) a2[i] = -expf(a2[i]) * kLog2e;
+#pragma unroll
+    for (int rr = 0; rr < RB; ++rr) {
+      if (n0 > 0) {
+        const float* src = g.ssm + (static_cast<size_t>(max(in[rr], 0)) * g.N + n0) * g.Di + d;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) h[rr][i] = in[rr] >= 0 && n0 + i < g.N ? src[static_cast<size_t>(i) * g.Di] : 0.f;
+      }
+      const float* B = s_p + rr * g.Nc + g.R + n0;
+      const bool keep = r0 + rr < g.rows && in_pool(g, to[rr]);
+      float* dst = g.ssm + (static_cast<size_t>(keep ? to[rr] : 0) * g.N + n0) * g.Di + d;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        if (n0 + i < g.N) {
+          const float v = fmaf(__builtin_amdgcn_exp2f(a2[i] * dt[rr]), h[rr][i], du[rr] * B[i]);
+          y[rr] = fmaf(B[g.N + i], v, y[rr]);
+          if (keep) dst[static_cast<size_t>(i) * g.Di] = v;
+        }
     }
   }
-  const int d = cb * 256 + static_cast<int>(threadIdx.x);
-  if (d >= g.Di) return;
-  float dt[RB];
-  dt_of<RB>(g, s_p, d, vec, dt);
 #pragma unroll
   for (int rr = 0; rr < RB; ++rr)
-    if (r0 + rr < g.rows) g.dt[static_cast<size_t>(r0 + rr) * g.Di + d] = dt[rr];
+    if (r0 + rr < g.rows) {
+      const bool padding = in[rr] < 0 && !in_pool(g, to[rr]);
+      g.y[static_cast<size_t>(r0 + rr) * g.Di + d] = from_f<E>(padding ? 0.f : y[rr] * silu_f(z[rr]));
+    }
+}
+
+// ---- prompts: the projections on the matrix cores -----------------------------------
+
+// x as the three bf16 terms of split_mfma.hpp, two values to a word; one that is not
+// finite as (x, 0, 0), one that would round past the largest bf16 as that and the rest.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&t)[3]) {
+  constexpr float kTop = 3.3895313892515355e38f;  // the largest bf16
+  const bool fa = fabsf(a) <= 3.4028234663852886e38f, fb = fabsf(b) <= 3.4028234663852886e38f;
+  t[0] = pack_bf16(fa ? fminf(fmaxf(a, -kTop), kTop) : a, fb ? fminf(fmaxf(b, -kTop), kTop) : b);
+  const float ra = fa ? a - bf16_lo(t[0]) : 0.f, rb = fb ? b - bf16_hi(t[0]) : 0.f;
+  t[1] = pack_bf16(ra, rb);
+  t[2] = pack_bf16(ra - bf16_lo(t[1]), rb - bf16_hi(t[1]));
+}
+
+// Rows of `width` (a multiple of 64) bf16 in LDS, in 16-byte chunks: chunk c of row r
+// sits at c ^ (r % 8), which spreads a fragment's rows over the banks.
+__device__ __forceinline__ int plane_at(int r, int k, int width) { return r * width + (((k >> 3) ^ (r & 7)) << 3) + (k & 7); }
+
+// A weight's fragment: eight values from k of row j, as its terms (zeros past the row).
+template <class E>
+struct Weight8;
+template <>
+struct Weight8<bf16_t> {
+  bf16x8 t[1];
+  __device__ __forceinline__ void load(const bf16_t* row, int k, int n, bool vec) {
+    if (vec && k + 8 <= n) {
+      t[0] = *reinterpret_cast<const bf16x8*>(row + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[0][i] = __builtin_bit_cast(__bf16, k + i < n ? row[k + i].bits : static_cast<uint16_t>(0));
+    }
+  }
+  __device__ __forceinline__ void split() {}
+};
+template <>
+struct Weight8<float> {
+  float x[8];
+  bf16x8 t[3];
+  __device__ __forceinline__ void load(const float* row, int k, int n, bool vec) { load8(row + (k < n ? k : 0), n - k, vec, x); }
+  __device__ __forceinline__ void split() {
+    const SplitFrag f = split8(x);
+    t[0] = f.t0;
+    t[1] = f.t1;
+    t[2] = f.t2;
+  }
+};
+
+// c += a b over 16 k, the terms of order up to two, smallest first (a bf16 weight is one term)
+__device__ __forceinline__ floatx16 mfma_terms(const bf16x8 (&a)[3], const Weight8<bf16_t>& b, floatx16 c) {
+  c = mfma_bf16(a[2], b.t[0], c);
+  c = mfma_bf16(a[1], b.t[0], c);
+  return mfma_bf16(a[0], b.t[0], c);
+}
+__device__ __forceinline__ floatx16 mfma_terms(const bf16x8 (&a)[3], const Weight8<float>& b, floatx16 c) {
+  return mfma_split(SplitFrag{a[0], a[1], a[2]}, SplitFrag{b.t[0], b.t[1], b.t[2]}, c);
+}
+
+// The sums of the second way wherever the first's are not finite.
+__device__ __forceinline__ void keep_finite(floatx16 (&acc)[2], const floatx16 (&first)[2]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[j][r] = fabsf(first[j][r]) <= 3.4028234663852886e38f ? first[j][r] : acc[j][r];
+}
+
+// The three terms of an LDS plane set at (r, k), added up again.
+__device__ __forceinline__ float planes_sum(const uint16_t* s, int plane, int at) {
+  return (to_f(bf16_t{s[2 * plane + at]}) + to_f(bf16_t{s[plane + at]})) + to_f(bf16_t{s[at]});
+}
+
+constexpr int kPtRows = 64, kPtK = 64, kPtCols = 128;  // prompt_proj_kernel's tile and k step
+
+// Conv + SiLU of a tile of kPtRows tokens, kPtK channels at a time, and x_proj's sums over
+// this split's channels for kPtCols of the Nc outputs.  u goes from registers into LDS as
+// three bf16 planes; a wave takes 32 rows and 64 outputs, the weights' fragments straight
+// from memory (all workgroups read the same few hundred kB).  Sums that are not
+// finite (a term of an infinite weight against a zero one) are formed again on the
+// fp32 instruction; finite ones stay as they are, whatever their neighbours.
+template <class E, int KT>
+__global__ __launch_bounds__(256) void prompt_proj_kernel(Mixer<E> g, int per_split, bool vec) {
+  __shared__ __align__(16) uint16_t s_u[3][kPtRows * kPtK];
+  __shared__ int s_start[kPtRows], s_slot[kPtRows];
+  const int groups = (g.Nc + kPtCols - 1) / kPtCols;
+  int id = static_cast<int>(blockIdx.x);
+  const int col0 = id % groups * kPtCols;
+  id /= groups;
+  const int split = id % g.n_blocks, r0 = id / g.n_blocks * kPtRows;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = wave_id();
+  if (tid < kPtRows) {
+    const int r = r0 + tid;
+    int start = INT_MAX, slot = -1;  // INT_MAX: padding
+    if (r < g.rows) {
+      const int s = seq_of(g, r);
+      if (s >= 0 && r < offset_of(g, s + 1)) { start = offset_of(g, s); slot = start_slot(g, s); }
+    }
+    s_start[tid] = start;
+    s_slot[tid] = slot;
+  }
+  __syncthreads();
+  const int skip_taps = KT - g.K;
+  const int pair = tid & 31, rg = tid >> 5;  // the conv's share: 2 channels of 8 rows
+  const int rf = (w & 1) * 32, cf = col0 + (w >> 1) * 64;  // the product's: 32 rows, 64 outputs
+  const int l32 = lane & 31, half = lane >> 5;
+  const int k_end = min(g.Di, (split + 1) * per_split);
+  floatx16 acc[2] = {}, first[2];
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      first[j] = acc[j];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+    }
+    for (int k0 = split * per_split; k0 < k_end; k0 += kPtK) {
+      Weight8<E> wt[kPtK / 16][2];
+      if (pass == 0) {
+#pragma unroll
+        for (int kk = 0; kk < kPtK / 16; ++kk)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            wt[kk][j].load(g.x_proj + static_cast<size_t>(min(cf + j * 32 + l32, g.Nc - 1)) * g.Di,
+                           k0 + kk * 16 + half * 8, g.Di, vec);
+      }
+      // ---- conv + SiLU
+      float x[2][8 + KT - 1], cw[2][KT], cb[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = min(k0 + 2 * pair + e, g.Di - 1);
+        cb[e] = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < KT; ++k) cw[e][k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d) * g.K + k - skip_taps]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8 + KT - 1; ++i) {
+          const int r = min(max(r0 + rg * 8 - (KT - 1) + i, 0), g.rows - 1);
+          x[e][i] = to_f(g.xz[static_cast<size_t>(r) * g.ld + d]);
+        }
+      }
+      __syncthreads();  // the last step's products have read s_u
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int rr = rg * 8 + i, start = s_start[rr];
+        float u[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = k0 + 2 * pair + e;
+          float p = cb[e];
+          if (r0 + rr - (g.K - 1) >= start) {
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+              if (k >= skip_taps) p = fmaf(cw[e][k], x[e][i + k], p);
+          } else {
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+              if (k >= skip_taps && start != INT_MAX) {
+                const int pos = r0 + rr - (KT - 1) + k;
+                p = fmaf(cw[e][k], pos >= start ? x[e][i + k] : conv_input(g, pos, start, s_slot[rr], min(d, g.Di - 1)), p);
+              }
+          }
+          u[e] = d < g.Di && start != INT_MAX ? silu_f(p) : 0.f;
+        }
+        uint32_t t[3];
+        split_pair(u[0], u[1], t);
+        const int at = plane_at(rr, 2 * pair, kPtK);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&s_u[q][at]) = t[q];
+      }
+      __syncthreads();
+      // ---- x_proj
+      if (pass == 0) {
+#pragma unroll
+        for (int kk = 0; kk < kPtK / 16; ++kk) {
+          bf16x8 a[3];
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            a[q] = *reinterpret_cast<const bf16x8*>(&s_u[q][plane_at(rf + l32, kk * 16 + half * 8, kPtK)]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            wt[kk][j].split();
+            acc[j] = mfma_terms(a, wt[kk][j], acc[j]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < kPtK; k += 2) {
+          const float a = planes_sum(&s_u[0][0], kPtRows * kPtK, plane_at(rf + l32, k + half, kPtK));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = k0 + k + half;
+            const float b = d < g.Di ? to_f(g.x_proj[static_cast<size_t>(min(cf + j * 32 + l32, g.Nc - 1)) * g.Di + d]) : 0.f;
+            acc[j] = mfma32(a, b, acc[j]);
+          }
+        }
+      }
+    }
+    if (pass == 0 && !__syncthreads_or(any_nonfinite(acc))) break;
+    if (pass == 1) keep_finite(acc, first);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = r0 + rf + 8 * (r >> 2) + 4 * half + (r & 3), col = cf + j * 32 + l32;
+      if (row < g.rows && col < g.Nc) g.part[(static_cast<size_t>(split) * g.rows + row) * g.Nc + col] = acc[j][r];
+    }
+}
+
+constexpr int kDtRows = 32, kDtCols = 256, kDtMaxR = 256;  // prompt_dt_kernel's tile, its stretch of R
+
+// B, C (float32) and dt = softplus(dt_proj p[:R] + bias) of a tile of tokens, from x_proj's
+// partial sums; blockIdx.y takes every gridDim.y-th block of kDtCols channels.  `width`:
+// the planes' row in LDS, at least the stretch of R, a multiple of 64.
+template <class E>
+__global__ __launch_bounds__(256) void prompt_dt_kernel(Mixer<E> g, int width, bool vec) {
+  extern __shared__ __align__(16) uint16_t s_dt[];  // [3][kDtRows * width]
+  const int r0 = static_cast<int>(blockIdx.x) * kDtRows;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = wave_id(), l32 = lane & 31, half = lane >> 5;
+  const int plane = kDtRows * width;
+  if (blockIdx.y == 0) {
+    for (int i = tid; i < kDtRows * 2 * g.Npad; i += 256) {
+      const int rr = i / (2 * g.Npad), k = i % (2 * g.Npad), second = k / g.Npad, n = k % g.Npad;
+      if (r0 + rr < g.rows)
+        g.bc[static_cast<size_t>(r0 + rr) * 2 * g.Npad + k] = n < g.N ? proj_of(g, r0 + rr, g.R + second * g.N + n) : 0.f;
+    }
+  }
+  const bool once = g.R <= kDtMaxR;  // the planes hold all of R for every block of channels
+  const auto fill = [&](int q0) {
+    for (int i = tid; i < kDtRows * (width / 2); i += 256) {
+      const int rr = i / (width / 2), k = i % (width / 2) * 2, r = min(r0 + rr, g.rows - 1);
+      uint32_t t[3];
+      split_pair(q0 + k < g.R ? proj_of(g, r, q0 + k) : 0.f, q0 + k + 1 < g.R ? proj_of(g, r, q0 + k + 1) : 0.f, t);
+      const int at = plane_at(rr, k, width);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&s_dt[q * plane + at]) = t[q];
+    }
+  };
+  if (once) {
+    fill(0);
+    __syncthreads();
+  }
+  for (int b0 = static_cast<int>(blockIdx.y) * kDtCols; b0 < g.Di; b0 += static_cast<int>(gridDim.y) * kDtCols) {
+    const int cw = b0 + w * 64;
+    floatx16 acc[2] = {}, first[2];
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        first[j] = acc[j];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+      }
+      for (int q0 = 0; q0 < g.R; q0 += kDtMaxR) {
+        if (!once) {
+          __syncthreads();
+          fill(q0);
+          __syncthreads();
+        }
+        const int n = min(g.R - q0, kDtMaxR);
+        if (pass == 0) {
+          for (int k = 0; k < n; k += 16) {
+            Weight8<E> wt[2];
+            bf16x8 a[3];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              wt[j].load(g.dt_proj + static_cast<size_t>(min(cw + j * 32 + l32, g.Di - 1)) * g.R, q0 + k + half * 8, g.R, vec);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+              a[q] = *reinterpret_cast<const bf16x8*>(&s_dt[q * plane + plane_at(l32, k + half * 8, width)]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              wt[j].split();
+              acc[j] = mfma_terms(a, wt[j], acc[j]);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < n; k += 2) {
+            const float a = k + half < n ? planes_sum(s_dt, plane, plane_at(l32, k + half, width)) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float b = k + half < n
+                  ? to_f(g.dt_proj[static_cast<size_t>(min(cw + j * 32 + l32, g.Di - 1)) * g.R + q0 + k + half]) : 0.f;
+              acc[j] = mfma32(a, b, acc[j]);
+            }
+          }
+        }
+      }
+      // (the waves agree: the passes hold barriers where R takes several stretches)
+      if (pass == 0 && !__syncthreads_or(any_nonfinite(acc))) break;
+      if (pass == 1) keep_finite(acc, first);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int d = cw + j * 32 + l32;
+      if (d >= g.Di) continue;
+      const float bias = g.dt_bias[d];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (row < g.rows) g.dt[static_cast<size_t>(row) * g.Di + d] = softplus_f(acc[j][r] + bias);
+      }
+    }
+  }
 }
 
 // The resumed states, copied before the scan that may overwrite their slots.
@@ -489,31 +771,56 @@ __global__ __launch_bounds__(kScanThreads) void mixer_scan_kernel(Mixer<E> g, co
   }
 }
 
-// carry[c + 1] = exp(A sum_dt[c]) carry[c] + local[c], a thread per state.
-template <class E>
-__global__ __launch_bounds__(256) void mixer_carry_kernel(Mixer<E> g) {
-  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-  const size_t nd = static_cast<size_t>(g.N) * g.Di;
-  if (i >= nd) return;
-  const int n = static_cast<int>(i / g.Di), d = static_cast<int>(i % g.Di);
-  const float a2 = -expf(g.a_log[static_cast<size_t>(d) * g.N + n]) * kLog2e;
-  float h = 0.f;
-  constexpr int kAhead = 8;
-  for (int c0 = 0; c0 + 1 < g.n_chunks; c0 += kAhead) {
-    float l[kAhead], sd[kAhead];
+constexpr int kCarryAhead = 8;  // chunks whose summaries are loaded together
+
+// h through `n` summaries from index c0: h = exp(A sum_dt) h + local (local alone where a
+// prompt starts inside); put(c, h) sees the state before each.
+template <class Put>
+__device__ __forceinline__ float fold(const float* local, const float* sum_dt, size_t nd, int Di, size_t i, int d,
+                                      float a2, int c0, int n, float h, float* total, Put put) {
+  for (int q = 0; q < n; q += kCarryAhead) {
+    float l[kCarryAhead], sd[kCarryAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int c = min(c0 + k, g.n_chunks - 2);
-      l[k] = g.local[c * nd + i];
-      sd[k] = g.sum_dt[static_cast<size_t>(c) * g.Di + d];
+    for (int k = 0; k < kCarryAhead; ++k) {
+      const int c = c0 + min(q + k, n - 1);
+      l[k] = local[c * nd + i];
+      sd[k] = sum_dt[static_cast<size_t>(c) * Di + d];
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (c0 + k + 1 >= g.n_chunks) break;
+    for (int k = 0; k < kCarryAhead; ++k) {
+      if (q + k >= n) break;
+      put(c0 + q + k, h);
       h = sd[k] < 0.f ? l[k] : fmaf(__builtin_amdgcn_exp2f(a2 * sd[k]), h, l[k]);
-      g.carry[(c0 + k + 1) * nd + i] = h;
+      *total = sd[k] < 0.f || *total < 0.f ? -1.f : *total + sd[k];
     }
   }
+  return h;
+}
+
+// The summary of each group of chunks (all but the last group's), a thread per state and group.
+template <class E>
+__global__ __launch_bounds__(256) void mixer_group_kernel(Mixer<E> g) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, nd = static_cast<size_t>(g.N) * g.Di;
+  if (i >= nd) return;
+  const int n = static_cast<int>(i / g.Di), d = static_cast<int>(i % g.Di), q = static_cast<int>(blockIdx.y);
+  const float a2 = -expf(g.a_log[static_cast<size_t>(d) * g.N + n]) * kLog2e;
+  float total = 0.f;
+  const float h = fold(g.local, g.sum_dt, nd, g.Di, i, d, a2, q * g.group, g.group, 0.f, &total, [](int, float) {});
+  g.group_local[q * nd + i] = h;
+  if (n == 0) g.group_dt[static_cast<size_t>(q) * g.Di + d] = total;
+}
+
+// carry[c], the state before chunk c: through the groups before, then the group's chunks.
+template <class E>
+__global__ __launch_bounds__(256) void mixer_carry_kernel(Mixer<E> g) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, nd = static_cast<size_t>(g.N) * g.Di;
+  if (i >= nd) return;
+  const int n = static_cast<int>(i / g.Di), d = static_cast<int>(i % g.Di), q = static_cast<int>(blockIdx.y);
+  const float a2 = -expf(g.a_log[static_cast<size_t>(d) * g.N + n]) * kLog2e;
+  float total = 0.f;
+  float h = fold(g.group_local, g.group_dt, nd, g.Di, i, d, a2, 0, q, 0.f, &total, [](int, float) {});
+  const int c0 = q * g.group, n_own = min(g.group, g.n_chunks - c0);
+  fold(g.local, g.sum_dt, nd, g.Di, i, d, a2, c0, n_own, h, &total, [&](int c, float v) { g.carry[c * nd + i] = v; });
 }
 
 // Every prompt's last K - 1 inputs, and the states of empty prompts.
@@ -543,7 +850,9 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 template <class E, int NB, int KT>
 int launch_scan(const Mixer<E>& g, bool out, int n_base, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((g.Di + kScanThreads - 1) / kScanThreads), static_cast<unsigned>(g.n_chunks));
+  // (nothing follows the last chunk: it needs no summary)
+  const dim3 grid(static_cast<unsigned>((g.Di + kScanThreads - 1) / kScanThreads),
+                  static_cast<unsigned>(out ? g.n_chunks : g.n_chunks - 1));
   if (out)
     hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, true>), grid, dim3(kScanThreads), 0, st, g, g.bc, n_base);
   else
@@ -577,29 +886,39 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.part = static_cast<float*>(ws);
   g.u = g.part + part;
   const bool vx = vec8(g.x_proj, g.Di), vd = vec8(g.dt_proj, g.R);
-  const bool many = g.rows >= 32;
+  // few rows: one each, in small workgroups, for the latency; many share the weights
+  const bool many = g.rows >= 32, k4 = g.K <= 4;
   const int rb = many ? 8 : 1;
   const dim3 ga(static_cast<unsigned>(g.n_blocks * ((g.rows + rb - 1) / rb)));
-  if (many) hipLaunchKernelGGL((mixer_proj_kernel<E, 8, false>), ga, dim3(kProjThreads), 0, st, g, vx);
-  else hipLaunchKernelGGL((mixer_proj_kernel<E, 1, false>), ga, dim3(kProjThreads), 0, st, g, vx);
-  if (int rc = launch_check("mixer_proj_kernel")) return rc;
+  auto proj = many ? (k4 ? token_proj_kernel<E, 8, 4> : token_proj_kernel<E, 8, 8>)
+                   : (k4 ? token_proj_kernel<E, 1, 4> : token_proj_kernel<E, 1, 8>);
+  hipLaunchKernelGGL(proj, ga, dim3(kProjThreads), 0, st, g, vx);
+  if (int rc = launch_check("token_proj_kernel")) return rc;
   const int rt = many ? 4 : 1, threads = many ? 256 : 64;
   const dim3 gb(static_cast<unsigned>((g.Di + threads - 1) / threads), static_cast<unsigned>((g.rows + rt - 1) / rt));
   const size_t lds = static_cast<size_t>(rt) * g.Nc * sizeof(float);
-  if (many) hipLaunchKernelGGL((mixer_token_kernel<E, 4>), gb, dim3(threads), lds, st, g, vd);
-  else hipLaunchKernelGGL((mixer_token_kernel<E, 1>), gb, dim3(threads), lds, st, g, vd);
-  return launch_check("mixer_token_kernel");
+  hipLaunchKernelGGL(many ? (token_scan_kernel<E, 4>) : (token_scan_kernel<E, 1>), gb, dim3(threads), lds, st, g, vd);
+  return launch_check("token_scan_kernel");
 }
 
 template <class E>
 int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
-  g.n_blocks = (g.Di + kProjBlock - 1) / kProjBlock;
+  const int64_t cus = std::max(1, device_cu_count(call.device()));
+  // the channels split among enough workgroups for four a CU, at most eight ways (each
+  // adds its sums' traffic)
+  const int64_t row_tiles = (g.rows + kPtRows - 1) / kPtRows, col_groups = (g.Nc + kPtCols - 1) / kPtCols;
+  const int64_t k_steps = (g.Di + kPtK - 1) / kPtK;
+  const int64_t ways = std::max<int64_t>(1, std::min<int64_t>({8, k_steps, 4 * cus / std::max<int64_t>(1, row_tiles * col_groups)}));
+  const int per_split = static_cast<int>((k_steps + ways - 1) / ways) * kPtK;
+  g.n_blocks = (g.Di + per_split - 1) / per_split;
   g.Npad = g.N <= 8 ? 8 : g.N <= 16 ? 16 : (g.N + 31) / 32 * 32;
-  // enough chunks for four waves on each SIMD, of 16 tokens at least
+  // enough chunks for four waves on each SIMD, of 32 tokens at least
   const int64_t waves = (g.Di + kWave - 1) / kWave;
-  const int64_t want = std::max<int64_t>(1, 16 * std::max(1, device_cu_count(call.device())) / waves);
-  g.chunk = static_cast<int>(std::max<int64_t>({16, (g.rows + want - 1) / want, (g.rows + 65534) / 65535}));
+  const int64_t want = std::max<int64_t>(1, 16 * cus / waves);
+  g.chunk = static_cast<int>(std::max<int64_t>({32, (g.rows + want - 1) / want, (g.rows + 65534) / 65535}));
   g.n_chunks = (g.rows + g.chunk - 1) / g.chunk;
+  g.group = 16;
+  g.n_groups = std::max(1, (g.n_chunks + g.group - 1) / g.group);
   const size_t nd = static_cast<size_t>(g.N) * g.Di;
   const bool carries = g.n_chunks > 1;
   size_t at = 0;
@@ -610,6 +929,8 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const size_t o_local = take(carries ? g.n_chunks * nd : 0);
   const size_t o_carry = take(carries ? g.n_chunks * nd : 0);
   const size_t o_sum = take(carries ? static_cast<size_t>(g.n_chunks) * g.Di : 0);
+  const size_t o_glocal = take(carries ? g.n_groups * nd : 0);
+  const size_t o_gsum = take(carries ? static_cast<size_t>(g.n_groups) * g.Di : 0);
   const size_t o_init = take(g.resume != nullptr ? g.n_seqs * nd : 0);
   const size_t o_y = take(g.N > 32 ? static_cast<size_t>(g.rows) * g.Di : 0);
   void* ws = nullptr;
@@ -621,16 +942,21 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.local = f + o_local;
   g.carry = f + o_carry;
   g.sum_dt = f + o_sum;
+  g.group_local = f + o_glocal;
+  g.group_dt = f + o_gsum;
   g.y_sum = f + o_y;
   if (g.rows > 0) {
-    constexpr int RB = 8;
-    const int64_t groups = (g.rows + RB - 1) / RB;
-    hipLaunchKernelGGL((mixer_proj_kernel<E, RB, true>), dim3(static_cast<unsigned>(groups * g.n_blocks)),
-                       dim3(kProjThreads), 0, st, g, vec8(g.x_proj, g.Di));
-    if (int rc = launch_check("mixer_proj_kernel")) return rc;
-    hipLaunchKernelGGL((mixer_dt_kernel<E, RB>), dim3(static_cast<unsigned>(groups * ((g.Di + 255) / 256))), dim3(256),
-                       static_cast<size_t>(RB) * g.Nc * sizeof(float), st, g, vec8(g.dt_proj, g.R));
-    if (int rc = launch_check("mixer_dt_kernel")) return rc;
+    const bool k4 = g.K <= 4;
+    hipLaunchKernelGGL(k4 ? (prompt_proj_kernel<E, 4>) : (prompt_proj_kernel<E, 8>),
+                       dim3(static_cast<unsigned>(row_tiles * g.n_blocks * col_groups)), dim3(256), 0, st, g, per_split,
+                       vec8(g.x_proj, g.Di));
+    if (int rc = launch_check("prompt_proj_kernel")) return rc;
+    const int64_t dt_tiles = (g.rows + kDtRows - 1) / kDtRows, dt_cols = (g.Di + kDtCols - 1) / kDtCols;
+    const int64_t dt_y = std::max<int64_t>(1, std::min<int64_t>(dt_cols, 4 * cus / dt_tiles));
+    const int width = (std::min(g.R, kDtMaxR) + 63) / 64 * 64;
+    hipLaunchKernelGGL(prompt_dt_kernel<E>, dim3(static_cast<unsigned>(dt_tiles), static_cast<unsigned>(dt_y)), dim3(256),
+                       static_cast<size_t>(3) * kDtRows * width * 2, st, g, width, vec8(g.dt_proj, g.R));
+    if (int rc = launch_check("prompt_dt_kernel")) return rc;
     if (g.resume != nullptr) {
       g.init = f + o_init;
       hipLaunchKernelGGL(mixer_gather_kernel<E>, dim3(static_cast<unsigned>(std::min<size_t>(64, (nd + 255) / 256)),
@@ -639,7 +965,12 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
     }
     if (carries) {
       if (int rc = launch_scans(g, false, st)) return rc;
-      hipLaunchKernelGGL(mixer_carry_kernel<E>, dim3(static_cast<unsigned>((nd + 255) / 256)), dim3(256), 0, st, g);
+      const unsigned nb = static_cast<unsigned>((nd + 255) / 256);
+      if (g.n_groups > 1) {
+        hipLaunchKernelGGL(mixer_group_kernel<E>, dim3(nb, static_cast<unsigned>(g.n_groups - 1)), dim3(256), 0, st, g);
+        if (int rc = launch_check("mixer_group_kernel")) return rc;
+      }
+      hipLaunchKernelGGL(mixer_carry_kernel<E>, dim3(nb, static_cast<unsigned>(g.n_groups)), dim3(256), 0, st, g);
       if (int rc = launch_check("mixer_carry_kernel")) return rc;
     }
     if (int rc = launch_scans(g, true, st)) return rc;
@@ -660,7 +991,7 @@ int check_mixer(const char* what, int dtype, int64_t rows, int64_t n_seqs, int64
                                                std::to_string(k));
   if (rows > 1 && ld < 2 * di) return set_error(OSSM_ERR_INVALID_ARGUMENT, w + ": row stride of xz below 2 d_inner");
   if (rows > (1 << 24) || n_seqs > 65535 || n_slots > INT_MAX / 8 || di > (1 << 20) || n > 1024 || r + 2 * n > 2048 ||
-      ((rows + 7) / 8) * ((di + 127) / 128) > INT_MAX / 2)
+      ((rows + 7) / 8) * ((di + 127) / 128) > INT_MAX / 2 || ((rows + 63) / 64) * 8 * ((r + 2 * n + 127) / 128) > INT_MAX)
     return set_error(OSSM_ERR_UNSUPPORTED, w + ": size exceeds launch limits");
   return OSSM_OK;
 }

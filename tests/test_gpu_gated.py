@@ -165,8 +165,7 @@ def test_values_that_are_not_finite(G, rows, dtype):
         announce(f"gated_linear {value} rows={rows} {dtype}")
         y = G.gated_linear(xi, wg, wi, activation="relu")
         keep_r, keep_c = [i for i in range(rows) if i != 1], list(range(69))
-        # (float32 sums near one that is not finite are formed another way: other roundings)
-        check(y[keep_r][:, keep_c], base[keep_r][:, keep_c].double().cpu().numpy(), dtype, "the others")
+        assert torch.equal(y[keep_r][:, keep_c], base[keep_r][:, keep_c])
         want = reference(xi, wg, wi, None, None, "relu")
         g = y.double().cpu().numpy()
         assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(np.isposinf(g), np.isposinf(want))

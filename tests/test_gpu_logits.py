@@ -88,7 +88,8 @@ def call(L, x, hist, n, first, rep, pres, freq, ids, vals, allowed, **kw):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("size", [(1, 1, 1, 1), (3, 31, 0, 0), (2, 33, 5, 2), (5, 1000, 700, 3), (4, 8191, 50, 7),
-                                  (3, 8192, 1, 0), (7, 8193, 300, 40), (2, 50001, 2000, 300), (33, 4099, 64, 16)],
+                                  (3, 8192, 1, 0), (7, 8193, 300, 40), (2, 50001, 2000, 300), (33, 4099, 64, 16),
+                                  (2, 300, 70000, 5), (1, 9000, 20, 70000)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_matches_float64(L, size, dtype):
     announce(f"control_logits {size} {dtype}")
