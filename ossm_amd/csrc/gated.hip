@@ -72,7 +72,7 @@ __device__ __forceinline__ ActGrad activate(float a) {
     default: {  // gelu, tanh form
       const float c = 0.79788456080286536f, k = 0.044715f;
       const float e = __expf(2.f * c * (a + k * a * a * a));
-      const float t = 1.f - 2.f / (e + 1.f);
+      const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
       return {0.5f * a * (1.f + t), 0.5f * (1.f + t) + 0.5f * a * (1.f - t * t) * c * (1.f + 3.f * k * a * a)};
     }
   }

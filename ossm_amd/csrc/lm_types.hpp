@@ -25,7 +25,9 @@ __device__ __forceinline__ bf16_t from_f<bf16_t>(float v) {  // to nearest, ties
   return bf16_t{__builtin_bit_cast(uint16_t, b)};
 }
 
-__device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + __expf(-x)); }
+// The hardware reciprocal (within 1 ulp): the exact division's ten instructions were a sixth
+// of the scans' time outside their states.
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 __device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
 
 // softplus(x) = max(x, 0) + log1p(exp(-|x|)), the logarithm by its series in
@@ -34,7 +36,7 @@ __device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
 // 1 + e would not).
 __device__ __forceinline__ float softplus_f(float x) {
   const float e = __expf(-fabsf(x));
-  const float z = e / (2.f + e), q = z * z;
+  const float z = e * __builtin_amdgcn_rcpf(2.f + e), q = z * z;
   float s = 1.f / 15.f;
   s = fmaf(s, q, 1.f / 13.f);
   s = fmaf(s, q, 1.f / 11.f);

@@ -43,7 +43,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxConv = 8;
 constexpr int kProjThreads = 256;
 constexpr int kProjWaves = kProjThreads / kWave;
-constexpr int kSub = 32;                       // channels of one wave's share of x_proj
+constexpr int kSub = 32;                       // channels of one wave's share of a token's x_proj
 constexpr int kProjBlock = kProjWaves * kSub;  // channels of a workgroup
 
 template <class E>
@@ -65,6 +65,7 @@ struct Mixer {
   E* y;
   float* part;   // [n_blocks][rows][Nc]: x_proj's sums over blocks (splits) of the channels
   float* u;      // tokens: [rows][Di]
+  uint16_t* planes;  // prompts: [3][rows][Rp], the projections' part for dt
   float* bc;     // prompts: [rows][2][Npad], B and C, zero from N on
   float* dt;     // prompts: [rows][Di]
   float* local;  // prompts: [n_chunks][N][Di], a chunk's end from a zero carry
@@ -75,7 +76,7 @@ struct Mixer {
   float* init;   // prompts: [n_seqs][N][Di] copies of the resumed states, or null
   float* y_sum;  // prompts with N past a block of states: [rows][Di]
   long long ld;
-  int rows, n_seqs, n_slots, Di, N, R, K, Nc, Npad, n_blocks, chunk, n_chunks, group, n_groups;
+  int rows, n_seqs, n_slots, Di, N, R, K, Nc, Npad, Rp, n_blocks, chunk, n_chunks, group, n_groups;
 };
 
 // Where sequence i starts, in range whatever the offsets hold.
@@ -112,6 +113,16 @@ __device__ __forceinline__ float conv_input(const Mixer<E>& g, int pos, int star
   const int j = g.K - 1 + pos - start;
   if (slot < 0 || j < 0) return 0.f;
   return to_f(g.conv_state[(static_cast<size_t>(slot) * (g.K - 1) + j) * g.Di + d]);
+}
+
+// Four consecutive elements.
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void load4(const bf16_t* p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
 }
 
 // Eight consecutive weights (zeros past the row's n), vector loads where `vec`.
@@ -156,7 +167,19 @@ __global__ __launch_bounds__(kProjThreads) void token_proj_kernel(Mixer<E> g, bo
   // kProjThreads / kProjBlock apart)
   constexpr int kRows = (RB * kProjBlock + kProjThreads - 1) / kProjThreads;
   const int c = tid % kProjBlock, d = min(c0 + c, g.Di - 1);
-  float x[kRows][KT], wt[KT];
+  float x[kRows][KT], wt[KT], v[kSub];
+  const auto weights = [&](int j0) {
+    const E* row = g.x_proj + static_cast<size_t>(min(j0 + lane, g.Nc - 1)) * g.Di;
+#pragma unroll
+    for (int q = 0; q < kSub; q += 8) {
+      const int left = g.Di - (c0 + w * kSub + q);
+      float e[8];
+      load8(row + (left > 0 ? c0 + w * kSub + q : 0), left, vec, e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q + i] = e[i];
+    }
+  };
+  weights(0);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int r = min(r0 + tid / kProjBlock + i * (kProjThreads / kProjBlock), g.rows - 1);
@@ -194,20 +217,15 @@ __global__ __launch_bounds__(kProjThreads) void token_proj_kernel(Mixer<E> g, bo
   }
   __syncthreads();
   for (int j0 = 0; j0 < g.Nc; j0 += kWave) {
-    const int j = min(j0 + lane, g.Nc - 1);
-    float acc[RB];
+    float acc[RB], now[kSub];
 #pragma unroll
-    for (int rr = 0; rr < RB; ++rr) acc[rr] = 0.f;
+    for (int i = 0; i < kSub; ++i) now[i] = v[i];
+    if (j0 + kWave < g.Nc) weights(j0 + kWave);  // in flight under this step's sums
 #pragma unroll
-    for (int q = 0; q < kSub; q += 8) {
-      const int c8 = w * kSub + q;
-      float v[8];
-      const int left = g.Di - (c0 + c8);
-      load8(g.x_proj + static_cast<size_t>(j) * g.Di + (left > 0 ? c0 + c8 : 0), left, vec, v);
+    for (int rr = 0; rr < RB; ++rr) {
+      acc[rr] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int rr = 0; rr < RB; ++rr) acc[rr] = fmaf(v[i], s_u[rr][c8 + i], acc[rr]);
+      for (int i = 0; i < kSub; ++i) acc[rr] = fmaf(now[i], s_u[rr][w * kSub + i], acc[rr]);
     }
 #pragma unroll
     for (int rr = 0; rr < RB; ++rr) s_sum[w][rr][lane] = acc[rr];
@@ -217,7 +235,7 @@ __global__ __launch_bounds__(kProjThreads) void token_proj_kernel(Mixer<E> g, bo
       if (r0 + rr < g.rows && j0 + l < g.Nc) {
         float t = s_sum[0][rr][l];
 #pragma unroll
-        for (int v = 1; v < kProjWaves; ++v) t += s_sum[v][rr][l];
+        for (int q = 1; q < kProjWaves; ++q) t += s_sum[q][rr][l];
         g.part[(static_cast<size_t>(blk) * g.rows + r0 + rr) * g.Nc + j0 + l] = t;
       }
     }
@@ -239,8 +257,9 @@ __device__ __forceinline__ float proj_of(const Mixer<E>& g, int r, int j) {
 // One token: a thread per channel, RB rows.  The first 16 states of all rows are asked
 // for before the projections are summed: the states' traffic is what bounds a large
 // batch, and this keeps 16 RB loads a thread in flight.
-template <class E, int RB>
-__global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, bool vec) {
+// VEC: A_log's and dt_proj's rows are whole 16-byte vectors.
+template <class E, int RB, bool VEC>
+__global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
   extern __shared__ float s_p[];  // [RB][Nc]
   const int r0 = static_cast<int>(blockIdx.y) * RB;
   const int d_own = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x), d = min(d_own, g.Di - 1);
@@ -258,8 +277,34 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, bool vec) {
     u[rr] = g.u[static_cast<size_t>(r) * g.Di + d];
     z[rr] = to_f(g.xz[static_cast<size_t>(r) * g.ld + g.Di + d]);
   }
+  const auto load_a = [&](int n0) {
+    const float* p = g.a_log + static_cast<size_t>(d) * g.N + n0;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) a2[i] = i < g.N ? g.a_log[static_cast<size_t>(d) * g.N + i] : 0.f;
+    for (int i = 0; i < NB; i += 4) {
+      if (VEC && n0 + i + 4 <= g.N) {
+        float q[4];
+        load4(p + i, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a2[i + k] = q[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a2[i + k] = n0 + i + k < g.N ? p[i + k] : 0.f;
+      }
+    }
+  };
+  load_a(0);
+  // dt_proj's first 32 weights of the channel
+  float wt[32];
+  const auto load_w = [&](int q0) {
+#pragma unroll
+    for (int q = 0; q < 32; q += 8) {
+      float e[8];
+      load8(g.dt_proj + static_cast<size_t>(d) * g.R + (q0 + q < g.R ? q0 + q : 0), g.R - q0 - q, VEC, e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wt[q + i] = e[i];
+    }
+  };
+  load_w(0);
   for (int i = threadIdx.x; i < RB * g.Nc; i += blockDim.x) {
     const int r = r0 + i / g.Nc;
     s_p[i] = r < g.rows ? proj_of(g, r, i % g.Nc) : 0.f;
@@ -269,14 +314,14 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, bool vec) {
   const float bias = g.dt_bias[d];
 #pragma unroll
   for (int rr = 0; rr < RB; ++rr) dt[rr] = bias;
-  for (int q = 0; q < g.R; q += 8) {
-    float wt[8];
-    load8(g.dt_proj + static_cast<size_t>(d) * g.R + q, g.R - q, vec, wt);
+  for (int q0 = 0; q0 < g.R; q0 += 32) {
+    if (q0 > 0) load_w(q0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = min(q + i, g.Nc - 1);
+    for (int i = 0; i < 32; ++i) {
+      if (q0 + i < g.R) {
 #pragma unroll
-      for (int rr = 0; rr < RB; ++rr) dt[rr] = q + i < g.R ? fmaf(wt[i], s_p[rr * g.Nc + k], dt[rr]) : dt[rr];
+        for (int rr = 0; rr < RB; ++rr) dt[rr] = fmaf(wt[i], s_p[rr * g.Nc + q0 + i], dt[rr]);
+      }
     }
   }
   if (d_own >= g.Di) return;
@@ -289,10 +334,7 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, bool vec) {
     y[rr] = skip * u[rr];
   }
   for (int n0 = 0; n0 < g.N; n0 += NB) {
-    if (n0 > 0) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) a2[i] = n0 + i < g.N ? g.a_log[static_cast<size_t>(d) * g.N + n0 + i] : 0.f;
-    }
+    if (n0 > 0) load_a(n0);
 #pragma unroll
     for (int i = 0; i < NB; ++i) a2[i] = -expf(a2[i]) * kLog2e;
 #pragma unroll
@@ -393,22 +435,120 @@ __device__ __forceinline__ float planes_sum(const uint16_t* s, int plane, int at
 
 constexpr int kPtRows = 64, kPtK = 64, kPtCols = 128;  // prompt_proj_kernel's tile and k step
 
+// A thread's share of a tile's conv: 4 channels of 4 rows, and the rows before them.
+// VEC: whole quads of channels, on 4-element boundaries.
+template <class E, int KT, bool VEC>
+struct ConvShare {
+  float x[4 + KT - 1][4], w[4][KT], b[4];
+
+  __device__ __forceinline__ void load(const Mixer<E>& g, int r_first, int d0) {
+    const int skip_taps = KT - g.K;
+    const int dv = VEC ? min(d0, g.Di - 4) : d0;
+#pragma unroll
+    for (int i = 0; i < 4 + KT - 1; ++i) {
+      const E* row = g.xz + static_cast<size_t>(min(max(r_first - (KT - 1) + i, 0), g.rows - 1)) * g.ld;
+      if constexpr (VEC) {
+        load4(row + dv, x[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = to_f(row[min(d0 + e, g.Di - 1)]);
+      }
+    }
+    if (VEC && KT == 4 && g.K == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float q[4];
+        load4(g.conv_w + static_cast<size_t>(dv + e) * 4, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[e][k] = q[k];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          w[e][k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(min(d0 + e, g.Di - 1)) * g.K + k - skip_taps]) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = g.conv_b != nullptr ? to_f(g.conv_b[min(d0 + e, g.Di - 1)]) : 0.f;
+  }
+
+  // u of the rows in `inside` (bit r: row r of the tile and the K - 1 before it are one
+  // prompt's), zeros for the rows in `padding`, as three planes in LDS
+  __device__ __forceinline__ void store(const Mixer<E>& g, int rr0, int quad, int d0, uint64_t inside, uint64_t padding,
+                                        uint16_t* s_u) const {
+    const int skip_taps = KT - g.K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = rr0 + i;
+      float u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = b[e];
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        if (k >= skip_taps)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = fmaf(w[e][k], x[i + k][e], u[e]);
+      const bool zero = (padding >> rr) & 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = d0 + e < g.Di && !zero ? silu_f(u[e]) : 0.f;
+      uint32_t t0[3], t1[3];
+      split_pair(u[0], u[1], t0);
+      split_pair(u[2], u[3], t1);
+      const int at = plane_at(rr, 4 * quad, kPtK);
+      if (((inside | padding) >> rr) & 1) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(&s_u[q * (kPtRows * kPtK) + at]) = make_uint2(t0[q], t1[q]);
+      }
+    }
+  }
+};
+
+// The other rows of the tile, a prompt's first K - 1: a wave a row, a lane a channel.
+template <class E>
+__device__ __forceinline__ void store_first_rows(const Mixer<E>& g, int r0, int k0, uint64_t others, const int* s_start,
+                                                 const int* s_slot, uint16_t* s_u) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), d = min(k0 + lane, g.Di - 1);
+  int turn = 0;
+#pragma unroll 1
+  for (; others != 0; others &= others - 1, ++turn) {
+    if ((turn & 3) != wave_id()) continue;
+    const int rr = __builtin_ctzll(others), start = s_start[rr], slot = s_slot[rr];
+    float p = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
+#pragma unroll 1
+    for (int k = 0; k < g.K; ++k)
+      p = fmaf(to_f(g.conv_w[static_cast<size_t>(d) * g.K + k]), conv_input(g, r0 + rr - (g.K - 1) + k, start, slot, d), p);
+    uint32_t t[3];
+    split_pair(k0 + lane < g.Di ? silu_f(p) : 0.f, 0.f, t);
+    const int at = plane_at(rr, lane, kPtK);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) s_u[q * (kPtRows * kPtK) + at] = static_cast<uint16_t>(t[q]);
+  }
+}
+
 // Conv + SiLU of a tile of kPtRows tokens, kPtK channels at a time, and x_proj's sums over
 // this split's channels for kPtCols of the Nc outputs.  u goes from registers into LDS as
 // three bf16 planes; a wave takes 32 rows and 64 outputs, the weights' fragments straight
 // from memory (all workgroups read the same few hundred kB).  Sums that are not
 // finite (a term of an infinite weight against a zero one) are formed again on the
 // fp32 instruction; finite ones stay as they are, whatever their neighbours.
-template <class E, int KT>
-__global__ __launch_bounds__(256) void prompt_proj_kernel(Mixer<E> g, int per_split, bool vec) {
-  __shared__ __align__(16) uint16_t s_u[3][kPtRows * kPtK];
+template <class E, int KT, bool VEC>
+__global__ __launch_bounds__(256, 2) void prompt_proj_kernel(Mixer<E> g, int per_split, bool vec) {
+  __shared__ __align__(16) uint16_t s_u[3 * kPtRows * kPtK];
   __shared__ int s_start[kPtRows], s_slot[kPtRows];
+  __shared__ uint64_t s_rows[2];  // rows inside a prompt, rows of padding
   const int groups = (g.Nc + kPtCols - 1) / kPtCols;
   int id = static_cast<int>(blockIdx.x);
   const int col0 = id % groups * kPtCols;
   id /= groups;
   const int split = id % g.n_blocks, r0 = id / g.n_blocks * kPtRows;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = wave_id();
+  const int quad = tid & 15, rr0 = (tid >> 4) * 4;  // the conv's share: 4 channels of 4 rows
+  const int rf = (w & 1) * 32, cf = col0 + (w >> 1) * 64;  // the product's: 32 rows, 64 outputs
+  const int l32 = lane & 31, half = lane >> 5;
+  const int k_first = split * per_split, k_end = min(g.Di, k_first + per_split);
+  ConvShare<E, KT, VEC> conv;
+  conv.load(g, r0 + rr0, k_first + 4 * quad);
   if (tid < kPtRows) {
     const int r = r0 + tid;
     int start = INT_MAX, slot = -1;  // INT_MAX: padding
@@ -418,104 +558,64 @@ __global__ __launch_bounds__(256) void prompt_proj_kernel(Mixer<E> g, int per_sp
     }
     s_start[tid] = start;
     s_slot[tid] = slot;
+    const uint64_t inside = __ballot(start != INT_MAX && r - (g.K - 1) >= start), padding = __ballot(start == INT_MAX);
+    if (tid == 0) { s_rows[0] = inside; s_rows[1] = padding; }
   }
   __syncthreads();
-  const int skip_taps = KT - g.K;
-  const int pair = tid & 31, rg = tid >> 5;  // the conv's share: 2 channels of 8 rows
-  const int rf = (w & 1) * 32, cf = col0 + (w >> 1) * 64;  // the product's: 32 rows, 64 outputs
-  const int l32 = lane & 31, half = lane >> 5;
-  const int k_end = min(g.Di, (split + 1) * per_split);
-  floatx16 acc[2] = {}, first[2];
-  for (int pass = 0; pass < 2; ++pass) {
+  const uint64_t inside = s_rows[0], padding = s_rows[1];
+  const E* rows_w[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      first[j] = acc[j];
+  for (int j = 0; j < 2; ++j) rows_w[j] = g.x_proj + static_cast<size_t>(min(cf + j * 32 + l32, g.Nc - 1)) * g.Di;
+  const bool idle = cf >= g.Nc;  // a wave without outputs
+  floatx16 acc[2] = {};
+  for (int k0 = k_first; k0 < k_end; k0 += kPtK) {
+    __syncthreads();  // the last step's products have read s_u
+    Weight8<E> wt[kPtK / 16][2];
+    if (!idle) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+      for (int kk = 0; kk < kPtK / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) wt[kk][j].load(rows_w[j], k0 + kk * 16 + half * 8, g.Di, vec);
     }
-    for (int k0 = split * per_split; k0 < k_end; k0 += kPtK) {
-      Weight8<E> wt[kPtK / 16][2];
-      if (pass == 0) {
+    conv.store(g, rr0, quad, k0 + 4 * quad, inside, padding, s_u);
+    store_first_rows(g, r0, k0, ~(inside | padding), s_start, s_slot, s_u);
+    if (k0 + kPtK < k_end) conv.load(g, r0 + rr0, k0 + kPtK + 4 * quad);  // in flight under the products
+    __syncthreads();
+    if (!idle) {
 #pragma unroll
-        for (int kk = 0; kk < kPtK / 16; ++kk)
+      for (int kk = 0; kk < kPtK / 16; ++kk) {
+        bf16x8 a[3];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            wt[kk][j].load(g.x_proj + static_cast<size_t>(min(cf + j * 32 + l32, g.Nc - 1)) * g.Di,
-                           k0 + kk * 16 + half * 8, g.Di, vec);
-      }
-      // ---- conv + SiLU
-      float x[2][8 + KT - 1], cw[2][KT], cb[2];
+        for (int q = 0; q < 3; ++q)
+          a[q] = *reinterpret_cast<const bf16x8*>(&s_u[q * (kPtRows * kPtK) + plane_at(rf + l32, kk * 16 + half * 8, kPtK)]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = min(k0 + 2 * pair + e, g.Di - 1);
-        cb[e] = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) cw[e][k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d) * g.K + k - skip_taps]) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8 + KT - 1; ++i) {
-          const int r = min(max(r0 + rg * 8 - (KT - 1) + i, 0), g.rows - 1);
-          x[e][i] = to_f(g.xz[static_cast<size_t>(r) * g.ld + d]);
+        for (int j = 0; j < 2; ++j) {
+          wt[kk][j].split();
+          acc[j] = mfma_terms(a, wt[kk][j], acc[j]);
         }
       }
-      __syncthreads();  // the last step's products have read s_u
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int rr = rg * 8 + i, start = s_start[rr];
-        float u[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = k0 + 2 * pair + e;
-          float p = cb[e];
-          if (r0 + rr - (g.K - 1) >= start) {
-#pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (k >= skip_taps) p = fmaf(cw[e][k], x[e][i + k], p);
-          } else {
-#pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (k >= skip_taps && start != INT_MAX) {
-                const int pos = r0 + rr - (KT - 1) + k;
-                p = fmaf(cw[e][k], pos >= start ? x[e][i + k] : conv_input(g, pos, start, s_slot[rr], min(d, g.Di - 1)), p);
-              }
-          }
-          u[e] = d < g.Di && start != INT_MAX ? silu_f(p) : 0.f;
-        }
-        uint32_t t[3];
-        split_pair(u[0], u[1], t);
-        const int at = plane_at(rr, 2 * pair, kPtK);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&s_u[q][at]) = t[q];
-      }
-      __syncthreads();
-      // ---- x_proj
-      if (pass == 0) {
-#pragma unroll
-        for (int kk = 0; kk < kPtK / 16; ++kk) {
-          bf16x8 a[3];
-#pragma unroll
-          for (int q = 0; q < 3; ++q)
-            a[q] = *reinterpret_cast<const bf16x8*>(&s_u[q][plane_at(rf + l32, kk * 16 + half * 8, kPtK)]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            wt[kk][j].split();
-            acc[j] = mfma_terms(a, wt[kk][j], acc[j]);
-          }
-        }
-      } else {
+    }
+  }
+  if (__syncthreads_or(any_nonfinite(acc))) {
+    floatx16 again[2] = {};
 #pragma unroll 1
-        for (int k = 0; k < kPtK; k += 2) {
-          const float a = planes_sum(&s_u[0][0], kPtRows * kPtK, plane_at(rf + l32, k + half, kPtK));
+    for (int k0 = k_first; k0 < k_end; k0 += kPtK) {
+      conv.load(g, r0 + rr0, k0 + 4 * quad);
+      __syncthreads();
+      conv.store(g, rr0, quad, k0 + 4 * quad, inside, padding, s_u);
+      store_first_rows(g, r0, k0, ~(inside | padding), s_start, s_slot, s_u);
+      __syncthreads();
+#pragma unroll 1
+      for (int q = 0; q < kPtK; q += 2) {
+        const int k = q + half;
+        const float a = planes_sum(s_u, kPtRows * kPtK, plane_at(rf + l32, k, kPtK));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int d = k0 + k + half;
-            const float b = d < g.Di ? to_f(g.x_proj[static_cast<size_t>(min(cf + j * 32 + l32, g.Nc - 1)) * g.Di + d]) : 0.f;
-            acc[j] = mfma32(a, b, acc[j]);
-          }
-        }
+        for (int j = 0; j < 2; ++j) again[j] = mfma32(a, k0 + k < g.Di ? to_f(rows_w[j][k0 + k]) : 0.f, again[j]);
       }
     }
-    if (pass == 0 && !__syncthreads_or(any_nonfinite(acc))) break;
-    if (pass == 1) keep_finite(acc, first);
+    keep_finite(again, acc);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[j] = again[j];
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -526,99 +626,84 @@ __global__ __launch_bounds__(256) void prompt_proj_kernel(Mixer<E> g, int per_sp
     }
 }
 
-constexpr int kDtRows = 32, kDtCols = 256, kDtMaxR = 256;  // prompt_dt_kernel's tile, its stretch of R
-
-// B, C (float32) and dt = softplus(dt_proj p[:R] + bias) of a tile of tokens, from x_proj's
-// partial sums; blockIdx.y takes every gridDim.y-th block of kDtCols channels.  `width`:
-// the planes' row in LDS, at least the stretch of R, a multiple of 64.
+// x_proj's sums over its splits: B and C in float32, the part for dt as three bf16 planes
+// [3][rows][Rp] (zeros from R on).
 template <class E>
-__global__ __launch_bounds__(256) void prompt_dt_kernel(Mixer<E> g, int width, bool vec) {
-  extern __shared__ __align__(16) uint16_t s_dt[];  // [3][kDtRows * width]
+__global__ __launch_bounds__(256) void prompt_sum_kernel(Mixer<E> g) {
+  const int cols = g.Rp + 2 * g.Npad;
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<long long>(g.rows) * cols) return;
+  const int r = static_cast<int>(i / cols), k = static_cast<int>(i % cols);
+  const size_t plane = static_cast<size_t>(g.rows) * g.Rp;
+  if (k < g.Rp) {
+    uint32_t t[3];
+    split_pair(k < g.R ? proj_of(g, r, k) : 0.f, 0.f, t);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) g.planes[q * plane + static_cast<size_t>(r) * g.Rp + k] = static_cast<uint16_t>(t[q]);
+  } else {
+    const int c = k - g.Rp, second = c >= g.Npad ? 1 : 0, n = c - second * g.Npad;
+    g.bc[static_cast<size_t>(r) * 2 * g.Npad + c] = n < g.N ? proj_of(g, r, g.R + second * g.N + n) : 0.f;
+  }
+}
+
+constexpr int kDtRows = 32, kDtCols = 256;  // prompt_dt_kernel's tile, a wave 32 x 64 of it
+
+// dt = softplus(dt_proj p[:R] + bias), both operands' fragments straight from memory (the
+// planes and the weights are read from the caches by every tile).
+template <class E>
+__global__ __launch_bounds__(256) void prompt_dt_kernel(Mixer<E> g, bool vec) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
   const int r0 = static_cast<int>(blockIdx.x) * kDtRows;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = wave_id(), l32 = lane & 31, half = lane >> 5;
-  const int plane = kDtRows * width;
-  if (blockIdx.y == 0) {
-    for (int i = tid; i < kDtRows * 2 * g.Npad; i += 256) {
-      const int rr = i / (2 * g.Npad), k = i % (2 * g.Npad), second = k / g.Npad, n = k % g.Npad;
-      if (r0 + rr < g.rows)
-        g.bc[static_cast<size_t>(r0 + rr) * 2 * g.Npad + k] = n < g.N ? proj_of(g, r0 + rr, g.R + second * g.N + n) : 0.f;
-    }
+  const int cw = static_cast<int>(blockIdx.y) * kDtCols + wave_id() * 64;
+  if (cw >= g.Di) return;  // no barriers below
+  const size_t plane = static_cast<size_t>(g.rows) * g.Rp;
+  const uint16_t* row = g.planes + static_cast<size_t>(min(r0 + l32, g.rows - 1)) * g.Rp;
+  const E* rows_w[2];
+  float bias[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int d = min(cw + j * 32 + l32, g.Di - 1);
+    rows_w[j] = g.dt_proj + static_cast<size_t>(d) * g.R;
+    bias[j] = g.dt_bias[d];
   }
-  const bool once = g.R <= kDtMaxR;  // the planes hold all of R for every block of channels
-  const auto fill = [&](int q0) {
-    for (int i = tid; i < kDtRows * (width / 2); i += 256) {
-      const int rr = i / (width / 2), k = i % (width / 2) * 2, r = min(r0 + rr, g.rows - 1);
-      uint32_t t[3];
-      split_pair(q0 + k < g.R ? proj_of(g, r, q0 + k) : 0.f, q0 + k + 1 < g.R ? proj_of(g, r, q0 + k + 1) : 0.f, t);
-      const int at = plane_at(rr, k, width);
+  floatx16 acc[2] = {};
+#pragma unroll 2
+  for (int k0 = 0; k0 < g.Rp; k0 += 16) {
+    const int k = k0 + half * 8;
+    bf16x8 a[3];
+    Weight8<E> wt[2];
 #pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&s_dt[q * plane + at]) = t[q];
-    }
-  };
-  if (once) {
-    fill(0);
-    __syncthreads();
-  }
-  for (int b0 = static_cast<int>(blockIdx.y) * kDtCols; b0 < g.Di; b0 += static_cast<int>(gridDim.y) * kDtCols) {
-    const int cw = b0 + w * 64;
-    floatx16 acc[2] = {}, first[2];
-    for (int pass = 0; pass < 2; ++pass) {
+    for (int q = 0; q < 3; ++q) a[q] = *reinterpret_cast<const bf16x8*>(row + q * plane + k);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        first[j] = acc[j];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
-      }
-      for (int q0 = 0; q0 < g.R; q0 += kDtMaxR) {
-        if (!once) {
-          __syncthreads();
-          fill(q0);
-          __syncthreads();
-        }
-        const int n = min(g.R - q0, kDtMaxR);
-        if (pass == 0) {
-          for (int k = 0; k < n; k += 16) {
-            Weight8<E> wt[2];
-            bf16x8 a[3];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              wt[j].load(g.dt_proj + static_cast<size_t>(min(cw + j * 32 + l32, g.Di - 1)) * g.R, q0 + k + half * 8, g.R, vec);
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-              a[q] = *reinterpret_cast<const bf16x8*>(&s_dt[q * plane + plane_at(l32, k + half * 8, width)]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              wt[j].split();
-              acc[j] = mfma_terms(a, wt[j], acc[j]);
-            }
-          }
-        } else {
-#pragma unroll 1
-          for (int k = 0; k < n; k += 2) {
-            const float a = k + half < n ? planes_sum(s_dt, plane, plane_at(l32, k + half, width)) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float b = k + half < n
-                  ? to_f(g.dt_proj[static_cast<size_t>(min(cw + j * 32 + l32, g.Di - 1)) * g.R + q0 + k + half]) : 0.f;
-              acc[j] = mfma32(a, b, acc[j]);
-            }
-          }
-        }
-      }
-      // (the waves agree: the passes hold barriers where R takes several stretches)
-      if (pass == 0 && !__syncthreads_or(any_nonfinite(acc))) break;
-      if (pass == 1) keep_finite(acc, first);
-    }
+    for (int j = 0; j < 2; ++j) wt[j].load(rows_w[j], k, g.R, vec);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int d = cw + j * 32 + l32;
-      if (d >= g.Di) continue;
-      const float bias = g.dt_bias[d];
+      wt[j].split();
+      acc[j] = mfma_terms(a, wt[j], acc[j]);
+    }
+  }
+  if (any_nonfinite(acc)) {
+    floatx16 again[2] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < g.Rp; k0 += 2) {
+      const int k = k0 + half;
+      const float a = (to_f(bf16_t{row[2 * plane + k]}) + to_f(bf16_t{row[plane + k]})) + to_f(bf16_t{row[k]});
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = r0 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (row < g.rows) g.dt[static_cast<size_t>(row) * g.Di + d] = softplus_f(acc[j][r] + bias);
-      }
+      for (int j = 0; j < 2; ++j) again[j] = mfma32(a, k < g.R ? to_f(rows_w[j][k]) : 0.f, again[j]);
+    }
+    keep_finite(again, acc);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[j] = again[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int d = cw + j * 32 + l32;
+    if (d >= g.Di) continue;
+    float* out = g.dt + static_cast<size_t>(r0) * g.Di + d;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = 8 * (r >> 2) + 4 * half + (r & 3);
+      if (r0 + at < g.rows) out[static_cast<size_t>(at) * g.Di] = softplus_f(acc[j][r] + bias[j]);
     }
   }
 }
@@ -719,6 +804,9 @@ __global__ __launch_bounds__(kScanThreads) void mixer_scan_kernel(Mixer<E> g, co
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
           if (t + i >= e) break;
+          // the scalar loads of B and C stay with their token: hoisted over the group they
+          // spill
+          __builtin_amdgcn_sched_barrier(0);
           const float* B = bc + static_cast<size_t>(t + i) * 2 * g.Npad + n_base;
           const float* C = B + g.Npad;
           float p = cb;
@@ -885,7 +973,7 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   if (int rc = acquire_workspace(call, (part + static_cast<size_t>(g.rows) * g.Di) * sizeof(float), &ws)) return rc;
   g.part = static_cast<float*>(ws);
   g.u = g.part + part;
-  const bool vx = vec8(g.x_proj, g.Di), vd = vec8(g.dt_proj, g.R);
+  const bool vx = vec8(g.x_proj, g.Di);
   // few rows: one each, in small workgroups, for the latency; many share the weights
   const bool many = g.rows >= 32, k4 = g.K <= 4;
   const int rb = many ? 8 : 1;
@@ -897,21 +985,25 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const int rt = many ? 4 : 1, threads = many ? 256 : 64;
   const dim3 gb(static_cast<unsigned>((g.Di + threads - 1) / threads), static_cast<unsigned>((g.rows + rt - 1) / rt));
   const size_t lds = static_cast<size_t>(rt) * g.Nc * sizeof(float);
-  hipLaunchKernelGGL(many ? (token_scan_kernel<E, 4>) : (token_scan_kernel<E, 1>), gb, dim3(threads), lds, st, g, vd);
+  const bool vec = vec8(g.dt_proj, g.R) && vec8(g.a_log, g.N);
+  hipLaunchKernelGGL(many ? (vec ? token_scan_kernel<E, 4, true> : token_scan_kernel<E, 4, false>)
+                          : (vec ? token_scan_kernel<E, 1, true> : token_scan_kernel<E, 1, false>),
+                     gb, dim3(threads), lds, st, g);
   return launch_check("token_scan_kernel");
 }
 
 template <class E>
 int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const int64_t cus = std::max(1, device_cu_count(call.device()));
-  // the channels split among enough workgroups for four a CU, at most eight ways (each
-  // adds its sums' traffic)
+  // the channels split among enough workgroups for four a CU: up to 32 ways where a few
+  // tiles of rows would leave the card empty, else eight (each adds its sums' traffic)
   const int64_t row_tiles = (g.rows + kPtRows - 1) / kPtRows, col_groups = (g.Nc + kPtCols - 1) / kPtCols;
   const int64_t k_steps = (g.Di + kPtK - 1) / kPtK;
-  const int64_t ways = std::max<int64_t>(1, std::min<int64_t>({8, k_steps, 4 * cus / std::max<int64_t>(1, row_tiles * col_groups)}));
+  const int64_t ways = std::max<int64_t>(1, std::min<int64_t>({row_tiles * col_groups * 32 <= cus ? 32 : 8, k_steps, 4 * cus / std::max<int64_t>(1, row_tiles * col_groups)}));
   const int per_split = static_cast<int>((k_steps + ways - 1) / ways) * kPtK;
   g.n_blocks = (g.Di + per_split - 1) / per_split;
   g.Npad = g.N <= 8 ? 8 : g.N <= 16 ? 16 : (g.N + 31) / 32 * 32;
+  g.Rp = (g.R + 15) / 16 * 16;
   // enough chunks for four waves on each SIMD, of 32 tokens at least
   const int64_t waves = (g.Di + kWave - 1) / kWave;
   const int64_t want = std::max<int64_t>(1, 16 * cus / waves);
@@ -924,6 +1016,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   size_t at = 0;
   const auto take = [&](size_t n) { const size_t o = at; at += (n + 63) / 64 * 64; return o; };
   const size_t o_part = take(static_cast<size_t>(g.n_blocks) * g.rows * g.Nc);
+  const size_t o_planes = take((3 * static_cast<size_t>(g.rows) * g.Rp + 1) / 2);
   const size_t o_bc = take(static_cast<size_t>(g.rows) * 2 * g.Npad);
   const size_t o_dt = take(static_cast<size_t>(g.rows) * g.Di);
   const size_t o_local = take(carries ? g.n_chunks * nd : 0);
@@ -937,6 +1030,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   if (int rc = acquire_workspace(call, at * sizeof(float), &ws)) return rc;
   float* f = static_cast<float*>(ws);
   g.part = f + o_part;
+  g.planes = reinterpret_cast<uint16_t*>(f + o_planes);
   g.bc = f + o_bc;
   g.dt = f + o_dt;
   g.local = f + o_local;
@@ -947,15 +1041,19 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.y_sum = f + o_y;
   if (g.rows > 0) {
     const bool k4 = g.K <= 4;
-    hipLaunchKernelGGL(k4 ? (prompt_proj_kernel<E, 4>) : (prompt_proj_kernel<E, 8>),
+    // quads of channels in one load each
+    const bool quads = g.Di % 4 == 0 && g.ld % 4 == 0 && aligned16(g.xz) && aligned16(g.conv_w);
+    hipLaunchKernelGGL(quads ? (k4 ? prompt_proj_kernel<E, 4, true> : prompt_proj_kernel<E, 8, true>)
+                             : (k4 ? prompt_proj_kernel<E, 4, false> : prompt_proj_kernel<E, 8, false>),
                        dim3(static_cast<unsigned>(row_tiles * g.n_blocks * col_groups)), dim3(256), 0, st, g, per_split,
                        vec8(g.x_proj, g.Di));
     if (int rc = launch_check("prompt_proj_kernel")) return rc;
-    const int64_t dt_tiles = (g.rows + kDtRows - 1) / kDtRows, dt_cols = (g.Di + kDtCols - 1) / kDtCols;
-    const int64_t dt_y = std::max<int64_t>(1, std::min<int64_t>(dt_cols, 4 * cus / dt_tiles));
-    const int width = (std::min(g.R, kDtMaxR) + 63) / 64 * 64;
-    hipLaunchKernelGGL(prompt_dt_kernel<E>, dim3(static_cast<unsigned>(dt_tiles), static_cast<unsigned>(dt_y)), dim3(256),
-                       static_cast<size_t>(3) * kDtRows * width * 2, st, g, width, vec8(g.dt_proj, g.R));
+    const int64_t sums = static_cast<int64_t>(g.rows) * (g.Rp + 2 * g.Npad);
+    hipLaunchKernelGGL(prompt_sum_kernel<E>, dim3(static_cast<unsigned>((sums + 255) / 256)), dim3(256), 0, st, g);
+    if (int rc = launch_check("prompt_sum_kernel")) return rc;
+    hipLaunchKernelGGL(prompt_dt_kernel<E>, dim3(static_cast<unsigned>((g.rows + kDtRows - 1) / kDtRows),
+                                                 static_cast<unsigned>((g.Di + kDtCols - 1) / kDtCols)),
+                       dim3(256), 0, st, g, vec8(g.dt_proj, g.R));
     if (int rc = launch_check("prompt_dt_kernel")) return rc;
     if (g.resume != nullptr) {
       g.init = f + o_init;
