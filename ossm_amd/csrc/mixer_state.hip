@@ -667,7 +667,6 @@ __global__ __launch_bounds__(256) void prompt_dt_kernel(Mixer<E> g, bool vec) {
     bias[j] = g.dt_bias[d];
   }
   floatx16 acc[2] = {};
-#pragma unroll 2
   for (int k0 = 0; k0 < g.Rp; k0 += 16) {
     const int k = k0 + half * 8;
     bf16x8 a[3];
@@ -720,28 +719,39 @@ __global__ __launch_bounds__(256) void mixer_gather_kernel(Mixer<E> g) {
 }
 
 constexpr int kScanThreads = 128;
-constexpr int kGroup = 4;  // tokens whose inputs are loaded together
+constexpr int kGroup = 4;   // tokens whose inputs are loaded together
+constexpr int kStage = 32;  // tokens whose B and C are in LDS
 
-// One thread per channel walks a chunk.  NB states in registers (from n_base), KT conv
-// taps (taps before the last K are skipped).  OUT: from the chunk's carry, writing y and
+// One thread per channel walks a chunk, NB states (from n_base) in registers and KT conv
+// taps (those before the last K are skipped).  OUT: from the chunk's carry, writing y and
 // the states of the prompts that end here; else from the last prompt start in the chunk
 // (or a zero carry), leaving the chunk's end and its sum of dt.
+//
+// Bound by the VALU: a token and channel take about 40 instructions, a state 5, one of
+// them an exponential of four issue slots.  B and C, the same for all channels, come from
+// LDS by broadcast reads, a stage of tokens at a time: as scalar loads they were
+// waited for token by token, 0.8 us each where few waves run.
 template <class E, int NB, int KT, bool OUT>
-__global__ __launch_bounds__(kScanThreads) void mixer_scan_kernel(Mixer<E> g, const float* __restrict__ bc, int n_base) {
-  const int d = static_cast<int>(blockIdx.x) * kScanThreads + static_cast<int>(threadIdx.x);
-  if (d >= g.Di) return;
+__global__ __launch_bounds__(kScanThreads, NB <= 16 ? 4 : 2) void mixer_scan_kernel(Mixer<E> g, int n_base) {
+  __shared__ __align__(16) float s_bc[kStage][2 * NB];
+  const int d_own = static_cast<int>(blockIdx.x) * kScanThreads + static_cast<int>(threadIdx.x);
+  const bool live = d_own < g.Di;
+  const int d = min(d_own, g.Di - 1);
   const int c = static_cast<int>(blockIdx.y);
   const int t0 = c * g.chunk, t1 = min(t0 + g.chunk, g.rows);
   const bool last_block = n_base + NB >= g.N;
-  float a2[NB], h[NB], cw[KT], win[KT - 1];
+  float a2[NB], h[NB], cw[KT], win[KT];
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
     a2[i] = n_base + i < g.N ? -expf(g.a_log[static_cast<size_t>(d) * g.N + n_base + i]) * kLog2e : 0.f;
+    h[i] = 0.f;
+  }
   const int skip_taps = KT - g.K;
 #pragma unroll
-  for (int k = 0; k < KT; ++k) cw[k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d) * g.K + k - skip_taps]) : 0.f;
-#pragma unroll
-  for (int i = 0; i < NB; ++i) h[i] = 0.f;
+  for (int k = 0; k < KT; ++k) {
+    cw[k] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d) * g.K + k - skip_taps]) : 0.f;
+    win[k] = 0.f;
+  }
   const float cb = g.conv_b != nullptr ? to_f(g.conv_b[d]) : 0.f;
   const float skip = g.skip != nullptr ? g.skip[d] : 0.f;
 
@@ -749,109 +759,117 @@ __global__ __launch_bounds__(kScanThreads) void mixer_scan_kernel(Mixer<E> g, co
   int t = t0;
   float dt_sum = 0.f;
   if constexpr (!OUT) {
-    if (s < 0) return;  // padding only: the next chunk starts a prompt
+    if (s < 0) return;  // padding only (of the whole workgroup): the next chunk starts a prompt
     const int start = offset_of(g, s);
     if (start >= t0) { t = start; dt_sum = -1.f; }
   }
-  while (t < t1) {
-    // the segment [t, e) of sequence s
-    int e, start = 0, slot = -1;
-    bool inside = false;
-    if (s >= 0 && t < offset_of(g, s + 1)) {
-      inside = true;
-      start = offset_of(g, s);
-      e = min(t1, offset_of(g, s + 1));
-      slot = start_slot(g, s);
-    } else {
-      e = s + 1 < g.n_seqs ? min(t1, max(offset_of(g, s + 1), t + 1)) : t1;  // padding
+  bool begun = false;  // h and the window are sequence s's at t
+#pragma unroll 1
+  for (int b0 = t0; b0 < t1; b0 += kStage) {
+    const int b1 = min(b0 + kStage, t1);
+    if (t >= b1) continue;  // (the same for the whole workgroup)
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kStage * 2 * NB / 4 / kScanThreads + 1; ++q) {
+      const int i = (q * kScanThreads + static_cast<int>(threadIdx.x)) * 4;
+      const int row = i / (2 * NB), k = i % (2 * NB);
+      if (row < kStage && b0 + row < t1) {
+        const float* src = g.bc + static_cast<size_t>(b0 + row) * 2 * g.Npad + n_base + (k < NB ? k : g.Npad + k - NB);
+        *reinterpret_cast<float4*>(&s_bc[row][k]) = *reinterpret_cast<const float4*>(src);
+      }
     }
-    if (!inside) {
-      if constexpr (OUT)
-        if (last_block)
-          for (int i = t; i < e; ++i) g.y[static_cast<size_t>(i) * g.Di + d] = from_f<E>(0.f);
-      t = e;
-    } else {
-      if (t == start) {
-        const float* src = g.init != nullptr ? g.init + (static_cast<size_t>(s) * g.N) * g.Di
-                                             : g.ssm + (static_cast<size_t>(max(slot, 0)) * g.N) * g.Di;
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          h[i] = slot >= 0 && n_base + i < g.N ? src[static_cast<size_t>(n_base + i) * g.Di + d] : 0.f;
+    __syncthreads();
+    while (t < b1) {
+      // the segment [t, e) of sequence s in this stage
+      if (s < 0 || t >= offset_of(g, s + 1)) {  // padding
+        const int e = s + 1 < g.n_seqs ? min(b1, max(offset_of(g, s + 1), t + 1)) : b1;
+        if constexpr (OUT)
+          if (last_block && live)
+            for (int i = t; i < e; ++i) g.y[static_cast<size_t>(i) * g.Di + d] = from_f<E>(0.f);
+        t = e;
       } else {
-        const bool carried = OUT && t == t0 && c > 0;
-        const float* src = g.carry + (static_cast<size_t>(c) * g.N) * g.Di;
+        const int start = offset_of(g, s), end = offset_of(g, s + 1), e = min(b1, end);
+        if (!begun) {
+          begun = true;
+          const int slot = start_slot(g, s);
+          const bool first = t == start, carried = OUT && !first && t == t0 && c > 0;
+          const float* src = first ? (g.init != nullptr ? g.init + (static_cast<size_t>(s) * g.N) * g.Di
+                                                        : g.ssm + (static_cast<size_t>(max(slot, 0)) * g.N) * g.Di)
+                                   : g.carry + (static_cast<size_t>(c) * g.N) * g.Di;
+          const bool any = first ? slot >= 0 : carried;
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-          h[i] = carried && n_base + i < g.N ? src[static_cast<size_t>(n_base + i) * g.Di + d] : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < KT - 1; ++k) {
-        const int pos = t - (KT - 1) + k;
-        win[k] = k >= skip_taps ? conv_input(g, pos, start, slot, d) : 0.f;
-      }
-      for (; t < e; t += kGroup) {
-        float x[kGroup], z[kGroup], dt[kGroup], ys[kGroup];
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {
-          const size_t r = static_cast<size_t>(min(t + i, e - 1));
-          x[i] = to_f(g.xz[r * g.ld + d]);
-          dt[i] = g.dt[r * g.Di + d];
-          if constexpr (OUT) {
-            z[i] = to_f(g.xz[r * g.ld + g.Di + d]);
-            ys[i] = n_base > 0 ? g.y_sum[r * g.Di + d] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {
-          if (t + i >= e) break;
-          // the scalar loads of B and C stay with their token: hoisted over the group they
-          // spill
-          __builtin_amdgcn_sched_barrier(0);
-          const float* B = bc + static_cast<size_t>(t + i) * 2 * g.Npad + n_base;
-          const float* C = B + g.Npad;
-          float p = cb;
+          for (int i = 0; i < NB; ++i)
+            h[i] = any && n_base + i < g.N ? src[static_cast<size_t>(n_base + i) * g.Di + d] : 0.f;
 #pragma unroll
           for (int k = 0; k < KT - 1; ++k)
-            if (k >= skip_taps) p = fmaf(cw[k], win[k], p);
-          p = fmaf(cw[KT - 1], x[i], p);
+            win[k] = k >= skip_taps ? conv_input(g, t - (KT - 1) + k, start, slot, d) : 0.f;
+        }
+#pragma unroll 1
+        for (; t < e; t += kGroup) {
+          float x[kGroup], z[kGroup], dt[kGroup], ys[kGroup];
 #pragma unroll
-          for (int k = 0; k + 1 < KT - 1; ++k) win[k] = win[k + 1];
-          if constexpr (KT > 1) win[KT - 2] = x[i];
-          const float u = silu_f(p);
-          const float du = dt[i] * u;
-          float y = OUT && n_base == 0 ? skip * u : ys[i];
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            const float decay = __builtin_amdgcn_exp2f(a2[n] * dt[i]);
-            h[n] = fmaf(decay, h[n], du * B[n]);
-            if constexpr (OUT) y = fmaf(C[n], h[n], y);
+          for (int i = 0; i < kGroup; ++i) {
+            const size_t r = static_cast<size_t>(min(t + i, e - 1));
+            x[i] = to_f(g.xz[r * g.ld + d]);
+            dt[i] = g.dt[r * g.Di + d];
+            if constexpr (OUT) {
+              z[i] = to_f(g.xz[r * g.ld + g.Di + d]);
+              ys[i] = n_base > 0 ? g.y_sum[r * g.Di + d] : 0.f;
+            }
           }
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            if (t + i >= e) break;
+            __builtin_amdgcn_sched_barrier(0);  // a token's B and C are read with it, not the group's at once
+            const float* B = s_bc[t + i - b0];
+            float p = cb;
+#pragma unroll
+            for (int k = 0; k < KT - 1; ++k)
+              if (k >= skip_taps) p = fmaf(cw[k], win[k], p);
+            p = fmaf(cw[KT - 1], x[i], p);
+#pragma unroll
+            for (int k = 0; k + 1 < KT - 1; ++k) win[k] = win[k + 1];
+            win[KT - 2] = x[i];
+            const float u = silu_f(p);
+            const float du = dt[i] * u;
+            float y = OUT && n_base == 0 ? skip * u : ys[i];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const float decay = __builtin_amdgcn_exp2f(a2[n] * dt[i]);
+              h[n] = fmaf(decay, h[n], du * B[n]);
+              if constexpr (OUT) y = fmaf(B[NB + n], h[n], y);
+            }
+            if constexpr (OUT) {
+              const size_t at = static_cast<size_t>(t + i) * g.Di + d;
+              if (live) {
+                if (last_block) g.y[at] = from_f<E>(y * silu_f(z[i]));
+                else g.y_sum[at] = y;
+              }
+            } else if (dt_sum >= 0.f) {
+              dt_sum += dt[i];
+            }
+          }
+        }
+        t = e;
+        if (e == end) {
+          begun = false;
           if constexpr (OUT) {
-            const size_t at = static_cast<size_t>(t + i) * g.Di + d;
-            if (last_block) g.y[at] = from_f<E>(y * silu_f(z[i]));
-            else g.y_sum[at] = y;
-          } else if (dt_sum >= 0.f) {
-            dt_sum += dt[i];
-          }
-        }
-      }
-      t = e;
-      if constexpr (OUT) {
-        if (e == offset_of(g, s + 1)) {
-          const int to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[s];
-          if (in_pool(g, to)) {
+            const int to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[s];
+            if (in_pool(g, to) && live) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-              if (n_base + i < g.N)
-                g.ssm[(static_cast<size_t>(to) * g.N + n_base + i) * g.Di + d] = h[i];
+              for (int i = 0; i < NB; ++i)
+                if (n_base + i < g.N)
+                  g.ssm[(static_cast<size_t>(to) * g.N + n_base + i) * g.Di + d] = h[i];
+            }
           }
         }
       }
+      // the sequence at t (empty ones are passed by; their states are the finish kernel's)
+      while (s + 1 < g.n_seqs && offset_of(g, s + 1) <= t) ++s;
     }
-    // the sequence at t (empty ones are passed by; their states are the finish kernel's)
-    while (s + 1 < g.n_seqs && offset_of(g, s + 1) <= t) ++s;
   }
   if constexpr (!OUT) {
+    if (!live) return;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       if (n_base + i < g.N) g.local[(static_cast<size_t>(c) * g.N + n_base + i) * g.Di + d] = h[i];
@@ -928,10 +946,18 @@ __global__ __launch_bounds__(256) void mixer_finish_kernel(Mixer<E> g) {
 #pragma unroll
   for (int k = 0; k < kMaxConv - 1; ++k)
     if (k < g.K - 1) g.conv_state[(static_cast<size_t>(to) * (g.K - 1) + k) * g.Di + d] = from_f<E>(x[k]);
-  if (start == end && to != slot)
-    for (int n = 0; n < g.N; ++n)
-      g.ssm[(static_cast<size_t>(to) * g.N + n) * g.Di + d] =
-          slot >= 0 ? g.ssm[(static_cast<size_t>(slot) * g.N + n) * g.Di + d] : 0.f;
+  if (start == end && to != slot) {
+    const float* src = g.ssm + (static_cast<size_t>(max(slot, 0)) * g.N) * g.Di + d;
+    float* dst = g.ssm + (static_cast<size_t>(to) * g.N) * g.Di + d;
+    for (int n0 = 0; n0 < g.N; n0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = slot >= 0 ? src[static_cast<size_t>(min(n0 + i, g.N - 1)) * g.Di] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n0 + i < g.N) dst[static_cast<size_t>(n0 + i) * g.Di] = v[i];
+    }
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -942,9 +968,9 @@ int launch_scan(const Mixer<E>& g, bool out, int n_base, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>((g.Di + kScanThreads - 1) / kScanThreads),
                   static_cast<unsigned>(out ? g.n_chunks : g.n_chunks - 1));
   if (out)
-    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, true>), grid, dim3(kScanThreads), 0, st, g, g.bc, n_base);
+    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, true>), grid, dim3(kScanThreads), 0, st, g, n_base);
   else
-    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, false>), grid, dim3(kScanThreads), 0, st, g, g.bc, n_base);
+    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, false>), grid, dim3(kScanThreads), 0, st, g, n_base);
   return launch_check("mixer_scan_kernel");
 }
 
@@ -1004,12 +1030,15 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.n_blocks = (g.Di + per_split - 1) / per_split;
   g.Npad = g.N <= 8 ? 8 : g.N <= 16 ? 16 : (g.N + 31) / 32 * 32;
   g.Rp = (g.R + 15) / 16 * 16;
-  // enough chunks for four waves on each SIMD, of 32 tokens at least
+  // enough chunks for four waves on each SIMD, of 16 tokens at least
   const int64_t waves = (g.Di + kWave - 1) / kWave;
   const int64_t want = std::max<int64_t>(1, 16 * cus / waves);
-  g.chunk = static_cast<int>(std::max<int64_t>({32, (g.rows + want - 1) / want, (g.rows + 65534) / 65535}));
+  g.chunk = static_cast<int>(std::max<int64_t>({16, (g.rows + want - 1) / want, (g.rows + 65534) / 65535}));
   g.n_chunks = (g.rows + g.chunk - 1) / g.chunk;
-  g.group = 16;
+  // groups of about the square root of the chunks: as many steps through the groups as
+  // through one's chunks
+  g.group = 8;
+  while (g.group * g.group < g.n_chunks) g.group += 8;
   g.n_groups = std::max(1, (g.n_chunks + g.group - 1) / g.group);
   const size_t nd = static_cast<size_t>(g.N) * g.Di;
   const bool carries = g.n_chunks > 1;
