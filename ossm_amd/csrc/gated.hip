@@ -43,7 +43,6 @@
 namespace ossm {
 namespace {
 
-constexpr int kTk = 64;           // k of a tile
 constexpr int kOutside = 0x7ffffff0;  // a buffer offset past every range: the load gives zeros
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -118,50 +117,61 @@ __device__ __forceinline__ int plane_b(int combo) { return (0x010210 >> (4 * com
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-// One operand's tile of R rows (of m or n) and kTk k, from element (i0, k0), into LDS.  An LDS
-// row is 64 k (row) or R columns (col) of 16-byte chunks; chunk c sits at c ^ (i % 8)
-// (row) or c ^ 4 (k % 4) (col), which spreads the fragments' reads over the banks.
-template <bool COL, int R, int THREADS>
-__device__ __forceinline__ void load_tile(uint16_t* lds, const uint16_t* p, long long ld, int i0, int rows, int k0,
-                                          int K) {
-  const int tid = static_cast<int>(threadIdx.x), w = wave_id();
-  constexpr int kRounds = R * (kTk / 8) / THREADS;
-  if constexpr (!COL) {
-    const int n = min(rows - i0, R);  // may be <= 0: every chunk is outside
-    const uint16_t* base = p + (n > 0 ? static_cast<long long>(i0) * ld + k0 : 0);
-    const int bytes = n > 0 ? static_cast<int>(((n - 1) * ld + ((K - k0 + 7) & ~7)) * 2) : 0;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, bytes, 0x00027000);
-    const int c = (tid & 7) ^ ((tid >> 3) & 7);
-    const bool in = k0 + c * 8 < K;
+// What the chunks of LDS row r of a row operand are turned by: eight neighbouring rows then
+// put a k in eight places.
+template <int TK>
+__device__ __forceinline__ int row_turn(int r) { return TK == 64 ? r & 7 : (r >> 1) & 3; }
+
+// One operand's tiles of R rows (of m or n) and TK k into LDS.  An LDS row is TK k (row) or R
+// columns (col) of 16-byte chunks; chunk c sits at c ^ row_turn (row) or c ^ 4 (k % 4)
+// (col), which spreads the fragments' reads over the banks.  A thread's chunks are the same
+// in every tile, so their offsets are kept; chunks of rows past the matrix have one
+// that the buffer's range turns into zeros, and the last tile of k masks its own.
+template <bool COL, int R, int TK, int THREADS>
+struct TileLoad {
+  static constexpr int kRounds = R * (TK / 8) / THREADS, kChunks = R / 8;
+  static constexpr int kRange = 0x40000000;  // every offset in a matrix is below it: 256 rows of 2^21 bytes
+  int off[kRounds];
+
+  // the chunk of its row that a thread's place in LDS holds (THREADS / 4 rows on: the same)
+  static __device__ __forceinline__ int row_chunk() {
+    const int tid = static_cast<int>(threadIdx.x);
+    return (tid % (TK / 8)) ^ row_turn<TK>(tid / (TK / 8));
+  }
+
+  __device__ __forceinline__ void init(long long ld, int i0, int rows) {
+    const int tid = static_cast<int>(threadIdx.x);
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
-      const int r = (tid >> 3) + i * (THREADS / 8);
-      const int off = in && r < n ? static_cast<int>(r * ld * 2) + c * 16 : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * THREADS + w * kWave) * 8), 16, off, 0, 0, 0);
-    }
-  } else {
-    constexpr int kChunks = R / 8;
-    const int n = min(K - k0, kTk), cols = rows - i0;
-    const uint16_t* base = p + (cols > 0 ? static_cast<long long>(k0) * ld + i0 : 0);
-    const int bytes = cols > 0 ? static_cast<int>(((n - 1) * ld + ((min(cols, R) + 7) & ~7)) * 2) : 0;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, bytes, 0x00027000);
-#pragma unroll
-    for (int i = 0; i < kRounds; ++i) {
-      const int q = i * THREADS + tid, k = q / kChunks, c = (q % kChunks) ^ (4 * (k & 3));
-      const int off = k < n && c * 8 < cols ? static_cast<int>(k * ld * 2) + c * 16 : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * THREADS + w * kWave) * 8), 16, off, 0, 0, 0);
+      const int q = i * THREADS + tid;
+      if constexpr (!COL) {
+        const int r = q / (TK / 8), c = row_chunk();
+        off[i] = i0 + r < rows ? static_cast<int>(r * ld * 2) + c * 16 : kOutside;
+      } else {
+        const int k = q / kChunks, c = (q % kChunks) ^ (4 * (k & 3));
+        off[i] = i0 + c * 8 < rows ? static_cast<int>(k * ld * 2) + c * 16 : kOutside;
+      }
     }
   }
-}
+
+  // round i of the tile at p, `left` k of it
+  __device__ __forceinline__ void load(int i, uint16_t* lds, const uint16_t* p, int left) const {
+    const int tid = static_cast<int>(threadIdx.x);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, kRange, 0x00027000);
+    const int k = COL ? (i * THREADS + tid) / kChunks : row_chunk() * 8;
+    const int o = k < left ? off[i] : kOutside;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (i * THREADS + wave_id() * kWave) * 8), 16, o, 0, 0, 0);
+  }
+};
 
 // The wave's fragment of 32 rows from i0 at k step kk (16 k) of a tile in LDS: lane l
 // holds row l % 32 at k = 8 (l / 32) .. + 7.
-template <bool COL, int R>
+template <bool COL, int R, int TK>
 __device__ __forceinline__ bf16x8 load_frag(const uint16_t* lds, int i0, int kk) {
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   if constexpr (!COL) {
     const int r = i0 + (lane & 31), c = kk * 2 + (lane >> 5);
-    return *reinterpret_cast<const bf16x8*>(lds + r * kTk + ((c ^ (r & 7)) * 8));
+    return *reinterpret_cast<const bf16x8*>(lds + r * TK + ((c ^ row_turn<TK>(r)) * 8));
   } else {
     // a group of 16 lanes reads 4 k of 16 columns, transposed: lane i gets column i
     const int g = lane >> 4, i16 = lane & 15, kr = i16 >> 2;
@@ -182,15 +192,46 @@ __device__ __forceinline__ float element(const Operand& o, int part, int i, int 
   return (to_f(bf16_t{p[2 * o.plane]}) + to_f(bf16_t{p[o.plane]})) + to_f(bf16_t{p[0]});
 }
 
+// Lays out a stretch of instructions: COUNT of a kind (0x100 LDS reads, 0x20 loads) spread
+// over MFMA matrix instructions.
+template <int KIND, int COUNT, int MFMA, int I = 0>
+__device__ __forceinline__ void interleave() {
+  constexpr int kGroups = COUNT < MFMA ? COUNT : MFMA;
+  if constexpr (I < kGroups) {
+    constexpr int kOfKind = (I + 1) * COUNT / kGroups - I * COUNT / kGroups;
+    constexpr int kOfMfma = (I + 1) * MFMA / kGroups - I * MFMA / kGroups;
+    __builtin_amdgcn_sched_group_barrier(KIND, kOfKind, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, kOfMfma, 0);
+    interleave<KIND, COUNT, MFMA, I + 1>();
+  }
+}
+
+// A tile's k and how many tiles LDS holds (one is read, the others are on their way): 64 and
+// two where both operands are rows (whole 128-byte lines of each), 32 and three where one
+// is not.  Both ways at [8192, 2048] -> 8192 in bf16, us: forward 480 and 520, dx 580 and
+// 488, dW 584 and 553.
+constexpr int tile_k(bool gated) { return gated ? 64 : 32; }
+constexpr int tile_stages(bool gated) { return gated ? 2 : 3; }
+
 // Workgroup tile: WM x WN waves of FM x FN fragments of 32 x 32.  GATED: the tile's
 // columns are 32-column pairs, gate and up rows of the same outputs (N counts outputs).
+//
+// Bound by the matrix cores and the loads into LDS, which share the waves: 256 x 256 tiles
+// take 128 bytes from L2 for 32 k of 4096 matrix cycles; alone the products of dx above take
+// 383 us (1.43 PFLOP/s) and the loads 399, together 488.  Eight waves of 4 x 2
+// fragments, two to a SIMD, since a wave that waits to issue a load issues no products: four
+// of 4 x 4, with less LDS traffic, took 612.  Hence also the loads a few at a time between
+// the products, a step's last fragments in registers before its barrier, and the next
+// step's first ones read under the last products.
 template <class E, bool ACOL, bool BCOL, bool GATED, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> g) {
+  constexpr int TK = tile_k(GATED), kStages = tile_stages(GATED);
   constexpr int THREADS = WM * WN * kWave, TM = WM * FM * 32, TN = WN * FN * 32;
   constexpr int NOUT = GATED ? TN / 2 : TN;  // output columns of a tile
-  static_assert(!GATED || (FN == 2 && !BCOL), "a wave holds 32 gate and 32 up columns");
-  extern __shared__ __align__(16) uint16_t s_tiles[];  // two buffers of (A, B)
-  constexpr int kA = TM * kTk, kBuf = (TM + TN) * kTk;
+  constexpr int HN = FN / 2;                 // gated: fragments of each kind
+  static_assert(!GATED || (FN % 2 == 0 && !BCOL), "a wave holds gate and up columns");
+  extern __shared__ __align__(16) uint16_t s_tiles[];  // kStages buffers of (A, B)
+  constexpr int kA = TM * TK, kBuf = (TM + TN) * TK;
   const int w = wave_id(), wm = w / WN, wn = w % WN;
 
   // consecutive ids share an XCD; bands of 8 tile rows keep their operands in its L2
@@ -203,21 +244,66 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
   const int m0 = (first + (id - band * 8 * g.tiles_n) % in_band) * TM;
   const int n0 = (id - band * 8 * g.tiles_n) / in_band * NOUT;
 
-  const int k_tiles = (g.K + kTk - 1) / kTk;
+  const int k_tiles = max(1, (g.K + TK - 1) / TK);
   const int kt0 = split * g.per_split, kt1 = min(kt0 + g.per_split, k_tiles);
   const int steps = (kt1 - kt0) * g.parts * g.combos;
 
-  const auto load = [&](int step, int buf) {
-    const int seg = step / (kt1 - kt0), k0 = (kt0 + step % (kt1 - kt0)) * kTk;
-    const int combo = seg / g.parts, part = seg % g.parts;
+  TileLoad<ACOL, TM, TK, THREADS> load_a;
+  TileLoad<BCOL, GATED ? TN / 2 : TN, TK, THREADS> load_b;
+  load_a.init(g.a.ld, m0, g.M);
+  load_b.init(g.b.ld, n0, g.N);
+  // where the next tile's elements (m0, k) and (n0, k) are, and how much k is left of its
+  // stretch (none past the last: zeros, unread)
+  int next_kt = kt0, part = 0, combo = 0, left = 0;
+  const uint16_t *pa, *pb[2];
+  const auto stretch = [&] {
+    const int k0 = next_kt * TK;
+    left = combo < g.combos ? g.K - k0 : 0;
+    const int c = combo < g.combos && g.combos > 1 ? combo : 5;  // 5: the first planes
+    const long long qa = plane_a(c) * g.a.plane + (ACOL ? m0 + k0 * g.a.ld : m0 * g.a.ld + k0);
+    const long long qb = plane_b(c) * g.b.plane + (BCOL ? n0 + k0 * g.b.ld : n0 * g.b.ld + k0);
+    pa = g.a.p[part] + qa;
+    pb[0] = g.b.p[GATED ? 0 : part] + qb;
+    pb[1] = GATED ? g.b.p[1] + qb : nullptr;
+  };
+  stretch();
+  const long long step_a = ACOL ? TK * g.a.ld : TK, step_b = BCOL ? TK * g.b.ld : TK;
+  constexpr int kRa = decltype(load_a)::kRounds, kRb = decltype(load_b)::kRounds;
+  constexpr int kLoads = kRa + (GATED ? 2 : 1) * kRb;
+  // loads q0 .. q1 - 1 of the next tile; the tile after it once all are asked for
+  const auto load = [&](int buf, int q0, int q1) {
     uint16_t* s = s_tiles + buf * kBuf;
-    const long long pa = (g.combos > 1 ? plane_a(combo) : 0) * g.a.plane, pb = (g.combos > 1 ? plane_b(combo) : 0) * g.b.plane;
-    load_tile<ACOL, TM, THREADS>(s, g.a.p[part] + pa, g.a.ld, m0, g.M, k0, g.K);
-    if constexpr (GATED) {
-      load_tile<BCOL, TN / 2, THREADS>(s + kA, g.b.p[0] + pb, g.b.ld, n0, g.N, k0, g.K);
-      load_tile<BCOL, TN / 2, THREADS>(s + kA + TN / 2 * kTk, g.b.p[1] + pb, g.b.ld, n0, g.N, k0, g.K);
+#pragma unroll
+    for (int q = q0; q < q1; ++q) {
+      if (q < kRa) load_a.load(q, s, pa, left);
+      else if (q < kRa + kRb) load_b.load(q - kRa, s + kA, pb[0], left);
+      else load_b.load(q - kRa - kRb, s + kA + TN / 2 * TK, pb[1], left);
+    }
+  };
+  const auto advance = [&] {
+    if (++next_kt == kt1) {
+      next_kt = kt0;
+      if (++part == g.parts) { part = 0; ++combo; }
+      stretch();
     } else {
-      load_tile<BCOL, TN, THREADS>(s + kA, g.b.p[part] + pb, g.b.ld, n0, g.N, k0, g.K);
+      left -= TK;
+      pa += step_a;
+      pb[0] += step_b;
+      if constexpr (GATED) pb[1] += step_b;
+    }
+  };
+  bf16x8 fa[2][FM], fb[2][FN];
+  const auto fragments = [&](int buf, int kk, int set) {
+    const uint16_t* sa = s_tiles + buf * kBuf;
+    const uint16_t* sb = sa + kA;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[set][i] = load_frag<ACOL, TM, TK>(sa, wm * FM * 32 + i * 32, kk);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      if constexpr (GATED)  // two tiles of TN / 2 rows, one after the other
+        fb[set][j] = load_frag<false, TN / 2, TK>(sb + (j / HN) * (TN / 2) * TK, wn * HN * 32 + (j % HN) * 32, kk);
+      else
+        fb[set][j] = load_frag<BCOL, TN, TK>(sb, wn * FN * 32 + j * 32, kk);
     }
   };
 
@@ -228,33 +314,64 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-  if (steps > 0) load(0, 0);
-  for (int step = 0; step < steps; ++step) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the tile has arrived
-    __syncthreads();  // everyone's has, and everyone is done with the other buffer
-    if (step + 1 < steps) load(step + 1, (step + 1) & 1);
-    const uint16_t* sa = s_tiles + (step & 1) * kBuf;
-    const uint16_t* sb = sa + kA;
+  const auto products = [&](int set) {
 #pragma unroll
-    for (int kk = 0; kk < kTk / 16; ++kk) {
-      bf16x8 fa[FM], fb[FN];
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = load_frag<ACOL, TM>(sa, wm * FM * 32 + i * 32, kk);
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fb[j] = load_frag<BCOL, TN>(sb, GATED ? j * (TN / 2) + wn * 32 : wn * FN * 32 + j * 32, kk);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_bf16(fa[i], fb[j], acc[i][j]);
-    }
+      for (int j = 0; j < FN; ++j) acc[i][j] = mfma_bf16(fa[set][i], fb[set][j], acc[i][j]);
+  };
+  // how a stretch of the loop is laid out: a products' share after every read or load
+  constexpr int kReads = (ACOL ? 2 : 1) * FM + (BCOL ? 2 : 1) * FN;  // LDS reads of a fragment set
+  constexpr int kMfma = FM * FN;
+  constexpr int kSteps = TK / 16;
+  static_assert(kSteps % 2 == 0 && kLoads * (kStages - 1) < 64, "an even number of k steps; loads in flight are counted in 6 bits");
+  // this wave's share of the oldest tile on its way has landed and its LDS reads so far
+  // have come back, then everyone's
+  const auto arrive = [&] {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads * (kStages - 2)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  for (int i = 0; i + 1 < kStages; ++i) {
+    load(i, 0, kLoads);
+    advance();
   }
+  arrive();
+  // a tile's loads are spread over its predecessor's steps, the first after its barrier
+  constexpr int kEarly = kLoads / kSteps;
+  load(kStages - 1, 0, kEarly);
+  fragments(0, 0, 0);
+  int buf = 0, last = kStages - 1;  // the tile read, the one whose loads are partly asked for
+  for (int step = 0; step < steps; ++step) {
+    const int next = buf + 1 == kStages ? 0 : buf + 1;
+#pragma unroll
+    for (int kk = 0; kk < kSteps - 1; ++kk) {
+      fragments(buf, kk + 1, (kk + 1) & 1);
+      load(last, kEarly + kk * (kLoads - kEarly) / (kSteps - 1), kEarly + (kk + 1) * (kLoads - kEarly) / (kSteps - 1));
+      __builtin_amdgcn_s_setprio(1);
+      products(kk & 1);
+      __builtin_amdgcn_s_setprio(0);
+      interleave<0x100, kReads, kMfma / 2>();
+      interleave<0x020, (kLoads - kEarly) / (kSteps - 1), kMfma - kMfma / 2>();
+    }
+    advance();
+    arrive();
+    fragments(next, 0, 0);
+    load(buf, 0, kEarly);
+    __builtin_amdgcn_s_setprio(1);
+    products(1);
+    __builtin_amdgcn_s_setprio(0);
+    interleave<0x100, kReads, kMfma / 2>();
+    interleave<0x020, kEarly, kMfma - kMfma / 2>();
+    last = buf;
+    buf = next;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into LDS at the end
 
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
   if constexpr (sizeof(E) == 4) {
     // the elements of a fragment that are not finite
-    const int k_end = min(kt1 * kTk, g.K);
+    const int k_end = min(kt1 * TK, g.K);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -264,9 +381,9 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
           floatx16 c = {};
           for (int part = 0; part < g.parts; ++part)
 #pragma unroll 1
-            for (int k = kt0 * kTk; k < k_end; k += 2) {
+            for (int k = kt0 * TK; k < k_end; k += 2) {
               const float va = element<ACOL>(g.a, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
-              const float vb = GATED ? element<BCOL>(g.b, j, n0 + wn * 32 + l32, g.N, k + half, k_end)
+              const float vb = GATED ? element<BCOL>(g.b, j / HN, n0 + wn * HN * 32 + (j % HN) * 32 + l32, g.N, k + half, k_end)
                                      : element<BCOL>(g.b, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
               c = mfma32(va, vb, c);
             }
@@ -279,25 +396,28 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
 
   // register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
   if constexpr (GATED) {
-    const int n = n0 + wn * 32 + l32;
-    const bool in = n < g.N;
-    const float bg = in && g.bias[0] != nullptr ? to_f(g.bias[0][n]) : 0.f;
-    const float bu = in && g.bias[1] != nullptr ? to_f(g.bias[1][n]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < HN; ++j) {
+      const int n = n0 + wn * HN * 32 + j * 32 + l32;
+      const bool in = n < g.N;
+      const float bg = in && g.bias[0] != nullptr ? to_f(g.bias[0][n]) : 0.f;
+      const float bu = in && g.bias[1] != nullptr ? to_f(g.bias[1][n]) : 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int m = m0 + wm * FM * 32 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        const float a = acc[i][0][r] + bg, b = acc[i][1][r] + bu;
-        if (in && m < g.M) {
-          const long long at = m * g.ldc + n;
-          g.c[0][at] = from_f<E>(activation_of(g.act, a) * b);
-          if (g.save[0] != nullptr) {
-            g.save[0][at] = a;
-            g.save[1][at] = b;
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + wm * FM * 32 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          const float a = acc[i][j][r] + bg, b = acc[i][j + HN][r] + bu;
+          if (in && m < g.M) {
+            const long long at = m * g.ldc + n;
+            g.c[0][at] = from_f<E>(activation_of(g.act, a) * b);
+            if (g.save[0] != nullptr) {
+              g.save[0][at] = a;
+              g.save[1][at] = b;
+            }
           }
         }
-      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -524,7 +644,7 @@ int pack(const Source<E>& m, uint16_t* ws, Operand* o, hipStream_t st) {
 template <class E, bool ACOL, bool BCOL, bool GATED, int WM, int WN, int FM, int FN>
 int launch_tiled(Product<E> g, hipStream_t st) {
   constexpr int TM = WM * FM * 32, TN = WN * FN * 32;
-  constexpr int lds = 2 * (TM + TN) * kTk * 2;
+  constexpr int lds = tile_stages(GATED) * (TM + TN) * tile_k(GATED) * 2;
   g.tiles_m = (g.M + TM - 1) / TM;
   g.tiles_n = (g.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
   const int64_t grid = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
@@ -546,7 +666,7 @@ int launch_tiled(Product<E> g, hipStream_t st) {
 int64_t tiles(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 
 // How many ways the k of an [M, N] product of `k_tiles` tiles is split: towards two
-// workgroups a CU, none with fewer than 8 tiles.
+// workgroups a CU, none with fewer than 16 tiles.
 int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t cus) {
   const int64_t t = std::max<int64_t>(1, tiles(m, n, 128, 128));  // an input without columns has none
   return static_cast<int>(std::max<int64_t>(1, std::min(2 * cus / t, k_tiles / 8)));
@@ -554,7 +674,7 @@ int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t cus) {
 
 template <class E, bool ACOL, bool BCOL, bool GATED>
 int launch_product(Product<E> g, int64_t cus, hipStream_t st) {
-  const int k_tiles = std::max(1, (g.K + kTk - 1) / kTk);
+  const int k_tiles = std::max(1, (g.K + tile_k(GATED) - 1) / tile_k(GATED));
   g.per_split = (k_tiles + g.splits - 1) / g.splits;
   g.splits = (k_tiles + g.per_split - 1) / g.per_split;
   if (g.splits == 1 && tiles(g.M, g.N, 256, GATED ? 128 : 256) >= cus)
@@ -621,8 +741,8 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   const int64_t dab_plane = p.T * 2 * Fp, rbs = (p.T + kRowsPer - 1) / kRowsPer;
   const int64_t cus = std::max(1, device_cu_count(call.device()));
   const bool want_w = gw[0] != nullptr || gw[1] != nullptr, want_b = gb[0] != nullptr || gb[1] != nullptr;
-  const int sx = choose_splits(p.T, p.D, (p.F + kTk - 1) / kTk, cus);
-  const int sw = choose_splits(2 * Fp, p.D, (p.T + kTk - 1) / kTk, cus);
+  const int sx = choose_splits(p.T, p.D, p.F / tile_k(false), cus);
+  const int sw = choose_splits(2 * Fp, p.D, p.T / tile_k(false), cus);
   const int64_t part = std::max<int64_t>(gx != nullptr && sx > 1 ? sx * p.T * p.D : 0, want_w && sw > 1 ? sw * 2 * Fp * p.D : 0);
   // bytes; every start a multiple of 16
   size_t at = 0;

@@ -877,7 +877,7 @@ __global__ __launch_bounds__(kScanThreads, NB <= 16 ? 4 : 2) void mixer_scan_ker
   }
 }
 
-constexpr int kCarryAhead = 8;  // chunks whose summaries are loaded together
+constexpr int kCarryAhead = 16;  // chunks whose summaries are loaded together
 
 // h through `n` summaries from index c0: h = exp(A sum_dt) h + local (local alone where a
 // prompt starts inside); put(c, h) sees the state before each.
