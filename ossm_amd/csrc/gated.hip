@@ -33,6 +33,7 @@
 #include <initializer_list>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #include "../../include/ossm_lm.h"
 #include "lm_types.hpp"
@@ -451,6 +452,122 @@ __global__ __launch_bounds__(256) void product_sum_kernel(Product<E> g) {
   g.c[second][row * g.ldc + col] = from_f<E>(s);
 }
 
+// ---- few rows ---------------------------------------------------------------------
+// Up to 32 NT rows of x: the weights' traffic is all there is (9.4 us for two of [5632, 2048]
+// in bf16), so each is read once, straight into fragments, and none goes through LDS.  A
+// workgroup takes 16 outputs, whose gate rows are rows 0-15 of a fragment and whose up rows
+// 16-31: a lane then holds a and b of an output 8 registers apart.  Its waves share k in
+// blocks of 64 (a lane reads 64 consecutive bytes in bf16) and add their sums in LDS in a
+// fixed order.  float32 takes the fp32 matrix instruction: nothing to split, and its rate
+// is above the memory's.
+constexpr int kRowWaves = 8, kRowOut = 16;
+
+template <class E>
+struct Frag8;
+template <>
+struct Frag8<bf16_t> {
+  bf16x8 v;
+  __device__ __forceinline__ void load(const bf16_t* row, int k, int n, bool vec) {
+    if (vec) {
+      v = k < n ? *reinterpret_cast<const bf16x8*>(row + k) : bf16x8{};  // n is a multiple of 8
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(__bf16, k + i < n ? row[k + i].bits : static_cast<uint16_t>(0));
+    }
+  }
+};
+template <>
+struct Frag8<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* row, int k, int n, bool vec) {
+    if (vec) {
+      const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 a = k < n ? reinterpret_cast<const float4*>(row + k)[0] : z;  // n is a multiple of 8
+      const float4 b = k < n ? reinterpret_cast<const float4*>(row + k)[1] : z;
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = k + i < n ? row[k + i] : 0.f;
+    }
+  }
+};
+__device__ __forceinline__ floatx16 mfma8(const Frag8<bf16_t>& a, const Frag8<bf16_t>& b, floatx16 c) { return mfma_bf16(a.v, b.v, c); }
+__device__ __forceinline__ floatx16 mfma8(const Frag8<float>& a, const Frag8<float>& b, floatx16 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = mfma32(a.v[i], b.v[i], c);
+  return c;
+}
+
+template <class E>
+struct FewRows {
+  const E* x;
+  const E* w[2];
+  const E* bias[2];
+  E* y;
+  float* save[2];
+  long long ld_x, ld_w[2];
+  int T, D, F, act;
+};
+
+template <class E, int NT>
+__global__ __launch_bounds__(kRowWaves * kWave, 2) void few_rows_kernel(FewRows<E> g, bool vec) {
+  __shared__ float s_sum[kRowWaves][NT][32 * 32];
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), w = wave_id(), l32 = lane & 31, half = lane >> 5;
+  const int f0 = static_cast<int>(blockIdx.x) * kRowOut;
+  const int f = min(f0 + (l32 & 15), g.F - 1), up = l32 >> 4;
+  const E* row_w = g.w[up] + f * g.ld_w[up];
+  const E* row_x[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) row_x[t] = g.x + min(t * 32 + l32, g.T - 1) * g.ld_x;
+  floatx16 acc[NT] = {};
+  const int blocks = (g.D + 63) / 64;
+  constexpr int kAhead = NT == 1 && sizeof(E) == 2 ? 4 : 1;  // blocks whose fragments are asked for together
+  for (int b0 = w; b0 < blocks; b0 += kRowWaves * kAhead) {
+    Frag8<E> fw[kAhead][4], fx[kAhead][4][NT];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = (b0 + q * kRowWaves) * 64 + half * 32 + i * 8;  // past D: zeros
+        fw[q][i].load(row_w, k, g.D, vec);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fx[q][i][t].load(row_x[t], k, g.D, vec);
+      }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = mfma8(fw[q][i], fx[q][i][t], acc[t]);
+  }
+  // row m (output) of token l32: register r holds m = 8 (r / 4) + 4 half + r % 4
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_sum[w][t][(8 * (r >> 2) + 4 * half + (r & 3)) * 32 + l32] = acc[t][r];
+  __syncthreads();
+  // outputs fastest, so that neighbouring lanes store neighbouring values
+  for (int i = threadIdx.x; i < NT * 32 * kRowOut; i += kRowWaves * kWave) {
+    const int m = i % kRowOut, token = i / kRowOut, t = token >> 5, l = token & 31, n = f0 + m;
+    if (token >= g.T || n >= g.F) continue;
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int v = 0; v < kRowWaves; ++v) {
+      a += s_sum[v][t][m * 32 + l];
+      b += s_sum[v][t][(m + 16) * 32 + l];
+    }
+    if (g.bias[0] != nullptr) a += to_f(g.bias[0][n]);
+    if (g.bias[1] != nullptr) b += to_f(g.bias[1][n]);
+    const long long at = static_cast<long long>(token) * g.F + n;
+    g.y[at] = from_f<E>(activation_of(g.act, a) * b);
+    if (g.save[0] != nullptr) {
+      g.save[0][at] = a;
+      g.save[1][at] = b;
+    }
+  }
+}
+
 // ---- operands as bf16 planes ---------------------------------------------------
 // x as the nearest bf16s of it and of what they leave; what is not finite as (x, 0, 0).
 __device__ __forceinline__ void split3(float x, uint16_t (&t)[3]) {
@@ -578,21 +695,30 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go
   }
 }
 
-// Column sums of [rows][2 Fp] in a fixed order: 64 columns, 4 lanes of rows each.
+// Column sums of [rows][2 Fp] in a fixed order, kBiasRows rows a workgroup: 64 columns, 4
+// lanes of rows each.  With more rows than that their sums go to `next` for another pass, else
+// to the gradients.
+constexpr int kBiasRows = 128;
+
 template <class E>
-__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int rows, int F, int Fp, E* ga,
-                                                        E* gb) {
+__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int rows, int F, int Fp,
+                                                        float* __restrict__ next, E* ga, E* gb) {
   __shared__ float s_p[4][kWave];
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), w = wave_id();
   const int c = static_cast<int>(blockIdx.x) * kWave + lane;
+  const int r0 = static_cast<int>(blockIdx.y) * kBiasRows, r1 = min(rows, r0 + kBiasRows);
   float s = 0.f;
   if (c < 2 * Fp)
-#pragma unroll 8
-    for (int r = w; r < rows; r += 4) s += sums[static_cast<long long>(r) * 2 * Fp + c];
+#pragma unroll 16
+    for (int r = r0 + w; r < r1; r += 4) s += sums[static_cast<long long>(r) * 2 * Fp + c];
   s_p[w][lane] = s;
   __syncthreads();
   if (w != 0 || c >= 2 * Fp) return;
   s = ((s_p[0][lane] + s_p[1][lane]) + s_p[2][lane]) + s_p[3][lane];
+  if (next != nullptr) {
+    next[static_cast<long long>(blockIdx.y) * 2 * Fp + c] = s;
+    return;
+  }
   E* out = c < Fp ? ga : gb;
   const int f = c < Fp ? c : c - Fp;
   if (f < F && out != nullptr) out[f] = from_f<E>(s);
@@ -709,8 +835,25 @@ struct Gated {
   Source<E> weights() const { return {{w[0], w[1]}, {ld_w[0], ld_w[1]}, F, D, 2}; }
 };
 
+// Rows up to which the weights' traffic bounds the forward and few_rows_kernel takes it.
+constexpr int64_t kFewRows = 64;
+
+template <class E>
+int few_rows(const Gated<E>& p, E* y, float* a, float* b, hipStream_t st) {
+  const FewRows<E> g{p.x, {p.w[0], p.w[1]}, {p.bias[0], p.bias[1]}, y, {a, b}, p.ld_x, {p.ld_w[0], p.ld_w[1]},
+                     static_cast<int>(p.T), static_cast<int>(p.D), static_cast<int>(p.F), p.act};
+  constexpr int e = sizeof(E);
+  const bool vec = p.D % 8 == 0 && aligned16(p.x) && aligned16(p.w[0]) && aligned16(p.w[1]) && p.ld_x * e % 16 == 0 &&
+                   p.ld_w[0] * e % 16 == 0 && p.ld_w[1] * e % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((p.F + kRowOut - 1) / kRowOut));
+  if (p.T <= 32) hipLaunchKernelGGL((few_rows_kernel<E, 1>), grid, dim3(kRowWaves * kWave), 0, st, g, vec);
+  else hipLaunchKernelGGL((few_rows_kernel<E, 2>), grid, dim3(kRowWaves * kWave), 0, st, g, vec);
+  return launch_check("few_rows_kernel");
+}
+
 template <class E>
 int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipStream_t st) {
+  if (p.T <= kFewRows) return few_rows(p, y, a, b, st);
   const Source<E> px = p.rows(), pw = p.weights();
   void* ws = nullptr;
   if (px.elems() + pw.elems() > 0)
@@ -749,7 +892,7 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   const auto take = [&](int64_t bytes) { const size_t o = at; at += static_cast<size_t>((bytes + 255) / 256 * 256); return o; };
   const size_t o_dab = take(dab_plane * planes * 2), o_x = take(want_w ? px.elems() * 2 : 0);
   const size_t o_w = take(gx != nullptr ? pw.elems() * 2 : 0), o_part = take(part * 4);
-  const size_t o_sums = take(want_b ? rbs * 2 * Fp * 4 : 0);
+  const size_t o_sums = take(want_b ? (rbs + (rbs + kBiasRows - 1) / kBiasRows) * 2 * Fp * 4 : 0);
   void* ws = nullptr;
   if (int rc = acquire_workspace(call, at, &ws)) return rc;
   char* base = static_cast<char*>(ws);
@@ -775,9 +918,19 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   };
   if (int rc = by_act()) return rc;
   if (want_b) {
-    hipLaunchKernelGGL(bias_grad_kernel<E>, dim3(static_cast<unsigned>((2 * Fp + kWave - 1) / kWave)), dim3(256), 0, st,
-                       static_cast<const float*>(sums), static_cast<int>(rbs), F, fp, gb[0], gb[1]);
-    if (int rc = launch_check("bias_grad_kernel")) return rc;
+    // the sums shrink 128 rows to one a pass; the passes alternate between two stretches
+    float* from = sums;
+    float* to = sums + rbs * 2 * Fp;
+    for (int64_t rows = rbs;;) {
+      const int64_t groups = (rows + kBiasRows - 1) / kBiasRows;
+      hipLaunchKernelGGL(bias_grad_kernel<E>, dim3(static_cast<unsigned>((2 * Fp + kWave - 1) / kWave), static_cast<unsigned>(groups)),
+                         dim3(256), 0, st, static_cast<const float*>(from), static_cast<int>(rows), F, fp,
+                         groups > 1 ? to : nullptr, gb[0], gb[1]);
+      if (int rc = launch_check("bias_grad_kernel")) return rc;
+      if (groups == 1) break;
+      std::swap(from, to);
+      rows = groups;
+    }
   }
   Product<E> g{};
   g.combos = kCombos(sizeof(E));

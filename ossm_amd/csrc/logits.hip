@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 8192;  // vocabulary entries of a workgroup
-constexpr int kAhead = 8;     // history loads in flight a thread
+constexpr int kAhead = 16;    // history loads in flight a thread
 
 // An entry's word in LDS.  Narrow: bias index + 1 in the upper half, set first (the
 // largest wins), then the mark of one seen at all and the count; it serves
@@ -81,6 +81,15 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   const bool same = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(E) % W) == shift;
   const int v0 = blk * kBlock - shift;  // the block's first entry, before the row's start in its first block
   const int n = min(kBlock, g.V - v0);
+  if (n <= 0) return;  // the block that a shifted row may need
+  // the block's logits are asked for first, and arrive under the history
+  constexpr int kVecs = kBlock / (kThreads * W);
+  Pack<E, W> p[kVecs];
+#pragma unroll
+  for (int q = 0; q < kVecs; ++q) {
+    const int i = (q * kThreads + tid) * W;
+    if (v0 + i >= 0 && i + W <= n) p[q] = *reinterpret_cast<const Pack<E, W>*>(in + v0 + i);
+  }
   const int lo = max(v0, 0), span = max(v0 + n - lo, 0);  // the entries that exist
 
   const int words = WIDE ? 2 * kBlock : kBlock;
@@ -127,8 +136,10 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
     return l;
   };
   const float kNone = -__builtin_inff();
-  for (int i = tid * W; i < n; i += kThreads * W) {
-    const int v = v0 + i;
+#pragma unroll
+  for (int q = 0; q < kVecs; ++q) {
+    const int i = (q * kThreads + tid) * W, v = v0 + i;
+    if (i >= n) break;
     // bits of entries v .. v + W - 1 (of which those in the row count)
     uint32_t bits = 0xffffffffu;
     if (allowed != nullptr) {
@@ -144,14 +155,18 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
           bits |= static_cast<uint32_t>(pair >> ((((e >> 5) != (lo >> 5)) ? 32 : 0) + (e & 31)) & 1u) << k;
       }
     }
-    if (same && v >= 0 && i + W <= n) {
-      Pack<E, W> p = *reinterpret_cast<const Pack<E, W>*>(in + v);
+    if (v >= 0 && i + W <= n) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float l = control(to_f(p.v[k]), i + k);
-        p.v[k] = from_f<E>((bits >> k) & 1 ? l : kNone);
+        const float l = control(to_f(p[q].v[k]), i + k);
+        p[q].v[k] = from_f<E>((bits >> k) & 1 ? l : kNone);
       }
-      *reinterpret_cast<Pack<E, W>*>(out + v) = p;
+      if (same) {
+        *reinterpret_cast<Pack<E, W>*>(out + v) = p[q];
+      } else {
+#pragma unroll
+        for (int k = 0; k < W; ++k) out[v + k] = p[q].v[k];
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < W; ++k)
