@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = 8192;  // vocabulary entries of a workgroup
 constexpr int kAhead = 16;    // history loads in flight a thread
+constexpr int kBiasInLds = 512;  // biases whose values are kept in LDS
 
 // An entry's word in LDS.  Narrow: bias index + 1 in the upper half, set first (the
 // largest wins), then the mark of one seen at all and the count; it serves
@@ -70,6 +71,7 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   constexpr int W = 16 / static_cast<int>(sizeof(E));
   constexpr uint32_t kSeen = Words<WIDE>::kSeen, kCount = Words<WIDE>::kCount;
   extern __shared__ uint32_t s_word[];
+  __shared__ float s_value[kBiasInLds];
   uint32_t* s_bias = WIDE ? s_word + kBlock : s_word;
   const int row = static_cast<int>(blockIdx.x / g.n_blocks);
   const int blk = static_cast<int>(blockIdx.x % g.n_blocks);
@@ -82,32 +84,59 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   const int v0 = blk * kBlock - shift;  // the block's first entry, before the row's start in its first block
   const int n = min(kBlock, g.V - v0);
   if (n <= 0) return;  // the block that a shifted row may need
-  // the block's logits are asked for first, and arrive under the history
+  const int lo = max(v0, 0), span = max(v0 + n - lo, 0);  // the entries that exist
+  // everything from memory that the block needs is asked for before the first barrier: a
+  // wait each for the history, the mask and the biases' values made three fourths of a
+  // small call's time
   constexpr int kVecs = kBlock / (kThreads * W);
   Pack<E, W> p[kVecs];
+  uint32_t mask[kVecs][2];
+  const int32_t* allowed = g.allowed != nullptr ? g.allowed + row * g.ld_a : nullptr;
 #pragma unroll
   for (int q = 0; q < kVecs; ++q) {
-    const int i = (q * kThreads + tid) * W;
-    if (v0 + i >= 0 && i + W <= n) p[q] = *reinterpret_cast<const Pack<E, W>*>(in + v0 + i);
+    const int i = (q * kThreads + tid) * W, v = v0 + i;
+    if (v >= 0 && i + W <= n) p[q] = *reinterpret_cast<const Pack<E, W>*>(in + v);
+    mask[q][0] = mask[q][1] = 0xffffffffu;
+    if (allowed != nullptr && i < n) {
+      mask[q][0] = static_cast<uint32_t>(allowed[max(v, 0) >> 5]);
+      mask[q][1] = static_cast<uint32_t>(allowed[(min(v + W, g.V) - 1) >> 5]);
+    }
   }
-  const int lo = max(v0, 0), span = max(v0 + n - lo, 0);  // the entries that exist
+  const int len = g.lengths != nullptr ? min(max(g.lengths[row], 0), g.H) : g.H;
+  const int first = g.prompts != nullptr ? min(max(g.prompts[row], 0), g.H) : 0;
+  const int32_t* hist = g.history + row * g.ld_h;
+  int id[kAhead];
+  const auto history = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) id[k] = i0 + k * kThreads < len ? hist[i0 + k * kThreads] : -1;
+  };
+  history(tid);
+  const float* bias = g.bias + row * g.ld_b;
+  const int32_t* bias_ids = g.bias_ids + row * g.ld_b;
+  int bias_id[kBiasInLds / kThreads];
+#pragma unroll
+  for (int k = 0; k < kBiasInLds / kThreads; ++k) {
+    const int i = k * kThreads + tid;
+    bias_id[k] = i < g.n_bias ? bias_ids[i] : -1;
+    if (i < g.n_bias) s_value[i] = bias[i];
+  }
+  const float rep = g.rep != nullptr ? g.rep[row] : g.rep_all;
+  const float pres = g.pres != nullptr ? g.pres[row] : g.pres_all;
+  const float freq = g.freq != nullptr ? g.freq[row] : g.freq_all;
 
   const int words = WIDE ? 2 * kBlock : kBlock;
   for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  for (int i = tid; i < g.n_bias; i += kThreads) {
-    const int id = g.bias_ids[row * g.ld_b + i];
-    if (static_cast<unsigned>(id - lo) < static_cast<unsigned>(span))
-      atomicMax(&s_bias[id - v0], static_cast<uint32_t>(i + 1) << (WIDE ? 0 : 16));
-  }
-  if (!WIDE && g.n_bias > 0) __syncthreads();
-  const int len = g.lengths != nullptr ? min(max(g.lengths[row], 0), g.H) : g.H;
-  const int first = g.prompts != nullptr ? min(max(g.prompts[row], 0), g.H) : 0;
-  const int32_t* hist = g.history + row * g.ld_h;
-  for (int i0 = tid; i0 < len; i0 += kThreads * kAhead) {
-    int id[kAhead];
+  const auto mark_bias = [&](int i, int t) {
+    if (t >= 0 && static_cast<unsigned>(t - lo) < static_cast<unsigned>(span))
+      atomicMax(&s_bias[t - v0], static_cast<uint32_t>(i + 1) << (WIDE ? 0 : 16));
+  };
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) id[k] = i0 + k * kThreads < len ? hist[i0 + k * kThreads] : -1;
+  for (int k = 0; k < kBiasInLds / kThreads; ++k) mark_bias(k * kThreads + tid, bias_id[k]);
+  for (int i = kBiasInLds + tid; i < g.n_bias; i += kThreads) mark_bias(i, bias_ids[i]);
+  if (!WIDE && g.n_bias > 0) __syncthreads();
+  for (int i0 = tid; i0 < len; i0 += kThreads * kAhead) {
+    if (i0 != tid) history(i0);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       // an id below zero is far outside as an unsigned number, and lo >= 0
@@ -119,11 +148,6 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   }
   __syncthreads();
 
-  const float rep = g.rep != nullptr ? g.rep[row] : g.rep_all;
-  const float pres = g.pres != nullptr ? g.pres[row] : g.pres_all;
-  const float freq = g.freq != nullptr ? g.freq[row] : g.freq_all;
-  const int32_t* allowed = g.allowed != nullptr ? g.allowed + row * g.ld_a : nullptr;
-  const float* bias = g.bias + row * g.ld_b;
   const auto control = [&](float l, int at) {
     const uint32_t w = s_word[at];
     if (w & (kSeen | kCount)) {
@@ -132,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
       if (c != 0) l -= freq * static_cast<float>(c) + pres;
     }
     const uint32_t b = WIDE ? s_bias[at] : w >> 16;
-    if (b != 0) l += bias[b - 1];
+    if (b != 0) l += b <= kBiasInLds ? s_value[b - 1] : bias[b - 1];
     return l;
   };
   const float kNone = -__builtin_inff();
@@ -140,21 +164,13 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   for (int q = 0; q < kVecs; ++q) {
     const int i = (q * kThreads + tid) * W, v = v0 + i;
     if (i >= n) break;
-    // bits of entries v .. v + W - 1 (of which those in the row count)
-    uint32_t bits = 0xffffffffu;
-    if (allowed != nullptr) {
-      const int lo = max(v, 0), hi = min(v + W, g.V) - 1;
-      const uint64_t pair = static_cast<uint32_t>(allowed[lo >> 5]) |
-                            (static_cast<uint64_t>(static_cast<uint32_t>(allowed[hi >> 5])) << 32);
-      // entry e's bit: word (e >> 5) - (lo >> 5) of the pair
-      bits = 0;
+    // bits of entries v .. v + W - 1: entry e's is bit e % 32 of the first word, or of the
+    // second where it lies in another
+    const int first_word = max(v, 0) >> 5;
+    uint32_t bits = 0;
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int e = v + k;
-        if (e >= lo && e <= hi)
-          bits |= static_cast<uint32_t>(pair >> ((((e >> 5) != (lo >> 5)) ? 32 : 0) + (e & 31)) & 1u) << k;
-      }
-    }
+    for (int k = 0; k < W; ++k)
+      bits |= ((mask[q][((v + k) >> 5) != first_word ? 1 : 0] >> ((v + k) & 31)) & 1u) << k;
     if (v >= 0 && i + W <= n) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
@@ -186,8 +202,12 @@ int run(Logits<E> g, int64_t rows, hipStream_t st) {
     return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
   const bool wide = g.H >= (1 << 15) || g.n_bias >= (1 << 16);
   const size_t lds = (wide ? 2 : 1) * kBlock * sizeof(uint32_t);
-  hipLaunchKernelGGL(wide ? (control_logits_kernel<E, true>) : (control_logits_kernel<E, false>),
-                     dim3(static_cast<unsigned>(rows * g.n_blocks)), dim3(kThreads), lds, st, g);
+  auto kern = wide ? control_logits_kernel<E, true> : control_logits_kernel<E, false>;
+  if (wide)  // past 64 KB with the biases' values
+    if (int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(lds)), "hipFuncSetAttribute"))
+      return rc;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows * g.n_blocks)), dim3(kThreads), lds, st, g);
   return launch_check("control_logits_kernel");
 }
 
