@@ -5,11 +5,13 @@
 //   l -= freq c + pres (c > 0)   c: v's count in the part after the prompt
 //   l += bias of v;  l = -inf where the mask forbids v
 //
-// A workgroup takes a row's block of kBlock vocabulary entries: it counts the row's
-// history and marks its biases for that block in LDS, then streams the block.
-// Integer LDS atomics only (the highest bias index, a mark, counts), so the result does not
-// depend on their order.  Every block of a row reads the row's history again (from
-// L2: a few kB against the block's logits).
+// A workgroup takes a row's block of kBlock vocabulary entries.  It copies the block
+// through the mask, without looking at a value; meanwhile it marks the row's biases
+// and counts its history for that block in LDS, and then forms the marked entries'
+// results, few against the vocabulary (doing all of it entry by entry took 45 instructions
+// an entry, two thirds of the time at [256, 131072]).  Integer LDS atomics only (the highest
+// bias index, a mark, counts): their order does not reach a result.  Every block of a row
+// reads the row's history again, from L2: a few kB against the block's logits.
 //
 // Vectors of 16 bytes are aligned to the row's address, whatever its offset (a
 // vocabulary of odd size puts every row at another one); the row's ends take single
@@ -36,12 +38,21 @@ constexpr int kBiasInLds = 512;  // biases whose values are kept in LDS
 // An entry's word in LDS.  Narrow: bias index + 1 in the upper half, set first (the
 // largest wins), then the mark of one seen at all and the count; it serves
 // histories below 2^15 tokens and up to 2^16 - 1 biases with one word an entry (32 KB:
-// five workgroups a CU).  Wide: the mark and the count in a word, biases in a second.
+// with the biases' values four workgroups a CU).  Wide: the mark and the count in a word,
+// biases in a second.
 template <bool WIDE>
 struct Words {
   static constexpr uint32_t kSeen = WIDE ? 0x80000000u : 0x8000u;
   static constexpr uint32_t kCount = kSeen - 1;
+  static constexpr int kWords = WIDE ? 2 * kBlock : kBlock;
 };
+
+template <class E>
+__device__ __forceinline__ E minus_inf();
+template <>
+__device__ __forceinline__ float minus_inf<float>() { return -__builtin_inff(); }
+template <>
+__device__ __forceinline__ bf16_t minus_inf<bf16_t>() { return bf16_t{0xff80}; }
 
 template <class E>
 struct Logits {
@@ -124,8 +135,7 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
   const float pres = g.pres != nullptr ? g.pres[row] : g.pres_all;
   const float freq = g.freq != nullptr ? g.freq[row] : g.freq_all;
 
-  const int words = WIDE ? 2 * kBlock : kBlock;
-  for (int i = tid * 4; i < words; i += kThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+  for (int i = tid * 4; i < Words<WIDE>::kWords; i += kThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
   const auto mark_bias = [&](int i, int t) {
     if (t >= 0 && static_cast<unsigned>(t - lo) < static_cast<unsigned>(span))
@@ -146,37 +156,38 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
       }
     }
   }
-  __syncthreads();
 
-  const auto control = [&](float l, int at) {
-    const uint32_t w = s_word[at];
-    if (w & (kSeen | kCount)) {
-      l = l > 0.f ? l / rep : l * rep;
-      const uint32_t c = w & kCount;
-      if (c != 0) l -= freq * static_cast<float>(c) + pres;
-    }
-    const uint32_t b = WIDE ? s_bias[at] : w >> 16;
-    if (b != 0) l += b <= kBiasInLds ? s_value[b - 1] : bias[b - 1];
-    return l;
-  };
-  const float kNone = -__builtin_inff();
+  __syncthreads();  // the marks are whole
+
+  // the block through the mask: entry e's bit is bit e % 32 of the first word, or of the
+  // second where it lies in another.  A thread's entries are the bits of a word, entry
+  // (q kThreads + tid) W + k bit q W + k: it copies them and forms the marked ones itself,
+  // and its second store to an entry follows its first without a wait.
+  static_assert(kBlock == 32 * kThreads, "a thread's entries are the bits of a word");
+  const E none = minus_inf<E>();
+  uint32_t marked = 0;
 #pragma unroll
   for (int q = 0; q < kVecs; ++q) {
     const int i = (q * kThreads + tid) * W, v = v0 + i;
     if (i >= n) break;
-    // bits of entries v .. v + W - 1: entry e's is bit e % 32 of the first word, or of the
-    // second where it lies in another
     const int first_word = max(v, 0) >> 5;
-    uint32_t bits = 0;
+    uint32_t bits = 0, marks = 0;
 #pragma unroll
     for (int k = 0; k < W; ++k)
       bits |= ((mask[q][((v + k) >> 5) != first_word ? 1 : 0] >> ((v + k) & 31)) & 1u) << k;
+#pragma unroll
+    for (int k = 0; k < W; k += 4) {
+      uint4 w = *reinterpret_cast<const uint4*>(&s_word[i + k]);
+      if constexpr (WIDE) {
+        const uint4 b = *reinterpret_cast<const uint4*>(&s_bias[i + k]);
+        w = make_uint4(w.x | b.x, w.y | b.y, w.z | b.z, w.w | b.w);
+      }
+      marks |= ((w.x != 0) | (w.y != 0) << 1 | (w.z != 0) << 2 | (w.w != 0) << 3) << k;
+    }
+    marked |= (marks & bits) << (q * W);
     if (v >= 0 && i + W <= n) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const float l = control(to_f(p[q].v[k]), i + k);
-        p[q].v[k] = from_f<E>((bits >> k) & 1 ? l : kNone);
-      }
+      for (int k = 0; k < W; ++k) p[q].v[k] = (bits >> k) & 1 ? p[q].v[k] : none;
       if (same) {
         *reinterpret_cast<Pack<E, W>*>(out + v) = p[q];
       } else {
@@ -186,10 +197,31 @@ __global__ __launch_bounds__(kThreads) void control_logits_kernel(Logits<E> g) {
     } else {
 #pragma unroll
       for (int k = 0; k < W; ++k)
-        if (v + k >= 0 && i + k < n) {
-          const float l = control(to_f(in[v + k]), i + k);
-          out[v + k] = from_f<E>((bits >> k) & 1 ? l : kNone);
-        }
+        if (v + k >= 0 && i + k < n) out[v + k] = (bits >> k) & 1 ? in[v + k] : none;
+    }
+  }
+  while (marked != 0) {
+    constexpr int kBatch = 4;  // entries whose logits are asked for together
+    int at[kBatch];
+    float l[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int bit = marked != 0 ? __builtin_ctz(marked) : -1;
+      marked &= marked - 1;
+      at[k] = bit < 0 ? -1 : ((bit / W) * kThreads + tid) * W + bit % W;
+      l[k] = at[k] >= 0 ? to_f(in[v0 + at[k]]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (at[k] < 0) continue;
+      const uint32_t w = s_word[at[k]], b = WIDE ? s_bias[at[k]] : w >> 16;
+      if (w & (kSeen | kCount)) {
+        l[k] = l[k] > 0.f ? l[k] / rep : l[k] * rep;
+        const uint32_t c = w & kCount;
+        if (c != 0) l[k] -= freq * static_cast<float>(c) + pres;
+      }
+      if (b != 0) l[k] += b <= kBiasInLds ? s_value[b - 1] : bias[b - 1];
+      out[v0 + at[k]] = from_f<E>(l[k]);
     }
   }
 }
@@ -201,7 +233,7 @@ int run(Logits<E> g, int64_t rows, hipStream_t st) {
   if (rows * g.n_blocks > INT_MAX)
     return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
   const bool wide = g.H >= (1 << 15) || g.n_bias >= (1 << 16);
-  const size_t lds = (wide ? 2 : 1) * kBlock * sizeof(uint32_t);
+  const size_t lds = (wide ? Words<true>::kWords : Words<false>::kWords) * sizeof(uint32_t);
   auto kern = wide ? control_logits_kernel<E, true> : control_logits_kernel<E, false>;
   if (wide)  // past 64 KB with the biases' values
     if (int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
