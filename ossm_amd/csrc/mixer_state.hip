@@ -256,11 +256,12 @@ __device__ __forceinline__ float proj_of(const Mixer<E>& g, int r, int j) {
 
 // One token: a thread per channel, RB rows.  The first 16 states of all rows are asked
 // for before the projections are summed: the states' traffic is what bounds a large
-// batch, and this keeps 16 RB loads a thread in flight.
-// VEC: A_log's and dt_proj's rows are whole 16-byte vectors.
+// batch, and this keeps 16 RB loads a thread in flight.  The rows' projections lie in LDS
+// in three stretches padded with zeros, dt's to Rq, B's and C's to Nq (multiples of 16), so
+// that four values come with a read.  VEC: A_log's and dt_proj's rows are whole 16-byte vectors.
 template <class E, int RB, bool VEC>
-__global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
-  extern __shared__ float s_p[];  // [RB][Nc]
+__global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, int Rq, int Nq) {
+  extern __shared__ __align__(16) float s_p[];  // [RB][Rq + 2 Nq]
   const int r0 = static_cast<int>(blockIdx.y) * RB;
   const int d_own = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x), d = min(d_own, g.Di - 1);
   constexpr int NB = 16;
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
     }
   };
   load_a(0);
-  // dt_proj's first 32 weights of the channel
+  // dt_proj's first 32 weights of the channel (zeros from R on)
   float wt[32];
   const auto load_w = [&](int q0) {
 #pragma unroll
@@ -305,9 +306,11 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
     }
   };
   load_w(0);
-  for (int i = threadIdx.x; i < RB * g.Nc; i += blockDim.x) {
-    const int r = r0 + i / g.Nc;
-    s_p[i] = r < g.rows ? proj_of(g, r, i % g.Nc) : 0.f;
+  const int width = Rq + 2 * Nq;
+  for (int i = threadIdx.x; i < RB * width; i += blockDim.x) {
+    const int rr = i / width, k = i % width, c = k - Rq, second = c >= Nq ? 1 : 0, n = c - second * Nq;
+    const int j = k < Rq ? (k < g.R ? k : -1) : (n < g.N ? g.R + second * g.N + n : -1);
+    s_p[i] = j >= 0 && r0 + rr < g.rows ? proj_of(g, r0 + rr, j) : 0.f;
   }
   __syncthreads();
   float dt[RB];
@@ -317,10 +320,13 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
   for (int q0 = 0; q0 < g.R; q0 += 32) {
     if (q0 > 0) load_w(q0);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (q0 + i < g.R) {
+    for (int i = 0; i < 32; i += 4) {
+      if (q0 + i < g.R) {  // (what a zero weight meets is a zero)
 #pragma unroll
-        for (int rr = 0; rr < RB; ++rr) dt[rr] = fmaf(wt[i], s_p[rr * g.Nc + q0 + i], dt[rr]);
+        for (int rr = 0; rr < RB; ++rr) {
+          const float4 p = *reinterpret_cast<const float4*>(s_p + rr * width + q0 + i);
+          dt[rr] = fmaf(wt[i + 3], p.w, fmaf(wt[i + 2], p.z, fmaf(wt[i + 1], p.y, fmaf(wt[i], p.x, dt[rr]))));
+        }
       }
     }
   }
@@ -344,16 +350,23 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) h[rr][i] = in[rr] >= 0 && n0 + i < g.N ? src[static_cast<size_t>(i) * g.Di] : 0.f;
       }
-      const float* B = s_p + rr * g.Nc + g.R + n0;
+      const float* B = s_p + rr * width + Rq + n0;
       const bool keep = r0 + rr < g.rows && in_pool(g, to[rr]);
       float* dst = g.ssm + (static_cast<size_t>(keep ? to[rr] : 0) * g.N + n0) * g.Di + d;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        if (n0 + i < g.N) {
-          const float v = fmaf(__builtin_amdgcn_exp2f(a2[i] * dt[rr]), h[rr][i], du[rr] * B[i]);
-          y[rr] = fmaf(B[g.N + i], v, y[rr]);
-          if (keep) dst[static_cast<size_t>(i) * g.Di] = v;
+      for (int i = 0; i < NB; i += 4) {
+        float b[4], c[4];
+        load4(B + i, b);
+        load4(B + Nq + i, c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v = fmaf(__builtin_amdgcn_exp2f(a2[i + k] * dt[rr]), h[rr][i + k], du[rr] * b[k]);
+          if (n0 + i + k < g.N) {
+            y[rr] = fmaf(c[k], v, y[rr]);
+            if (keep) dst[static_cast<size_t>(i + k) * g.Di] = v;
+          }
         }
+      }
     }
   }
 #pragma unroll
@@ -991,6 +1004,8 @@ int launch_scans(const Mixer<E>& g, bool out, hipStream_t st) {
 template <class E>
 bool vec8(const E* p, int row) { return aligned16(p) && row % (16 / static_cast<int>(sizeof(E))) == 0; }
 
+constexpr int kTokenRows = 2;  // rows of a workgroup of token_scan_kernel where there are many
+
 template <class E>
 int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.n_blocks = (g.Di + kProjBlock - 1) / kProjBlock;
@@ -1008,13 +1023,14 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
                    : (k4 ? token_proj_kernel<E, 1, 4> : token_proj_kernel<E, 1, 8>);
   hipLaunchKernelGGL(proj, ga, dim3(kProjThreads), 0, st, g, vx);
   if (int rc = launch_check("token_proj_kernel")) return rc;
-  const int rt = many ? 4 : 1, threads = many ? 256 : 64;
+  const int rt = many ? kTokenRows : 1, threads = many ? 256 : 64;
   const dim3 gb(static_cast<unsigned>((g.Di + threads - 1) / threads), static_cast<unsigned>((g.rows + rt - 1) / rt));
-  const size_t lds = static_cast<size_t>(rt) * g.Nc * sizeof(float);
+  const int Rq = (g.R + 15) / 16 * 16, Nq = (g.N + 15) / 16 * 16;
+  const size_t lds = static_cast<size_t>(rt) * (Rq + 2 * Nq) * sizeof(float);
   const bool vec = vec8(g.dt_proj, g.R) && vec8(g.a_log, g.N);
-  hipLaunchKernelGGL(many ? (vec ? token_scan_kernel<E, 4, true> : token_scan_kernel<E, 4, false>)
+  hipLaunchKernelGGL(many ? (vec ? token_scan_kernel<E, kTokenRows, true> : token_scan_kernel<E, kTokenRows, false>)
                           : (vec ? token_scan_kernel<E, 1, true> : token_scan_kernel<E, 1, false>),
-                     gb, dim3(threads), lds, st, g);
+                     gb, dim3(threads), lds, st, g, Rq, Nq);
   return launch_check("token_scan_kernel");
 }
 
