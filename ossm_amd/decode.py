@@ -26,7 +26,7 @@ from torch import Tensor
 
 from . import _lib
 
-__all__ = ["MixerState", "mixer_prompt", "mixer_step"]
+__all__ = ["MixerState", "mixer_prompt", "mixer_step", "prompt", "step"]
 
 
 class MixerState:
@@ -146,3 +146,31 @@ def mixer_prompt(xz: Tensor, conv_weight: Tensor, conv_bias: Optional[Tensor], x
              conv_state.data_ptr(), ssm_state.data_ptr(), slots.data_ptr(), _lib.ptr(out_slots), offsets.data_ptr(),
              _lib.ptr(resume), y.data_ptr(), rows, n, n_slots, Di, N, R, K)
     return y
+
+
+# ------------------------------------------------------------------ the module's calls
+def _weights(mixer, dtype: torch.dtype):
+    """A ``MambaMixer``'s parameters as the functions take them."""
+    bias = mixer.conv1d.bias
+    like = [mixer.conv1d.weight.to(dtype), None if bias is None else bias.to(dtype), mixer.x_proj.weight.to(dtype),
+            mixer.dt_proj.weight.to(dtype)]
+    return (*like, mixer.dt_proj.bias.float(), mixer.A_log.float())
+
+
+@torch.no_grad()
+def prompt(mixer, inputs: Tensor, state: MixerState, slots: Tensor, offsets: Tensor,
+           resume: Optional[Tensor] = None) -> Tensor:
+    """``mixer`` (a ``MambaMixer``) over packed prompts, inputs [rows, d_model]; states and
+    offsets as ``mixer_prompt``'s."""
+    xz = mixer.in_proj(inputs)
+    skip = None if mixer.D is None else mixer.D.float()
+    y = mixer_prompt(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots, offsets, resume, skip=skip)
+    return mixer.out_proj(y)
+
+
+@torch.no_grad()
+def step(mixer, inputs: Tensor, state: MixerState, slots: Tensor) -> Tensor:
+    """``mixer`` (a ``MambaMixer``) on the next token of each sequence, inputs [rows, d_model]."""
+    xz = mixer.in_proj(inputs)
+    skip = None if mixer.D is None else mixer.D.float()
+    return mixer.out_proj(mixer_step(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots, skip=skip))
