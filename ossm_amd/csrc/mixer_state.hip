@@ -16,7 +16,7 @@
 // A prompt batch is one row of packed tokens cut into chunks of equal length,
 // whatever the prompts' lengths (the host never reads the offsets): a prompt's
 // first token resets the recurrence, so a chunk may hold many prompts or a
-// piece of one.  prompt_proj_kernel (conv and x_proj) and prompt_dt_kernel (dt_proj) put both
+// piece of one.  prompt_proj_kernel (conv and x_proj) and the first scan (dt_proj) put both
 // projections on the matrix cores, u and p as three bf16 terms (split_mfma.hpp has
 // the error).  mixer_scan_kernel<summary> finds what each chunk leaves to a zero
 // carry and the sum of its dt (the decay over the chunk is exp(A sum dt)),
@@ -659,67 +659,6 @@ __global__ __launch_bounds__(256) void prompt_sum_kernel(Mixer<E> g) {
   }
 }
 
-constexpr int kDtRows = 32, kDtCols = 256;  // prompt_dt_kernel's tile, a wave 32 x 64 of it
-
-// dt = softplus(dt_proj p[:R] + bias), both operands' fragments straight from memory (the
-// planes and the weights are read from the caches by every tile).
-template <class E>
-__global__ __launch_bounds__(256) void prompt_dt_kernel(Mixer<E> g, bool vec) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
-  const int r0 = static_cast<int>(blockIdx.x) * kDtRows;
-  const int cw = static_cast<int>(blockIdx.y) * kDtCols + wave_id() * 64;
-  if (cw >= g.Di) return;  // no barriers below
-  const size_t plane = static_cast<size_t>(g.rows) * g.Rp;
-  const uint16_t* row = g.planes + static_cast<size_t>(min(r0 + l32, g.rows - 1)) * g.Rp;
-  const E* rows_w[2];
-  float bias[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int d = min(cw + j * 32 + l32, g.Di - 1);
-    rows_w[j] = g.dt_proj + static_cast<size_t>(d) * g.R;
-    bias[j] = g.dt_bias[d];
-  }
-  floatx16 acc[2] = {};
-  for (int k0 = 0; k0 < g.Rp; k0 += 16) {
-    const int k = k0 + half * 8;
-    bf16x8 a[3];
-    Weight8<E> wt[2];
-#pragma unroll
-    for (int q = 0; q < 3; ++q) a[q] = *reinterpret_cast<const bf16x8*>(row + q * plane + k);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) wt[j].load(rows_w[j], k, g.R, vec);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      wt[j].split();
-      acc[j] = mfma_terms(a, wt[j], acc[j]);
-    }
-  }
-  if (any_nonfinite(acc)) {
-    floatx16 again[2] = {};
-#pragma unroll 1
-    for (int k0 = 0; k0 < g.Rp; k0 += 2) {
-      const int k = k0 + half;
-      const float a = (to_f(bf16_t{row[2 * plane + k]}) + to_f(bf16_t{row[plane + k]})) + to_f(bf16_t{row[k]});
-#pragma unroll
-      for (int j = 0; j < 2; ++j) again[j] = mfma32(a, k < g.R ? to_f(rows_w[j][k]) : 0.f, again[j]);
-    }
-    keep_finite(again, acc);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[j] = again[j];
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int d = cw + j * 32 + l32;
-    if (d >= g.Di) continue;
-    float* out = g.dt + static_cast<size_t>(r0) * g.Di + d;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int at = 8 * (r >> 2) + 4 * half + (r & 3);
-      if (r0 + at < g.rows) out[static_cast<size_t>(at) * g.Di] = softplus_f(acc[j][r] + bias[j]);
-    }
-  }
-}
-
 // The resumed states, copied before the scan that may overwrite their slots.
 template <class E>
 __global__ __launch_bounds__(256) void mixer_gather_kernel(Mixer<E> g) {
@@ -735,6 +674,91 @@ constexpr int kScanThreads = 128;
 constexpr int kGroup = 4;   // tokens whose inputs are loaded together
 constexpr int kStage = 32;  // tokens whose B and C are in LDS
 
+// dt_proj's sums of 32 tokens (from r0) and the wave's 64 channels (from cw), both operands'
+// fragments straight from memory: the planes and the weights are read from the caches by
+// every tile.  Register r of lane l: token 8 (r / 4) + 4 (l / 32) + r % 4, channel l % 32
+// of each half.
+template <class E>
+__device__ __forceinline__ void dt_sums(const Mixer<E>& g, int r0, int cw, bool vec, floatx16 (&acc)[2]) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
+  const size_t plane = static_cast<size_t>(g.rows) * g.Rp;
+  const uint16_t* row = g.planes + static_cast<size_t>(min(r0 + l32, g.rows - 1)) * g.Rp;
+  const E* rows_w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    rows_w[j] = g.dt_proj + static_cast<size_t>(min(cw + j * 32 + l32, g.Di - 1)) * g.R;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+  }
+  constexpr int kAhead = 2;  // k steps whose fragments are asked for together
+#pragma unroll 1
+  for (int k0 = 0; k0 < g.Rp; k0 += 16 * kAhead) {
+    bf16x8 a[kAhead][3];
+    Weight8<E> wt[kAhead][2];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int k = min(k0 + q * 16, g.Rp - 16) + half * 8;
+#pragma unroll
+      for (int t = 0; t < 3; ++t) a[q][t] = *reinterpret_cast<const bf16x8*>(row + t * plane + k);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) wt[q][j].load(rows_w[j], k, g.R, vec);
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (k0 + q * 16 < g.Rp) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          wt[q][j].split();
+          acc[j] = mfma_terms(a[q], wt[q][j], acc[j]);
+        }
+      }
+  }
+  if (any_nonfinite(acc)) {
+    floatx16 again[2] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < g.Rp; k0 += 2) {
+      const int k = k0 + half;
+      const float a = (to_f(bf16_t{row[2 * plane + k]}) + to_f(bf16_t{row[plane + k]})) + to_f(bf16_t{row[k]});
+#pragma unroll
+      for (int j = 0; j < 2; ++j) again[j] = mfma32(a, k < g.R ? to_f(rows_w[j][k]) : 0.f, again[j]);
+    }
+    keep_finite(again, acc);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[j] = again[j];
+  }
+}
+
+constexpr int kDtRows = 32, kDtCols = 256;  // prompt_dt_kernel's tile, a wave 32 x 64 of it
+
+// dt of a batch large enough to fill the card without the scans' help.  Many small waves:
+// weights kept in registers over several tiles cost the occupancy that hides the loads
+// (75 us against 68 at [16384, 2048], whose write alone takes 27).
+template <class E>
+__global__ __launch_bounds__(256, 4) void prompt_dt_kernel(Mixer<E> g, bool vec) {
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
+  const int r0 = static_cast<int>(blockIdx.x) * kDtRows;
+  const int cw = static_cast<int>(blockIdx.y) * kDtCols + wave_id() * 64;
+  if (cw >= g.Di) return;  // no barriers below
+  float bias[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) bias[j] = g.dt_bias[min(cw + j * 32 + l32, g.Di - 1)];
+  floatx16 acc[2];
+  dt_sums(g, r0, cw, vec, acc);
+  const bool whole = r0 + kDtRows <= g.rows;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int d = cw + j * 32 + l32;
+    if (d >= g.Di) continue;
+    float* out = g.dt + static_cast<size_t>(r0) * g.Di + d;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = 8 * (r >> 2) + 4 * half + (r & 3);
+      const float v = softplus_f(acc[j][r] + bias[j]);
+      if (whole || r0 + at < g.rows) out[static_cast<size_t>(at) * g.Di] = v;
+    }
+  }
+}
+
 // One thread per channel walks a chunk, NB states (from n_base) in registers and KT conv
 // taps (those before the last K are skipped).  OUT: from the chunk's carry, writing y and
 // the states of the prompts that end here; else from the last prompt start in the chunk
@@ -744,9 +768,13 @@ constexpr int kStage = 32;  // tokens whose B and C are in LDS
 // them an exponential of four issue slots.  B and C, the same for all channels, come from
 // LDS by broadcast reads, a stage of tokens at a time: as scalar loads they were
 // waited for token by token, 0.8 us each where few waves run.
-template <class E, int NB, int KT, bool OUT>
-__global__ __launch_bounds__(kScanThreads, NB <= 16 ? 4 : 2) void mixer_scan_kernel(Mixer<E> g, int n_base) {
+//
+// DT: this pass forms dt of its stages on the matrix cores (the first of the passes, where
+// the chunks leave the card half empty) and, where another follows, leaves it in memory.
+template <class E, int NB, int KT, bool OUT, bool DT>
+__global__ __launch_bounds__(kScanThreads, NB <= 16 ? (DT ? 3 : 4) : 2) void mixer_scan_kernel(Mixer<E> g, int n_base, bool vec) {
   __shared__ __align__(16) float s_bc[kStage][2 * NB];
+  __shared__ float s_dt[DT ? kStage : 1][DT ? kScanThreads : 1];
   const int d_own = static_cast<int>(blockIdx.x) * kScanThreads + static_cast<int>(threadIdx.x);
   const bool live = d_own < g.Di;
   const int d = min(d_own, g.Di - 1);
@@ -772,16 +800,35 @@ __global__ __launch_bounds__(kScanThreads, NB <= 16 ? 4 : 2) void mixer_scan_ker
   int t = t0;
   float dt_sum = 0.f;
   if constexpr (!OUT) {
-    if (s < 0) return;  // padding only (of the whole workgroup): the next chunk starts a prompt
-    const int start = offset_of(g, s);
+    // (none: padding only, and the next chunk starts a prompt)
+    const int start = s >= 0 ? offset_of(g, s) : t1;
     if (start >= t0) { t = start; dt_sum = -1.f; }
+    if (c + 1 == g.n_chunks) t = t1;  // nothing follows: it needs no summary
   }
   bool begun = false;  // h and the window are sequence s's at t
 #pragma unroll 1
   for (int b0 = t0; b0 < t1; b0 += kStage) {
     const int b1 = min(b0 + kStage, t1);
-    if (t >= b1) continue;  // (the same for the whole workgroup)
+    if (!DT && t >= b1) continue;  // (the same for the whole workgroup)
     __syncthreads();
+    if constexpr (DT) {
+      const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5, w = wave_id();
+      const int cw = static_cast<int>(blockIdx.x) * kScanThreads + w * kWave;
+      floatx16 acc[2];
+      dt_sums(g, b0, cw, vec, acc);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int ch = cw + j * 32 + l32;
+        const float bias = g.dt_bias[min(ch, g.Di - 1)];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+          const float v = softplus_f(acc[j][r] + bias);
+          s_dt[row][w * kWave + j * 32 + l32] = v;
+          if (g.dt != nullptr && ch < g.Di && b0 + row < b1) g.dt[static_cast<size_t>(b0 + row) * g.Di + ch] = v;
+        }
+      }
+    }
 #pragma unroll
     for (int q = 0; q < kStage * 2 * NB / 4 / kScanThreads + 1; ++q) {
       const int i = (q * kScanThreads + static_cast<int>(threadIdx.x)) * 4;
@@ -824,7 +871,7 @@ __global__ __launch_bounds__(kScanThreads, NB <= 16 ? 4 : 2) void mixer_scan_ker
           for (int i = 0; i < kGroup; ++i) {
             const size_t r = static_cast<size_t>(min(t + i, e - 1));
             x[i] = to_f(g.xz[r * g.ld + d]);
-            dt[i] = g.dt[r * g.Di + d];
+            dt[i] = DT ? s_dt[min(t + i, e - 1) - b0][threadIdx.x] : g.dt[r * g.Di + d];
             if constexpr (OUT) {
               z[i] = to_f(g.xz[r * g.ld + g.Di + d]);
               ys[i] = n_base > 0 ? g.y_sum[r * g.Di + d] : 0.f;
@@ -976,26 +1023,25 @@ __global__ __launch_bounds__(256) void mixer_finish_kernel(Mixer<E> g) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <class E, int NB, int KT>
-int launch_scan(const Mixer<E>& g, bool out, int n_base, hipStream_t st) {
-  // (nothing follows the last chunk: it needs no summary)
-  const dim3 grid(static_cast<unsigned>((g.Di + kScanThreads - 1) / kScanThreads),
-                  static_cast<unsigned>(out ? g.n_chunks : g.n_chunks - 1));
-  if (out)
-    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, true>), grid, dim3(kScanThreads), 0, st, g, n_base);
-  else
-    hipLaunchKernelGGL((mixer_scan_kernel<E, NB, KT, false>), grid, dim3(kScanThreads), 0, st, g, n_base);
+int launch_scan(const Mixer<E>& g, bool out, bool dt, int n_base, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((g.Di + kScanThreads - 1) / kScanThreads), static_cast<unsigned>(g.n_chunks));
+  auto kern = out ? (dt ? mixer_scan_kernel<E, NB, KT, true, true> : mixer_scan_kernel<E, NB, KT, true, false>)
+                  : (dt ? mixer_scan_kernel<E, NB, KT, false, true> : mixer_scan_kernel<E, NB, KT, false, false>);
+  const bool vec = aligned16(g.dt_proj) && g.R % (16 / static_cast<int>(sizeof(E))) == 0;
+  hipLaunchKernelGGL(kern, grid, dim3(kScanThreads), 0, st, g, n_base, vec);
   return launch_check("mixer_scan_kernel");
 }
 
+// One pass over all states, a block of them at a time; `dt`: the first block forms dt.
 template <class E>
-int launch_scans(const Mixer<E>& g, bool out, hipStream_t st) {
-  for (int n_base = 0; n_base < g.N; n_base += 32) {
+int launch_scans(const Mixer<E>& g, bool out, bool dt, hipStream_t st) {
+  for (int n_base = 0; n_base < g.N; n_base += 32, dt = false) {
     const int left = g.N - n_base;
     const bool k4 = g.K <= 4;
     int rc;
-    if (left <= 8) rc = k4 ? launch_scan<E, 8, 4>(g, out, n_base, st) : launch_scan<E, 8, 8>(g, out, n_base, st);
-    else if (left <= 16) rc = k4 ? launch_scan<E, 16, 4>(g, out, n_base, st) : launch_scan<E, 16, 8>(g, out, n_base, st);
-    else rc = k4 ? launch_scan<E, 32, 4>(g, out, n_base, st) : launch_scan<E, 32, 8>(g, out, n_base, st);
+    if (left <= 8) rc = k4 ? launch_scan<E, 8, 4>(g, out, dt, n_base, st) : launch_scan<E, 8, 8>(g, out, dt, n_base, st);
+    else if (left <= 16) rc = k4 ? launch_scan<E, 16, 4>(g, out, dt, n_base, st) : launch_scan<E, 16, 8>(g, out, dt, n_base, st);
+    else rc = k4 ? launch_scan<E, 32, 4>(g, out, dt, n_base, st) : launch_scan<E, 32, 8>(g, out, dt, n_base, st);
     if (rc) return rc;
   }
   return OSSM_OK;
@@ -1063,7 +1109,8 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const size_t o_part = take(static_cast<size_t>(g.n_blocks) * g.rows * g.Nc);
   const size_t o_planes = take((3 * static_cast<size_t>(g.rows) * g.Rp + 1) / 2);
   const size_t o_bc = take(static_cast<size_t>(g.rows) * 2 * g.Npad);
-  const size_t o_dt = take(static_cast<size_t>(g.rows) * g.Di);
+  const bool keep_dt = carries || g.N > 32;  // a pass reads what an earlier one formed
+  const size_t o_dt = take(keep_dt ? static_cast<size_t>(g.rows) * g.Di : 0);
   const size_t o_local = take(carries ? g.n_chunks * nd : 0);
   const size_t o_carry = take(carries ? g.n_chunks * nd : 0);
   const size_t o_sum = take(carries ? static_cast<size_t>(g.n_chunks) * g.Di : 0);
@@ -1077,7 +1124,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.part = f + o_part;
   g.planes = reinterpret_cast<uint16_t*>(f + o_planes);
   g.bc = f + o_bc;
-  g.dt = f + o_dt;
+  g.dt = keep_dt ? f + o_dt : nullptr;
   g.local = f + o_local;
   g.carry = f + o_carry;
   g.sum_dt = f + o_sum;
@@ -1096,18 +1143,24 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
     const int64_t sums = static_cast<int64_t>(g.rows) * (g.Rp + 2 * g.Npad);
     hipLaunchKernelGGL(prompt_sum_kernel<E>, dim3(static_cast<unsigned>((sums + 255) / 256)), dim3(256), 0, st, g);
     if (int rc = launch_check("prompt_sum_kernel")) return rc;
-    hipLaunchKernelGGL(prompt_dt_kernel<E>, dim3(static_cast<unsigned>((g.rows + kDtRows - 1) / kDtRows),
-                                                 static_cast<unsigned>((g.Di + kDtCols - 1) / kDtCols)),
-                       dim3(256), 0, st, g, vec8(g.dt_proj, g.R));
-    if (int rc = launch_check("prompt_dt_kernel")) return rc;
     if (g.resume != nullptr) {
       g.init = f + o_init;
       hipLaunchKernelGGL(mixer_gather_kernel<E>, dim3(static_cast<unsigned>(std::min<size_t>(64, (nd + 255) / 256)),
                                                       static_cast<unsigned>(g.n_seqs)), dim3(256), 0, st, g);
       if (int rc = launch_check("mixer_gather_kernel")) return rc;
     }
+    // dt in the first scan saves a launch where there are few waves (one prompt of 117
+    // tokens at d_inner 2048 55 -> 49 us), and costs the scan its occupancy where there
+    // are many (16384 tokens 456 -> 478, 25600 at d_inner 128 122 -> 126)
+    const bool dt_in_scan = !carries || g.n_chunks * waves <= 4 * cus;
+    if (!dt_in_scan) {
+      const dim3 grid(static_cast<unsigned>((g.rows + kDtRows - 1) / kDtRows), static_cast<unsigned>((g.Di + kDtCols - 1) / kDtCols));
+      hipLaunchKernelGGL(prompt_dt_kernel<E>, grid, dim3(256), 0, st, g,
+                         aligned16(g.dt_proj) && g.R % (16 / static_cast<int>(sizeof(E))) == 0);
+      if (int rc = launch_check("prompt_dt_kernel")) return rc;
+    }
     if (carries) {
-      if (int rc = launch_scans(g, false, st)) return rc;
+      if (int rc = launch_scans(g, false, dt_in_scan, st)) return rc;
       const unsigned nb = static_cast<unsigned>((nd + 255) / 256);
       if (g.n_groups > 1) {
         hipLaunchKernelGGL(mixer_group_kernel<E>, dim3(nb, static_cast<unsigned>(g.n_groups - 1)), dim3(256), 0, st, g);
@@ -1116,7 +1169,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
       hipLaunchKernelGGL(mixer_carry_kernel<E>, dim3(nb, static_cast<unsigned>(g.n_groups)), dim3(256), 0, st, g);
       if (int rc = launch_check("mixer_carry_kernel")) return rc;
     }
-    if (int rc = launch_scans(g, true, st)) return rc;
+    if (int rc = launch_scans(g, true, !carries, st)) return rc;
   }
   hipLaunchKernelGGL(mixer_finish_kernel<E>, dim3(static_cast<unsigned>((g.Di + 255) / 256), static_cast<unsigned>(g.n_seqs)),
                      dim3(256), 0, st, g);
