@@ -9,8 +9,8 @@
 // All of it in float32 whatever E is: u, p, dt and h are never rounded to E (h is an
 // output in float32, and a u rounded to bf16 would leave 2^-9 in it).
 //
-// A token's launches: token_proj_kernel (conv, its state's update, x_proj over a block
-// of channels) and token_scan_kernel (the blocks' sums, dt, the state's update, the
+// A token's launches: token_proj_kernel or token_tile_kernel (conv, its state's update,
+// x_proj over a block of channels) and token_scan_kernel (the blocks' sums, dt, the state's update, the
 // gate).  x_proj sums over all channels, so two launches is the least.
 //
 // A prompt batch is one row of packed tokens cut into chunks of equal length,
@@ -446,6 +446,140 @@ __device__ __forceinline__ float planes_sum(const uint16_t* s, int plane, int at
   return (to_f(bf16_t{s[2 * plane + at]}) + to_f(bf16_t{s[plane + at]})) + to_f(bf16_t{s[at]});
 }
 
+// Eight consecutive elements, on a 16-byte boundary.
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(bf16_t* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+constexpr int kTileRows = 32, kTileK = 128;  // token_tile_kernel's
+constexpr int kTileThreads = kTileRows * kTileK / 8;
+
+// token_proj_kernel for many rows of whole vectors: a tile of 32 sequences and 128 channels, a
+// thread 8 channels of a sequence, x_proj on the matrix cores, a wave 32 of its outputs at a
+// time over half of the channels.  All of it is asked for before the first barrier; latency
+// bounds it (8 us of a step of 256 sequences, 17 by token_proj_kernel).
+template <class E, int KT>
+__global__ __launch_bounds__(kTileThreads, 2) void token_tile_kernel(Mixer<E> g) {
+  __shared__ __align__(16) uint16_t s_u[3 * kTileRows * kTileK];
+  __shared__ float s_half[4][16][kWave];
+  constexpr int kSteps = kTileK / 32;  // a wave's k steps
+  constexpr int kPlane = kTileRows * kTileK;
+  const int blk = static_cast<int>(blockIdx.x % g.n_blocks), c0 = blk * kTileK;
+  const int r0 = static_cast<int>(blockIdx.x / g.n_blocks) * kTileRows;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), l32 = lane & 31, half = lane >> 5;
+  const int w = wave_id() & 3, kh = wave_id() >> 2, kb = kh * (kTileK / 2);  // the wave's outputs, its half of the channels
+  constexpr int kChunks = kTileK / 8;
+  const int row = tid / kChunks, r = min(r0 + row, g.rows - 1), ch = c0 + tid % kChunks * 8, d = min(ch, g.Di - 8);
+  const bool live = r0 + row < g.rows && ch < g.Di;
+  const int skip_taps = KT - g.K;
+  Weight8<E> wt[kSteps];
+  const auto weights = [&](int j0) {
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk)
+      wt[kk].load(g.x_proj + static_cast<size_t>(min(j0 + l32, g.Nc - 1)) * g.Di, c0 + kb + kk * 16 + half * 8, g.Di, true);
+  };
+  weights(w * 32);
+  const int slot = start_slot(g, r), to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
+  float x[KT][8], cw[KT][8], u[8];
+#pragma unroll
+  for (int k = 0; k < KT - 1; ++k) {
+    if (k >= skip_taps && slot >= 0) {
+      load8(g.conv_state + (static_cast<size_t>(slot) * (g.K - 1) + k - skip_taps) * g.Di + d, 8, true, x[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+    }
+  }
+  load8(g.xz + static_cast<size_t>(r) * g.ld + d, 8, true, x[KT - 1]);
+  if (KT == 4 && g.K == 4) {  // a channel's taps side by side: two channels to eight
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float q[8];
+      load8(g.conv_w + static_cast<size_t>(d + e) * 4, 8, true, q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        cw[k % KT][e] = q[k];
+        cw[k % KT][e + 1] = q[4 + k];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cw[k][e] = k >= skip_taps ? to_f(g.conv_w[static_cast<size_t>(d + e) * g.K + k - skip_taps]) : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = 0.f;
+  if (g.conv_b != nullptr) load8(g.conv_b + d, 8, true, u);
+#pragma unroll
+  for (int k = 0; k < KT; ++k)
+    if (k >= skip_taps)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = fmaf(cw[k][e], x[k][e], u[e]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = live ? silu_f(u[e]) : 0.f;
+  uint32_t t[4][3];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split_pair(u[2 * e], u[2 * e + 1], t[e]);
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+    *reinterpret_cast<uint4*>(&s_u[q * kPlane + plane_at(row, tid % kChunks * 8, kTileK)]) = make_uint4(t[0][q], t[1][q], t[2][q], t[3][q]);
+  if (live) {
+    store8(g.u + static_cast<size_t>(r) * g.Di + d, u);
+    if (in_pool(g, to)) {
+#pragma unroll
+      for (int k = 1; k < KT; ++k)
+        if (k > skip_taps) store8(g.conv_state + (static_cast<size_t>(to) * (g.K - 1) + k - 1 - skip_taps) * g.Di + d, x[k]);
+    }
+  }
+  __syncthreads();
+  for (int base = 0; base < g.Nc; base += 128) {
+    const int j0 = base + w * 32;
+    if (base > 0) weights(j0);
+    floatx16 acc[2] = {};  // (the second stays zero)
+    if (j0 < g.Nc) {
+#pragma unroll
+      for (int kk = 0; kk < kSteps; ++kk) {
+        bf16x8 a[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          a[q] = *reinterpret_cast<const bf16x8*>(&s_u[q * kPlane + plane_at(l32, kb + kk * 16 + half * 8, kTileK)]);
+        wt[kk].split();
+        acc[0] = mfma_terms(a, wt[kk], acc[0]);
+      }
+      if (any_nonfinite(acc)) {
+        floatx16 again[2] = {};
+        const E* row_w = g.x_proj + static_cast<size_t>(min(j0 + l32, g.Nc - 1)) * g.Di;
+#pragma unroll 1
+        for (int q = 0; q < kTileK / 2; q += 2) {
+          const int k = kb + q + half;
+          again[0] = mfma32(planes_sum(s_u, kPlane, plane_at(l32, k, kTileK)), c0 + k < g.Di ? to_f(row_w[c0 + k]) : 0.f, again[0]);
+        }
+        keep_finite(again, acc);
+        acc[0] = again[0];
+      }
+    }
+    if (base > 0) __syncthreads();
+    if (kh == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s_half[w][i][lane] = acc[0][i];
+    }
+    __syncthreads();
+    if (kh == 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = r0 + 8 * (i >> 2) + 4 * half + (i & 3), col = j0 + l32;
+        if (at < g.rows && col < g.Nc)
+          g.part[(static_cast<size_t>(blk) * g.rows + at) * g.Nc + col] = acc[0][i] + s_half[w][i][lane];
+      }
+    }
+  }
+}
+
 constexpr int kPtRows = 64, kPtK = 64, kPtCols = 128;  // prompt_proj_kernel's tile and k step
 
 // A thread's share of a tile's conv: 4 channels of 4 rows, and the rows before them.
@@ -639,10 +773,50 @@ __global__ __launch_bounds__(256, 2) void prompt_proj_kernel(Mixer<E> g, int per
     }
 }
 
-// x_proj's sums over its splits: B and C in float32, the part for dt as three bf16 planes
-// [3][rows][Rp] (zeros from R on).
+// Prompt s's last K - 1 inputs, and its state where it is empty.
 template <class E>
-__global__ __launch_bounds__(256) void prompt_sum_kernel(Mixer<E> g) {
+__device__ __forceinline__ void finish(const Mixer<E>& g, int d, int s) {
+  if (d >= g.Di) return;
+  const int to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[s];
+  if (!in_pool(g, to)) return;
+  const int start = offset_of(g, s), end = max(offset_of(g, s + 1), start);
+  const int slot = start_slot(g, s);
+  float x[kMaxConv - 1];
+#pragma unroll
+  for (int k = 0; k < kMaxConv - 1; ++k)
+    if (k < g.K - 1) x[k] = conv_input(g, end - (g.K - 1) + k, start, slot, d);
+#pragma unroll
+  for (int k = 0; k < kMaxConv - 1; ++k)
+    if (k < g.K - 1) g.conv_state[(static_cast<size_t>(to) * (g.K - 1) + k) * g.Di + d] = from_f<E>(x[k]);
+  if (start == end && to != slot) {
+    const float* src = g.ssm + (static_cast<size_t>(max(slot, 0)) * g.N) * g.Di + d;
+    float* dst = g.ssm + (static_cast<size_t>(to) * g.N) * g.Di + d;
+    for (int n0 = 0; n0 < g.N; n0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = slot >= 0 ? src[static_cast<size_t>(min(n0 + i, g.N - 1)) * g.Di] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n0 + i < g.N) dst[static_cast<size_t>(n0 + i) * g.Di] = v[i];
+    }
+  }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void mixer_finish_kernel(Mixer<E> g) {
+  finish(g, static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x), static_cast<int>(blockIdx.y));
+}
+
+// x_proj's sums over its splits: B and C in float32, the part for dt as three bf16 planes
+// [3][rows][Rp] (zeros from R on).  Workgroups from `sums` on finish the prompts, where
+// nothing is resumed: no later kernel then reads what they write.
+template <class E>
+__global__ __launch_bounds__(256) void prompt_sum_kernel(Mixer<E> g, unsigned sums) {
+  if (blockIdx.x >= sums) {
+    const int blocks = (g.Di + 255) / 256, id = static_cast<int>(blockIdx.x - sums);
+    finish(g, id % blocks * 256 + static_cast<int>(threadIdx.x), id / blocks);
+    return;
+  }
   const int cols = g.Rp + 2 * g.Npad;
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= static_cast<long long>(g.rows) * cols) return;
@@ -989,37 +1163,6 @@ __global__ __launch_bounds__(256) void mixer_carry_kernel(Mixer<E> g) {
   fold(g.local, g.sum_dt, nd, g.Di, i, d, a2, c0, n_own, h, &total, [&](int c, float v) { g.carry[c * nd + i] = v; });
 }
 
-// Every prompt's last K - 1 inputs, and the states of empty prompts.
-template <class E>
-__global__ __launch_bounds__(256) void mixer_finish_kernel(Mixer<E> g) {
-  const int d = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
-  if (d >= g.Di) return;
-  const int s = static_cast<int>(blockIdx.y);
-  const int to = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[s];
-  if (!in_pool(g, to)) return;
-  const int start = offset_of(g, s), end = max(offset_of(g, s + 1), start);
-  const int slot = start_slot(g, s);
-  float x[kMaxConv - 1];
-#pragma unroll
-  for (int k = 0; k < kMaxConv - 1; ++k)
-    if (k < g.K - 1) x[k] = conv_input(g, end - (g.K - 1) + k, start, slot, d);
-#pragma unroll
-  for (int k = 0; k < kMaxConv - 1; ++k)
-    if (k < g.K - 1) g.conv_state[(static_cast<size_t>(to) * (g.K - 1) + k) * g.Di + d] = from_f<E>(x[k]);
-  if (start == end && to != slot) {
-    const float* src = g.ssm + (static_cast<size_t>(max(slot, 0)) * g.N) * g.Di + d;
-    float* dst = g.ssm + (static_cast<size_t>(to) * g.N) * g.Di + d;
-    for (int n0 = 0; n0 < g.N; n0 += 16) {
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = slot >= 0 ? src[static_cast<size_t>(min(n0 + i, g.N - 1)) * g.Di] : 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n0 + i < g.N) dst[static_cast<size_t>(n0 + i) * g.Di] = v[i];
-    }
-  }
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <class E, int NB, int KT>
@@ -1054,21 +1197,31 @@ constexpr int kTokenRows = 2;  // rows of a workgroup of token_scan_kernel where
 
 template <class E>
 int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
-  g.n_blocks = (g.Di + kProjBlock - 1) / kProjBlock;
+  // few rows: one each, in small workgroups, for the latency; many share the weights, on the
+  // matrix cores where every row is whole vectors
+  const bool many = g.rows >= 32, k4 = g.K <= 4;
+  const int e16 = 16 / static_cast<int>(sizeof(E));
+  const bool tiles = many && g.Di % 8 == 0 && g.ld % e16 == 0 && aligned16(g.xz) && aligned16(g.conv_state) &&
+                     aligned16(g.conv_w) && aligned16(g.conv_b) && aligned16(g.x_proj);
+  g.n_blocks = (g.Di + (tiles ? kTileK : kProjBlock) - 1) / (tiles ? kTileK : kProjBlock);
   const size_t part = static_cast<size_t>(g.n_blocks) * g.rows * g.Nc;
   void* ws = nullptr;
   if (int rc = acquire_workspace(call, (part + static_cast<size_t>(g.rows) * g.Di) * sizeof(float), &ws)) return rc;
   g.part = static_cast<float*>(ws);
   g.u = g.part + part;
   const bool vx = vec8(g.x_proj, g.Di);
-  // few rows: one each, in small workgroups, for the latency; many share the weights
-  const bool many = g.rows >= 32, k4 = g.K <= 4;
-  const int rb = many ? 8 : 1;
-  const dim3 ga(static_cast<unsigned>(g.n_blocks * ((g.rows + rb - 1) / rb)));
-  auto proj = many ? (k4 ? token_proj_kernel<E, 8, 4> : token_proj_kernel<E, 8, 8>)
-                   : (k4 ? token_proj_kernel<E, 1, 4> : token_proj_kernel<E, 1, 8>);
-  hipLaunchKernelGGL(proj, ga, dim3(kProjThreads), 0, st, g, vx);
-  if (int rc = launch_check("token_proj_kernel")) return rc;
+  if (tiles) {
+    const dim3 grid(static_cast<unsigned>(g.n_blocks * ((g.rows + kTileRows - 1) / kTileRows)));
+    hipLaunchKernelGGL(k4 ? (token_tile_kernel<E, 4>) : (token_tile_kernel<E, 8>), grid, dim3(kTileThreads), 0, st, g);
+    if (int rc = launch_check("token_tile_kernel")) return rc;
+  } else {
+    const int rb = many ? 8 : 1;
+    const dim3 grid(static_cast<unsigned>(g.n_blocks * ((g.rows + rb - 1) / rb)));
+    auto proj = many ? (k4 ? token_proj_kernel<E, 8, 4> : token_proj_kernel<E, 8, 8>)
+                     : (k4 ? token_proj_kernel<E, 1, 4> : token_proj_kernel<E, 1, 8>);
+    hipLaunchKernelGGL(proj, grid, dim3(kProjThreads), 0, st, g, vx);
+    if (int rc = launch_check("token_proj_kernel")) return rc;
+  }
   const int rt = many ? kTokenRows : 1, threads = many ? 256 : 64;
   const dim3 gb(static_cast<unsigned>((g.Di + threads - 1) / threads), static_cast<unsigned>((g.rows + rt - 1) / rt));
   const int Rq = (g.R + 15) / 16 * 16, Nq = (g.N + 15) / 16 * 16;
@@ -1141,7 +1294,9 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
                        vec8(g.x_proj, g.Di));
     if (int rc = launch_check("prompt_proj_kernel")) return rc;
     const int64_t sums = static_cast<int64_t>(g.rows) * (g.Rp + 2 * g.Npad);
-    hipLaunchKernelGGL(prompt_sum_kernel<E>, dim3(static_cast<unsigned>((sums + 255) / 256)), dim3(256), 0, st, g);
+    const unsigned sum_groups = static_cast<unsigned>((sums + 255) / 256);
+    const unsigned finishers = g.resume == nullptr ? static_cast<unsigned>((g.Di + 255) / 256) * static_cast<unsigned>(g.n_seqs) : 0;
+    hipLaunchKernelGGL(prompt_sum_kernel<E>, dim3(sum_groups + finishers), dim3(256), 0, st, g, sum_groups);
     if (int rc = launch_check("prompt_sum_kernel")) return rc;
     if (g.resume != nullptr) {
       g.init = f + o_init;
@@ -1170,6 +1325,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
       if (int rc = launch_check("mixer_carry_kernel")) return rc;
     }
     if (int rc = launch_scans(g, true, !carries, st)) return rc;
+    if (g.resume == nullptr) return OSSM_OK;  // the sums' launch has finished the prompts
   }
   hipLaunchKernelGGL(mixer_finish_kernel<E>, dim3(static_cast<unsigned>((g.Di + 255) / 256), static_cast<unsigned>(g.n_seqs)),
                      dim3(256), 0, st, g);
