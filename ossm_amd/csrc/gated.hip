@@ -123,14 +123,20 @@ typedef __attribute__((address_space(3))) void lds_void;
 template <int TK>
 __device__ __forceinline__ int row_turn(int r) { return TK == 64 ? r & 7 : (r >> 1) & 3; }
 
+// The same for LDS row k of a col operand of R columns: the four k of a transposing read then
+// lie in four stretches of 64 bytes.
+template <int R>
+__device__ __forceinline__ int col_turn(int k) { return R == 64 ? 4 * ((k >> 1) & 1) : 4 * (k & 3); }
+
 // One operand's tiles of R rows (of m or n) and TK k into LDS.  An LDS row is TK k (row) or R
-// columns (col) of 16-byte chunks; chunk c sits at c ^ row_turn (row) or c ^ 4 (k % 4)
+// columns (col) of 16-byte chunks; chunk c sits at c ^ row_turn (row) or c ^ col_turn
 // (col), which spreads the fragments' reads over the banks.  A thread's chunks are the same
 // in every tile, so their offsets are kept; chunks of rows past the matrix have one
 // that the buffer's range turns into zeros, and the last tile of k masks its own.
 template <bool COL, int R, int TK, int THREADS>
 struct TileLoad {
   static constexpr int kRounds = R * (TK / 8) / THREADS, kChunks = R / 8;
+  static_assert(!COL || R >= 64, "col_turn stays in a row");
   static constexpr int kRange = 0x40000000;  // every offset in a matrix is below it: 256 rows of 2^21 bytes
   int off[kRounds];
 
@@ -149,7 +155,7 @@ struct TileLoad {
         const int r = q / (TK / 8), c = row_chunk();
         off[i] = i0 + r < rows ? static_cast<int>(r * ld * 2) + c * 16 : kOutside;
       } else {
-        const int k = q / kChunks, c = (q % kChunks) ^ (4 * (k & 3));
+        const int k = q / kChunks, c = (q % kChunks) ^ col_turn<R>(k);
         off[i] = i0 + c * 8 < rows ? static_cast<int>(k * ld * 2) + c * 16 : kOutside;
       }
     }
@@ -177,7 +183,7 @@ __device__ __forceinline__ bf16x8 load_frag(const uint16_t* lds, int i0, int kk)
     // a group of 16 lanes reads 4 k of 16 columns, transposed: lane i gets column i
     const int g = lane >> 4, i16 = lane & 15, kr = i16 >> 2;
     const int k = kk * 16 + (g >> 1) * 8 + kr, col = i0 + (g & 1) * 16 + (i16 & 3) * 4;
-    const uint16_t* q = lds + k * R + (((col >> 3) ^ (4 * kr)) * 8) + (col & 7);
+    const uint16_t* q = lds + k * R + (((col >> 3) ^ col_turn<R>(k)) * 8) + (col & 7);  // (of k + 4 too)
     typedef __attribute__((address_space(3))) s16x4 lds4;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)q);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(q + 4 * R));
@@ -587,29 +593,55 @@ __device__ __forceinline__ void put8(uint16_t* dst, const uint16_t (&v)[8]) {
   *reinterpret_cast<u32x4*>(dst) = q;
 }
 
-// rows of C elements as 1 (bf16) or 3 (float32) planes of rows of Cp, zeros from C on
+// Rows of C elements as 1 (bf16) or 3 (float32) planes of rows of Cp, zeros from C on; up to
+// three matrices in a launch, each from its own workgroup on.
 template <class E>
-__global__ __launch_bounds__(256) void pack_kernel(const E* __restrict__ src, long long ld, uint16_t* __restrict__ dst,
-                                                   long long plane, long long rows, int C, int Cp) {
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const int chunks = Cp / 8;
-  if (i >= rows * chunks) return;
-  const long long r = i / chunks;
-  const int c = static_cast<int>(i % chunks) * 8;
-  const E* s = src + r * ld + c;
+struct PackJobs {
+  const E* src[3];
+  uint16_t* dst[3];
+  long long ld[3], plane[3], chunks[3];  // chunks of 8 in all
+  int C[3], Cp[3];
+  bool pairs[3];  // every pair of elements is aligned
+  unsigned first[3];
+  int n;
+};
+
+template <class E>
+__global__ __launch_bounds__(256) void pack_kernel(PackJobs<E> g) {
+  int job = 0;
+#pragma unroll
+  for (int i = 1; i < 3; ++i)
+    if (i < g.n && blockIdx.x >= g.first[i]) job = i;
+  const long long i = static_cast<long long>(blockIdx.x - g.first[job]) * 256 + threadIdx.x;
+  if (i >= g.chunks[job]) return;
+  const int C = g.C[job], Cp = g.Cp[job], row = Cp / 8;
+  const long long r = i / row;
+  const int c = static_cast<int>(i % row) * 8;
+  const E* s = g.src[job] + r * g.ld[job] + c;
+  E x[8];
+  if (c + 8 <= C && g.pairs[job]) {
+    struct alignas(2 * sizeof(E)) Pair { E v[2]; };
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const Pair q = *reinterpret_cast<const Pair*>(s + k);
+      x[k] = q.v[0];
+      x[k + 1] = q.v[1];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < C ? s[k] : E{};
+  }
   uint16_t t[3][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     uint16_t v[3] = {0, 0, 0};
-    if (c + k < C) {
-      if constexpr (sizeof(E) == 4) split3(s[k], v);
-      else v[0] = s[k].bits;
-    }
+    if constexpr (sizeof(E) == 4) split3(x[k], v);
+    else v[0] = x[k].bits;
 #pragma unroll
     for (int j = 0; j < 3; ++j) t[j][k] = v[j];
   }
 #pragma unroll
-  for (int j = 0; j < (sizeof(E) == 4 ? 3 : 1); ++j) put8(dst + j * plane + r * Cp + c, t[j]);
+  for (int j = 0; j < (sizeof(E) == 4 ? 3 : 1); ++j) put8(g.dst[job] + j * g.plane[job] + r * Cp + c, t[j]);
 }
 
 // ---- da, db ----------------------------------------------------------------------
@@ -745,26 +777,43 @@ struct Source {
   int64_t elems() const { return direct() ? 0 : n * plane() * (sizeof(E) == 4 ? 3 : 1); }  // of bf16
 };
 
+// The operand that m makes, its planes (if it needs any) at ws, as more of `jobs`.
 template <class E>
-int pack(const Source<E>& m, uint16_t* ws, Operand* o, hipStream_t st) {
-  if (m.direct()) {
-    for (int i = 0; i < m.n; ++i) o->p[i] = reinterpret_cast<const uint16_t*>(m.src[i]);
-    o->ld = m.ld[0];
-    o->plane = 0;
-    return OSSM_OK;
-  }
-  const int64_t cp = up8(m.cols), chunks = m.rows * (cp / 8);
-  if (chunks == 0) return OSSM_OK;  // nothing is read
-  o->ld = cp;
-  o->plane = m.plane();
+Operand operand(const Source<E>& m, uint16_t* ws, PackJobs<E>* jobs) {
+  Operand o{};
+  o.ld = m.ld[0];
+  for (int i = 0; i < m.n; ++i) o.p[i] = reinterpret_cast<const uint16_t*>(m.src[i]);
+  if (m.direct()) return o;
+  const int64_t cp = up8(m.cols);
+  o.ld = cp;
+  o.plane = m.plane();
   for (int i = 0; i < m.n; ++i) {
     uint16_t* dst = ws + i * (m.elems() / m.n);
-    o->p[i] = dst;
-    hipLaunchKernelGGL(pack_kernel<E>, dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, st, m.src[i], m.ld[i],
-                       dst, o->plane, m.rows, static_cast<int>(m.cols), static_cast<int>(cp));
-    if (int rc = launch_check("pack_kernel")) return rc;
+    o.p[i] = dst;
+    const int j = jobs->n++;
+    jobs->src[j] = m.src[i];
+    jobs->dst[j] = dst;
+    jobs->ld[j] = m.ld[i];
+    jobs->plane[j] = o.plane;
+    jobs->chunks[j] = m.rows * (cp / 8);
+    jobs->pairs[j] = m.ld[i] % 2 == 0 && (reinterpret_cast<uintptr_t>(m.src[i]) & (2 * sizeof(E) - 1)) == 0;
+    jobs->C[j] = static_cast<int>(m.cols);
+    jobs->Cp[j] = static_cast<int>(cp);
   }
-  return OSSM_OK;
+  return o;
+}
+
+template <class E>
+int pack(PackJobs<E> jobs, hipStream_t st) {
+  int64_t blocks = 0;
+  for (int i = 0; i < jobs.n; ++i) {
+    jobs.first[i] = static_cast<unsigned>(blocks);
+    blocks += (jobs.chunks[i] + 255) / 256;
+  }
+  if (blocks == 0) return OSSM_OK;  // nothing to copy, or nothing in it
+  if (blocks > INT_MAX) return set_error(OSSM_ERR_UNSUPPORTED, "gated: size exceeds launch limits");
+  hipLaunchKernelGGL(pack_kernel<E>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, jobs);
+  return launch_check("pack_kernel");
 }
 
 template <class E, bool ACOL, bool BCOL, bool GATED, int WM, int WN, int FM, int FN>
@@ -792,7 +841,8 @@ int launch_tiled(Product<E> g, hipStream_t st) {
 int64_t tiles(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 
 // How many ways the k of an [M, N] product of `k_tiles` tiles is split: towards two
-// workgroups a CU, none with fewer than 16 tiles.
+// workgroups a CU, none with fewer than 8 tiles (dx of [25600, 128] from 2 x 512 in float32,
+// 200 tiles: two ways and their sum 96 us, unsplit in tiles half as high 129).
 int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t cus) {
   const int64_t t = std::max<int64_t>(1, tiles(m, n, 128, 128));  // an input without columns has none
   return static_cast<int>(std::max<int64_t>(1, std::min(2 * cus / t, k_tiles / 8)));
@@ -805,6 +855,10 @@ int launch_product(Product<E> g, int64_t cus, hipStream_t st) {
   g.splits = (k_tiles + g.per_split - 1) / g.per_split;
   if (g.splits == 1 && tiles(g.M, g.N, 256, GATED ? 128 : 256) >= cus)
     return launch_tiled<E, ACOL, BCOL, GATED, 2, 4, 4, 2>(g, st);
+  // too few tiles for two workgroups a CU: half as high ([1001, 1022] -> 2730 in float32, 344
+  // tiles: 97 -> 89 us)
+  if (g.splits == 1 && tiles(g.M, g.N, 128, GATED ? 64 : 128) < 2 * cus)
+    return launch_tiled<E, ACOL, BCOL, GATED, 2, 2, 1, 2>(g, st);
   return launch_tiled<E, ACOL, BCOL, GATED, 2, 2, 2, 2>(g, st);
 }
 
@@ -860,8 +914,10 @@ int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipSt
     if (int rc = acquire_workspace(call, static_cast<size_t>(px.elems() + pw.elems()) * 2, &ws)) return rc;
   Product<E> g{};
   uint16_t* q = static_cast<uint16_t*>(ws);
-  if (int rc = pack(px, q, &g.a, st)) return rc;
-  if (int rc = pack(pw, q + px.elems(), &g.b, st)) return rc;
+  PackJobs<E> jobs{};
+  g.a = operand(px, q, &jobs);
+  g.b = operand(pw, q + px.elems(), &jobs);
+  if (int rc = pack(jobs, st)) return rc;
   g.M = static_cast<int>(p.T);
   g.N = static_cast<int>(p.F);
   g.K = static_cast<int>(p.D);
@@ -941,8 +997,12 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   g.a.ld = 2 * Fp;
   g.N = D;
   g.ldc = p.D;
+  PackJobs<E> jobs{};
+  const Operand w_op = gx != nullptr ? operand(pw, reinterpret_cast<uint16_t*>(base + o_w), &jobs) : Operand{};
+  const Operand x_op = want_w ? operand(px, reinterpret_cast<uint16_t*>(base + o_x), &jobs) : Operand{};
+  if (int rc = pack(jobs, st)) return rc;
   if (gx != nullptr) {
-    if (int rc = pack(pw, reinterpret_cast<uint16_t*>(base + o_w), &g.b, st)) return rc;
+    g.b = w_op;
     g.M = T;
     g.K = F;
     g.parts = 2;
@@ -952,7 +1012,7 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
     if (int rc = launch_product<E, false, true, false>(g, cus, st)) return rc;
   }
   if (want_w) {
-    if (int rc = pack(px, reinterpret_cast<uint16_t*>(base + o_x), &g.b, st)) return rc;
+    g.b = x_op;
     g.M = 2 * fp;
     g.K = T;
     g.parts = 1;
