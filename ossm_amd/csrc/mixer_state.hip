@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, int Rq, int
     to[rr] = (g.out_slots != nullptr ? g.out_slots : g.in_slots)[r];
     const float* src = g.ssm + (static_cast<size_t>(max(in[rr], 0)) * g.N) * g.Di + d;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) h[rr][i] = in[rr] >= 0 && i < g.N ? src[static_cast<size_t>(i) * g.Di] : 0.f;
+    for (int i = 0; i < NB; ++i) h[rr][i] = in[rr] >= 0 && i < g.N ? __builtin_nontemporal_load(src + static_cast<size_t>(i) * g.Di) : 0.f;
     u[rr] = g.u[static_cast<size_t>(r) * g.Di + d];
     z[rr] = to_f(g.xz[static_cast<size_t>(r) * g.ld + g.Di + d]);
   }
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void token_scan_kernel(Mixer<E> g, int Rq, int
           const float v = fmaf(__builtin_amdgcn_exp2f(a2[i + k] * dt[rr]), h[rr][i + k], du[rr] * b[k]);
           if (n0 + i + k < g.N) {
             y[rr] = fmaf(c[k], v, y[rr]);
-            if (keep) dst[static_cast<size_t>(i + k) * g.Di] = v;
+            if (keep) __builtin_nontemporal_store(v, dst + static_cast<size_t>(i + k) * g.Di);
           }
         }
       }
