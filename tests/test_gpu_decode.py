@@ -135,6 +135,46 @@ def test_step_matches_float64(D, size, rows, dtype):
     check(c.ssm, want[2], torch.float32, "ssm state")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size, lengths", [
+    ((600, 16, 10, 4), [700, 0, 1, 1300, 15]),  # over a hundred chunks: dt by its own kernel, chunks in groups
+    ((1030, 40, 33, 5), [513, 1, 700, 2]),  # two passes over the states, odd ranks
+    ((128, 16, 8, 4), [9000, 3, 17, 160])], ids=["600", "1030", "128"])
+def test_large_prompts(D, size, lengths, dtype):
+    for resumed in (False, True):
+        c = Case(*size, lengths, dtype, seed=20, pad=9)
+        announce(f"mixer_prompt {size} {lengths} {dtype} resumed={resumed}")
+        want = reference(c, c.resume.tolist() if resumed else [False] * c.S)
+        y = run_prompt(D, c, c.resume if resumed else None)
+        check(y, want[0], dtype, "y")
+        check(c.conv, want[1], torch.float32, "conv state")
+        check(c.ssm, want[2], torch.float32, "ssm state")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [(600, 16, 38, 4), (1030, 40, 33, 5)], ids=["600", "1030"])
+def test_large_steps(D, size, dtype):
+    c = Case(*size, [1] * 301, dtype, seed=21)
+    announce(f"mixer_step {size} rows=301 {dtype}")
+    want = reference(c, [True] * 301)
+    y = D.mixer_step(c.xz, *c.args(), skip=c.skip)
+    check(y, want[0], dtype, "y")
+    check(c.conv, want[1], torch.float32, "conv state")
+    check(c.ssm, want[2], torch.float32, "ssm state")
+
+
+def test_values_of_one_large_prompt_stay_in_it(D):
+    lengths = [700, 800, 900]
+    a, b = Case(600, 16, 10, 4, lengths, seed=22), Case(600, 16, 10, 4, lengths, seed=22)
+    b.xz[900] = float("nan")  # in the second prompt
+    announce("mixer_prompt of three large prompts, NaN in one")
+    ya, yb = run_prompt(D, a), run_prompt(D, b)
+    assert torch.equal(ya[:900], yb[:900]) and torch.equal(ya[1500:], yb[1500:])
+    assert torch.isnan(yb[900:1500]).all()
+    others = [s for s in range(a.ssm.size(0)) if s != int(a.slots[1])]
+    assert torch.equal(a.ssm[others], b.ssm[others]) and torch.isnan(b.ssm[int(a.slots[1])]).all()
+
+
 @pytest.mark.parametrize("rows", [4, 40])
 def test_slots_outside_the_pool_and_forks(D, rows):
     """-1 starts from zeros or keeps nothing; a row with neither is padding; other out
