@@ -3,7 +3,10 @@
 ``ossm_amd._kernels`` is the drop-in module (same names and signatures as the
 reference extension); ``ossm_amd.bridge`` holds autograd wrappers with the
 reference bridges' semantics; the C ABI is ``include/ossm_scan.h``, built by
-``python -m ossm_amd.build`` into ``ossm_amd/_lib/libossm_scan.so``.
+``python -m ossm_amd.build`` into ``ossm_amd/_lib/libossm_scan.so``.  The operators of
+language models (``include/ossm_lm.h``) are ``ossm_amd.decode`` (the Mamba mixer served),
+``ossm_amd.gated`` (gated feed-forward) and ``ossm_amd.logits`` (control of the logits);
+``ossm_amd.decoder`` is a small model that runs them together.
 """
 
 from __future__ import annotations
