@@ -460,49 +460,38 @@ __global__ __launch_bounds__(256) void product_sum_kernel(Product<E> g) {
 }
 
 // ---- few rows ---------------------------------------------------------------------
-// Up to 32 NT rows of x: the weights' traffic is all there is (9.4 us for two of [5632, 2048]
-// in bf16), so each is read once, straight into fragments, and none goes through LDS.  A
-// workgroup takes 16 outputs, whose gate rows are rows 0-15 of a fragment and whose up rows
-// 16-31: a lane then holds a and b of an output 8 registers apart.  Its waves share k in
-// blocks of 64 (a lane reads 64 consecutive bytes in bf16) and add their sums in LDS in a
-// fixed order.  float32 takes the fp32 matrix instruction: nothing to split, and its rate
-// is above the memory's.
+// Few rows of x, 16 NT to a workgroup: the weights' traffic is all there is (9.4 us for two of
+// [5632, 2048] in bf16; 11 at 4 rows), so each is read once, straight into fragments, and
+// none goes through LDS.  A workgroup takes 16 outputs of both projections.  Its waves share k in blocks of 128 bytes
+// of a row, whole lines (where a lane read 128 bytes by itself, lines left the L1 between its
+// loads: 118 us for 16 rows of float32, 28 now), ask for kAhead blocks together, and add their
+// sums in LDS in a fixed order.  float32 takes the fp32 matrix instruction: nothing to
+// split, and its rate is above the memory's.
 constexpr int kRowWaves = 8, kRowOut = 16;
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 
+// 16 bytes of a row: an operand of a 16 x 16 product, lane l's row l % 16, its k the
+// (l / 16)-th stretch of 16 bytes in 64.
 template <class E>
-struct Frag8;
-template <>
-struct Frag8<bf16_t> {
-  bf16x8 v;
-  __device__ __forceinline__ void load(const bf16_t* row, int k, int n, bool vec) {
-    if (vec) {
-      v = k < n ? *reinterpret_cast<const bf16x8*>(row + k) : bf16x8{};  // n is a multiple of 8
-    } else {
+struct Piece {
+  static constexpr int kN = 16 / static_cast<int>(sizeof(E));
+  E v[kN];
+  __device__ __forceinline__ void load(const E* p) {
+    struct __attribute__((packed, aligned(sizeof(E)))) Any { u32x4 q; };
+    const u32x4 q = reinterpret_cast<const Any*>(p)->q;  // whatever its alignment
+    __builtin_memcpy(v, &q, 16);
+  }
+  __device__ __forceinline__ void load_some(const E* row, int k, int n) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(__bf16, k + i < n ? row[k + i].bits : static_cast<uint16_t>(0));
-    }
+    for (int i = 0; i < kN; ++i) v[i] = k + i < n ? row[k + i] : E{};
   }
 };
-template <>
-struct Frag8<float> {
-  float v[8];
-  __device__ __forceinline__ void load(const float* row, int k, int n, bool vec) {
-    if (vec) {
-      const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 a = k < n ? reinterpret_cast<const float4*>(row + k)[0] : z;  // n is a multiple of 8
-      const float4 b = k < n ? reinterpret_cast<const float4*>(row + k)[1] : z;
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+__device__ __forceinline__ floatx4 product16(const Piece<bf16_t>& a, const Piece<bf16_t>& b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 product16(const Piece<float>& a, const Piece<float>& b, floatx4 c) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = k + i < n ? row[k + i] : 0.f;
-    }
-  }
-};
-__device__ __forceinline__ floatx16 mfma8(const Frag8<bf16_t>& a, const Frag8<bf16_t>& b, floatx16 c) { return mfma_bf16(a.v, b.v, c); }
-__device__ __forceinline__ floatx16 mfma8(const Frag8<float>& a, const Frag8<float>& b, floatx16 c) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c = mfma32(a.v[i], b.v[i], c);
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
   return c;
 }
 
@@ -518,51 +507,78 @@ struct FewRows {
 };
 
 template <class E, int NT>
-__global__ __launch_bounds__(kRowWaves * kWave, 2) void few_rows_kernel(FewRows<E> g, bool vec) {
-  __shared__ float s_sum[kRowWaves][NT][32 * 32];
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), w = wave_id(), l32 = lane & 31, half = lane >> 5;
+__global__ __launch_bounds__(kRowWaves * kWave, 4) void few_rows_kernel(FewRows<E> g) {
+  constexpr int kAhead = NT == 1 ? 4 : NT == 2 ? 2 : 1;
+  constexpr int kPiece = Piece<E>::kN, kStep = 4 * kPiece, kBlockK = 2 * kStep;
+  __shared__ float s_sum[kRowWaves][2][NT][16 * 16];
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), w = wave_id(), l16 = lane & 15, part = lane >> 4;
   const int f0 = static_cast<int>(blockIdx.x) * kRowOut;
-  const int f = min(f0 + (l32 & 15), g.F - 1), up = l32 >> 4;
-  const E* row_w = g.w[up] + f * g.ld_w[up];
+  const int t0 = static_cast<int>(blockIdx.y) * 16 * NT;
+  const E* row_w[2];
   const E* row_x[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) row_x[t] = g.x + min(t * 32 + l32, g.T - 1) * g.ld_x;
-  floatx16 acc[NT] = {};
-  const int blocks = (g.D + 63) / 64;
-  constexpr int kAhead = NT == 1 && sizeof(E) == 2 ? 4 : 1;  // blocks whose fragments are asked for together
-  for (int b0 = w; b0 < blocks; b0 += kRowWaves * kAhead) {
-    Frag8<E> fw[kAhead][4], fx[kAhead][4][NT];
+  for (int j = 0; j < 2; ++j) row_w[j] = g.w[j] + min(f0 + l16, g.F - 1) * g.ld_w[j];
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q)
+  for (int t = 0; t < NT; ++t) row_x[t] = g.x + min(t0 + t * 16 + l16, g.T - 1) * g.ld_x;
+  floatx4 acc[2][NT] = {};
+  const auto products = [&](const Piece<E> (&pw)[2], const Piece<E> (&px)[NT]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = (b0 + q * kRowWaves) * 64 + half * 32 + i * 8;  // past D: zeros
-        fw[q][i].load(row_w, k, g.D, vec);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) fx[q][i][t].load(row_x[t], k, g.D, vec);
+      for (int j = 0; j < 2; ++j) acc[j][t] = product16(px[t], pw[j], acc[j][t]);
+  };
+  const int whole = g.D / kBlockK;
+  for (int b0 = w; b0 < whole; b0 += kRowWaves * kAhead) {
+    Piece<E> fw[kAhead][2][2], fx[kAhead][2][NT];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int b = b0 + q * kRowWaves;
+      if (b >= whole) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = b * kBlockK + i * kStep + part * kPiece;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) fw[q][i][j].load(row_w[j] + k);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fx[q][i][t].load(row_x[t] + k);
       }
+    }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q)
+      if (b0 + q * kRowWaves < whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t] = mfma8(fw[q][i], fx[q][i][t], acc[t]);
+        for (int i = 0; i < 2; ++i) products(fw[q][i], fx[q][i]);
+      }
   }
-  // row m (output) of token l32: register r holds m = 8 (r / 4) + 4 half + r % 4
+  if (w == whole % kRowWaves) {  // the rest, zeros past D
+#pragma unroll 1
+    for (int k0 = whole * kBlockK; k0 < g.D; k0 += kStep) {
+      Piece<E> fw[2], fx[NT];
+      const int k = k0 + part * kPiece;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+      for (int j = 0; j < 2; ++j) fw[j].load_some(row_w[j], k, g.D);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s_sum[w][t][(8 * (r >> 2) + 4 * half + (r & 3)) * 32 + l32] = acc[t][r];
+      for (int t = 0; t < NT; ++t) fx[t].load_some(row_x[t], k, g.D);
+      products(fw, fx);
+    }
+  }
+  // a lane's output l % 16, its tokens 4 (l / 16) + r
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_sum[w][j][t][(4 * part + r) * 16 + l16] = acc[j][t][r];
   __syncthreads();
   // outputs fastest, so that neighbouring lanes store neighbouring values
-  for (int i = threadIdx.x; i < NT * 32 * kRowOut; i += kRowWaves * kWave) {
-    const int m = i % kRowOut, token = i / kRowOut, t = token >> 5, l = token & 31, n = f0 + m;
+  for (int i = threadIdx.x; i < NT * 16 * kRowOut; i += kRowWaves * kWave) {
+    const int t = i / (16 * kRowOut), at_sum = i % (16 * kRowOut), token = t0 + i / kRowOut, n = f0 + i % kRowOut;
     if (token >= g.T || n >= g.F) continue;
     float a = 0.f, b = 0.f;
 #pragma unroll
     for (int v = 0; v < kRowWaves; ++v) {
-      a += s_sum[v][t][m * 32 + l];
-      b += s_sum[v][t][(m + 16) * 32 + l];
+      a += s_sum[v][0][t][at_sum];
+      b += s_sum[v][1][t][at_sum];
     }
     if (g.bias[0] != nullptr) a += to_f(g.bias[0][n]);
     if (g.bias[1] != nullptr) b += to_f(g.bias[1][n]);
@@ -894,26 +910,30 @@ struct Gated {
   Source<E> weights() const { return {{w[0], w[1]}, {ld_w[0], ld_w[1]}, F, D, 2}; }
 };
 
-// Rows up to which the weights' traffic bounds the forward and few_rows_kernel takes it.
-constexpr int64_t kFewRows = 64;
+// Whether few_rows_kernel takes a forward, by itself and by the products, us: 64 rows of
+// [2048] -> 5632 in bf16 25 and 25, 96 37 and 25; where the operands would be packed first, 128
+// of them in float32 94 and 154, 192 151 and 156, and of [1022] -> 2730 in bf16 16 and 24.
+// Small products leave the products' tiles few: [512] -> 2048 in bf16 5.5 and 8.3 at 64 rows,
+// 8.6 and 8.7 at 256, 15 and 9.2 at 512; in float32 19 and 40 at 256, 36 and 43 at 512.
+bool few(int64_t T, int64_t D, int64_t F, bool packed, int64_t small) {
+  return T <= (packed ? 128 : 64) || (T <= 512 && T * D * F <= small);
+}
 
 template <class E>
 int few_rows(const Gated<E>& p, E* y, float* a, float* b, hipStream_t st) {
   const FewRows<E> g{p.x, {p.w[0], p.w[1]}, {p.bias[0], p.bias[1]}, y, {a, b}, p.ld_x, {p.ld_w[0], p.ld_w[1]},
                      static_cast<int>(p.T), static_cast<int>(p.D), static_cast<int>(p.F), p.act};
-  constexpr int e = sizeof(E);
-  const bool vec = p.D % 8 == 0 && aligned16(p.x) && aligned16(p.w[0]) && aligned16(p.w[1]) && p.ld_x * e % 16 == 0 &&
-                   p.ld_w[0] * e % 16 == 0 && p.ld_w[1] * e % 16 == 0;
-  const dim3 grid(static_cast<unsigned>((p.F + kRowOut - 1) / kRowOut));
-  if (p.T <= 32) hipLaunchKernelGGL((few_rows_kernel<E, 1>), grid, dim3(kRowWaves * kWave), 0, st, g, vec);
-  else hipLaunchKernelGGL((few_rows_kernel<E, 2>), grid, dim3(kRowWaves * kWave), 0, st, g, vec);
+  const dim3 grid(static_cast<unsigned>((p.F + kRowOut - 1) / kRowOut), static_cast<unsigned>((p.T + 63) / 64));
+  hipLaunchKernelGGL((p.T <= 16 ? few_rows_kernel<E, 1> : p.T <= 32 ? few_rows_kernel<E, 2> : few_rows_kernel<E, 4>), grid,
+                     dim3(kRowWaves * kWave), 0, st, g);
   return launch_check("few_rows_kernel");
 }
 
 template <class E>
 int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipStream_t st) {
-  if (p.T <= kFewRows) return few_rows(p, y, a, b, st);
   const Source<E> px = p.rows(), pw = p.weights();
+  if (few(p.T, p.D, p.F, !px.direct() || !pw.direct(), int64_t(1) << (sizeof(E) == 4 ? 29 : 28)))
+    return few_rows(p, y, a, b, st);
   void* ws = nullptr;
   if (px.elems() + pw.elems() > 0)
     if (int rc = acquire_workspace(call, static_cast<size_t>(px.elems() + pw.elems()) * 2, &ws)) return rc;

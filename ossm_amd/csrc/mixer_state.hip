@@ -1197,9 +1197,13 @@ constexpr int kTokenRows = 2;  // rows of a workgroup of token_scan_kernel where
 
 template <class E>
 int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
-  // few rows: one each, in small workgroups, for the latency; many share the weights, on the
-  // matrix cores where every row is whole vectors
-  const bool many = g.rows >= 32, k4 = g.K <= 4;
+  // Few rows: one each, in small workgroups, for the latency.  Many share the weights, the
+  // projection's on the matrix cores where every row is whole vectors, from 400 channels a CU
+  // on (a row at a time and shared, us of a step: 32 rows of d_inner 2048 15 and 16, 64 18.5 and
+  // 17.4, 128 28 and 21; 128 of 512 13 and 14, 384 21 and 17), the scan's from 16 waves of
+  // channels a CU on, what it holds at once (128 of 2048 21 and 24, 192 32 and 27).
+  const int64_t channels = static_cast<int64_t>(g.rows) * g.Di, cus = std::max(1, device_cu_count(call.device()));
+  const bool many = channels >= 400 * cus, many_scan = channels >= 16 * kWave * cus, k4 = g.K <= 4;
   const int e16 = 16 / static_cast<int>(sizeof(E));
   const bool tiles = many && g.Di % 8 == 0 && g.ld % e16 == 0 && aligned16(g.xz) && aligned16(g.conv_state) &&
                      aligned16(g.conv_w) && aligned16(g.conv_b) && aligned16(g.x_proj);
@@ -1222,12 +1226,12 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
     hipLaunchKernelGGL(proj, grid, dim3(kProjThreads), 0, st, g, vx);
     if (int rc = launch_check("token_proj_kernel")) return rc;
   }
-  const int rt = many ? kTokenRows : 1, threads = many ? 256 : 64;
+  const int rt = many_scan ? kTokenRows : 1, threads = many_scan ? 256 : 64;
   const dim3 gb(static_cast<unsigned>((g.Di + threads - 1) / threads), static_cast<unsigned>((g.rows + rt - 1) / rt));
   const int Rq = (g.R + 15) / 16 * 16, Nq = (g.N + 15) / 16 * 16;
   const size_t lds = static_cast<size_t>(rt) * (Rq + 2 * Nq) * sizeof(float);
   const bool vec = vec8(g.dt_proj, g.R) && vec8(g.a_log, g.N);
-  hipLaunchKernelGGL(many ? (vec ? token_scan_kernel<E, kTokenRows, true> : token_scan_kernel<E, kTokenRows, false>)
+  hipLaunchKernelGGL(many_scan ? (vec ? token_scan_kernel<E, kTokenRows, true> : token_scan_kernel<E, kTokenRows, false>)
                           : (vec ? token_scan_kernel<E, 1, true> : token_scan_kernel<E, 1, false>),
                      gb, dim3(threads), lds, st, g, Rq, Nq);
   return launch_check("token_scan_kernel");

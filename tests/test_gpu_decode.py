@@ -163,6 +163,45 @@ def test_large_steps(D, size, dtype):
     check(c.ssm, want[2], torch.float32, "ssm state")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("channels", [103000, 263000])  # weights shared by the projection, and by the scan
+@pytest.mark.parametrize("size", [s for s in SIZES if s[0] >= 64], ids=lambda s: "x".join(map(str, s)))
+def test_steps_of_many_sequences(D, size, channels, dtype):
+    rows = channels // size[0] + 2
+    c = Case(*size, [1] * rows, dtype, seed=23, skip=channels < 200000, bias=channels > 200000)
+    announce(f"mixer_step {size} rows={rows} {dtype}")
+    want = reference(c, [True] * rows)
+    y = D.mixer_step(c.xz, *c.args(), skip=c.skip)
+    check(y, want[0], dtype, "y")
+    check(c.conv, want[1], torch.float32, "conv state")
+    check(c.ssm, want[2], torch.float32, "ssm state")
+
+
+@pytest.mark.parametrize("Di", [128, 130])
+def test_slots_and_values_among_many_sequences(D, Di):
+    """Padding, rows from zeros, rows that keep nothing; NaN in one row leaves the others' bits."""
+    rows = 2100
+    c = Case(Di, 16, 8, 4, [1] * rows, seed=24)
+    c.slots[1], c.slots[3] = -1, 10 ** 6
+    used = set(c.slots.tolist())
+    outs = torch.tensor([s for s in range(c.ssm.size(0)) if s not in used][:rows], dtype=torch.int32).cuda()
+    outs[2], outs[3] = -1, -1
+    announce(f"mixer_step among {rows} sequences, d_inner {Di}")
+    want = reference(c, [True] * rows, outs)
+    want[0][3] = 0  # padding
+    conv, ssm = c.conv.clone(), c.ssm.clone()
+    y = D.mixer_step(c.xz, *c.args(), skip=c.skip, out_slots=outs)
+    for got, w in zip((y, c.conv, c.ssm), want):
+        check(got, w)
+    bad = c.xz.clone()
+    bad[40] = float("nan")
+    z = D.mixer_step(bad, *c.args(conv, ssm), skip=c.skip, out_slots=outs)
+    keep = [i for i in range(rows) if i != 40]
+    assert torch.equal(y[keep], z[keep]) and torch.isnan(z[40]).all()
+    others = [s for s in range(ssm.size(0)) if s != int(outs[40])]
+    assert torch.equal(c.ssm[others], ssm[others]) and torch.isnan(ssm[int(outs[40])]).all()
+
+
 def test_values_of_one_large_prompt_stay_in_it(D):
     lengths = [700, 800, 900]
     a, b = Case(600, 16, 10, 4, lengths, seed=22), Case(600, 16, 10, 4, lengths, seed=22)

@@ -116,6 +116,54 @@ def test_large_tiles(G, dtype):
             check(g, w, dtype, f"grad {n}", True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(513, 40, 70), (520, 130, 33), (700, 264, 40), (1025, 7, 5)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_forward_past_few_rows(G, shape, dtype):
+    """Products over the whole batch, however small."""
+    for i, act in enumerate(ACTS):
+        args, _ = inputs(*shape, dtype, i % 2 == 0, seed=20 + i)
+        announce(f"gated_linear products {shape} {dtype} {act}")
+        with torch.no_grad():
+            check(G.gated_linear(*args, activation=act), reference(*args, act), dtype, act)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_values_that_are_not_finite_past_few_rows(G, dtype):
+    args, _ = inputs(600, 40, 70, dtype, False, seed=21)
+    x, wg, wu = args[:3]
+    base = G.gated_linear(x, wg, wu, activation="relu")
+    for value in (float("inf"), -float("inf"), float("nan")):
+        xi, wi = x.clone(), wu.clone()
+        xi[1, 3] = value
+        wi[69, 5] = value
+        announce(f"gated_linear {value} rows=600 {dtype}")
+        y = G.gated_linear(xi, wg, wi, activation="relu")
+        keep = [i for i in range(600) if i != 1]
+        assert torch.equal(y[keep][:, :69], base[keep][:, :69])
+        want = reference(xi, wg, wi, None, None, "relu")
+        g = y.double().cpu().numpy()
+        assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(np.isposinf(g), np.isposinf(want))
+        assert np.array_equal(np.isneginf(g), np.isneginf(want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_few_rows_of_any_alignment(G, dtype):
+    """Rows and sizes at every offset, D from below a block to several, several groups of rows."""
+    for T, D, n in ((1, 31, 17), (15, 33, 16), (16, 128, 40), (31, 300, 15), (33, 2050, 48), (63, 513, 31), (127, 1025, 50),
+                    (200, 1000, 70)):
+        args, _ = inputs(T, D, n, dtype, True, seed=T)
+        want = reference(*args, "silu")
+        for off in (0, 1, 3, 8):
+            wide = [torch.full((t.size(0), D + 11), float("nan"), dtype=dtype, device="cuda") for t in args[:3]]
+            for w, t in zip(wide, args):
+                w[:, off:off + D] = t
+            announce(f"gated_linear few rows {T} {D} {n} offset {off} {dtype}")
+            with torch.no_grad():
+                y = G.gated_linear(*(w[:, off:off + D] for w in wide), *args[3:])
+            check(y, want, dtype, f"offset {off}")
+
+
 def test_gradients_against_differences(G):
     """Central differences of a random projection of y, along random directions."""
     (args, go) = inputs(40, 24, 50, torch.float32, True, seed=4)
