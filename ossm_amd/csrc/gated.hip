@@ -22,7 +22,7 @@
 //
 // bfloat16: da and db are rounded to bf16 between the elementwise kernel and the products
 // (relative 2^-9, random; gradients then are 0.0024 off, where an exact sum rounded to
-// bf16 is 0.0017 off); sums are float32 throughout, and so are the stored a and b: in
+// bf16 is 0.0017 off), or, where they are few, held as two terms; sums are float32 throughout, and so are the stored a and b: in
 // bf16 they left 0.0031.
 
 #include <hip/hip_runtime.h>
@@ -100,7 +100,7 @@ template <class E>
 struct Product {
   Operand a, b;
   int M, N, K;       // K: of one part
-  int parts, combos; // stretches of k: parts x (1, or 6 products of planes)
+  int parts, combos; // stretches of k: parts x (1, or 2 or 6 products of planes)
   int tiles_m, tiles_n, splits, per_split;  // per_split: k tiles of one split
   // outputs
   E* c[2];           // plain: rows below `half` to c[0], from it on to c[1] (less half); gated: y in c[0]
@@ -191,12 +191,14 @@ __device__ __forceinline__ bf16x8 load_frag(const uint16_t* lds, int i0, int kk)
   }
 }
 
-// Element (i, k) of an operand as its planes' sum (0 outside).
+// Element (i, k) of an operand as the sum of its planes, smallest first (0 outside).
 template <bool COL>
-__device__ __forceinline__ float element(const Operand& o, int part, int i, int rows, int k, int K) {
+__device__ __forceinline__ float element(const Operand& o, int planes, int part, int i, int rows, int k, int K) {
   if (i >= rows || k >= K) return 0.f;
   const uint16_t* p = o.p[part] + (COL ? static_cast<long long>(k) * o.ld + i : static_cast<long long>(i) * o.ld + k);
-  return (to_f(bf16_t{p[2 * o.plane]}) + to_f(bf16_t{p[o.plane]})) + to_f(bf16_t{p[0]});
+  float s = to_f(bf16_t{p[(planes - 1) * o.plane]});
+  for (int j = planes - 2; j >= 0; --j) s += to_f(bf16_t{p[j * o.plane]});
+  return s;
 }
 
 // Lays out a stretch of instructions: COUNT of a kind (0x100 LDS reads, 0x20 loads) spread
@@ -266,7 +268,8 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
   const auto stretch = [&] {
     const int k0 = next_kt * TK;
     left = combo < g.combos ? g.K - k0 : 0;
-    const int c = combo < g.combos && g.combos > 1 ? combo : 5;  // 5: the first planes
+    // the last of them: (0,0); two: (1,0) before it
+    const int c = combo >= g.combos || g.combos == 1 ? 5 : g.combos == 2 ? 3 + 2 * combo : combo;
     const long long qa = plane_a(c) * g.a.plane + (ACOL ? m0 + k0 * g.a.ld : m0 * g.a.ld + k0);
     const long long qb = plane_b(c) * g.b.plane + (BCOL ? n0 + k0 * g.b.ld : n0 * g.b.ld + k0);
     pa = g.a.p[part] + qa;
@@ -376,22 +379,23 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into LDS at the end
 
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), l32 = lane & 31, half = lane >> 5;
-  if constexpr (sizeof(E) == 4) {
+  if (!GATED || sizeof(E) == 4) {
     // the elements of a fragment that are not finite
+    const int pla = g.combos == 6 ? 3 : g.combos, plb = g.combos == 6 ? 3 : 1;
     const int k_end = min(kt1 * TK, g.K);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const floatx16 one[1] = {acc[i][j]};
-        if (any_nonfinite(one)) {
+        if (g.combos > 1 && any_nonfinite(one)) {
           floatx16 c = {};
           for (int part = 0; part < g.parts; ++part)
 #pragma unroll 1
             for (int k = kt0 * TK; k < k_end; k += 2) {
-              const float va = element<ACOL>(g.a, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
-              const float vb = GATED ? element<BCOL>(g.b, j / HN, n0 + wn * HN * 32 + (j % HN) * 32 + l32, g.N, k + half, k_end)
-                                     : element<BCOL>(g.b, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
+              const float va = element<ACOL>(g.a, pla, part, m0 + wm * FM * 32 + i * 32 + l32, g.M, k + half, k_end);
+              const float vb = GATED ? element<BCOL>(g.b, plb, j / HN, n0 + wn * HN * 32 + (j % HN) * 32 + l32, g.N, k + half, k_end)
+                                     : element<BCOL>(g.b, plb, part, n0 + wn * FN * 32 + j * 32 + l32, g.N, k + half, k_end);
               c = mfma32(va, vb, c);
             }
 #pragma unroll
@@ -682,11 +686,11 @@ __device__ __forceinline__ void read8(const bf16_t* p, float (&v)[8]) {
   }
 }
 
-// da and db side by side, [T][2 Fp] (1 or 3 planes), zeros from F on, and each thread's
+// da and db side by side, [T][2 Fp] (1 or 3 planes, 2 in bf16 where TWO), zeros from F on, and each thread's
 // sums over its rows for the biases' gradients (in float32, before any rounding).  Bound by
 // memory: 12 bytes read and 4 written an element in bf16.  VEC: F and every row are
 // multiples of 16 bytes, and a thread's eight columns move in vectors.
-template <class E, int ACT, bool VEC>
+template <class E, int ACT, bool VEC, bool TWO>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go, long long ld_go,
                                                         const float* __restrict__ a, const float* __restrict__ b,
                                                         uint16_t* __restrict__ dab, long long plane,
@@ -724,7 +728,7 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go
       sa[i] += ga;
       sb[i] += gb;
       uint16_t va[3] = {0, 0, 0}, vb[3] = {0, 0, 0};
-      if constexpr (sizeof(E) == 4) {
+      if constexpr (sizeof(E) == 4 || TWO) {
         split3(ga, va);
         split3(gb, vb);
       } else {
@@ -735,7 +739,7 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const E* __restrict__ go
       for (int j = 0; j < 3; ++j) { ta[j][i] = va[j]; tb[j][i] = vb[j]; }
     }
 #pragma unroll
-    for (int j = 0; j < (sizeof(E) == 4 ? 3 : 1); ++j) {
+    for (int j = 0; j < (sizeof(E) == 4 ? 3 : TWO ? 2 : 1); ++j) {
       uint16_t* dst = dab + j * plane + static_cast<long long>(r) * 2 * Fp + f0;
       put8(dst, ta[j]);
       put8(dst + Fp, tb[j]);
@@ -861,12 +865,12 @@ int launch_tiled(Product<E> g, hipStream_t st) {
 
 int64_t tiles(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 
-// How many ways the k of an [M, N] product of `k_tiles` tiles is split: towards two
-// workgroups a CU, none with fewer than 8 tiles (dx of [25600, 128] from 2 x 512 in float32,
-// 200 tiles: two ways and their sum 96 us, unsplit in tiles half as high 129).
-int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t cus) {
+// How many ways the k of an [M, N] product of `k_tiles` tiles, each `combos` steps, is split:
+// towards two workgroups a CU, none with fewer than 8 steps (dx of [25600, 128] from 2 x 512
+// in float32, 200 tiles: two ways and their sum 96 us, unsplit in tiles half as high 129).
+int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t combos, int64_t cus) {
   const int64_t t = std::max<int64_t>(1, tiles(m, n, 128, 128));  // an input without columns has none
-  return static_cast<int>(std::max<int64_t>(1, std::min(2 * cus / t, k_tiles / 8)));
+  return static_cast<int>(std::max<int64_t>(1, std::min({2 * cus / t, k_tiles * combos / 8, k_tiles})));
 }
 
 template <class E, bool ACOL, bool BCOL, bool GATED>
@@ -957,17 +961,25 @@ int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipSt
   return launch_product<E, false, false, true>(g, std::max(1, device_cu_count(call.device())), st);
 }
 
+// bfloat16: up to this many da the gradients take them as two terms.  Rounded to one, their
+// errors average out over all of them and leave 1.41 times that of an exact sum rounded to
+// bf16, but where some are much larger than others it is up to 1.53 times with 2^16 of them,
+// 1.47 with 2^18 and 1.44 with 2^19 (relu, twelve draws); few products cost hardly more for it
+// ([16, 2048] -> 5632 91 and 93 us), many twice as much.
+constexpr int64_t kTwoPlanes = 1 << 18;
+
 template <class E>
 int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, const float* b, E* gx, E* const gw[2], E* const gb[2],
              StreamCall& call, hipStream_t st) {
   const Source<E> px = p.rows(), pw = p.weights();
-  const int64_t Fp = up8(p.F), planes = sizeof(E) == 4 ? 3 : 1;
+  const bool two = sizeof(E) == 2 && p.T * p.F <= kTwoPlanes;
+  const int64_t Fp = up8(p.F), planes = sizeof(E) == 4 ? 3 : two ? 2 : 1, combos = sizeof(E) == 4 ? 6 : planes;
   const int64_t cus = std::max(1, device_cu_count(call.device()));
   const bool want_w = gw[0] != nullptr || gw[1] != nullptr, want_b = gb[0] != nullptr || gb[1] != nullptr;
   const int rows_per = want_b ? kRowsPerSum : kRowsPer;
   const int64_t dab_plane = p.T * 2 * Fp, rbs = (p.T + rows_per - 1) / rows_per;
-  const int sx = choose_splits(p.T, p.D, p.F / tile_k(false), cus);
-  const int sw = choose_splits(2 * Fp, p.D, p.T / tile_k(false), cus);
+  const int sx = choose_splits(p.T, p.D, p.F / tile_k(false), combos, cus);
+  const int sw = choose_splits(2 * Fp, p.D, p.T / tile_k(false), combos, cus);
   const int64_t part = std::max<int64_t>(gx != nullptr && sx > 1 ? sx * p.T * p.D : 0, want_w && sw > 1 ? sw * 2 * Fp * p.D : 0);
   // bytes; every start a multiple of 16
   size_t at = 0;
@@ -984,7 +996,9 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   const bool vec = F % 8 == 0 && aligned16(go) && aligned16(a) && aligned16(b) && ld_go * static_cast<int64_t>(sizeof(E)) % 16 == 0;
   const auto grads = [&](auto act) {
     constexpr int ACT = decltype(act)::value;
-    auto kern = vec ? gate_grad_kernel<E, ACT, true> : gate_grad_kernel<E, ACT, false>;
+    auto kern = vec ? gate_grad_kernel<E, ACT, true, false> : gate_grad_kernel<E, ACT, false, false>;
+    if constexpr (sizeof(E) == 2)
+      if (two) kern = vec ? gate_grad_kernel<E, ACT, true, true> : gate_grad_kernel<E, ACT, false, true>;
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((rbs * (Fp / 8) + 255) / 256)), dim3(256), 0, st, go, ld_go, a, b, dab,
                        static_cast<long long>(dab_plane), sums, T, F, fp, rows_per);
     return launch_check("gate_grad_kernel");
@@ -1015,7 +1029,7 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
     }
   }
   Product<E> g{};
-  g.combos = kCombos(sizeof(E));
+  g.combos = static_cast<int>(combos);
   g.part = reinterpret_cast<float*>(base + o_part);
   g.a.p[0] = dab;
   g.a.p[1] = dab + Fp;

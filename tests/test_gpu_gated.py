@@ -164,6 +164,34 @@ def test_few_rows_of_any_alignment(G, dtype):
             check(y, want, dtype, f"offset {off}")
 
 
+@pytest.mark.parametrize("shape", [(1, 100, 64), (1, 256, 2000), (2, 64, 4096), (40, 33, 70), (5, 130, 600)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_few_gradients_lose_nothing_before_their_rounding(G, shape):
+    """bfloat16, few da and db: what is off is the rounding of the result alone.  It moves a
+    value by at most 2^-8 of it, uniformly, so by at most 2^-8 / sqrt(3) in the root mean
+    square; a twentieth more is room for chance and the float32 sums."""
+    for seed, act in enumerate(ACTS * 2):
+        args, go = inputs(*shape, torch.bfloat16, False, seed=40 + seed)
+        announce(f"gated_linear few gradients {shape} {act}")
+        want = reference(*args, act, go)[1:4]
+        leaves = [t.requires_grad_(True) for t in args[:3]]
+        for g, w, n in zip(torch.autograd.grad(G.gated_linear(*leaves, activation=act), leaves, go), want, ("x", "gate", "up")):
+            off = np.sqrt(((g.double().cpu().numpy() - w) ** 2).sum() / (w ** 2).sum())
+            assert off <= 1.05 * 2.0 ** -8 / math.sqrt(3), f"{act} grad {n}: {off:.5f}"
+
+
+def test_few_gradients_of_infinite_weights(G):
+    """An infinite weight reaches x's gradient in its column alone, as an infinity."""
+    args, go = inputs(3, 40, 70, torch.bfloat16, False, seed=60)
+    announce("gated_linear gradient through an infinite weight")
+    go[:] = 1
+    x, wg, wu = (t.requires_grad_(True) for t in args[:3])
+    y = G.gated_linear(x, wg, wu, activation="sigmoid")
+    wu.data[7, 5] = float("inf")  # db = sigmoid(a) > 0
+    g = torch.autograd.grad(y, [x], go)[0]
+    assert torch.isposinf(g[:, 5]).all() and torch.isfinite(g[:, :5]).all() and torch.isfinite(g[:, 6:]).all()
+
+
 def test_gradients_against_differences(G):
     """Central differences of a random projection of y, along random directions."""
     (args, go) = inputs(40, 24, 50, torch.float32, True, seed=4)
