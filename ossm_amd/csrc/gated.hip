@@ -22,8 +22,8 @@
 //
 // bfloat16: da and db are rounded to bf16 between the elementwise kernel and the products
 // (relative 2^-9, random; gradients then are 0.0024 off, where an exact sum rounded to
-// bf16 is 0.0017 off), or, where they are few, held as two terms; sums are float32 throughout, and so are the stored a and b: in
-// bf16 they left 0.0031.
+// bf16 is 0.0017 off), or, where they are few, held as two terms; sums are float32
+// throughout, and so are the stored a and b: in bf16 they left 0.0031.
 
 #include <hip/hip_runtime.h>
 
@@ -466,11 +466,11 @@ __global__ __launch_bounds__(256) void product_sum_kernel(Product<E> g) {
 // ---- few rows ---------------------------------------------------------------------
 // Few rows of x, 16 NT to a workgroup: the weights' traffic is all there is (9.4 us for two of
 // [5632, 2048] in bf16; 11 at 4 rows), so each is read once, straight into fragments, and
-// none goes through LDS.  A workgroup takes 16 outputs of both projections.  Its waves share k in blocks of 128 bytes
-// of a row, whole lines (where a lane read 128 bytes by itself, lines left the L1 between its
-// loads: 118 us for 16 rows of float32, 28 now), ask for kAhead blocks together, and add their
-// sums in LDS in a fixed order.  float32 takes the fp32 matrix instruction: nothing to
-// split, and its rate is above the memory's.
+// none goes through LDS.  A workgroup takes 16 outputs of both projections.  Its waves share
+// k in blocks of 128 bytes of a row, whole lines (where a lane read 128 bytes by itself,
+// lines left the L1 between its loads: 118 us for 16 rows of float32, 28 now), ask for kAhead
+// blocks together, and add their sums in LDS in a fixed order.  float32 takes the fp32
+// matrix instruction: nothing to split, and its rate is above the memory's.
 constexpr int kRowWaves = 8, kRowOut = 16;
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 

@@ -288,6 +288,28 @@ def test_strides_leading_dimensions_and_streams(G, dtype):
     assert all(torch.equal(a, b) for a, b in zip(wide, dense))  # a broadcast gradient
 
 
+def test_rows_past_32_bits(G):
+    """More outputs than 32 bits count; gradients only in the first and last rows, whose
+    float64 formulas give all there is of the weights'."""
+    T, D, n, ends = (1 << 20) + 77, 32, 2056, 40
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(T, D, device="cuda", generator=g).bfloat16()
+    wg, wu = (torch.randn(n, D, device="cuda", generator=g).mul(2 / math.sqrt(D)).bfloat16() for _ in range(2))
+    rows = torch.cat([torch.arange(ends), torch.arange(T - ends, T)]).cuda()
+    go = torch.zeros(T, n, dtype=torch.bfloat16, device="cuda")
+    go[rows] = torch.randn(2 * ends, n, device="cuda", generator=g).bfloat16()
+    want = reference(x[rows], wg, wu, None, None, "silu", go[rows])
+    announce(f"gated_linear past 32 bits {(T, D, n)}")
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
+    y = G.gated_linear(*leaves)
+    check(y[rows], want[0], torch.bfloat16, "y")
+    gx, *gw = torch.autograd.grad(y, leaves, go)
+    check(gx[rows], want[1], torch.bfloat16, "grad x", True)
+    assert not gx[ends:T - ends].any()
+    for got, w, name in zip(gw, want[2:], ("gate", "up")):
+        check(got, w, torch.bfloat16, f"grad {name}", True)
+
+
 def test_empty(G):
     z = lambda *s: torch.zeros(*s, device="cuda", requires_grad=True)  # noqa: E731
     announce("gated_linear empty")
