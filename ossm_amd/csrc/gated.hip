@@ -106,7 +106,7 @@ struct Product {
   E* c[2];           // plain: rows below `half` to c[0], from it on to c[1] (less half); gated: y in c[0]
   long long ldc;
   int half, half_rows;  // rows of each half that exist
-  float* part;       // splits > 1: [splits][M][N]
+  float* part;       // splits > 1: [splits][M][N]; gated: [splits][2][M][N]
   const E* bias[2];  // gated
   float* save[2];    // gated: a, b or null
   int act;
@@ -407,6 +407,21 @@ __global__ __launch_bounds__(WM * WN * kWave, 2) void product_kernel(Product<E> 
 
   // register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
   if constexpr (GATED) {
+    if (g.splits > 1) {  // gated_sum_kernel has the epilogue
+#pragma unroll
+      for (int q = 0; q < FN; ++q) {
+        const int n = n0 + wn * HN * 32 + q % HN * 32 + l32;
+        float* at = g.part + (split * 2 + q / HN) * (static_cast<size_t>(g.M) * g.N) + n;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int m = m0 + wm * FM * 32 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            if (n < g.N && m < g.M) at[static_cast<size_t>(m) * g.N] = acc[i][q][r];
+          }
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < HN; ++j) {
       const int n = n0 + wn * HN * 32 + j * 32 + l32;
@@ -461,6 +476,27 @@ __global__ __launch_bounds__(256) void product_sum_kernel(Product<E> g) {
 #pragma unroll 8
   for (int k = 0; k < g.splits; ++k) s += g.part[k * n + i];
   g.c[second][row * g.ldc + col] = from_f<E>(s);
+}
+
+// The same of a gated product, and its epilogue.
+template <class E>
+__global__ __launch_bounds__(256) void gated_sum_kernel(Product<E> g) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, n = static_cast<long long>(g.M) * g.N;
+  if (i >= n) return;
+  const int col = static_cast<int>(i % g.N);
+  float a = 0.f, b = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < g.splits; ++k) {
+    a += g.part[2 * k * n + i];
+    b += g.part[(2 * k + 1) * n + i];
+  }
+  if (g.bias[0] != nullptr) a += to_f(g.bias[0][col]);
+  if (g.bias[1] != nullptr) b += to_f(g.bias[1][col]);
+  g.c[0][i] = from_f<E>(activation_of(g.act, a) * b);
+  if (g.save[0] != nullptr) {
+    g.save[0][i] = a;
+    g.save[1][i] = b;
+  }
 }
 
 // ---- few rows ---------------------------------------------------------------------
@@ -857,8 +893,9 @@ int launch_tiled(Product<E> g, hipStream_t st) {
   if (int rc = launch_check("product_kernel")) return rc;
   if (g.splits > 1) {
     const int64_t n = static_cast<int64_t>(g.M) * g.N;
-    hipLaunchKernelGGL(product_sum_kernel<E>, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, g);
-    return launch_check("product_sum_kernel");
+    hipLaunchKernelGGL((GATED ? gated_sum_kernel<E> : product_sum_kernel<E>), dim3(static_cast<unsigned>((n + 255) / 256)),
+                       dim3(256), 0, st, g);
+    return launch_check(GATED ? "gated_sum_kernel" : "product_sum_kernel");
   }
   return OSSM_OK;
 }
@@ -871,6 +908,16 @@ int64_t tiles(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 
 int choose_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t combos, int64_t cus) {
   const int64_t t = std::max<int64_t>(1, tiles(m, n, 128, 128));  // an input without columns has none
   return static_cast<int>(std::max<int64_t>(1, std::min({2 * cus / t, k_tiles * combos / 8, k_tiles})));
+}
+
+// The same for a forward, where few tiles have much to add: [626, 1954] -> 86 in float32, 20
+// tiles, 120 us unsplit and 30 split, [384, 3540] -> 562 242 and 54.  Splitting has to save 24
+// steps, of about 0.4 us, to pay for the sums' launch and traffic: in bf16 2686 k of 45 tiles
+// 41 and 30, but 1096 k 15.5 and 19.6, 2112 k of 245 tiles in two 30 and 37.
+int forward_splits(int64_t m, int64_t n, int64_t k_tiles, int64_t combos, int64_t cus) {
+  const int splits = choose_splits(m, n, k_tiles, combos, cus);
+  const int64_t steps = k_tiles * combos;
+  return steps - steps / splits >= 24 ? splits : 1;
 }
 
 template <class E, bool ACOL, bool BCOL, bool GATED>
@@ -938,9 +985,14 @@ int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipSt
   const Source<E> px = p.rows(), pw = p.weights();
   if (few(p.T, p.D, p.F, !px.direct() || !pw.direct(), int64_t(1) << (sizeof(E) == 4 ? 29 : 28)))
     return few_rows(p, y, a, b, st);
+  const int64_t cus = std::max(1, device_cu_count(call.device()));
+  const int combos = kCombos(sizeof(E)), splits = forward_splits(p.T, 2 * p.F, p.D / tile_k(true), combos, cus);
+  // planes, then the splits' sums; a plane's rows are multiples of 16 bytes
+  const size_t o_part = static_cast<size_t>(px.elems() + pw.elems()) * 2;
+  const size_t bytes = o_part + (splits > 1 ? static_cast<size_t>(splits) * 2 * p.T * p.F * 4 : 0);
   void* ws = nullptr;
-  if (px.elems() + pw.elems() > 0)
-    if (int rc = acquire_workspace(call, static_cast<size_t>(px.elems() + pw.elems()) * 2, &ws)) return rc;
+  if (bytes > 0)
+    if (int rc = acquire_workspace(call, bytes, &ws)) return rc;
   Product<E> g{};
   uint16_t* q = static_cast<uint16_t*>(ws);
   PackJobs<E> jobs{};
@@ -950,15 +1002,17 @@ int forward(const Gated<E>& p, E* y, float* a, float* b, StreamCall& call, hipSt
   g.M = static_cast<int>(p.T);
   g.N = static_cast<int>(p.F);
   g.K = static_cast<int>(p.D);
-  g.parts = g.splits = 1;
-  g.combos = kCombos(sizeof(E));
+  g.parts = 1;
+  g.splits = splits;
+  g.combos = combos;
+  g.part = reinterpret_cast<float*>(static_cast<char*>(ws) + o_part);
   g.c[0] = y;
   g.ldc = p.F;
   for (int i = 0; i < 2; ++i) g.bias[i] = p.bias[i];
   g.save[0] = a;
   g.save[1] = b;
   g.act = p.act;
-  return launch_product<E, false, false, true>(g, std::max(1, device_cu_count(call.device())), st);
+  return launch_product<E, false, false, true>(g, cus, st);
 }
 
 // bfloat16: up to this many da the gradients take them as two terms.  Rounded to one, their

@@ -288,6 +288,46 @@ def test_strides_leading_dimensions_and_streams(G, dtype):
     assert all(torch.equal(a, b) for a, b in zip(wide, dense))  # a broadcast gradient
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(626, 1954, 86), (1679, 1549, 94), (530, 2048, 264), (2161, 600, 1)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_few_tiles_share_k(G, shape, dtype):
+    """Long products of few tiles: with and without biases and saved projections."""
+    for bias, act in ((True, "sigmoid"), (False, "gelu")):
+        args, go = inputs(*shape, dtype, bias, seed=30)
+        want = reference(*args, act, go)
+        announce(f"gated_linear shared k {shape} {dtype} {act} bias={bias}")
+        with torch.no_grad():
+            y = G.gated_linear(*args, activation=act)
+            check(y, want[0], dtype, act)
+            assert torch.equal(y, G.gated_linear(*args, activation=act))
+        leaves = [t.requires_grad_(True) for t in args if t is not None]
+        y = G.gated_linear(*args, activation=act)
+        check(y, want[0], dtype, "y, training")
+        for g, w, n in zip(torch.autograd.grad(y, leaves, go), want[1:], ("x", "gate", "up", "gate bias", "up bias")):
+            check(g, w, dtype, f"{act} grad {n}", True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_values_that_are_not_finite_among_few_tiles(G, dtype):
+    """An infinite and a NaN input reach their own rows and no other's bits."""
+    args, _ = inputs(700, 1100, 70, dtype, False, seed=31)
+    x, wg, wu = args[:3]
+    announce(f"gated_linear shared k, not finite {dtype}")
+    base = G.gated_linear(x, wg, wu, activation="sigmoid")
+    bad = x.clone()
+    bad[5, 1090] = float("nan")
+    bad[650, 3] = float("inf")
+    got = G.gated_linear(bad, wg, wu, activation="sigmoid")
+    keep = [r for r in range(700) if r not in (5, 650)]
+    assert torch.equal(got[keep], base[keep])
+    assert got[5].isnan().all()
+    # sigmoid(+-inf) of +-inf: 0 inf is NaN, 1 inf is inf with the up weight's sign
+    g, u = wg[:, 3].float(), wu[:, 3].float()
+    want = torch.where(g > 0, u.sign() * float("inf"), float("nan"))
+    assert torch.equal(got[650].float().nan_to_num(7.0, 8.0, -8.0), want.nan_to_num(7.0, 8.0, -8.0))
+
+
 def test_rows_past_32_bits(G):
     """More outputs than 32 bits count; gradients only in the first and last rows, whose
     float64 formulas give all there is of the weights'."""
