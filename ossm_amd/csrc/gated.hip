@@ -925,11 +925,15 @@ int launch_product(Product<E> g, int64_t cus, hipStream_t st) {
   const int k_tiles = std::max(1, (g.K + tile_k(GATED) - 1) / tile_k(GATED));
   g.per_split = (k_tiles + g.splits - 1) / g.splits;
   g.splits = (k_tiles + g.per_split - 1) / g.per_split;
-  if (g.splits == 1 && tiles(g.M, g.N, 256, GATED ? 128 : 256) >= cus)
+  // Eight waves and tiles of 256 where they fill three quarters of the CUs and pad no more than a
+  // quarter beyond tiles of 128 (training [5255, 2518] -> 717 in float32, dx of 210 tiles, 1350 ->
+  // 1024 us, [2128, 2524] -> 1906 488 -> 321; [25534, 289] -> 479 in bf16, dx's 289 columns padded to 512, 270 -> 290, so not there).
+  const int64_t large = tiles(g.M, g.N, 256, GATED ? 128 : 256), small = tiles(g.M, g.N, 128, GATED ? 64 : 128);
+  if (g.splits == 1 && large * 4 >= 3 * cus && large * 16 <= small * 5)
     return launch_tiled<E, ACOL, BCOL, GATED, 2, 4, 4, 2>(g, st);
-  // too few tiles for two workgroups a CU: half as high ([1001, 1022] -> 2730 in float32, 344
-  // tiles: 97 -> 89 us)
-  if (g.splits == 1 && tiles(g.M, g.N, 128, GATED ? 64 : 128) < 2 * cus)
+  // too few tiles to give every CU one and half of them two: half as high ([1001, 1022] -> 2730 in
+  // float32, 344 tiles: 97 -> 89 us; not from 384 on)
+  if (g.splits == 1 && small * 2 < 3 * cus)
     return launch_tiled<E, ACOL, BCOL, GATED, 2, 2, 1, 2>(g, st);
   return launch_tiled<E, ACOL, BCOL, GATED, 2, 2, 2, 2>(g, st);
 }
