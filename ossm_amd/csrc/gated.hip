@@ -965,13 +965,13 @@ struct Gated {
   Source<E> weights() const { return {{w[0], w[1]}, {ld_w[0], ld_w[1]}, F, D, 2}; }
 };
 
-// Whether few_rows_kernel takes a forward, by itself and by the products, us: 64 rows of
-// [2048] -> 5632 in bf16 25 and 25, 96 37 and 25; where the operands would be packed first, 128
-// of them in float32 94 and 154, 192 151 and 156, and of [1022] -> 2730 in bf16 16 and 24.
-// Small products leave the products' tiles few: [512] -> 2048 in bf16 5.5 and 8.3 at 64 rows,
-// 8.6 and 8.7 at 256, 15 and 9.2 at 512; in float32 19 and 40 at 256, 36 and 43 at 512.
+// Whether few_rows_kernel takes a forward, by itself and by the products, us: 32 rows of
+// [2048] -> 5632 in bf16 17 and 17, 64 25 and 18; where the operands would be packed first, 128
+// of them in float32 94 and 99, 32 39 and 86, and of [1022] -> 2730 in bf16 15 and 24.  Small
+// products leave the products' tiles few: [512] -> 2048 in float32 18 and 31 at 256 rows, 34
+// and 39 at 512; in bf16 both are the call's own 11.
 bool few(int64_t T, int64_t D, int64_t F, bool packed, int64_t small) {
-  return T <= (packed ? 128 : 64) || (T <= 512 && T * D * F <= small);
+  return T <= (packed ? 128 : 32) || (T <= 512 && T * D * F <= small);
 }
 
 template <class E>
