@@ -33,14 +33,16 @@ def _separate(x: Tensor, wg: Tensor, wu: Tensor, bg: Optional[Tensor], bu: Optio
 
 
 def _matrix(t: Tensor) -> Tensor:
-    """``t`` itself where its rows are whole and do not overlap, else a dense copy."""
-    return t if t.size(1) <= 1 or t.stride(1) == 1 and (t.size(0) <= 1 or t.size(1) <= t.stride(0) <= 1 << 20) \
+    """``t`` itself where its rows are whole and do not overlap, else a dense copy (of rows
+    broadcast from one, too, where they are single columns)."""
+    rows, cols = t.shape
+    return t if (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or max(cols, 1) <= t.stride(0) <= 1 << 20) \
         else t.contiguous()
 
 
 def _ld(t: Tensor) -> int:
-    """The row stride of such a matrix (of a single row, any that holds it)."""
-    return max(t.stride(0), t.size(1)) if t.size(0) > 1 else t.size(1)
+    """The row stride of such a matrix (where nothing is read at it, any that holds a row)."""
+    return max(t.stride(0), t.size(1)) if t.size(0) > 1 and t.size(1) > 0 else t.size(1)
 
 
 def _forward(x: Tensor, wg: Tensor, wu: Tensor, bg: Optional[Tensor], bu: Optional[Tensor], act: str, save: bool):

@@ -422,3 +422,28 @@ def test_refusals(G):
     wide = torch.zeros(2, 2 ** 20 + 8, device="cuda")
     with pytest.raises(RuntimeError, match="row strides up to"):
         G.gated_linear(wide, wide, wide)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_single_columns_of_any_row_stride(G, dtype):
+    """One column broadcast from one row (a summed loss's gradient, an expanded input or
+    weight), or of a matrix whose rows lie further apart than the kernels take."""
+    far = (1 << 20) + 8
+    for T, D, n in ((9, 24, 1), (70, 1, 50), (700, 1, 1), (3, 1, 200)):
+        args, _ = inputs(T, D, n, dtype, True, seed=T)
+        cases = [("dense", args)]
+        if D == 1:
+            cases.append(("expanded", [args[0][:1].expand(T, 1), *(w[:1].expand(n, 1) for w in args[1:3]), *args[3:]]))
+        if D == 1 and T <= 70:
+            wide = torch.empty(T, far, dtype=dtype, device="cuda")
+            wide[:, :1] = args[0]
+            cases.append(("far apart", [wide[:, :1], *args[1:]]))
+        for name, given in cases:
+            announce(f"gated_linear single columns {(T, D, n)} {dtype} {name}")
+            want = reference(*given, "gelu", torch.ones(T, n))
+            with torch.no_grad():
+                check(G.gated_linear(*given, activation="gelu"), want[0], dtype, f"{name} y")
+            leaves = [t.detach().requires_grad_(True) for t in given]
+            y = G.gated_linear(*leaves, activation="gelu")
+            for g, w, what in zip(torch.autograd.grad(y.sum(), leaves), want[1:], ("x", "gate", "up", "gate bias", "up bias")):
+                check(g, w, dtype, f"{name} grad {what}", True)
