@@ -16,7 +16,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _lib
-from .linear import linear
+from .linear import aliases, linear
 
 __all__ = ["ACTIVATIONS", "GatedFeedForward", "GatedLinearFn", "gated_linear"]
 
@@ -74,7 +74,7 @@ class GatedLinearFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():
             # create_graph: differentiable again, as separate steps
-            inputs = (x, wg, wu, bg, bu)
+            inputs = aliases(x, wg, wu, bg, bu)
             wanted = [t for t, n in zip(inputs, need) if n]
             got = iter(torch.autograd.grad(_separate(*inputs, ctx.act), wanted, gy, create_graph=True))
             return (*(next(got) if n else None for n in need[:5]), None)

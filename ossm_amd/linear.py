@@ -8,7 +8,7 @@ with R (every batch row and step) much larger than M and N
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -16,7 +16,7 @@ from torch import Tensor, nn
 
 from . import _lib
 
-__all__ = ["rows_product", "linear", "linear_weight", "LinearFn", "is_plain",
+__all__ = ["rows_product", "linear", "linear_weight", "LinearFn", "aliases", "is_plain",
            "MIN_ROWS", "BLOCK_ROWS"]
 
 # The least the kernel takes, and where the layers' and the mixer's own backwards, which
@@ -56,6 +56,14 @@ def rows_product(a: Tensor, b: Tensor, pairs: bool = False) -> Tensor:
     _lib.run(_lib.load().ossm_rows_product, a, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
              out.data_ptr(), *strides, R, M, N)
     return out
+
+
+def aliases(*ts: Optional[Tensor]) -> Tuple[Optional[Tensor], ...]:
+    """Each tensor as a view with a node of its own, for a backward that differentiates a
+    composition of its inputs under create_graph: gradients with respect to the views stop
+    there, where the inputs' own may depend on one another or be one tensor twice, and a
+    path between them would count once inside and once more outside."""
+    return tuple(None if t is None else t.view_as(t) for t in ts)
 
 
 class LinearFn(torch.autograd.Function):

@@ -44,3 +44,42 @@ def test_a_matrix_is_described_as_it_lies(name):
     end = m.storage_offset() + (rows - 1) * gated._ld(m) + cols
     assert end <= m.untyped_storage().nbytes() // m.element_size()
     assert torch.equal(m.as_strided((rows, cols), (gated._ld(m), 1)), t)
+
+
+class _OnHost:
+    """GatedLinearFn with its forward as torch's steps: the backward under create_graph
+    runs no kernel."""
+
+    def __init__(self, monkeypatch):
+        monkeypatch.setattr(gated, "_forward", lambda x, wg, wu, bg, bu, act, save: (
+            gated._separate(x, wg, wu, bg, bu, act), *(torch.nn.functional.linear(x, *p) for p in ((wg, bg), (wu, bu)))))
+
+    def __call__(self, *args):
+        return gated.GatedLinearFn.apply(*args, "silu")
+
+
+def _tied(f):
+    """The gate's weight is the up weight too, as are the biases."""
+    g = torch.Generator().manual_seed(1)
+    x, w, b = (torch.randn(*s, dtype=torch.float64, generator=g).requires_grad_(True) for s in ((6, 5), (4, 5), (4,)))
+    return f(x, w, w, b, b), [x, w, b]
+
+
+def _twice(f):
+    """One block applied to its own output."""
+    g = torch.Generator().manual_seed(2)
+    x, wg, wu, b = (torch.randn(*s, dtype=torch.float64, generator=g).requires_grad_(True)
+                    for s in ((6, 5), (5, 5), (5, 5), (5,)))
+    return f(f(x, wg, wu, b, None), wg, wu, b, None), [x, wg, wu, b]
+
+
+@pytest.mark.parametrize("use", [_tied, _twice])
+def test_shared_inputs_differentiate_twice(monkeypatch, use):
+    """Under create_graph each path to a shared tensor counts once, in the gradients and in theirs."""
+    seen = []
+    for f in (_OnHost(monkeypatch), lambda *a: gated._separate(*a, "silu")):
+        y, leaves = use(f)
+        grads = torch.autograd.grad(y.square().sum(), leaves, create_graph=True)
+        seen.append((*grads, *torch.autograd.grad(sum(t.square().sum() for t in grads), leaves, create_graph=True)))
+    for a, b in zip(*seen):
+        assert torch.allclose(a, b, rtol=1e-10, atol=1e-10 * float(b.detach().abs().max()))

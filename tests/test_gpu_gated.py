@@ -447,3 +447,22 @@ def test_single_columns_of_any_row_stride(G, dtype):
             y = G.gated_linear(*leaves, activation="gelu")
             for g, w, what in zip(torch.autograd.grad(y.sum(), leaves), want[1:], ("x", "gate", "up", "gate bias", "up bias")):
                 check(g, w, dtype, f"{name} grad {what}", True)
+
+
+def test_shared_inputs_differentiate_twice(G):
+    """create_graph where gate and up share a weight and a bias, and where a block is applied
+    twice: gradients and second derivatives as float64's of the separate steps."""
+    args, _ = inputs(20, 24, 24, torch.float32, True, seed=10, scale=1.0)
+    x, w, v, b, c = (t * 0.5 for t in args)
+    tied = lambda f, x, w, b: f(x, w, w, b, b)  # noqa: E731
+    twice = lambda f, x, w, v, b, c: f(f(x, w, v, b, c), w, v, b, c)  # noqa: E731
+    for name, use, given in (("tied", tied, (x, w, b)), ("twice", twice, (x, w, v, b, c))):
+        announce(f"gated_linear create_graph {name}")
+        seen = []
+        for cast, f in ((torch.Tensor.cuda, G.gated_linear), (lambda t: t.double().cpu(), lambda *a: G._separate(*a, "silu"))):
+            leaves = [cast(t.detach()).clone().requires_grad_(True) for t in given]
+            grads = torch.autograd.grad(use(f, *leaves).square().sum(), leaves, create_graph=True)
+            seen.append((*grads, *torch.autograd.grad(sum(t.square().sum() for t in grads), leaves)))
+        for got, want in zip(*seen):
+            # the float32 steps of two blocks and three derivatives, sums of at most 24 x 20 terms
+            assert torch.allclose(got.double().cpu(), want, rtol=1e-4, atol=1e-4 * float(want.abs().max())), name
