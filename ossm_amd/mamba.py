@@ -28,7 +28,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _lib
-from .linear import is_plain, linear, linear_weight, rows_product
+from .linear import aliases, is_plain, linear, linear_weight, rows_product
 
 __all__ = ["MambaMixer", "mamba_conv_silu", "selective_scan_mamba", "ConvSiluFn", "MambaScanFn",
            "MixerCoreFn"]
@@ -299,7 +299,7 @@ class MixerCoreFn(torch.autograd.Function):
         xz, u, proj, dt, A, ck, raw, conv_w, conv_b, xproj_w, dt_w, dt_b, A_log = ctx.saved_tensors
         if torch.is_grad_enabled():
             # create_graph: differentiable again, as separate steps
-            inputs = (xz, conv_w, conv_b, xproj_w, dt_w, dt_b, A_log)
+            inputs = aliases(xz, conv_w, conv_b, xproj_w, dt_w, dt_b, A_log)
             wanted = [t for t, n in zip(inputs, ctx.needs_input_grad) if n]
             got = iter(torch.autograd.grad(_mixer_core(*inputs), wanted, gy, create_graph=True, allow_unused=True))
             return tuple(next(got) if n else None for n in ctx.needs_input_grad)

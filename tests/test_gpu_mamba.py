@@ -411,3 +411,28 @@ def test_mixer_core_with_segment_carries(M, shape, monkeypatch):
         g, r = to_np(g), to_np(r)
         np.testing.assert_allclose(g, r, rtol=1e-4, atol=1e-5 * max(1.0, float(np.abs(r).max())))
     no_device_errors()
+
+
+def test_mixer_applied_twice_under_create_graph(M, monkeypatch):
+    """Its parameters then reach its own input: create_graph gives the gradients that a
+    plain backward gives, and those of the separate Functions."""
+    torch.manual_seed(6)
+    mixer = M.MambaMixer(8, d_state=4, d_conv=4, expand=2, dt_rank=3).cuda()
+    x = torch.randn(2, 70, 8, device="cuda", requires_grad=True)
+    go = torch.randn(2, 70, 8, device="cuda")
+    announce("mixer applied twice, create_graph")
+    wrt = [x, *mixer.parameters()]
+    plain = torch.autograd.grad(mixer(mixer(x)), wrt, go)
+
+    def second():
+        first = torch.autograd.grad(mixer(mixer(x)), wrt, go, create_graph=True)
+        return [t.detach() for t in first] + list(
+            torch.autograd.grad(sum(g.square().sum() for g in first if g.requires_grad), wrt, allow_unused=True))
+
+    got, ref = _both_ways(M, second, monkeypatch)
+    for g, r in zip((*got, *got), (*ref, *plain)):
+        assert (g is None) == (r is None)
+        if r is not None:
+            g, r = to_np(g), to_np(r)
+            np.testing.assert_allclose(g, r, rtol=1e-3, atol=1e-3 * float(np.abs(r).max()))
+    no_device_errors()
