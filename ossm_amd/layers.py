@@ -33,7 +33,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .bridge import run_dlinoss
-from .linear import BLOCK_ROWS, rows_product
+from .linear import BLOCK_ROWS, aliases, rows_product
 
 __all__ = ["DampedLinOSSLayer", "dlinoss_layer_forward", "dlinoss_layer_backward", "DlinossLayerFn",
            "project_parameters", "unfused_layer_forward", "LayerParamsFn", "fused_layer_supported"]
@@ -104,7 +104,7 @@ class LayerParamsFn(torch.autograd.Function):
         params, grads = ctx.saved_tensors, grads[:3]
         if torch.is_grad_enabled():
             # create_graph: differentiable again, as torch operations
-            A, G, s = params
+            params = A, G, s = aliases(*params)
             outs = project_parameters(A, G, s) if ctx.damped else \
                 (torch.relu(A), None, torch.sigmoid(s))
             pairs = [(o, g) for o, g in zip(outs, grads) if o is not None and g is not None]
@@ -322,7 +322,7 @@ class DlinossLayerFn(torch.autograd.Function):
             grads = dlinoss_layer_backward(ctx.variant, *saved[:1], grad_out, *saved[1:], carries, lo)
             return (None, *[gr if n else None for gr, n in zip(grads, needs)], *tail)
         with torch.enable_grad():
-            args = saved if again else [t.detach().requires_grad_(bool(n)) for t, n in zip(saved, needs)]
+            args = aliases(*saved) if again else [t.detach().requires_grad_(bool(n)) for t, n in zip(saved, needs)]
             wanted = [t for t, n in zip(args, needs) if n]
             y = ctx.unfused(ctx.variant, *args)
             got = iter(torch.autograd.grad(y, wanted, grad_out, create_graph=again, allow_unused=True)

@@ -403,3 +403,20 @@ def test_layer_split_projections_vs_float64(layers, variant, shape):
         err = float((x.detach().double() - r.detach()).norm() / r.detach().norm())
         assert err < (2e-5 if name in ("a", "g", "step") else 2e-6), f"{name}: {err:.2g}"
     no_device_errors()
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_layer_applied_twice_under_create_graph(layers, variant):
+    """Its weights and parameters then reach its own input: create_graph gives the gradients
+    that a plain backward gives."""
+    announce(f"layer applied twice, create_graph {variant}")
+    args = _layer_inputs(2, 40, 12, 9, 59, variant)
+    go = to_dev(np.random.default_rng(60).normal(size=args[0].shape).astype(np.float32))
+    leaves = [to_dev(x).requires_grad_() for x in args]
+    f = layers.DlinossLayerFn.apply
+    y = f(variant, f(variant, *leaves), *leaves[1:])
+    want = torch.autograd.grad(y, leaves, go, retain_graph=True)
+    got = torch.autograd.grad(y, leaves, go, create_graph=True)
+    for x, r, name in zip(got, want, ("u", "B", "C", "D", "a", "g", "step")):
+        np.testing.assert_allclose(to_np(x), to_np(r), rtol=1e-3, atol=1e-4 * max(1.0, float(r.abs().max())),
+                                   err_msg=name)

@@ -131,3 +131,21 @@ def test_layers_with_parameters_that_broadcast(disc):
         layer.steps = torch.nn.Parameter(torch.zeros(9, device="cuda"))
         with pytest.raises(RuntimeError):
             layer(u)
+
+
+def test_layer_params_of_one_another_under_create_graph():
+    """Parameters computed from one another, or one tensor in two places: create_graph gives
+    the gradients that a plain backward gives."""
+    need_gpu()
+    from ossm_amd.layers import LayerParamsFn
+
+    announce("layer params of one another, create_graph")
+    A, G, s = (t.cuda().requires_grad_() for t in _inputs(17, 6))
+    for damped, given, leaves in ((True, (A + G * s, G, s), (A, G, s)), (True, (A, s, s), (A, s)), (False, (s * s, None, s), (s,))):
+        outs = [o for o, used in zip(LayerParamsFn.apply(damped, *given), (True, damped, True)) if used]
+        loss = sum(o.square().sum() for o in outs)
+        want = torch.autograd.grad(loss, leaves, retain_graph=True)
+        got = torch.autograd.grad(loss, leaves, create_graph=True)
+        for x, r in zip(got, want):
+            np.testing.assert_allclose(x.detach().cpu().numpy(), r.cpu().numpy(), rtol=1e-4,
+                                       atol=1e-4 * max(1.0, float(r.abs().max())))

@@ -142,3 +142,29 @@ def test_linoss_layer_second_derivatives(linoss, disc, monkeypatch):
         if r is not None:
             np.testing.assert_allclose(x.cpu().numpy(), r.cpu().numpy(), rtol=1e-3,
                                        atol=1e-4 * max(1.0, float(r.abs().max())))
+
+
+@pytest.mark.parametrize("disc", ["IM", "IMEX"])
+def test_linoss_layer_applied_twice_under_create_graph(linoss, disc, monkeypatch):
+    """Its parameters then reach its own input: create_graph gives the gradients that a
+    plain backward gives, and the composition's second derivatives."""
+    torch.manual_seed(8)
+    layer = linoss.LinOSSLayer(9, 12, disc).cuda()
+    u = torch.randn(2, 40, 12, device="cuda", requires_grad=True)
+    go = torch.randn(2, 40, 12, device="cuda")
+    announce(f"linoss layer applied twice, create_graph {disc}")
+    wrt = [u, *layer.parameters()]
+    plain = torch.autograd.grad(layer(layer(u)), wrt, go)
+
+    def second():
+        first = torch.autograd.grad(layer(layer(u)), wrt, go, create_graph=True)
+        return [t.detach() for t in first] + list(
+            torch.autograd.grad(sum(g.square().sum() for g in first if g.requires_grad), wrt, allow_unused=True))
+
+    got = second()
+    monkeypatch.setattr(linoss, "fused_layer_supported", lambda *a: False)
+    for x, r in zip((*got, *got), (*second(), *plain)):
+        assert (x is None) == (r is None)
+        if r is not None:
+            np.testing.assert_allclose(x.cpu().numpy(), r.cpu().numpy(), rtol=1e-3,
+                                       atol=1e-4 * max(1.0, float(r.abs().max())))
