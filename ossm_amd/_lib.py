@@ -14,6 +14,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch  # noqa: F401  (must precede the library load)
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libossm_scan.so"
 
@@ -230,6 +231,13 @@ def run(fn, t: torch.Tensor, *args) -> None:
     else:
         with torch.cuda.device(dev):
             check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def has_tangent(ts) -> bool:
+    """Whether one of the tensors (or Nones) carries a forward-mode tangent, which a call that
+    hands out raw pointers would drop."""
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

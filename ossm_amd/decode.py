@@ -14,7 +14,8 @@ sequence from zeros, or keeps nothing.
 
 xz, conv and projection weights are float32 or bfloat16, all of one dtype; dt_bias,
 A_log and the skip are float32.  Sums and states are float32 and each output is
-rounded once.  Inference only: a call that would need a gradient raises.
+rounded once.  Inference only: a call that would need a gradient or carries a
+forward-mode tangent raises.
 """
 
 from __future__ import annotations
@@ -88,8 +89,10 @@ def _args(what: str, xz: Tensor, conv_weight: Tensor, conv_bias: Optional[Tensor
                                    f"(got a {t.dtype} tensor of shape {tuple(t.shape)} on {t.device})")
     if not (ssm_state.is_contiguous() and conv_state.is_contiguous()):
         raise RuntimeError(f"{what}: the state pools are updated in place and must be contiguous")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (xz, *like, *full)):
-        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad() (MambaMixer.forward trains)")
+    given = (xz, *like, *full)
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given)) or _lib.has_tangent(given):
+        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad() and on tensors without tangents "
+                           "(MambaMixer.forward trains)")
     if xz.stride(1) != 1 or xz.stride(0) < 2 * Di:
         xz = xz.contiguous()
     weights = [t if t is None else t.contiguous() for t in (conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A_log, skip)]

@@ -94,8 +94,8 @@ def gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate_bias: O
     [..., D] and weights [F, D] (as two ``nn.Linear`` hold them): float32 or bfloat16
     tensors of one dtype on one GPU, any strides.  activation: silu, gelu, gelu_tanh,
     sigmoid or relu.  Sums are float32, and float32 products keep its 24 bits; the
-    result is rounded once.  Differentiable in every argument, twice as torch's
-    separate steps; training keeps the two projections' outputs in float32.  Under a bfloat16
+    result is rounded once.  Differentiable in every argument (in reverse mode; a
+    forward-mode tangent raises), twice as torch's separate steps; training keeps the two projections' outputs in float32.  Under a bfloat16
     autocast, float32 arguments are cast as ``F.linear``'s are."""
     args = [x, gate_weight, up_weight, gate_bias, up_bias]
     if activation not in ACTIVATIONS:
@@ -114,6 +114,8 @@ def gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate_bias: O
             any(b is not None and b.shape != (n,) for b in (gate_bias, up_bias)):
         raise RuntimeError("gated_linear: expected x (..., D), weights (F, D), biases (F,), got "
                            f"{[None if t is None else tuple(t.shape) for t in args]}")
+    if _lib.has_tangent(args):
+        raise RuntimeError("gated_linear has no forward-mode derivative, and an argument carries a tangent")
     x2 = x if x.dim() == 2 else x.reshape(-1, D) if D > 0 else x.reshape(x.shape[:-1].numel(), 0)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         y = GatedLinearFn.apply(x2, gate_weight, up_weight, gate_bias, up_bias, activation)

@@ -81,14 +81,17 @@ def control_logits(logits: Tensor, history: Optional[Tensor] = None, lengths: Op
     penalties are numbers or float32 tensors [rows]; history, biases and allowed may
     have one row for all.  A row whose mask allows nothing is all -inf.  ``out``
     (``logits`` itself to work in place) takes the result, else a new tensor; it is
-    computed in float32 and rounded once."""
+    computed in float32 and rounded once.  Inference only: a call that would need a
+    gradient or carries a forward-mode tangent raises."""
     dev = logits.get_device()
     if logits.dtype not in _lib.LM_DTYPES or dev < 0 or logits.dim() != 2:
         raise RuntimeError("control_logits: logits must be a float32 or bfloat16 GPU tensor (rows, vocabulary), got "
                            f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
     rows, V = logits.shape
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("control_logits is for inference: call it under torch.no_grad()")
+    given = (logits, repetition, presence, frequency, bias_values, out)
+    needs_grad = torch.is_grad_enabled() and logits.requires_grad
+    if needs_grad or _lib.has_tangent(given):
+        raise RuntimeError("control_logits is for inference: call it under torch.no_grad() and on tensors without tangents")
     if (bias_ids is None) != (bias_values is None):
         raise RuntimeError("control_logits: give both bias_ids and bias_values, or neither")
     if history is None and (lengths is not None or prompt_lengths is not None):

@@ -400,3 +400,20 @@ def test_refusals(D):
         run_prompt(D, e)
     with pytest.raises(RuntimeError, match="slots must be a 1-D tensor of 5"):
         D.mixer_step(c.xz, *a)
+
+
+def test_forward_mode_is_refused(D):
+    """A tangent raises, under no_grad too, whichever argument carries it."""
+    from torch.autograd import forward_ad
+
+    c = Case(64, 16, 4, 4, [1, 1], seed=14)
+    announce("mixer calls with tangents")
+    given = [c.xz, *c.w, c.conv, c.ssm]
+    with forward_ad.dual_level(), torch.no_grad():
+        run_prompt(D, c)
+        for i, t in enumerate((*given, c.skip)):
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else u for j, u in enumerate((*given, c.skip))]
+            with pytest.raises(RuntimeError, match="tangents"):
+                D.mixer_step(*dual[:-1], c.slots, skip=dual[-1])
+            with pytest.raises(RuntimeError, match="tangents"):
+                D.mixer_prompt(*dual[:-1], c.slots, c.offsets, skip=dual[-1])

@@ -466,3 +466,19 @@ def test_shared_inputs_differentiate_twice(G):
         for got, want in zip(*seen):
             # the float32 steps of two blocks and three derivatives, sums of at most 24 x 20 terms
             assert torch.allclose(got.double().cpu(), want, rtol=1e-4, atol=1e-4 * float(want.abs().max())), name
+
+
+def test_forward_mode_is_refused(G):
+    """A tangent raises, whichever argument carries it, under no_grad too."""
+    from torch.autograd import forward_ad
+
+    args, _ = inputs(5, 8, 6, torch.float32, True)
+    announce("gated_linear with tangents")
+    with forward_ad.dual_level():
+        G.gated_linear(*args)
+        for i, t in enumerate(args):
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else u for j, u in enumerate(args)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                G.gated_linear(*dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                G.gated_linear(*dual)

@@ -224,3 +224,17 @@ def test_refusals(L):
                       ("logits must be", {"logits": x[0]}), ("logits must be", {"logits": x.cpu()})):
         with pytest.raises(RuntimeError, match=match):
             L.control_logits(**{"logits": x, **kw})
+
+
+def test_forward_mode_is_refused(L):
+    """A tangent raises, under no_grad too, whichever argument carries it."""
+    from torch.autograd import forward_ad
+
+    floats = {"logits": torch.randn(2, 40).cuda(), "bias_values": torch.randn(2, 3).cuda(),
+              **{k: torch.ones(2).cuda() for k in ("repetition", "presence", "frequency")}}
+    ids = torch.arange(3, dtype=torch.int32).cuda()[None]
+    announce("control_logits with tangents")
+    L.control_logits(**floats, bias_ids=ids)
+    for k, t in floats.items():
+        with torch.no_grad(), forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangents"):
+            L.control_logits(**{**floats, k: forward_ad.make_dual(t, torch.ones_like(t))}, bias_ids=ids)
