@@ -89,7 +89,7 @@ def control_logits(logits: Tensor, history: Optional[Tensor] = None, lengths: Op
                            f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
     rows, V = logits.shape
     given = (logits, repetition, presence, frequency, bias_values, out)
-    needs_grad = torch.is_grad_enabled() and logits.requires_grad
+    needs_grad = torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in given)
     if needs_grad or _lib.has_tangent(given):
         raise RuntimeError("control_logits is for inference: call it under torch.no_grad() and on tensors without tangents")
     if (bias_ids is None) != (bias_values is None):

@@ -238,3 +238,17 @@ def test_forward_mode_is_refused(L):
     for k, t in floats.items():
         with torch.no_grad(), forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangents"):
             L.control_logits(**{**floats, k: forward_ad.make_dual(t, torch.ones_like(t))}, bias_ids=ids)
+
+
+def test_gradients_are_refused(L):
+    """Of the logits and of every penalty and bias, where one is wanted."""
+    floats = {"logits": torch.randn(2, 40).cuda(), "bias_values": torch.randn(2, 3).cuda(),
+              **{k: torch.ones(2).cuda() for k in ("repetition", "presence", "frequency")}}
+    ids = torch.arange(3, dtype=torch.int32).cuda()[None]
+    announce("control_logits with gradients")
+    for k, t in floats.items():
+        grad = {**floats, k: t.clone().requires_grad_(True)}
+        with pytest.raises(RuntimeError, match="inference"):
+            L.control_logits(**grad, bias_ids=ids)
+        with torch.no_grad():
+            L.control_logits(**grad, bias_ids=ids)
