@@ -164,16 +164,13 @@ def _weights(mixer, dtype: torch.dtype):
 def prompt(mixer, inputs: Tensor, state: MixerState, slots: Tensor, offsets: Tensor,
            resume: Optional[Tensor] = None) -> Tensor:
     """``mixer`` (a ``MambaMixer``) over packed prompts, inputs [rows, d_model]; states and
-    offsets as ``mixer_prompt``'s."""
+    offsets as ``mixer_prompt``'s.  As in ``MambaMixer.forward`` there is no skip."""
     xz = mixer.in_proj(inputs)
-    skip = None if mixer.D is None else mixer.D.float()
-    y = mixer_prompt(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots, offsets, resume, skip=skip)
-    return mixer.out_proj(y)
+    return mixer.out_proj(mixer_prompt(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots, offsets, resume))
 
 
 @torch.no_grad()
 def step(mixer, inputs: Tensor, state: MixerState, slots: Tensor) -> Tensor:
     """``mixer`` (a ``MambaMixer``) on the next token of each sequence, inputs [rows, d_model]."""
     xz = mixer.in_proj(inputs)
-    skip = None if mixer.D is None else mixer.D.float()
-    return mixer.out_proj(mixer_step(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots, skip=skip))
+    return mixer.out_proj(mixer_step(xz, *_weights(mixer, xz.dtype), state.conv, state.ssm, slots))

@@ -417,3 +417,28 @@ def test_forward_mode_is_refused(D):
                 D.mixer_step(*dual[:-1], c.slots, skip=dual[-1])
             with pytest.raises(RuntimeError, match="tangents"):
                 D.mixer_prompt(*dual[:-1], c.slots, c.offsets, skip=dual[-1])
+
+
+def _mixer():
+    from ossm_amd.mamba import MambaMixer
+
+    torch.manual_seed(3)
+    return MambaMixer(24, d_state=8, d_conv=4, expand=2).cuda()
+
+
+def _served(D, m, x):
+    """What a mixer answers to x [1, L, d_model] as a prompt of all but the last two and two steps."""
+    st, slot = D.MixerState.of(m, 1), torch.zeros(1, dtype=torch.int32).cuda()
+    L = x.size(1)
+    head = D.prompt(m, x[0, :-2], st, slot, torch.tensor([0, L - 2], dtype=torch.int32).cuda())
+    return torch.cat([head, *(D.step(m, x[0, t:t + 1], st, slot) for t in (L - 2, L - 1))])
+
+
+def test_a_skip_that_the_mixer_does_not_train_is_not_served(D):
+    """MambaMixer.forward has no D skip, whatever its ``D`` holds."""
+    m = _mixer()
+    m.D = torch.nn.Parameter(torch.randn(48).cuda())
+    x = torch.randn(1, 30, 24).cuda()
+    announce("decode of a mixer with D set")
+    with torch.no_grad():
+        check(_served(D, m, x), m(x)[0].double().cpu().numpy(), what="mixer with D")
