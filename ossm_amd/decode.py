@@ -23,7 +23,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 from . import _lib
 
@@ -154,8 +154,13 @@ def mixer_prompt(xz: Tensor, conv_weight: Tensor, conv_bias: Optional[Tensor], x
 # ------------------------------------------------------------------ the module's calls
 def _weights(mixer, dtype: torch.dtype):
     """A ``MambaMixer``'s parameters as the functions take them."""
-    bias = mixer.conv1d.bias
-    like = [mixer.conv1d.weight.to(dtype), None if bias is None else bias.to(dtype), mixer.x_proj.weight.to(dtype),
+    x_proj, bias = mixer.x_proj, mixer.conv1d.bias
+    # the kernels take its weight alone; MambaMixer.forward calls one that does more
+    if not isinstance(x_proj, nn.Linear) or type(x_proj).forward is not nn.Linear.forward or "forward" in x_proj.__dict__ \
+            or x_proj.bias is not None or x_proj._forward_hooks or x_proj._forward_pre_hooks:
+        raise RuntimeError("decode needs a mixer whose x_proj is an nn.Linear without bias, hooks or a forward of its own, "
+                           f"got {x_proj}")
+    like = [mixer.conv1d.weight.to(dtype), None if bias is None else bias.to(dtype), x_proj.weight.to(dtype),
             mixer.dt_proj.weight.to(dtype)]
     return (*like, mixer.dt_proj.bias.float(), mixer.A_log.float())
 

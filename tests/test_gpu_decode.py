@@ -442,3 +442,32 @@ def test_a_skip_that_the_mixer_does_not_train_is_not_served(D):
     announce("decode of a mixer with D set")
     with torch.no_grad():
         check(_served(D, m, x), m(x)[0].double().cpu().numpy(), what="mixer with D")
+
+
+@pytest.mark.parametrize("how", ["bias", "hook", "replaced"])
+def test_an_x_proj_that_is_more_than_its_weight_is_refused(D, how):
+    m = _mixer()
+    if how == "bias":
+        m.x_proj = torch.nn.Linear(48, m.x_proj.out_features).cuda()
+    elif how == "hook":
+        m.x_proj.register_forward_hook(lambda mod, args, out: 2 * out)
+    else:
+        m.x_proj = torch.nn.Sequential(m.x_proj, torch.nn.Identity())
+    x = torch.randn(1, 30, 24).cuda()
+    announce(f"decode of a mixer, x_proj {how}")
+    with pytest.raises(RuntimeError, match="x_proj"):
+        _served(D, m, x)
+    st, slot = D.MixerState.of(m, 1), torch.zeros(1, dtype=torch.int32).cuda()
+    with pytest.raises(RuntimeError, match="x_proj"):
+        D.step(m, x[0, :1], st, slot)
+
+
+def test_a_computed_x_proj_weight_is_served(D):
+    """A parametrized weight is the module's weight: what trains is what answers."""
+    m = _mixer()
+    torch.nn.utils.parametrizations.weight_norm(m.x_proj)
+    x = torch.randn(1, 30, 24).cuda()
+    announce("decode of a mixer, x_proj parametrized")
+    with torch.no_grad():
+        m.x_proj.parametrizations.weight.original0.mul_(1.5)
+        check(_served(D, m, x), m(x)[0].double().cpu().numpy(), what="mixer with a parametrized x_proj")
