@@ -16,7 +16,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _lib
-from .linear import aliases, linear
+from .linear import aliases, is_linear, linear
 
 __all__ = ["ACTIVATIONS", "GatedFeedForward", "GatedLinearFn", "gated_linear"]
 
@@ -138,6 +138,9 @@ class GatedFeedForward(nn.Module):
         self.down_proj = nn.Linear(d_hidden, d_model, bias=bias)
 
     def forward(self, x: Tensor) -> Tensor:
-        h = gated_linear(x, self.gate_proj.weight, self.up_proj.weight, self.gate_proj.bias, self.up_proj.bias,
-                         self.activation)
+        if is_linear(self.gate_proj) and is_linear(self.up_proj):
+            h = gated_linear(x, self.gate_proj.weight, self.up_proj.weight, self.gate_proj.bias, self.up_proj.bias,
+                             self.activation)
+        else:  # a replaced or hooked projection is called as it is
+            h = _TORCH[self.activation](linear(self.gate_proj, x)) * linear(self.up_proj, x)
         return linear(self.down_proj, h)

@@ -16,7 +16,7 @@ from torch import Tensor, nn
 
 from . import _lib
 
-__all__ = ["rows_product", "linear", "linear_weight", "LinearFn", "aliases", "is_plain",
+__all__ = ["rows_product", "linear", "linear_weight", "LinearFn", "aliases", "is_linear", "is_plain",
            "MIN_ROWS", "BLOCK_ROWS"]
 
 # The least the kernel takes, and where the layers' and the mixer's own backwards, which
@@ -88,15 +88,20 @@ class LinearFn(torch.autograd.Function):
         return gx, gw, (g2.sum(0) if need_b and ctx.has_bias else None)
 
 
-def is_plain(module: nn.Module) -> bool:
-    """Whether calling ``module`` is F.linear on its own weight and nothing else
-    (no subclass, no hooks, its own or global, no replaced forward)."""
+def is_linear(module: nn.Module) -> bool:
+    """Whether calling ``module`` is F.linear on its weight and bias and nothing else (no
+    hooks, its own or global, no replaced forward; the weight may be a computed one)."""
     glob = nn.modules.module
-    return (type(module) is nn.Linear and "forward" not in module.__dict__
+    return (isinstance(module, nn.Linear) and type(module).forward is nn.Linear.forward and "forward" not in module.__dict__
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
                      or module._backward_pre_hooks or glob._global_forward_hooks
                      or glob._global_forward_pre_hooks or glob._global_backward_hooks
                      or glob._global_backward_pre_hooks))
+
+
+def is_plain(module: nn.Module) -> bool:
+    """The same of an ``nn.Linear`` itself (no subclass), whose weight is its own."""
+    return type(module) is nn.Linear and is_linear(module)
 
 
 def linear(module: nn.Module, x: Tensor) -> Tensor:

@@ -482,3 +482,21 @@ def test_forward_mode_is_refused(G):
                 G.gated_linear(*dual)
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 G.gated_linear(*dual)
+
+
+@pytest.mark.parametrize("which", ["gate_proj", "up_proj"])
+def test_module_runs_replaced_and_hooked_projections(G, which):
+    """A projection that is more than its weight and bias is called as it is."""
+    torch.manual_seed(1)
+    m = G.GatedFeedForward(20, 36, bias=True).cuda()
+    x = torch.randn(7, 20, device="cuda")
+    getattr(m, which).register_forward_hook(lambda mod, args, out: 2 * out + 1)
+    announce(f"GatedFeedForward with a hook on {which}")
+    want = m.down_proj(torch.nn.functional.silu(m.gate_proj(x)) * m.up_proj(x))
+    assert torch.allclose(m(x), want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
+    setattr(m, which, torch.nn.Sequential(torch.nn.Linear(20, 36), torch.nn.Dropout(0.0)).cuda())
+    want = m.down_proj(torch.nn.functional.silu(m.gate_proj(x)) * m.up_proj(x))
+    assert torch.allclose(m(x), want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
+    setattr(m, which, torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(20, 36)).cuda())
+    want = m.down_proj(torch.nn.functional.silu(m.gate_proj(x)) * m.up_proj(x))
+    assert torch.allclose(m(x), want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
