@@ -434,6 +434,7 @@ def _served(D, m, x):
     return torch.cat([head, *(D.step(m, x[0, t:t + 1], st, slot) for t in (L - 2, L - 1))])
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 def test_a_skip_that_the_mixer_does_not_train_is_not_served(D):
     """MambaMixer.forward has no D skip, whatever its ``D`` holds."""
     m = _mixer()
@@ -444,6 +445,7 @@ def test_a_skip_that_the_mixer_does_not_train_is_not_served(D):
         check(_served(D, m, x), m(x)[0].double().cpu().numpy(), what="mixer with D")
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 @pytest.mark.parametrize("how", ["bias", "hook", "replaced"])
 def test_an_x_proj_that_is_more_than_its_weight_is_refused(D, how):
     m = _mixer()
@@ -462,6 +464,7 @@ def test_an_x_proj_that_is_more_than_its_weight_is_refused(D, how):
         D.step(m, x[0, :1], st, slot)
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 def test_a_computed_x_proj_weight_is_served(D):
     """A parametrized weight is the module's weight: what trains is what answers."""
     m = _mixer()

@@ -484,6 +484,7 @@ def test_forward_mode_is_refused(G):
                 G.gated_linear(*dual)
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 @pytest.mark.parametrize("which", ["gate_proj", "up_proj"])
 def test_module_runs_replaced_and_hooked_projections(G, which):
     """A projection that is more than its weight and bias is called as it is."""

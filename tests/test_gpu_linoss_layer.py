@@ -144,6 +144,7 @@ def test_linoss_layer_second_derivatives(linoss, disc, monkeypatch):
                                        atol=1e-4 * max(1.0, float(r.abs().max())))
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 @pytest.mark.parametrize("disc", ["IM", "IMEX"])
 def test_linoss_layer_applied_twice_under_create_graph(linoss, disc, monkeypatch):
     """Its parameters then reach its own input: create_graph gives the gradients that a

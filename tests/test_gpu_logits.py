@@ -226,6 +226,7 @@ def test_refusals(L):
             L.control_logits(**{"logits": x, **kw})
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 def test_forward_mode_is_refused(L):
     """A tangent raises, under no_grad too, whichever argument carries it."""
     from torch.autograd import forward_ad
@@ -240,6 +241,7 @@ def test_forward_mode_is_refused(L):
             L.control_logits(**{**floats, k: forward_ad.make_dual(t, torch.ones_like(t))}, bias_ids=ids)
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 def test_gradients_are_refused(L):
     """Of the logits and of every penalty and bias, where one is wanted."""
     floats = {"logits": torch.randn(2, 40).cuda(), "bias_values": torch.randn(2, 3).cuda(),

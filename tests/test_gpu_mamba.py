@@ -413,6 +413,7 @@ def test_mixer_core_with_segment_carries(M, shape, monkeypatch):
     no_device_errors()
 
 
+@torch.random.fork_rng()  # later tests draw what they drew
 def test_mixer_applied_twice_under_create_graph(M, monkeypatch):
     """Its parameters then reach its own input: create_graph gives the gradients that a
     plain backward gives, and those of the separate Functions."""
