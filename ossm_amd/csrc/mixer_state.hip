@@ -1113,8 +1113,17 @@ __global__ __launch_bounds__(kScanThreads, NB <= 16 ? (DT ? 3 : 4) : 2) void mix
 
 constexpr int kCarryAhead = 16;  // chunks whose summaries are loaded together
 
-// h through `n` summaries from index c0: h = exp(A sum_dt) h + local (local alone where a
-// prompt starts inside); put(c, h) sees the state before each.
+// h after a chunk that ends at `local` from zero, its sum of dt `sum`: the transition
+// exp(A sum) in two halves, since it may underflow where its product with the state does
+// not (1e33 under e^-96), and each at least the smallest normal number, since an infinite
+// state stays infinite under every decay (what that adds to a finite one is below 2^-124).
+__device__ __forceinline__ float past_chunk(float a2, float sum, float h, float local) {
+  const float f = fmaxf(__builtin_amdgcn_exp2f(0.5f * a2 * sum), 1.17549435e-38f);
+  return fmaf(f * h, f, local);
+}
+
+// h through `n` summaries from index c0 (local alone where a prompt starts inside);
+// put(c, h) sees the state before each.
 template <class Put>
 __device__ __forceinline__ float fold(const float* local, const float* sum_dt, size_t nd, int Di, size_t i, int d,
                                       float a2, int c0, int n, float h, float* total, Put put) {
@@ -1130,7 +1139,7 @@ __device__ __forceinline__ float fold(const float* local, const float* sum_dt, s
     for (int k = 0; k < kCarryAhead; ++k) {
       if (q + k >= n) break;
       put(c0 + q + k, h);
-      h = sd[k] < 0.f ? l[k] : fmaf(__builtin_amdgcn_exp2f(a2 * sd[k]), h, l[k]);
+      h = sd[k] < 0.f ? l[k] : past_chunk(a2, sd[k], h, l[k]);
       *total = sd[k] < 0.f || *total < 0.f ? -1.f : *total + sd[k];
     }
   }

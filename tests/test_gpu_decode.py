@@ -474,3 +474,26 @@ def test_a_computed_x_proj_weight_is_served(D):
     with torch.no_grad():
         m.x_proj.parametrizations.weight.original0.mul_(1.5)
         check(_served(D, m, x), m(x)[0].double().cpu().numpy(), what="mixer with a parametrized x_proj")
+
+
+@pytest.mark.parametrize("rows", [64, 400])
+def test_states_past_the_range_of_a_chunks_decay(D, rows):
+    """exp(A sum dt) of a chunk of tokens leaves float32's range where its product with the
+    state does not (1e33 under e^-96), and an infinite state stays infinite.  The exponent of
+    138 binary digits is rounded in 16 steps, 138 * 16 * 2^-24 * ln 2 = 9e-5 of the state."""
+    c = Case(64, 3, 1, 1, [rows], seed=15, skip=False, bias=False)
+    cw, _, xp, dp, db, al = c.w
+    for t, v in ((cw, 1), (xp, 0), (dp, 1), (db, -8), (al, 0)):
+        t.fill_(v)
+    # p = (u_0, for dt; u_1 = 0 for B: nothing is added to the state; u_2 = 1.3 for C)
+    xp[0, 0], xp[1:4, 1], xp[4:, 2] = 1, 1, 1
+    c.xz[:, :3] = torch.tensor([-30.0, 0.0, 1.6]).cuda()
+    c.xz[17:31, 0] = 6.857 + 8  # 14 tokens of one chunk, whatever its ends: dt = 6.857
+    for value in (1e33, float("inf"), -float("inf")):
+        c.ssm.fill_(value)
+        announce(f"mixer_prompt of {rows} rows from states of {value}")
+        with np.errstate(invalid="ignore"):
+            want = reference(c, [True])
+        y = run_prompt(D, c, torch.ones(1, dtype=torch.bool).cuda()).double().cpu().numpy()
+        np.testing.assert_allclose(y, want[0], rtol=5e-4)
+        np.testing.assert_allclose(c.ssm[c.slots.long()].double().cpu().numpy(), want[2][c.slots.tolist()], rtol=5e-4)
