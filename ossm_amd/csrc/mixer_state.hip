@@ -1202,6 +1202,11 @@ int launch_scans(const Mixer<E>& g, bool out, bool dt, hipStream_t st) {
 template <class E>
 bool vec8(const E* p, int row) { return aligned16(p) && row % (16 / static_cast<int>(sizeof(E))) == 0; }
 
+// A stretch of the workspace of at least n floats whose end, the next one's start, is on 256
+// bytes: vectors of 16 bytes are stored to it.
+constexpr size_t stretch(size_t n) { return (n + 63) / 64 * 64; }
+static_assert(stretch(18 * 299 * 83) % 4 == 0, "16-byte starts");
+
 constexpr int kTokenRows = 2;  // rows of a workgroup of token_scan_kernel where there are many
 
 template <class E>
@@ -1217,7 +1222,7 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const bool tiles = many && g.Di % 8 == 0 && g.ld % e16 == 0 && aligned16(g.xz) && aligned16(g.conv_state) &&
                      aligned16(g.conv_w) && aligned16(g.conv_b) && aligned16(g.x_proj);
   g.n_blocks = (g.Di + (tiles ? kTileK : kProjBlock) - 1) / (tiles ? kTileK : kProjBlock);
-  const size_t part = static_cast<size_t>(g.n_blocks) * g.rows * g.Nc;
+  const size_t part = stretch(static_cast<size_t>(g.n_blocks) * g.rows * g.Nc);
   void* ws = nullptr;
   if (int rc = acquire_workspace(call, (part + static_cast<size_t>(g.rows) * g.Di) * sizeof(float), &ws)) return rc;
   g.part = static_cast<float*>(ws);
@@ -1271,7 +1276,7 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const size_t nd = static_cast<size_t>(g.N) * g.Di;
   const bool carries = g.n_chunks > 1;
   size_t at = 0;
-  const auto take = [&](size_t n) { const size_t o = at; at += (n + 63) / 64 * 64; return o; };
+  const auto take = [&](size_t n) { const size_t o = at; at += stretch(n); return o; };
   const size_t o_part = take(static_cast<size_t>(g.n_blocks) * g.rows * g.Nc);
   const size_t o_planes = take((3 * static_cast<size_t>(g.rows) * g.Rp + 1) / 2);
   const size_t o_bc = take(static_cast<size_t>(g.rows) * 2 * g.Npad);

@@ -497,3 +497,18 @@ def test_states_past_the_range_of_a_chunks_decay(D, rows):
         y = run_prompt(D, c, torch.ones(1, dtype=torch.bool).cuda()).double().cpu().numpy()
         np.testing.assert_allclose(y, want[0], rtol=5e-4)
         np.testing.assert_allclose(c.ssm[c.slots.long()].double().cpu().numpy(), want[2][c.slots.tolist()], rtol=5e-4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_step_in_tiles_of_an_odd_number_of_sums(D, dtype):
+    """Rows in tiles whose projections' sums are no multiple of four: what lies behind them in
+    the workspace is stored in vectors."""
+    Di, N, R, rows = 2184, 7, 69, 299  # 18 blocks of channels x 299 x 83 sums, 2 over a multiple of 4
+    assert -(-Di // 128) * rows * (R + 2 * N) % 4 == 2
+    c = Case(Di, N, R, 4, [1] * rows, dtype, seed=16)
+    announce(f"mixer_step tiles, odd sums {dtype}")
+    want = reference(c, [True] * rows)
+    y = D.mixer_step(c.xz, *c.args(), skip=c.skip)
+    check(y, want[0], dtype, "y")
+    check(c.conv, want[1], torch.float32, "conv state")
+    check(c.ssm, want[2], torch.float32, "ssm state")
