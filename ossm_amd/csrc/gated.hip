@@ -872,7 +872,7 @@ int pack(PackJobs<E> jobs, hipStream_t st) {
     blocks += (jobs.chunks[i] + 255) / 256;
   }
   if (blocks == 0) return OSSM_OK;  // nothing to copy, or nothing in it
-  if (blocks > INT_MAX) return set_error(OSSM_ERR_UNSUPPORTED, "gated: size exceeds launch limits");
+  if (int rc = check_grid("gated", blocks, 256)) return rc;
   hipLaunchKernelGGL(pack_kernel<E>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, jobs);
   return launch_check("pack_kernel");
 }
@@ -884,7 +884,7 @@ int launch_tiled(Product<E> g, hipStream_t st) {
   g.tiles_m = (g.M + TM - 1) / TM;
   g.tiles_n = (g.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
   const int64_t grid = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
-  if (grid > INT_MAX) return set_error(OSSM_ERR_UNSUPPORTED, "gated: size exceeds launch limits");
+  if (int rc = check_grid("gated", grid, WM * WN * kWave)) return rc;
   auto kern = product_kernel<E, ACOL, BCOL, GATED, WM, WN, FM, FN>;
   if (int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
                          "hipFuncSetAttribute"))
@@ -1052,12 +1052,14 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
   float* sums = want_b ? reinterpret_cast<float*>(base + o_sums) : nullptr;
   const int T = static_cast<int>(p.T), F = static_cast<int>(p.F), D = static_cast<int>(p.D), fp = static_cast<int>(Fp);
   const bool vec = F % 8 == 0 && aligned16(go) && aligned16(a) && aligned16(b) && ld_go * static_cast<int64_t>(sizeof(E)) % 16 == 0;
+  const int64_t grad_groups = (rbs * (Fp / 8) + 255) / 256;
+  if (int rc = check_grid("gated", grad_groups, 256)) return rc;
   const auto grads = [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     auto kern = vec ? gate_grad_kernel<E, ACT, true, false> : gate_grad_kernel<E, ACT, false, false>;
     if constexpr (sizeof(E) == 2)
       if (two) kern = vec ? gate_grad_kernel<E, ACT, true, true> : gate_grad_kernel<E, ACT, false, true>;
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((rbs * (Fp / 8) + 255) / 256)), dim3(256), 0, st, go, ld_go, a, b, dab,
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grad_groups)), dim3(256), 0, st, go, ld_go, a, b, dab,
                        static_cast<long long>(dab_plane), sums, T, F, fp, rows_per);
     return launch_check("gate_grad_kernel");
   };
@@ -1125,14 +1127,14 @@ int backward(const Gated<E>& p, const E* go, int64_t ld_go, const float* a, cons
 }
 
 __global__ __launch_bounds__(256) void gated_zero_kernel(uint16_t* p, int64_t n) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) p[i] = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) p[i] = 0;
 }
 
 int zero(void* p, int64_t bytes, hipStream_t st) {
   if (p == nullptr || bytes == 0) return OSSM_OK;
-  const int64_t n = bytes / 2;
-  hipLaunchKernelGGL(gated_zero_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, static_cast<uint16_t*>(p), n);
+  const int64_t n = bytes / 2, groups = std::min<int64_t>((n + 255) / 256, 1 << 16);
+  hipLaunchKernelGGL(gated_zero_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, static_cast<uint16_t*>(p), n);
   return launch_check("gated_zero_kernel");
 }
 

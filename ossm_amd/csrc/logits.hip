@@ -230,8 +230,8 @@ template <class E>
 int run(Logits<E> g, int64_t rows, hipStream_t st) {
   constexpr int W = 16 / static_cast<int>(sizeof(E));
   g.n_blocks = (g.V + W - 1 + kBlock - 1) / kBlock;  // the shift may need one more
-  if (rows * g.n_blocks > INT_MAX)
-    return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
+  if (rows > INT_MAX) return set_error(OSSM_ERR_UNSUPPORTED, "control_logits: size exceeds launch limits");
+  if (int rc = check_grid("control_logits", rows * g.n_blocks, kThreads)) return rc;
   const bool wide = g.H >= (1 << 15) || g.n_bias >= (1 << 16);
   const size_t lds = (wide ? Words<true>::kWords : Words<false>::kWords) * sizeof(uint32_t);
   auto kern = wide ? control_logits_kernel<E, true> : control_logits_kernel<E, false>;

@@ -1222,6 +1222,9 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const bool tiles = many && g.Di % 8 == 0 && g.ld % e16 == 0 && aligned16(g.xz) && aligned16(g.conv_state) &&
                      aligned16(g.conv_w) && aligned16(g.conv_b) && aligned16(g.x_proj);
   g.n_blocks = (g.Di + (tiles ? kTileK : kProjBlock) - 1) / (tiles ? kTileK : kProjBlock);
+  const int rows_per = tiles ? kTileRows : many ? 8 : 1;
+  const int64_t groups = static_cast<int64_t>(g.n_blocks) * ((g.rows + rows_per - 1) / rows_per);
+  if (int rc = check_grid("mixer_step", groups, tiles ? kTileThreads : kProjThreads)) return rc;
   const size_t part = stretch(static_cast<size_t>(g.n_blocks) * g.rows * g.Nc);
   void* ws = nullptr;
   if (int rc = acquire_workspace(call, (part + static_cast<size_t>(g.rows) * g.Di) * sizeof(float), &ws)) return rc;
@@ -1229,15 +1232,12 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   g.u = g.part + part;
   const bool vx = vec8(g.x_proj, g.Di);
   if (tiles) {
-    const dim3 grid(static_cast<unsigned>(g.n_blocks * ((g.rows + kTileRows - 1) / kTileRows)));
-    hipLaunchKernelGGL(k4 ? (token_tile_kernel<E, 4>) : (token_tile_kernel<E, 8>), grid, dim3(kTileThreads), 0, st, g);
+    hipLaunchKernelGGL(k4 ? (token_tile_kernel<E, 4>) : (token_tile_kernel<E, 8>), dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, st, g);
     if (int rc = launch_check("token_tile_kernel")) return rc;
   } else {
-    const int rb = many ? 8 : 1;
-    const dim3 grid(static_cast<unsigned>(g.n_blocks * ((g.rows + rb - 1) / rb)));
     auto proj = many ? (k4 ? token_proj_kernel<E, 8, 4> : token_proj_kernel<E, 8, 8>)
                      : (k4 ? token_proj_kernel<E, 1, 4> : token_proj_kernel<E, 1, 8>);
-    hipLaunchKernelGGL(proj, grid, dim3(kProjThreads), 0, st, g, vx);
+    hipLaunchKernelGGL(proj, dim3(static_cast<unsigned>(groups)), dim3(kProjThreads), 0, st, g, vx);
     if (int rc = launch_check("token_proj_kernel")) return rc;
   }
   const int rt = many_scan ? kTokenRows : 1, threads = many_scan ? 256 : 64;
@@ -1251,6 +1251,15 @@ int step(Mixer<E> g, StreamCall& call, hipStream_t st) {
   return launch_check("token_scan_kernel");
 }
 
+int64_t padded_states(int64_t n) { return n <= 8 ? 8 : n <= 16 ? 16 : (n + 31) / 32 * 32; }
+int64_t padded_rank(int64_t r) { return (r + 15) / 16 * 16; }
+
+// prompt_sum_kernel's workgroups: of the sums, and of the prompts it finishes.
+int64_t prompt_sum_groups(int64_t rows, int64_t r, int64_t n) {
+  return (rows * (padded_rank(r) + 2 * padded_states(n)) + 255) / 256;
+}
+int64_t prompt_finishers(int64_t di, int64_t n_seqs) { return (di + 255) / 256 * n_seqs; }
+
 template <class E>
 int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const int64_t cus = std::max(1, device_cu_count(call.device()));
@@ -1261,8 +1270,8 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
   const int64_t ways = std::max<int64_t>(1, std::min<int64_t>({row_tiles * col_groups * 32 <= cus ? 32 : 8, k_steps, 4 * cus / std::max<int64_t>(1, row_tiles * col_groups)}));
   const int per_split = static_cast<int>((k_steps + ways - 1) / ways) * kPtK;
   g.n_blocks = (g.Di + per_split - 1) / per_split;
-  g.Npad = g.N <= 8 ? 8 : g.N <= 16 ? 16 : (g.N + 31) / 32 * 32;
-  g.Rp = (g.R + 15) / 16 * 16;
+  g.Npad = static_cast<int>(padded_states(g.N));
+  g.Rp = static_cast<int>(padded_rank(g.R));
   // enough chunks for four waves on each SIMD, of 16 tokens at least
   const int64_t waves = (g.Di + kWave - 1) / kWave;
   const int64_t want = std::max<int64_t>(1, 16 * cus / waves);
@@ -1311,9 +1320,8 @@ int prompt(Mixer<E> g, StreamCall& call, hipStream_t st) {
                        dim3(static_cast<unsigned>(row_tiles * g.n_blocks * col_groups)), dim3(256), 0, st, g, per_split,
                        vec8(g.x_proj, g.Di));
     if (int rc = launch_check("prompt_proj_kernel")) return rc;
-    const int64_t sums = static_cast<int64_t>(g.rows) * (g.Rp + 2 * g.Npad);
-    const unsigned sum_groups = static_cast<unsigned>((sums + 255) / 256);
-    const unsigned finishers = g.resume == nullptr ? static_cast<unsigned>((g.Di + 255) / 256) * static_cast<unsigned>(g.n_seqs) : 0;
+    const unsigned sum_groups = static_cast<unsigned>(prompt_sum_groups(g.rows, g.R, g.N));
+    const unsigned finishers = g.resume == nullptr ? static_cast<unsigned>(prompt_finishers(g.Di, g.n_seqs)) : 0;
     hipLaunchKernelGGL(prompt_sum_kernel<E>, dim3(sum_groups + finishers), dim3(256), 0, st, g, sum_groups);
     if (int rc = launch_check("prompt_sum_kernel")) return rc;
     if (g.resume != nullptr) {
@@ -1440,6 +1448,8 @@ int ossm_mixer_prompt(int dtype, const void* xz, int64_t ld_xz, const void* conv
   if (int rc = check_mixer("mixer_prompt", dtype, rows, n_seqs, n_slots, d_inner, d_state, dt_rank, d_conv, ld_xz)) return rc;
   if (d_inner == 0 || (rows == 0 && n_seqs == 0)) return OSSM_OK;
   if (n_seqs == 0) return set_error(OSSM_ERR_INVALID_ARGUMENT, "mixer_prompt: rows without a sequence");
+  if (int rc = check_grid("mixer_prompt", prompt_sum_groups(rows, dt_rank, d_state) + prompt_finishers(d_inner, n_seqs), 256))
+    return rc;
   if ((rows > 0 && (!xz || !y)) || !conv_w || !x_proj || !dt_proj || !dt_bias || !a_log || !in_slots || !offsets ||
       (n_slots > 0 && (!ssm_state || (d_conv > 1 && !conv_state))))
     return set_error(OSSM_ERR_INVALID_ARGUMENT, "mixer_prompt: null pointer");

@@ -75,6 +75,12 @@ int hip_check(hipError_t e, const char* what) {
   return set_error(OSSM_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
+int check_grid(const char* what, int64_t groups, int threads) {
+  if (groups < 0 || groups > (int64_t(1) << 32) / threads - 1)
+    return set_error(OSSM_ERR_UNSUPPORTED, std::string(what) + ": size exceeds launch limits");
+  return OSSM_OK;
+}
+
 int launch_check(const char* what) {
   return hip_check(hipGetLastError(), what);
 }

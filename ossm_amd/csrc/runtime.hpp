@@ -144,6 +144,10 @@ int acquire_scratch(StreamCall& call, size_t payload_bytes, int64_t n_workgroups
 // would have to grow.
 int acquire_workspace(StreamCall& call, size_t bytes, void** ptr);
 
+// Whether HIP takes a launch of `groups` workgroups of `threads` along x (it counts their
+// threads in 32 bits): OSSM_OK, or OSSM_ERR_UNSUPPORTED.
+int check_grid(const char* what, int64_t groups, int threads);
+
 // Launch-error check after a kernel launch (reference: C10_CUDA_KERNEL_LAUNCH_CHECK).
 int launch_check(const char* what);
 

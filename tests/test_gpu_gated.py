@@ -501,3 +501,16 @@ def test_module_runs_replaced_and_hooked_projections(G, which):
     setattr(m, which, torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(20, 36)).cuda())
     want = m.down_proj(torch.nn.functional.silu(m.gate_proj(x)) * m.up_proj(x))
     assert torch.allclose(m(x), want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
+
+
+def test_empty_batch_of_large_weights(G):
+    """Zeros for more of a weight's gradient than a launch has threads for, two bytes each."""
+    from ossm_amd import _lib
+
+    n, D = 1 << 19, 4100
+    grad = torch.ones(n, D, device="cuda")
+    assert grad.numel() * 4 > 2 ** 33
+    announce("gated_linear backward of an empty batch, 8.6 GB of weights")
+    _lib.run(_lib.load().ossm_gated_backward, grad, 0, None, n, None, D, None, D, None, D, 0, None, None, None,
+             grad.data_ptr(), None, None, None, 0, D, n)
+    assert not grad.any()

@@ -123,3 +123,11 @@ def test_gated_refuses_host_tensors_and_unknown_activations():
         gated_linear(z, z, z, activation="tanh")
     with pytest.raises(ValueError, match="activation"):
         GatedFeedForward(8, 8, activation="tanh")
+
+
+def test_launches_past_32_bits_of_threads_are_refused_before_any_hip_call():
+    assert _call("ossm_control_logits", rows=2**24, vocab=1) == (3, "control_logits: size exceeds launch limits")
+    assert _call("ossm_control_logits", rows=2**62, vocab=1) == (3, "control_logits: size exceeds launch limits")
+    big = {"d_inner": 2**17, "ld_xz": 2**18}
+    assert _call("ossm_mixer_prompt", rows=2**24, ld_xz=2, dt_rank=240, d_state=64)[0] == 3  # x_proj's sums
+    assert _call("ossm_mixer_prompt", rows=2**16, n_seqs=2**15, **big) == (3, "mixer_prompt: size exceeds launch limits")
