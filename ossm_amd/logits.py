@@ -114,8 +114,8 @@ def control_logits(logits: Tensor, history: Optional[Tensor] = None, lengths: Op
     allowed, ld_a = _rows(allowed, rows, (V + 31) // 32, torch.int32, "allowed", dev)
     if out is None:
         out = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev or out.stride(1) != 1 or \
-            (rows > 1 and out.stride(0) < V):
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev or \
+            (V > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < V):
         raise RuntimeError("control_logits: out must have the logits' shape, dtype and device and whole rows, got "
                            f"{out.dtype} {tuple(out.shape)} strides {out.stride()} on {out.device}")
     if logits.stride(1) != 1 and V > 1:

@@ -254,3 +254,16 @@ def test_gradients_are_refused(L):
             L.control_logits(**grad, bias_ids=ids)
         with torch.no_grad():
             L.control_logits(**grad, bias_ids=ids)
+
+
+def test_a_vocabulary_of_one_at_any_stride(L):
+    """A single column has no column stride to check, in place too."""
+    wide = torch.arange(1.0, 41.0).cuda().view(5, 8)
+    x, out = wide[:, 2:3].T.T, wide[:, ::3][:, 2:3]
+    one = torch.as_strided(wide, (5, 1), (8, 3), 4)
+    announce("control_logits of one column, strided")
+    want = one.clone() * 0.5
+    hist = torch.zeros(1, 1, dtype=torch.int32).cuda()
+    assert L.control_logits(one, hist, repetition=2.0, out=one) is one
+    assert torch.equal(one, want)
+    assert torch.equal(L.control_logits(x, hist, repetition=2.0, out=out), x * 0.5)
