@@ -7,10 +7,10 @@
  * The conventions are ossm_scan.h's: device pointers, sizes and a HIP stream (as
  * void*), asynchronous launches on that stream, status 0 or an error with
  * ossm_last_error(), outputs written and never allocated, scratch from the
- * library's workspace of the stream (grown on demand outside stream capture,
- * refused under capture with OSSM_ERR_UNSUPPORTED).  No call synchronises, reads
- * device memory on the host or uses atomics on floating-point values: results are
- * bitwise repeatable.
+ * library's workspace of the stream (grown on demand outside stream capture, which
+ * waits for the stream and allocates; refused under capture with OSSM_ERR_UNSUPPORTED).
+ * No other call synchronises; none reads device memory on the host or uses atomics on
+ * floating-point values: results are bitwise repeatable.
  *
  * dtype: OSSM_F32 (0) or OSSM_BF16 (1), of the tensors marked E below; everything
  * else is float32.  Sums, states and statistics are held in float32, and each
@@ -48,7 +48,8 @@ int ossm_lm_abi_version(void);
  *
  * Weights: conv_w E [Di, K], conv_bias E [Di] or null, x_proj E [R + 2N, Di],
  * dt_proj E [Di, R], dt_bias f32 [Di], a_log f32 [Di, N], skip f32 [Di] or null.
- * xz E [rows, 2 Di] with row stride ld_xz, y E [rows, Di] dense.  1 <= K <= 8.
+ * xz E [rows, 2 Di] with row stride ld_xz, y E [rows, Di] dense.  1 <= K <= 8; up to
+ * 65535 sequences a call.
  *
  * ossm_mixer_step: one token of each of `rows` sequences; a row whose in and out
  * slot are both outside the pool is padding: its y is zero.
@@ -106,8 +107,10 @@ enum { OSSM_ACT_SILU = 0, OSSM_ACT_GELU = 1, OSSM_ACT_GELU_TANH = 2, OSSM_ACT_SI
  * ossm_gated_backward: with grad_y E [rows, d_out] (row stride ld_grad) and the
  * forward's a and b, the gradients of x, of the weights and of the biases, all dense E;
  * a null gradient is not computed.  float32 products take three bf16 terms of
- * each operand (24 bits); in bfloat16 the gradients of a and b are rounded to
- * bfloat16 before their products.
+ * each operand (24 bits).  In bfloat16 the gradients of a and b enter their products
+ * as two bfloat16 terms (16 bits) where rows * d_out <= 2^18, and rounded to one past
+ * that: their errors then average out, and a gradient is about 1.41 times as far from the
+ * exact one as that one's own rounding to bfloat16.
  */
 int ossm_gated_forward(int dtype, const void* x, int64_t ld_x, const void* w_gate, int64_t ld_gate, const void* w_up,
                        int64_t ld_up, const void* b_gate, const void* b_up, int activation, void* y, float* a, float* b,
