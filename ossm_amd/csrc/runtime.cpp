@@ -180,7 +180,10 @@ int acquire_scratch(StreamCall& call, size_t payload_bytes, int64_t n_workgroups
     cap = (cap + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
     void* p = nullptr;
     if (int rc = hip_check(hipMalloc(&p, kHdrBytes + cap), "hipMalloc(scratch)")) return rc;
-    if (int rc = hip_check(hipMemset(p, 0, kHdrBytes + cap), "hipMemset(scratch)")) {
+    // on the call's own stream: hipMemset runs on the null stream and may return before it is
+    // done, and a stream that does not wait for that one would have its first records cleared
+    // under it, or read what the memory held before (no capture gets here)
+    if (int rc = hip_check(hipMemsetAsync(p, 0, kHdrBytes + cap, call.stream()), "hipMemsetAsync(scratch)")) {
       (void)hipFree(p);
       return rc;
     }
@@ -271,7 +274,7 @@ uint32_t ossm_device_error_bits(ossm_stream_t stream_v) {
     t = (t | (ossm::kEpochSpan - 1)) + 1;
     (void)hipMemcpy(base + ossm::kHdrTicket, &t, sizeof(t), hipMemcpyHostToDevice);
   }
-  if (bits != 0) (void)hipMemset(base + ossm::kHdrErr, 0, sizeof(bits));
+  if (bits != 0) (void)hipMemsetAsync(base + ossm::kHdrErr, 0, sizeof(bits), stream);
   return bits | fixed_bits;
 }
 
