@@ -1,8 +1,9 @@
 /*
  * ossm_lm.h — C ABI of libossm_scan.so's operators for serving and training language
  * models built on the Mamba mixer: the mixer over ragged prompts and over single
- * tokens with its states in a pool, the gated projection of a feed-forward block,
- * and the control of logits.
+ * tokens with its states in a pool, the gated linear recurrence in the same forms and in
+ * training, the gated projection of a feed-forward block, layer norm, the control of
+ * logits and the choice of a token from them.
  *
  * The conventions are ossm_scan.h's: device pointers, sizes and a HIP stream (as
  * void*), asynchronous launches on that stream, status 0 or an error with
@@ -120,6 +121,91 @@ int ossm_gated_backward(int dtype, const void* grad_y, int64_t ld_grad, const vo
                         int64_t ld_gate, const void* w_up, int64_t ld_up, int activation, const float* a, const float* b,
                         void* grad_x, void* grad_w_gate, void* grad_w_up, void* grad_b_gate, void* grad_b_up,
                         int64_t rows, int64_t d_in, int64_t d_out, ossm_stream_t stream);
+
+/*
+ * Layer norm of rows, alone or of a residual sum:
+ *   s = x + residual, rounded to E (x itself where residual is null)
+ *   y = (s - mean(s)) rstd weight + bias,  rstd = (mean((s - mean(s))^2) + eps)^-1/2
+ * x, residual E [rows, dim] with row strides ld_*; weight, bias [dim] of weight_dtype (the
+ * same as dtype, or OSSM_F32), or null for ones and zeros; y, sum E [rows, dim] dense, sum
+ * given exactly where residual is.  mean, rstd f32 [rows], written for the backward, or both null.
+ *
+ * ossm_layer_norm_backward: with grad_y, grad_sum (null where nothing reaches the sum) E
+ * [rows, dim] and s, the forward's sum (or x), the gradients of x (and of the residual,
+ * which is the same) E dense, and of weight and bias in their type; a null gradient is
+ * not computed.
+ */
+int ossm_layer_norm_forward(int dtype, int weight_dtype, const void* x, int64_t ld_x, const void* residual,
+                            int64_t ld_residual, const void* weight, const void* bias, float eps, void* y, void* sum,
+                            float* mean, float* rstd, int64_t rows, int64_t dim, ossm_stream_t stream);
+
+int ossm_layer_norm_backward(int dtype, int weight_dtype, const void* grad_y, int64_t ld_grad_y, const void* grad_sum,
+                             int64_t ld_grad_sum, const void* s, int64_t ld_s, const void* weight, const float* mean,
+                             const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, int64_t rows,
+                             int64_t dim, ossm_stream_t stream);
+
+/*
+ * The gated linear recurrence, per channel d of dim:
+ *   a_t = exp(-scale softplus(decay[d]) sigmoid(decay_gate_t))
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t
+ *   y_t = h_t, or h_t silu(output_gate_t) where output_gate is given
+ * x and the gates E, rows of dim with row strides ld_*; decay f32 [dim]; y E dense.
+ *
+ * ossm_recurrence_forward: [batch, length] rows of each tensor; start f32 [batch, dim] or
+ * null (zeros); last f32 [batch, dim] takes h of the last step.  saved: f32, of
+ * ossm_recurrence_saved(batch, length, dim) elements, written for the backward, or null.
+ *
+ * ossm_recurrence_backward: with grad_y E and grad_last f32 [batch, dim] (or null), the
+ * gradients of x and the gates E with row stride ld_grads, of decay and start f32; a null
+ * gradient is not computed.
+ *
+ * ossm_recurrence_prompt, ossm_recurrence_step: packed prompts and single tokens with
+ * states in a pool, state f32 [n_slots, dim]; slots, offsets, resume and padding as
+ * ossm_mixer_prompt's and ossm_mixer_step's.
+ */
+int64_t ossm_recurrence_saved(int64_t batch, int64_t length, int64_t dim);
+
+int ossm_recurrence_forward(int dtype, const void* x, int64_t ld_x, const void* input_gate, int64_t ld_input_gate,
+                            const void* decay_gate, int64_t ld_decay_gate, const void* output_gate, int64_t ld_output_gate,
+                            const float* decay, float scale, const float* start, void* y, float* last, float* saved,
+                            int64_t batch, int64_t length, int64_t dim, ossm_stream_t stream);
+
+int ossm_recurrence_backward(int dtype, const void* grad_y, int64_t ld_grad, const float* grad_last, const void* x,
+                             int64_t ld_x, const void* input_gate, int64_t ld_input_gate, const void* decay_gate,
+                             int64_t ld_decay_gate, const void* output_gate, int64_t ld_output_gate, const float* decay,
+                             float scale, const float* saved, void* grad_x, void* grad_input_gate, void* grad_decay_gate,
+                             void* grad_output_gate, int64_t ld_grads, float* grad_decay, float* grad_start,
+                             int64_t batch, int64_t length, int64_t dim, ossm_stream_t stream);
+
+int ossm_recurrence_prompt(int dtype, const void* x, int64_t ld_x, const void* input_gate, int64_t ld_input_gate,
+                           const void* decay_gate, int64_t ld_decay_gate, const void* output_gate, int64_t ld_output_gate,
+                           const float* decay, float scale, float* state, const int32_t* in_slots, const int32_t* out_slots,
+                           const int32_t* offsets, const uint8_t* resume, void* y, int64_t rows, int64_t n_seqs,
+                           int64_t n_slots, int64_t dim, ossm_stream_t stream);
+
+int ossm_recurrence_step(int dtype, const void* x, int64_t ld_x, const void* input_gate, int64_t ld_input_gate,
+                         const void* decay_gate, int64_t ld_decay_gate, const void* output_gate, int64_t ld_output_gate,
+                         const float* decay, float scale, float* state, const int32_t* in_slots, const int32_t* out_slots,
+                         void* y, int64_t rows, int64_t n_slots, int64_t dim, ossm_stream_t stream);
+
+/*
+ * The next token of each row from its logits E [rows, vocab] (row stride ld_logits) and a
+ * given random number uniform[row] in [0, 1):
+ *   w_v = exp((logits[v] - max) / temperature), the largest's is 1; NaN counts as -inf
+ *   kept, in falling order of the logits (equal ones by their index): the first top_k (0 or
+ *   less: all); of those each before which less than top_p of their sum lies (1 or more: all);
+ *   of those each with w_v >= min_p; the first always
+ *   tokens[row] = the least v at which the sum of the kept weights up to it passes
+ *   uniform of their whole sum; with a temperature that is not above 0 the first kept
+ * tokens int64 [rows]; -1 for a row of which every logit is -inf.  temperature, top_p,
+ * min_p f32 [rows] and top_k int32 [rows], or null and the value *_all for every row.
+ * Weights are whole multiples of a power of two from 2^-46 to 2^-43, by the vocabulary's
+ * size, so that their sums do not depend on an order; vocab is at most 2^20.
+ */
+int ossm_sample_logits(int dtype, const void* logits, int64_t ld_logits, const float* uniform, const float* temperature,
+                       float temperature_all, const int32_t* top_k, int64_t top_k_all, const float* top_p, float top_p_all,
+                       const float* min_p, float min_p_all, int64_t* tokens, int64_t rows, int64_t vocab,
+                       ossm_stream_t stream);
 
 #ifdef __cplusplus
 }

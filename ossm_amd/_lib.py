@@ -170,6 +170,30 @@ _LM_SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_int, _vp, _c_int64, _vp, _c_int64, _vp, _c_int64, _c_int64, _vp, _vp, _fp, ctypes.c_float, _fp,
          ctypes.c_float, _fp, ctypes.c_float, _vp, _fp, _c_int64, _c_int64, _vp, _c_int64, _c_int64, _c_int64, _vp]),
+    "ossm_layer_norm_forward": (
+        ctypes.c_int,
+        [ctypes.c_int] * 2 + [_vp, _c_int64] * 2 + [_vp] * 2 + [ctypes.c_float] + [_vp] * 4 + [_c_int64] * 2 + [_vp]),
+    "ossm_layer_norm_backward": (
+        ctypes.c_int, [ctypes.c_int] * 2 + [_vp, _c_int64] * 3 + [_vp] * 6 + [_c_int64] * 2 + [_vp]),
+    "ossm_recurrence_saved": (_c_int64, [_c_int64] * 3),
+    "ossm_recurrence_forward": (
+        ctypes.c_int,
+        [ctypes.c_int] + [_vp, _c_int64] * 4 + [_fp, ctypes.c_float] + [_vp] * 4 + [_c_int64] * 3 + [_vp]),
+    "ossm_recurrence_backward": (
+        ctypes.c_int,
+        [ctypes.c_int, _vp, _c_int64, _fp] + [_vp, _c_int64] * 4 + [_fp, ctypes.c_float] + [_vp] * 5
+        + [_c_int64] + [_vp] * 2 + [_c_int64] * 3
+        + [_vp]),
+    "ossm_recurrence_prompt": (
+        ctypes.c_int,
+        [ctypes.c_int] + [_vp, _c_int64] * 4 + [_fp, ctypes.c_float] + [_vp] * 6 + [_c_int64] * 4 + [_vp]),
+    "ossm_recurrence_step": (
+        ctypes.c_int,
+        [ctypes.c_int] + [_vp, _c_int64] * 4 + [_fp, ctypes.c_float] + [_vp] * 4 + [_c_int64] * 3 + [_vp]),
+    "ossm_sample_logits": (
+        ctypes.c_int,
+        [ctypes.c_int, _vp, _c_int64, _fp, _fp, ctypes.c_float, _vp, _c_int64, _fp, ctypes.c_float, _fp, ctypes.c_float,
+         _vp, _c_int64, _c_int64, _vp]),
 }
 
 LM_EXPORTED = tuple(_LM_SIGNATURES)

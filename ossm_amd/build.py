@@ -25,7 +25,7 @@ LIB = LIBDIR / "libossm_scan.so"
 
 SOURCES = ["runtime.cpp", "oscillator_scan.hip", "selective_scan.hip", "sdlinoss_scan.hip",
            "diag_scan.hip", "dlinoss_layer.hip", "gated.hip", "layer_params.hip", "logits.hip", "mamba_conv.hip",
-           "mixer_state.hip", "rows_product.hip", "scan_f64.hip",
+           "mixer_state.hip", "norm.hip", "recurrence.hip", "rows_product.hip", "sample.hip", "scan_f64.hip",
            "shard_scan.hip"]
 # standalone measurement program (not linked into the library)
 ISSUE_RATE_SRC = "valu_issue_rate.hip"

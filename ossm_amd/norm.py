@@ -1,0 +1,150 @@
+"""Layer norm, alone or of a residual sum, forward and backward in this library's kernels
+(``ossm_layer_norm_forward``, ``ossm_layer_norm_backward``).
+
+The reference's backbones and a language model's blocks add what a block computed to the
+residual stream and norm the sum for the next block; ``add_layer_norm`` is both in one
+pass, and its backward joins the two gradients that reach the sum.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor, nn
+
+from . import _lib
+from .gated import _ld, _matrix
+from .linear import aliases
+
+__all__ = ["LayerNorm", "LayerNormFn", "add_layer_norm", "layer_norm"]
+
+
+def _separate(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
+    """The same as torch's separate steps."""
+    s = x if residual is None else x + residual
+    cast = [t if t is None or t.dtype == s.dtype else t.to(s.dtype) for t in (weight, bias)]
+    if cast[0] is weight and cast[1] is bias:
+        y = F.layer_norm(s, s.shape[-1:], weight, bias, eps)
+    else:  # float32 weights are not rounded
+        y = F.layer_norm(s.float(), s.shape[-1:], weight, bias, eps).to(s.dtype)
+    return y if residual is None else (y, s)
+
+
+def _forward(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float, save: bool):
+    T, D = x.shape
+    x, residual = _matrix(x), None if residual is None else _matrix(residual)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    y = torch.empty((T, D), dtype=x.dtype, device=x.device)
+    s = None if residual is None else torch.empty_like(y)
+    mean, rstd = (torch.empty(T, dtype=torch.float32, device=x.device) if save else None for _ in range(2))
+    if y.numel() > 0:
+        wt = weight if weight is not None else bias
+        _lib.run(_lib.load().ossm_layer_norm_forward, x, _lib.LM_DTYPES[x.dtype], _lib.LM_DTYPES[(x if wt is None else wt).dtype],
+                 x.data_ptr(), _ld(x), _lib.ptr(residual), 0 if residual is None else _ld(residual), _lib.ptr(weight),
+                 _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(s), _lib.ptr(mean), _lib.ptr(rstd), T, D)
+    return y, s, mean, rstd
+
+
+class LayerNormFn(torch.autograd.Function):
+    """``layer_norm`` and ``add_layer_norm`` on matrices; saves the sum and two numbers a row."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor],  # type: ignore[override]
+                eps: float):
+        y, s, mean, rstd = _forward(x, residual, weight, bias, eps, True)
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if s is None else s, weight, bias, mean, rstd)
+        return y if s is None else (y, s)
+
+    @staticmethod
+    def backward(ctx, gy: Optional[Tensor], gs: Optional[Tensor] = None):  # type: ignore[override]
+        s, weight, bias, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if torch.is_grad_enabled():
+            # create_graph: differentiable again, as separate steps on the sum
+            if gy is None:
+                return gs if need[0] else None, gs if need[1] else None, None, None, None
+            inputs = aliases(s, weight, bias)
+            wanted = [t for t, n in zip(inputs, (need[0] or need[1], *need[2:4])) if n]
+            got = iter(torch.autograd.grad(_separate(inputs[0], None, *inputs[1:], ctx.eps), wanted, gy, create_graph=True))
+            ds = next(got) if need[0] or need[1] else None
+            if ds is not None and gs is not None:
+                ds = ds + gs
+            return (ds if need[0] else None, ds if need[1] else None, *(next(got) if n else None for n in need[2:4]), None)
+        if gy is None:
+            gy = torch.zeros_like(s)
+        T, D = s.shape
+        s, gy = _matrix(s), _matrix(gy)
+        gs = None if gs is None else _matrix(gs)
+        weight = None if weight is None else weight.contiguous()
+        make = torch.empty if s.numel() > 0 else torch.zeros
+        ds = make((T, D), dtype=s.dtype, device=s.device) if need[0] or need[1] else None
+        wt = weight if weight is not None else bias
+        dw, db = (make((D,), dtype=wt.dtype, device=s.device) if n else None for n in need[2:4])
+        if s.numel() > 0:
+            _lib.run(_lib.load().ossm_layer_norm_backward, s, _lib.LM_DTYPES[s.dtype],
+                     _lib.LM_DTYPES[(s if wt is None else wt).dtype], gy.data_ptr(), _ld(gy), _lib.ptr(gs),
+                     0 if gs is None else _ld(gs), s.data_ptr(), _ld(s), _lib.ptr(weight), mean.data_ptr(), rstd.data_ptr(),
+                     _lib.ptr(ds), _lib.ptr(dw), _lib.ptr(db), T, D)
+        return ds if need[0] else None, ds if need[1] else None, dw, db, None
+
+
+def _apply(what: str, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
+    args = [x, residual, weight, bias]
+    if torch.is_autocast_enabled("cuda"):  # as F.layer_norm: in float32
+        args = [t if t is None or t.dtype not in (torch.bfloat16, torch.float16) else t.float() for t in args]
+        x, residual, weight, bias = args
+    index, dtype = x.get_device(), x.dtype
+    if dtype not in _lib.LM_DTYPES or index < 0 or x.dim() == 0:
+        raise RuntimeError(f"{what}: x must be a float32 or bfloat16 GPU tensor of at least one dimension, got {dtype} "
+                           f"{tuple(x.shape)} on {x.device}")
+    if residual is not None and (residual.dtype != dtype or residual.shape != x.shape or residual.get_device() != index):
+        raise RuntimeError(f"{what}: residual must be as x, {dtype} {tuple(x.shape)}, got {residual.dtype} "
+                           f"{tuple(residual.shape)} on {residual.device}")
+    D = x.size(-1)
+    types = {t.dtype for t in (weight, bias) if t is not None}
+    for t in (weight, bias):
+        if t is not None and (t.shape != (D,) or t.get_device() != index or len(types) > 1
+                              or t.dtype not in (dtype, torch.float32)):
+            raise RuntimeError(f"{what}: weight and bias must be of shape ({D},), both of x's dtype or both float32, on x's GPU, "
+                               f"got {[None if t is None else (t.dtype, tuple(t.shape), str(t.device)) for t in (weight, bias)]}")
+    if _lib.has_tangent(args):
+        raise RuntimeError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
+    two = [t if t is None or t.dim() == 2 else t.reshape(-1, D) if D > 0 else t.reshape(t.shape[:-1].numel(), 0)
+           for t in (x, residual)]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        out = LayerNormFn.apply(*two, weight, bias, float(eps))
+        y, s = (out, None) if residual is None else out
+    else:
+        y, s, _, _ = _forward(*two, weight, bias, float(eps), False)
+    return (y, s) if x.dim() == 2 else (y.view(x.shape), None if s is None else s.view(x.shape))
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """``F.layer_norm(x, x.shape[-1:], weight, bias, eps)`` for x [..., D], float32 or
+    bfloat16 on a GPU, any strides; weight and bias [D], both of x's dtype or both float32.
+    Sums and statistics are float32, the variance is about the mean; the result is rounded once.  Differentiable in
+    x, weight and bias (in reverse mode; a forward-mode tangent raises), twice as torch's
+    separate steps.  Under autocast it runs in float32, as ``F.layer_norm`` does."""
+    return _apply("layer_norm", x, None, weight, bias, eps)[0]
+
+
+def add_layer_norm(x: Tensor, residual: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+                   eps: float = 1e-5) -> Tuple[Tensor, Tensor]:
+    """``(layer_norm(s), s)`` with ``s = x + residual`` rounded to their dtype: the next
+    block's input and residual stream.  Both outputs are differentiable."""
+    return _apply("add_layer_norm", x, residual, weight, bias, eps)
+
+
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` over the last dimension in this library's kernels; with a residual
+    it returns the norm of the sum and the sum."""
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+        if len(self.normalized_shape) != 1 or x.shape[-1:] != torch.Size(self.normalized_shape):
+            raise RuntimeError(f"LayerNorm norms a last dimension of {tuple(self.normalized_shape)}, got {tuple(x.shape)}")
+        y, s = _apply("LayerNorm", x, residual, self.weight, self.bias, self.eps)
+        return y if residual is None else (y, s)

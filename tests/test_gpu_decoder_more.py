@@ -1,0 +1,132 @@
+"""GPU tests of the example model with the gated recurrence as its mixer, and of drawn
+answers: norm, recurrence, control and choice run together as a server runs them.
+
+Tolerance, derived before the first run: as in test_gpu_decoder, two orders of float32 sums
+of up to 256 terms, 1e-4 of the largest logit."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.gpu_util import announce, need_gpu, no_device_errors
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", params=["recurrent", ("mamba", "recurrent")], ids=["recurrent", "mixed"])
+def model(request):
+    need_gpu()
+    from ossm_amd.decoder import MambaDecoder
+
+    with torch.random.fork_rng():
+        torch.manual_seed(0)
+        return MambaDecoder(97, 64, 2, d_hidden=120, mixer=request.param).cuda()
+
+
+def close(a, b):
+    assert (a - b).abs().max() <= 1e-4 * b.abs().max()
+
+
+@torch.random.fork_rng()
+def test_prompts_and_tokens_match_the_whole_sequence(model):
+    tokens = torch.randint(0, 97, (3, 40)).cuda()
+    announce("recurrent decoder prompt and steps against forward")
+    with torch.no_grad():
+        whole = model(tokens)
+    states = model.states(8)
+    slots = torch.tensor([5, 0, 7]).cuda()
+    cuts = [30, 1, 37]
+    packed = torch.cat([tokens[i, :n] for i, n in enumerate(cuts)])
+    logits = model.prompt(packed, torch.tensor([0, 30, 31, 68]).cuda(), states, slots)
+    for i, n in enumerate(cuts):
+        close(logits[i], whole[i, n - 1])
+    for t in range(3):
+        at = torch.tensor([n + t for n in cuts]).cuda()
+        logits = model.step(tokens[torch.arange(3).cuda(), at], states, slots)
+        for i, n in enumerate(cuts):
+            close(logits[i], whole[i, n + t])
+    packed = torch.cat([tokens[0, 33:35], tokens[1, 4:10]])
+    logits = model.prompt(packed, torch.tensor([0, 2, 8, 8]).cuda(), states, slots, torch.ones(3, dtype=torch.bool).cuda())
+    close(logits[0], whole[0, 34])
+    close(logits[1], whole[1, 9])
+    no_device_errors()
+
+
+@torch.random.fork_rng()
+def test_training_step_reaches_every_parameter(model):
+    tokens = torch.randint(0, 97, (2, 50)).cuda()
+    announce("recurrent decoder training step")
+    loss = torch.nn.functional.cross_entropy(model(tokens)[:, :-1].flatten(0, 1), tokens[:, 1:].flatten())
+    grads = torch.autograd.grad(loss, list(model.parameters()))
+    assert all(torch.isfinite(g).all() and g.abs().max() > 0 for g in grads)
+
+
+@torch.random.fork_rng()
+def test_the_norms_are_the_separate_sums(model):
+    """The residual stream with its sums taken inside the norms is the plain stream's: logits
+    and gradients against the same modules put together step by step."""
+    tokens = torch.randint(0, 97, (2, 33)).cuda()
+    params = list(model.parameters())
+    weights = torch.randn(2, 33, 97).cuda()
+
+    def plain():
+        x = model.embedding(tokens)
+        for b in model.blocks:
+            norm = lambda m, v: torch.nn.functional.layer_norm(v, (64,), m.weight, m.bias)  # noqa: E731
+            x = x + b.mixer(norm(b.norm1, x))
+            x = x + b.feed_forward(norm(b.norm2, x))
+        return torch.nn.functional.linear(norm(model.norm, x), model.embedding.weight)
+
+    announce("recurrent decoder norms")
+    got, want = model(tokens), plain()
+    close(got, want)
+    for p, q in zip(torch.autograd.grad(got, params, weights), torch.autograd.grad(want, params, weights)):
+        assert (p - q).abs().max() <= 1e-3 * q.abs().max()
+
+
+@torch.random.fork_rng()
+def test_drawn_answers(model):
+    prompts = [torch.tensor([1, 2, 3]), torch.tensor([50]), torch.arange(20)]
+    allowed = torch.zeros(3, 97, dtype=torch.bool)
+    allowed[0, 10:20] = allowed[1, ::7] = True  # the third may answer nothing
+    gen = lambda s: torch.Generator(device="cuda").manual_seed(s)  # noqa: E731
+    announce("recurrent decoder drawn answers")
+    out = model.answer(prompts, 12, allowed=allowed, temperature=1.5, top_p=0.95, generator=gen(1))
+    for i in range(2):
+        assert allowed[i].cuda()[out[i]].all()
+    assert not out[2].any()
+    again = model.answer(prompts, 12, allowed=allowed, temperature=1.5, top_p=0.95, generator=gen(1))
+    assert torch.equal(out, again)
+    # one token left, or no temperature to speak of: the greedy answer
+    greedy = model.answer(prompts, 6)
+    assert torch.equal(model.answer(prompts, 6, temperature=1.0, top_k=1, generator=gen(2)), greedy)
+    assert torch.equal(model.answer(prompts, 6, temperature=0.0, generator=gen(2)), greedy)
+    assert len({tuple(model.answer(prompts, 6, temperature=5.0, generator=gen(s))[0].tolist()) for s in range(5)}) > 1
+    with pytest.raises(ValueError, match="need one"):
+        model.answer(prompts, 3, top_k=4)
+
+
+@torch.random.fork_rng()
+def test_bfloat16_weights(model):
+    """The same model cast to bfloat16 serves, and agrees to bfloat16's rounding."""
+    import copy
+
+    half = copy.deepcopy(model).bfloat16()
+    tokens = torch.randint(0, 97, (2, 20)).cuda()
+    announce("recurrent decoder in bfloat16")
+    offsets, slots = torch.tensor([0, 20, 40]).cuda(), torch.arange(2).cuda()
+    a = model.prompt(tokens.flatten(), offsets, model.states(2), slots)
+    states = half.states(2)
+    b = half.prompt(tokens.flatten(), offsets, states, slots)
+    assert b.dtype == torch.bfloat16
+    assert (a - b.float()).abs().max() <= 0.1 * a.abs().max()
+    assert half.step(tokens[:, 0], states, slots).shape == (2, 97)
+
+
+def test_refuses_unknown_mixers():
+    from ossm_amd.decoder import MambaDecoder
+
+    for mixer in ("attention", ("mamba",), ("mamba", "recurrent", "mamba")):
+        with pytest.raises(ValueError, match="mixer must be"):
+            MambaDecoder(10, 16, 2, mixer=mixer)
