@@ -156,8 +156,8 @@ int ossm_layer_norm_backward(int dtype, int weight_dtype, const void* grad_y, in
  * ossm_recurrence_saved(batch, length, dim) elements, written for the backward, or null.
  *
  * ossm_recurrence_backward: with grad_y E and grad_last f32 [batch, dim] (or null), the
- * gradients of x and the gates E with row stride ld_grads, of decay and start f32; a null
- * gradient is not computed.
+ * gradients of x and the gates E with row stride ld_grads (of the output gate exactly where
+ * it is given), of decay and start f32 (or null).
  *
  * ossm_recurrence_prompt, ossm_recurrence_step: packed prompts and single tokens with
  * states in a pool, state f32 [n_slots, dim]; slots, offsets, resume and padding as

@@ -91,8 +91,8 @@ def _forward(x, i, r, z, decay, start, scale: float, save: bool):
 
 
 def _backward(x, i, r, z, decay, gy, glast, saved, grads, scale: float, need_decay: bool, need_start: bool):
-    """Gradients of x, i, r, z into ``grads`` (views of one row stride, or Nones); returns
-    those of decay and start."""
+    """Gradients of x, i, r and (where there is one) z into ``grads``, tensors of one row
+    stride; returns those of decay and start."""
     B, L, D = x.shape
     keep, args = _pairs(x, i, r, z)
     (gy,), gargs = _pairs(gy)
@@ -101,7 +101,7 @@ def _backward(x, i, r, z, decay, gy, glast, saved, grads, scale: float, need_dec
         glast = glast.contiguous()
     gdecay = torch.empty(D, dtype=torch.float32, device=x.device) if need_decay else None
     gstart = torch.empty((B, D), dtype=torch.float32, device=x.device) if need_start else None
-    ld = next((g.stride(1) for g in grads if g is not None), D)
+    ld = grads[0].stride(1) if B * L > 1 else D
     _lib.run(_lib.load().ossm_recurrence_backward, x, _lib.LM_DTYPES[x.dtype], *gargs, _lib.ptr(glast), *args,
              decay.data_ptr(), scale, saved.data_ptr(), *(_lib.ptr(g) for g in grads), ld, _lib.ptr(gdecay), _lib.ptr(gstart),
              B, L, D)
@@ -109,7 +109,7 @@ def _backward(x, i, r, z, decay, gy, glast, saved, grads, scale: float, need_dec
 
 
 class GatedRecurrenceFn(torch.autograd.Function):
-    """``gated_recurrence``; saves the state before every 64th step."""
+    """``gated_recurrence``; saves the state before every 32nd step."""
 
     @staticmethod
     def forward(ctx, x, i, r, z, decay, start, scale):  # type: ignore[override]
@@ -133,9 +133,9 @@ class GatedRecurrenceFn(torch.autograd.Function):
             return (*(next(got) if n else None for n in need[:6]), None)
         if gy is None:
             gy = torch.zeros_like(x)
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if n else None for n in need[:4]]
+        grads = [None if t is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for t in (x, i, r, z)]
         gdecay, gstart = _backward(x, i, r, z, decay, gy, glast, saved, grads, ctx.scale, need[4], need[5])
-        return (*grads, gdecay, gstart, None)
+        return (*(g if n else None for g, n in zip(grads, need)), gdecay, gstart, None)
 
 
 class PackedRecurrenceFn(torch.autograd.Function):
@@ -160,10 +160,9 @@ class PackedRecurrenceFn(torch.autograd.Function):
             got = iter(torch.autograd.grad(y, wanted, gy, create_graph=True))
             return (*(next(got) if n else None for n in ctx.needs_input_grad[:2]), None)
         need_p, need_d = ctx.needs_input_grad[:2]
-        grad = torch.empty_like(packed) if need_p else None
-        parts = grad.chunk(4, -1) if need_p else (None,) * 4
-        gdecay, _ = _backward(*packed.chunk(4, -1), decay, gy, None, saved, parts, ctx.scale, need_d, False)
-        return grad, gdecay, None
+        grad = torch.empty_like(packed)
+        gdecay, _ = _backward(*packed.chunk(4, -1), decay, gy, None, saved, grad.chunk(4, -1), ctx.scale, need_d, False)
+        return grad if need_p else None, gdecay, None
 
 
 def _check(what: str, x: Tensor, i: Tensor, r: Tensor, z: Optional[Tensor], decay: Tensor, dims: int) -> None:

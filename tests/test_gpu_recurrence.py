@@ -249,9 +249,9 @@ def test_strides_and_other_streams(R, dtype):
     stream: all what dense tensors give."""
     B, L, D = 2, 150, 66
     args, gy, glast = inputs(B, L, D, dtype, True, True, seed=4)
-    want = run(R, args, gy, glast)
-    for off in (0, 1, 2, 3):
-        wide = torch.zeros(B, L, 4 * D + 9, dtype=dtype, device="cuda")
+    want, exact = run(R, args, gy, glast), reference(*args, 8.0, gy, glast)
+    for off, more in ((0, 8), (2, 8), (0, 9), (1, 9), (2, 9), (3, 8)):
+        wide = torch.zeros(B, L, 4 * D + more, dtype=dtype, device="cuda")
         views = [wide[..., off + k * D:off + (k + 1) * D].copy_(t) for k, t in enumerate(args[:4])]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -260,8 +260,9 @@ def test_strides_and_other_streams(R, dtype):
             got = run(R, [*views, *args[4:]], gy, glast)
         torch.cuda.synchronize()
         for n, t in got.items():
-            check(t, (f64(want[n]), 64 * U * np.abs(f64(want[n])) + 1e-6), n) if off % 2 else None
-            assert off % 2 or torch.equal(t, want[n]), n
+            check(t, exact[n], n)
+            # 16-bit rows off whole words take chunks of other lengths, and round otherwise
+            assert off % 2 or more % 2 or torch.equal(t, want[n]), n
     turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in args[:4]]
     got = run(R, [*turned, *args[4:]], gy.transpose(0, 1).contiguous().transpose(0, 1), glast)
     assert all(torch.equal(t, want[n]) for n, t in got.items())

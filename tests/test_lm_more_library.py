@@ -34,7 +34,8 @@ def test_recurrence_training_checks_before_any_hip_call(name):
     for size in ("batch", "length", "dim"):
         assert _call(name, **{size: -1})[0] == 1 and _call(name, **{size: 2**40})[0] == 3
         assert _call(name, **{size: 0}) == (0, "")
-    for p in ("x", "input_gate", "decay_gate", "decay", *(("y", "last") if name.endswith("forward") else ("grad_y", "saved"))):
+    for p in ("x", "input_gate", "decay_gate", "decay", *(("y", "last") if name.endswith("forward") else ("grad_y", "saved", "grad_x", "grad_input_gate", "grad_decay_gate",
+                                                                "grad_output_gate", "output_gate"))):
         assert _call(name, **{p: None}) == (1, f"{name[5:]}: null pointer")
     assert _call(name, length=2, dim=8) == (1, f"{name[5:]}: row stride below the row")
 
@@ -62,9 +63,9 @@ def test_sampler_checks_before_any_hip_call():
     assert _call(name, rows=0) == (0, "")
 
 
-def test_saved_states_are_one_every_64_steps():
+def test_saved_states_are_one_every_32_steps():
     lib = _lib.load()
-    assert [lib.ossm_recurrence_saved(2, n, 3) for n in (1, 64, 65, 128, 129)] == [6, 6, 12, 12, 18]
+    assert [lib.ossm_recurrence_saved(2, n, 3) for n in (1, 32, 33, 64, 65)] == [6, 6, 12, 12, 18]
     assert "ossm_recurrence_saved" in _declarations()
 
 
