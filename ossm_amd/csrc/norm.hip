@@ -56,7 +56,7 @@ struct Norm {
 
 // Threads of a workgroup whose rows take G lanes each.
 template <int G>
-constexpr int kBlockOf = G > kThreads ? G : kThreads;
+constexpr int kBlockOf = G > 64 ? G : kThreads;
 
 // Two sums over a row's lanes at once.
 template <int G>
@@ -83,10 +83,11 @@ __device__ __forceinline__ void load_weights(const WT* p, int D, int lane, float
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * G + lane) * W;
-    WT t[W];
-    if (p != nullptr && at < D) load_part(p + at, D - at, t);
+    Vec<WT, W> t;
+    t.zero();
+    if (p != nullptr && at < D) t.load(p + at, D - at);
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[j][k] = p != nullptr && at < D ? to_f(t[k]) : none;
+    for (int k = 0; k < W; ++k) w[j][k] = p != nullptr ? t.get(k) : none;
   }
 }
 
@@ -100,41 +101,57 @@ __device__ __forceinline__ Row row_of(float2 sums, float inv, float eps) {
   return {rest, 1.f / sqrtf(fmaf(-rest, rest, sums.x * inv) + eps)};
 }
 
-template <class E, class WT, int G, int NV>
+// RAGGED: D is no multiple of a vector, and rows share lines.
+template <class E, class WT, int G, int NV, bool RAGGED>
 __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g) {
   constexpr int W = kVec<E>, kRows = kBlockOf<G> / G;
   __shared__ float2 s_sum[G > 64 ? G / 64 : 1];
   const int lane = threadIdx.x % G;
+  const auto left_of = [&](int at) { return RAGGED ? g.D - at : W; };  // a vector's elements in the row
   const float inv = 1.f / static_cast<float>(g.D);
   float w[NV][W], b[NV][W];
   load_weights<WT, NV, W, G>(g.weight, g.D, lane, 1.f, w);
   load_weights<WT, NV, W, G>(g.bias, g.D, lane, 0.f, b);
-  for (long long r = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G; r < g.rows;
-       r += static_cast<long long>(gridDim.x) * kRows) {
-    float v[NV][W], total = 0.f;
-    {
-      E raw[NV][W], res[NV][W];
+  const long long step = static_cast<long long>(gridDim.x) * kRows;
+  long long r = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G;
+  Vec<E, W> raw[NV], res[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int at = (j * G + lane) * W;
-        if (at < g.D) load_part(g.x + r * g.ld_x + at, g.D - at, raw[j]);
-        if (at < g.D && g.residual != nullptr) load_part(g.residual + r * g.ld_res + at, g.D - at, res[j]);
+  for (int j = 0; j < NV; ++j) raw[j].zero(), res[j].zero();
+  const auto fetch = [&](long long row) {
+    if (row >= g.rows) return;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = (j * G + lane) * W;
+      if (at < g.D) raw[j].load(g.x + row * g.ld_x + at, left_of(at), RAGGED ? (g.rows - 1 - row) * g.ld_x + g.D - at : 0);
+      if (at < g.D && g.residual != nullptr)
+        res[j].load(g.residual + row * g.ld_res + at, left_of(at), RAGGED ? (g.rows - 1 - row) * g.ld_res + g.D - at : 0);
+    }
+  };
+  fetch(r);
+  for (; r < g.rows; r += step) {
+    float v[NV][W], total = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = (j * G + lane) * W;
+      if (RAGGED && at < g.D) {
+        raw[j].keep(g.D - at);
+        res[j].keep(g.D - at);
+      }
+      if (at < g.D && g.residual != nullptr) {
+        float t[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) t[k] = raw[j].get(k) + res[j].get(k);
+        raw[j].set(t);
+        raw[j].template store<!RAGGED>(g.sum + r * g.D + at, left_of(at));
       }
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int at = (j * G + lane) * W;
-        if (at < g.D && g.residual != nullptr) {
-#pragma unroll
-          for (int k = 0; k < W; ++k) raw[j][k] = from_f<E>(to_f(raw[j][k]) + to_f(res[j][k]));
-          store_part(g.sum + r * g.D + at, g.D - at, raw[j]);
-        }
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          v[j][k] = at < g.D ? to_f(raw[j][k]) : 0.f;
-          total += v[j][k];
-        }
+      for (int k = 0; k < W; ++k) {
+        v[j][k] = raw[j].get(k);
+        total += v[j][k];
       }
     }
+    fetch(r + step);  // the next row comes in while this one is summed
+    __builtin_amdgcn_sched_barrier(0);
     const float mean = row_sums<G>(total, 0.f, s_sum).x / static_cast<float>(g.D);
     float square = 0.f, rest = 0.f;
 #pragma unroll
@@ -153,20 +170,23 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * G + lane) * W;
-      E out[W];
+      float t[W];
+      Vec<E, W> out;
 #pragma unroll
-      for (int k = 0; k < W; ++k) out[k] = from_f<E>(fmaf((v[j][k] - row.rest) * row.rstd, w[j][k], b[j][k]));
-      if (at < g.D) store_part(g.y + r * g.D + at, g.D - at, out);
+      for (int k = 0; k < W; ++k) t[k] = fmaf((v[j][k] - row.rest) * row.rstd, w[j][k], b[j][k]);
+      out.set(t);
+      if (at < g.D) out.template store<!RAGGED>(g.y + r * g.D + at, left_of(at));
     }
   }
 }
 
-template <class E, class WT, int G, int NV>
+template <class E, class WT, int G, int NV, bool RAGGED>
 __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> g) {
   constexpr int W = kVec<E>, kRows = kBlockOf<G> / G;
   __shared__ float2 s_sum[G > 64 ? G / 64 : 1];
   __shared__ float s_part[G <= 64 ? 2 : 1][G <= 64 ? G * NV * W : 1];
   const int lane = threadIdx.x % G;
+  const auto left_of = [&](int at) { return RAGGED ? g.D - at : W; };  // a vector's elements in the row
   const float inv = 1.f / static_cast<float>(g.D);
   float w[NV][W], dw[NV][W], db[NV][W];
   load_weights<WT, NV, W, G>(g.weight, g.D, lane, 1.f, w);
@@ -174,26 +194,52 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> 
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int k = 0; k < W; ++k) dw[j][k] = db[j][k] = 0.f;
-  for (long long r = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G; r < g.rows;
-       r += static_cast<long long>(gridDim.x) * kRows) {
-    E s[NV][W], gy[NV][W], gs[NV][W];
-    const float mean = g.mean[r], rstd = g.rstd[r];
+  const long long step = static_cast<long long>(gridDim.x) * kRows;
+  long long r = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G;
+  Vec<E, W> s_in[NV], gy_in[NV], gs_in[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) s_in[j].zero(), gy_in[j].zero(), gs_in[j].zero();
+  float mean_in = 0.f, rstd_in = 0.f;
+  const auto fetch = [&](long long row) {
+    if (row >= g.rows) return;
+    mean_in = g.mean[row];
+    rstd_in = g.rstd[row];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * G + lane) * W;
       if (at < g.D) {
-        load_part(g.x + r * g.ld_x + at, g.D - at, s[j]);
-        load_part(g.gy + r * g.ld_gy + at, g.D - at, gy[j]);
-        if (g.gs != nullptr) load_part(g.gs + r * g.ld_gs + at, g.D - at, gs[j]);
+        const long long left = g.rows - 1 - row;
+        s_in[j].load(g.x + row * g.ld_x + at, left_of(at), RAGGED ? left * g.ld_x + g.D - at : 0);
+        gy_in[j].load(g.gy + row * g.ld_gy + at, left_of(at), RAGGED ? left * g.ld_gy + g.D - at : 0);
+        if (g.gs != nullptr) gs_in[j].load(g.gs + row * g.ld_gs + at, left_of(at), RAGGED ? left * g.ld_gs + g.D - at : 0);
       }
     }
-    float m1 = 0.f, m2 = 0.f;
+  };
+  constexpr bool kAhead = NV * W <= 8;  // where there are registers for a second row
+  if (kAhead) fetch(r);
+  for (; r < g.rows; r += step) {
+    if (!kAhead) fetch(r);
+    const float rstd = rstd_in, mean = mean_in;
+    Vec<E, W> s[NV], gy[NV], gs[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      s[j] = s_in[j], gy[j] = gy_in[j], gs[j] = gs_in[j];
+      const int at = (j * G + lane) * W;
+      if (RAGGED && at < g.D) {
+        s[j].keep(g.D - at);
+        gy[j].keep(g.D - at);
+      }
+    }
+    if (kAhead) {
+      fetch(r + step);  // the next row comes in while this one is summed
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float m1 = 0.f, m2 = 0.f;  // past the row's end gy is zero
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        if ((j * G + lane) * W + k >= g.D) continue;
-        const float n = (to_f(s[j][k]) - mean) * rstd, o = to_f(gy[j][k]), q = o * w[j][k];
+        const float n = (s[j].get(k) - mean) * rstd, o = gy[j].get(k), q = o * w[j][k];
         dw[j][k] = fmaf(o, n, dw[j][k]);
         db[j][k] += o;
         m1 += q;
@@ -202,19 +248,25 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> 
     const float2 m = row_sums<G>(m1, m2, s_sum);
     m1 = m.x * inv;
     m2 = m.y * inv;
+    // n and gy w are formed again from the packed row: kept, they would take four times its registers
+#pragma unroll
+    for (int j = 0; j < NV && kAhead; ++j)
+#pragma unroll
+      for (int i = 0; i < Vec<E, W>::kWords; ++i) asm volatile("" : "+v"(s[j].w[i]), "+v"(gy[j].w[i]));
     if (g.gx != nullptr) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int at = (j * G + lane) * W;
         if (at >= g.D) continue;
-        E out[W];
+        float t[W];
+        Vec<E, W> out;
 #pragma unroll
         for (int k = 0; k < W; ++k) {
-          const float n = (to_f(s[j][k]) - mean) * rstd;
-          const float d = rstd * (fmaf(-n, m2, to_f(gy[j][k]) * w[j][k] - m1));
-          out[k] = from_f<E>(g.gs != nullptr ? d + to_f(gs[j][k]) : d);
+          const float n = (s[j].get(k) - mean) * rstd;
+          t[k] = fmaf(rstd, fmaf(-n, m2, gy[j].get(k) * w[j][k] - m1), gs[j].get(k));  // no gs: zeros
         }
-        store_part(g.gx + r * g.D + at, g.D - at, out);
+        out.set(t);
+        out.template store<!RAGGED>(g.gx + r * g.D + at, left_of(at));
       }
     }
   }
@@ -253,104 +305,160 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> 
     for (int j = 0; j < NV; ++j) {
       const int at = (j * G + lane) * W;
       if (at >= g.D) continue;
-      store_part(part + at, g.D - at, dw[j]);
-      store_part(part + g.D + at, g.D - at, db[j]);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        if (at + k >= g.D) break;
+        part[at + k] = dw[j][k];
+        part[g.D + at + k] = db[j][k];
+      }
     }
   }
 }
 
-// Rows longer than a workgroup's registers hold: the same sums in three passes over the row.
+// Rows longer than a workgroup's registers hold: the same sums in passes over the row, from
+// the caches after the first.  f(first element, its elements, vectors of each tensor).
+template <class E, int N, class F>
+__device__ __forceinline__ void each_vector(const E* const (&rows)[N], int D, F f) {
+  constexpr int W = kVec<E>;
+  for (int at = static_cast<int>(threadIdx.x) * W; at < D; at += kMaxThreads * W) {
+    Vec<E, W> v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i].zero();
+      if (rows[i] != nullptr) v[i].load(rows[i] + at, D - at);
+    }
+    f(at, min(W, D - at), v);
+  }
+}
+
 template <class E, class WT>
 __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g) {
+  constexpr int W = kVec<E>;
   __shared__ float2 s_sum[kMaxThreads / 64];
   const float inv = 1.f / static_cast<float>(g.D);
   for (long long r = blockIdx.x; r < g.rows; r += gridDim.x) {
-    const E* in = g.x + r * g.ld_x;
-    if (g.residual != nullptr) {
-      for (int i = threadIdx.x; i < g.D; i += kMaxThreads)
-        g.sum[r * g.D + i] = from_f<E>(to_f(in[i]) + to_f(g.residual[r * g.ld_res + i]));
-      in = g.sum + r * g.D;  // a thread reads back its own elements
-    }
+    const E* in[1] = {g.x + r * g.ld_x};
     float total = 0.f;
-    for (int i = threadIdx.x; i < g.D; i += kMaxThreads) total += to_f(in[i]);
+    if (g.residual != nullptr) {
+      const E* const both[2] = {in[0], g.residual + r * g.ld_res};
+      each_vector(both, g.D, [&](int at, int n, Vec<E, W>(&v)[2]) {
+        float t[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) t[k] = v[0].get(k) + v[1].get(k);
+        v[0].set(t);
+#pragma unroll
+        for (int k = 0; k < W; ++k) total += v[0].get(k);
+        v[0].template store<false>(g.sum + r * g.D + at, n);
+      });
+      in[0] = g.sum + r * g.D;  // a thread reads back its own elements
+    } else {
+      each_vector(in, g.D, [&](int, int, Vec<E, W>(&v)[1]) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) total += v[0].get(k);
+      });
+    }
     const float mean = row_sums<kMaxThreads>(total, 0.f, s_sum).x / static_cast<float>(g.D);
     float square = 0.f, rest = 0.f;
-    for (int i = threadIdx.x; i < g.D; i += kMaxThreads) {
-      const float c = to_f(in[i]) - mean;
-      square = fmaf(c, c, square);
-      rest += c;
-    }
+    each_vector(in, g.D, [&](int, int n, Vec<E, W>(&v)[1]) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float c = k < n ? v[0].get(k) - mean : 0.f;
+        square = fmaf(c, c, square);
+        rest += c;
+      }
+    });
     const Row row = row_of(row_sums<kMaxThreads>(square, rest, s_sum), inv, g.eps);
     if (threadIdx.x == 0 && g.mean != nullptr) {
       g.mean[r] = mean + row.rest;
       g.rstd[r] = row.rstd;
     }
-    for (int i = threadIdx.x; i < g.D; i += kMaxThreads)
-      g.y[r * g.D + i] = from_f<E>(fmaf((to_f(in[i]) - mean - row.rest) * row.rstd, g.weight != nullptr ? to_f(g.weight[i]) : 1.f,
-                                        g.bias != nullptr ? to_f(g.bias[i]) : 0.f));
+    each_vector(in, g.D, [&](int at, int n, Vec<E, W>(&v)[1]) {
+      float w[1][W], b[1][W], t[W];
+      load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
+      load_weights<WT, 1, W, kMaxThreads>(g.bias, g.D, at / W, 0.f, b);
+#pragma unroll
+      for (int k = 0; k < W; ++k) t[k] = fmaf((v[0].get(k) - mean - row.rest) * row.rstd, w[0][k], b[0][k]);
+      v[0].set(t);
+      v[0].template store<false>(g.y + r * g.D + at, n);
+    });
   }
 }
 
 template <class E, class WT>
 __global__ __launch_bounds__(kMaxThreads) void long_backward_kernel(Norm<E, WT> g) {
+  constexpr int W = kVec<E>;
   __shared__ float2 s_sum[kMaxThreads / 64];
   const float inv = 1.f / static_cast<float>(g.D);
   for (long long r = blockIdx.x; r < g.rows; r += gridDim.x) {
-    const E* s = g.x + r * g.ld_x;
-    const E* gy = g.gy + r * g.ld_gy;
+    const E* const in[3] = {g.x + r * g.ld_x, g.gy + r * g.ld_gy, g.gs != nullptr ? g.gs + r * g.ld_gs : nullptr};
+    const E* const two[2] = {in[0], in[1]};
     const float mean = g.mean[r], rstd = g.rstd[r];
     float m1 = 0.f, m2 = 0.f;
-    for (int i = threadIdx.x; i < g.D; i += kMaxThreads) {
-      const float q = to_f(gy[i]) * (g.weight != nullptr ? to_f(g.weight[i]) : 1.f);
-      m1 += q;
-      m2 = fmaf(q, (to_f(s[i]) - mean) * rstd, m2);
-    }
+    each_vector(two, g.D, [&](int at, int, Vec<E, W>(&v)[2]) {
+      float w[1][W];
+      load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float q = v[1].get(k) * w[0][k];
+        m1 += q;
+        m2 = fmaf(q, (v[0].get(k) - mean) * rstd, m2);
+      }
+    });
     const float2 m = row_sums<kMaxThreads>(m1, m2, s_sum);
-    for (int i = threadIdx.x; i < g.D; i += kMaxThreads) {
-      const float q = to_f(gy[i]) * (g.weight != nullptr ? to_f(g.weight[i]) : 1.f);
-      const float d = rstd * fmaf(-(to_f(s[i]) - mean) * rstd, m.y * inv, q - m.x * inv);
-      g.gx[r * g.D + i] = from_f<E>(g.gs != nullptr ? d + to_f(g.gs[r * g.ld_gs + i]) : d);
-    }
+    m1 = m.x * inv;
+    m2 = m.y * inv;
+    each_vector(in, g.D, [&](int at, int n, Vec<E, W>(&v)[3]) {
+      float w[1][W], t[W];
+      load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        t[k] = fmaf(rstd, fmaf(-(v[0].get(k) - mean) * rstd, m2, v[1].get(k) * w[0][k] - m1), v[2].get(k));
+      v[0].set(t);
+      v[0].template store<false>(g.gx + r * g.D + at, n);
+    });
   }
 }
 
-// dw and db of such rows: a workgroup's rows, 64 columns a wave.
+// dw and db of such rows: every n_parts-th row for the vectors of a workgroup's threads.
 template <class E, class WT>
-__global__ __launch_bounds__(kThreads) void long_columns_kernel(Norm<E, WT> g, int n_parts) {
-  const int n_cols = (g.D + kThreads - 1) / kThreads;
-  const int part = static_cast<int>(blockIdx.x) / n_cols, i = static_cast<int>(blockIdx.x) % n_cols * kThreads + threadIdx.x;
-  if (i >= g.D) return;
-  float dw = 0.f, db = 0.f;
+__global__ __launch_bounds__(kThreads) void long_columns_kernel(Norm<E, WT> g, int n_parts, int n_cols) {
+  constexpr int W = kVec<E>;
+  const int part = static_cast<int>(blockIdx.x) / n_cols, at = (static_cast<int>(blockIdx.x) % n_cols * kThreads + threadIdx.x) * W;
+  if (at >= g.D) return;
+  float dw[W] = {}, db[W] = {};
   for (long long r = part; r < g.rows; r += n_parts) {
-    const float o = to_f(g.gy[r * g.ld_gy + i]);
-    dw = fmaf(o, (to_f(g.x[r * g.ld_x + i]) - g.mean[r]) * g.rstd[r], dw);
-    db += o;
+    Vec<E, W> s, gy;
+    s.load(g.x + r * g.ld_x + at, g.D - at);
+    gy.load(g.gy + r * g.ld_gy + at, g.D - at);
+    const float mean = g.mean[r], rstd = g.rstd[r];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      dw[k] = fmaf(gy.get(k), (s.get(k) - mean) * rstd, dw[k]);
+      db[k] += gy.get(k);
+    }
   }
   float* out = g.partial + static_cast<size_t>(part) * 2 * g.D;
-  out[i] = dw;
-  out[g.D + i] = db;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if (at + k >= g.D) break;
+    out[at + k] = dw[k];
+    out[g.D + at + k] = db[k];
+  }
 }
 
-// dw and db from n partial sums: a column takes 16 rows of lanes, each every sixteenth
-// partial sum, in 64 bits.
+// dw and db from n partial sums.
 template <class WT>
-__global__ __launch_bounds__(kMaxThreads) void norm_sum_kernel(const float* partial, int n, int D, WT* dw, WT* db) {
-  __shared__ double s_sum[kMaxThreads / 64][64];
-  const long long cols = 2ll * D, i = static_cast<long long>(blockIdx.x) * 64 + threadIdx.x % 64;
-  const int w = threadIdx.x / 64;
-  double t = 0;
-  if (i < cols)
-    for (int r = w; r < n; r += kMaxThreads / 64) t += partial[r * cols + i];
-  s_sum[w][threadIdx.x % 64] = t;
-  __syncthreads();
-  if (w != 0 || i >= cols) return;
-  for (int v = 1; v < kMaxThreads / 64; ++v) t += s_sum[v][threadIdx.x];
+__global__ __launch_bounds__(kSumThreads) void norm_sum_kernel(const float* partial, int n, int D, WT* dw, WT* db) {
+  const long long cols = 2ll * D, i = static_cast<long long>(blockIdx.x) * kSumColumns + threadIdx.x;
+  const double t = column_sum(partial, n, cols, cols);
+  if (threadIdx.x >= kSumColumns || i >= cols) return;
   WT* out = i < D ? dw : db;
   if (out != nullptr) out[i < D ? i : i - D] = from_f<WT>(static_cast<float>(t));
 }
 
-// Calls f(G, NV) with the least group that holds D elements, or returns false.
-template <class E, class F>
+// Calls f(G, NV) with the least group of lanes that holds D elements in up to MAXV vectors each
+// where there are lanes enough (or more of 1024 lanes), or returns false.
+template <class E, int MAXV, class F>
 bool with_group(int64_t D, F f) {
   constexpr int W = kVec<E>;
   using std::integral_constant;
@@ -360,14 +468,28 @@ bool with_group(int64_t D, F f) {
   OSSM_GROUP(16, 1);
   OSSM_GROUP(32, 1);
   OSSM_GROUP(64, 1);
-  OSSM_GROUP(64, 2);
-  OSSM_GROUP(64, 4);
-  OSSM_GROUP(256, 2);
-  OSSM_GROUP(256, 4);
-  OSSM_GROUP(1024, (sizeof(E) == 2 ? 2 : 4));
+  if constexpr (MAXV > 1) {
+    OSSM_GROUP(64, 2);
+    OSSM_GROUP(128, 2);
+    OSSM_GROUP(256, 2);
+    OSSM_GROUP(512, 2);
+  } else {
+    OSSM_GROUP(128, 1);
+    OSSM_GROUP(256, 1);
+    OSSM_GROUP(512, 1);
+    OSSM_GROUP(1024, 1);
+  }
+  if constexpr (sizeof(E) == 4) OSSM_GROUP(1024, 2);
+  if constexpr (MAXV > 1) OSSM_GROUP(1024, 16 / W);
 #undef OSSM_GROUP
   return false;
 }
+
+// The forward takes two vectors a lane, the backward, whose sums take twice the registers, one:
+// forward and backward of [32768, 2048] in bf16 with a residual at one vector 98 and 115 us, at
+// two 91 and 131, at four 93 and 138.
+constexpr int kForwardVecs = 2, kBackwardVecs = 1;
+constexpr int kForwardWaves = 32, kBackwardWaves = 16;  // a CU
 
 // Workgroups that walk the rows: as many as the card holds at once.
 int64_t walkers(int64_t rows, int rows_each, int threads, int cus, int waves) {
@@ -376,14 +498,21 @@ int64_t walkers(int64_t rows, int rows_each, int threads, int cus, int waves) {
   return need < most ? need : most;
 }
 
-constexpr int kForwardWaves = 32, kBackwardWaves = 12;  // a CU
+// In the backward each leaves two rows of partial sums too: at least four rows each, where
+// that still leaves one for every CU.
+int64_t summing_walkers(int64_t rows, int rows_each, int threads, int cus) {
+  const int64_t need = (rows + rows_each - 1) / rows_each, few = need < cus ? need : cus;
+  const int64_t most = walkers(rows, rows_each, threads, cus, kBackwardWaves);
+  const int64_t want = need / 4 > few ? need / 4 : few;
+  return want < most ? want : most;
+}
 
 template <class E, class WT>
 int forward(Norm<E, WT> g, int cus, hipStream_t st) {
-  const bool held = with_group<E>(g.D, [&](auto G, auto NV) {
+  const bool held = with_group<E, kForwardVecs>(g.D, [&](auto G, auto NV) {
     constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value, kB = kBlockOf<kG>;
-    hipLaunchKernelGGL((norm_forward_kernel<E, WT, kG, kNV>),
-                       dim3(static_cast<unsigned>(walkers(g.rows, kB / kG, kB, cus, kForwardWaves))), dim3(kB), 0, st, g);
+    const auto kern = g.D % kVec<E> != 0 ? norm_forward_kernel<E, WT, kG, kNV, true> : norm_forward_kernel<E, WT, kG, kNV, false>;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(walkers(g.rows, kB / kG, kB, cus, kForwardWaves))), dim3(kB), 0, st, g);
   });
   if (!held)
     hipLaunchKernelGGL((long_forward_kernel<E, WT>),
@@ -396,21 +525,22 @@ template <class E, class WT>
 int backward(Norm<E, WT> g, WT* dw, WT* db, StreamCall& call, int cus) {
   hipStream_t st = call.stream();
   int64_t parts = 0;
-  const bool held = with_group<E>(g.D, [&](auto G, auto) {
+  const bool held = with_group<E, kBackwardVecs>(g.D, [&](auto G, auto) {
     constexpr int kG = decltype(G)::value, kB = kBlockOf<kG>;
-    parts = walkers(g.rows, kB / kG, kB, cus, kBackwardWaves);
+    parts = summing_walkers(g.rows, kB / kG, kB, cus > 0 ? cus : 256);
   });
-  const int n_cols = (g.D + kThreads - 1) / kThreads;
-  if (!held) parts = walkers(g.rows, 64, kThreads, cus, 16 / (n_cols < 16 ? n_cols : 16));
+  const int n_cols = (g.D + kThreads * kVec<E> - 1) / (kThreads * kVec<E>);
+  if (!held) parts = walkers(g.rows, 16, kThreads, cus, 16 / (n_cols < 16 ? n_cols : 16));
   const bool sums = dw != nullptr || db != nullptr;
   if (sums) {
     void* p = nullptr;
     if (int rc = acquire_workspace(call, static_cast<size_t>(parts) * 2 * g.D * sizeof(float), &p)) return rc;
     g.partial = static_cast<float*>(p);
   }
-  with_group<E>(g.D, [&](auto G, auto NV) {
+  with_group<E, kBackwardVecs>(g.D, [&](auto G, auto NV) {
     constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value, kB = kBlockOf<kG>;
-    hipLaunchKernelGGL((norm_backward_kernel<E, WT, kG, kNV>), dim3(static_cast<unsigned>(parts)), dim3(kB), 0, st, g);
+    const auto kern = g.D % kVec<E> != 0 ? norm_backward_kernel<E, WT, kG, kNV, true> : norm_backward_kernel<E, WT, kG, kNV, false>;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(parts)), dim3(kB), 0, st, g);
   });
   if (!held) {
     if (g.gx != nullptr)
@@ -420,12 +550,13 @@ int backward(Norm<E, WT> g, WT* dw, WT* db, StreamCall& call, int cus) {
     if (sums) {
       if (int rc = check_grid("layer_norm_backward", parts * n_cols, kThreads)) return rc;
       hipLaunchKernelGGL((long_columns_kernel<E, WT>), dim3(static_cast<unsigned>(parts * n_cols)), dim3(kThreads), 0, st, g,
-                         static_cast<int>(parts));
+                         static_cast<int>(parts), n_cols);
     }
   }
   if (int rc = launch_check("norm_backward_kernel")) return rc;
   if (!sums) return OSSM_OK;
-  hipLaunchKernelGGL(norm_sum_kernel<WT>, dim3(static_cast<unsigned>((2ll * g.D + 63) / 64)), dim3(kMaxThreads), 0, st,
+  hipLaunchKernelGGL(norm_sum_kernel<WT>, dim3(static_cast<unsigned>((2ll * g.D + kSumColumns - 1) / kSumColumns)),
+                     dim3(kSumThreads), 0, st,
                      g.partial, static_cast<int>(parts), g.D, dw, db);
   return launch_check("norm_sum_kernel");
 }
@@ -483,6 +614,7 @@ int ossm_layer_norm_backward(int dtype, int weight_dtype, const void* grad_y, in
   const char* what = "layer_norm_backward";
   if (int rc = check_types(what, dtype, weight_dtype, rows, dim)) return rc;
   if (rows == 0 || dim == 0) return OSSM_OK;
+  if (int rc = check_grid(what, (2 * dim + kSumColumns - 1) / kSumColumns, kSumThreads)) return rc;
   if (!grad_y || !s || !mean || !rstd) return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": null pointer");
   if (rows > 1 && (ld_s < dim || ld_grad_y < dim || (grad_sum && ld_grad_sum < dim)))
     return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": row stride below the row");

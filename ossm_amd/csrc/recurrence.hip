@@ -118,16 +118,10 @@ __device__ __forceinline__ float decay_rate(float decay, float scale) {
   return kLog2e * scale * (greatest(decay, 0.f) + 2.f * z * s);
 }
 
-__global__ void decay_grad_kernel(const float* partial, int n, int D, const float* decay, float* out) {
-  __shared__ double s_sum[16][64];
-  const int i = static_cast<int>(blockIdx.x) * 64 + threadIdx.x % 64, w = threadIdx.x / 64;
-  double t = 0;
-  if (i < D)
-    for (int r = w; r < n; r += 16) t += partial[static_cast<size_t>(r) * D + i];
-  s_sum[w][threadIdx.x % 64] = t;
-  __syncthreads();
-  if (w != 0 || i >= D) return;
-  for (int v = 1; v < 16; ++v) t += s_sum[v][threadIdx.x];
+__global__ __launch_bounds__(kSumThreads) void decay_grad_kernel(const float* partial, int n, int D, const float* decay, float* out) {
+  const double t = column_sum(partial, n, D, D);
+  const int i = static_cast<int>(blockIdx.x) * kSumColumns + threadIdx.x;
+  if (threadIdx.x >= kSumColumns || i >= D) return;
   const double x = decay[i];
   // sigmoid / softplus goes to one below; past -40 the quotient's own terms vanish
   const double ratio = x < -40 ? 1. : 1. / ((1. + exp(-x)) * (fmax(x, 0.) + log1p(exp(-fabs(x)))));
@@ -770,8 +764,8 @@ int backward_tile(Backward<E> g, float* gdecay, StreamCall& call) {
                      static_cast<unsigned long long*>(records), sync);
   if (int rc = launch_check("recurrence_backward_kernel")) return rc;
   if (gdecay == nullptr) return OSSM_OK;
-  hipLaunchKernelGGL(decay_grad_kernel, dim3(static_cast<unsigned>((g.D + 63) / 64)), dim3(1024), 0, call.stream(), g.partial,
-                     g.n_chunks * g.B, g.D, g.decay, gdecay);
+  hipLaunchKernelGGL(decay_grad_kernel, dim3(static_cast<unsigned>((g.D + kSumColumns - 1) / kSumColumns)),
+                     dim3(kSumThreads), 0, call.stream(), g.partial, g.n_chunks * g.B, g.D, g.decay, gdecay);
   return launch_check("decay_grad_kernel");
 }
 

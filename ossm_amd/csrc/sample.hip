@@ -157,11 +157,11 @@ struct Shared {
 template <class E, class F>
 __device__ __forceinline__ void each_key(const E* row, int V, F f) {
   for (int at = static_cast<int>(threadIdx.x) * kEach; at < V; at += kThreads * kEach) {
-    E v[kEach];
-    load_part(row + at, V - at, v);
+    Vec<E, kEach> v;
+    v.load(row + at, V - at);
 #pragma unroll
     for (int k = 0; k < kEach; ++k)
-      if (at + k < V) f(at + k, key_of(to_f(v[k])));
+      if (at + k < V) f(at + k, key_of(v.get(k)));
   }
 }
 
@@ -303,11 +303,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     for (int st = wave; st < n_stretches; st += kWavesOf) {
       const int at = st * kStretch + lane * kEach;
       uint32_t n = 0;
-      E v[kEach];
-      if (at < g.V) load_part(row + at, g.V - at, v);
+      Vec<E, kEach> v;
+      v.zero();
+      if (at < g.V) v.load(row + at, g.V - at);
 #pragma unroll
       for (int q = 0; q < kEach; ++q)
-        if (at + q < g.V) n += key_of(to_f(v[q])) == kept.key;
+        if (at + q < g.V) n += key_of(v.get(q)) == kept.key;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
       if (lane == 0) s.ties[st] = n;
@@ -326,12 +327,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   // a stretch's weights, one a lane's entry; their sums over the lane in w[kEach]
   const auto weigh = [&](int st, u64 (&w)[kEach]) {
     const int at = st * kStretch + lane * kEach;
-    E v[kEach];
-    if (at < g.V) load_part(row + at, g.V - at, v);
+    Vec<E, kEach> v;
+    v.zero();
+    if (at < g.V) v.load(row + at, g.V - at);
     uint32_t key[kEach], n = 0;
 #pragma unroll
     for (int q = 0; q < kEach; ++q) {
-      key[q] = at + q < g.V ? key_of(to_f(v[q])) : kLowest;
+      key[q] = at + q < g.V ? key_of(v.get(q)) : kLowest;
       n += key[q] == kept.key;
     }
     uint32_t before = 0;
