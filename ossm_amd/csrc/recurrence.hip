@@ -340,7 +340,9 @@ __device__ __forceinline__ Lane<E, V> lane_load(const E* row, unsigned ch) {
 }
 template <class E, int V>
 __device__ __forceinline__ void lane_store(E* row, unsigned ch, const Lane<E, V>& v) {
-  *reinterpret_cast<Lane<E, V>*>(row + ch) = v;
+  // past the caches: written once, read by later kernels only
+  if constexpr (V * sizeof(E) == 4) __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, v), reinterpret_cast<uint32_t*>(row + ch));
+  else __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, v), reinterpret_cast<uint16_t*>(row + ch));
 }
 
 // h of a prompt before its first token
