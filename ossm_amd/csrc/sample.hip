@@ -11,18 +11,22 @@
 // answer does not depend on how the row is cut, and a result next to a border
 // is the exact one but for the weights' own rounding.  In float32 the sums' error of some 1e-7 times the
 // 1e5 borders of a vocabulary would move one row in a hundred to a neighbouring token.  The
-// exponential is 2^y = 2^(j/64) 2^e e^r, a table and five terms in 64 bits (error 2^-50):
-// ten instructions, at the rate of float32's.
+// exponential is 2^y = 2^(j/256) 2^e 2^f, a table and four terms in 64 bits (error 2^-52): some
+// twenty operations, at the rate of float32's.
 //
-// A workgroup takes a row, in passes over it (from the caches after the first).  Logits are
-// compared by their bits as an unsigned number in their order (a key).  The first pass finds
-// the largest.  Where top-k or top-p is set, the next counts the row (or sums its weights) in
-// 2048 bins of equal width below the largest, which gives the bin in which the last kept token lies;
-// that bin's tokens are gathered in LDS, sorted, and give the last kept key and how many of
-// the tokens that share it are kept, the first by index.  Where all that top-k keeps
-// fits LDS the row is not looked at again.  Else a last pass sums the kept weights by stretches of
-// 512 entries, and the one that passes the target is looked at entry by entry.  A bin that does not fit (a row
-// of mostly equal logits) is cut by the keys' bits instead, in up to three further rounds (select).
+// A workgroup takes a row, in passes over it (from the caches after the first) that are bound by
+// the operations an entry takes.  The first finds the largest logit.
+//   top-k: of 1024 threads' own largest, the k-th is at least k logits' lower bound, and few more than
+//     k reach it: those are gathered in LDS, sorted, and hold all that is kept; the row is not
+//     looked at again.  For larger k (or where too many reach it) the row is counted in 8192 bins of equal
+//     width below the largest first, which gives the bin of the k-th.
+//   top-p: the counts by bins times the weights of the bins' middles give the border to a
+//     quarter of a percent.  A pass then sums the weights, exactly, above those bins and in all, and
+//     gathers the bins' tokens, which are sorted and give the last kept one.
+//   Then a pass sums the kept weights by stretches of 512 entries, and the one that passes the
+//     target is looked at entry by entry.
+// Where a bin's tokens do not fit (a row of mostly equal logits) the last kept one is found by
+// its bits, 11 at a time (select).
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -40,30 +44,80 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 1024, kWavesOf = kThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 8192, kPerBins = kBins / kThreads;
+constexpr int kDigits = 2048;                         // of a round of select
 constexpr int kList = 4096, kPer = kList / kThreads;  // gathered tokens, and a thread's
 constexpr int kEach = 8;                              // consecutive entries of a lane
 constexpr int kStretch = 64 * kEach;                  // entries of a wave at a time
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kStretches = kMaxVocab / kStretch;
 
-__constant__ double kPowers[64] = {  // 2^(j / 64)
-    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
-    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
-    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
-    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
-    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
-    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
-    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
-    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
-    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
-    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
-    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
-    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
-    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
-    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
-    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
-    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,};
+__constant__ double kPowers[256] = {  // 2^(j / 256)
+    1.0, 1.0027112750502025, 1.0054299011128027, 1.0081558981184175,
+    1.0108892860517005, 1.0136300849514894, 1.016378314910953, 1.019133996077738,
+    1.0218971486541166, 1.0246677928971357, 1.0274459491187637, 1.030231637686041,
+    1.0330248790212284, 1.0358256936019572, 1.0386341019613787, 1.041450124688316,
+    1.0442737824274138, 1.0471050958792898, 1.0499440858006872, 1.0527907730046264,
+    1.0556451783605572, 1.0585073227945128, 1.061377227289262, 1.0642549128844645,
+    1.0671404006768237, 1.0700337118202419, 1.0729348675259756, 1.075843889062791,
+    1.0787607977571199, 1.0816856149932152, 1.0846183622133092, 1.0875590609177697,
+    1.0905077326652577, 1.0934643990728858, 1.0964290818163769, 1.099401802630222,
+    1.102382583307841, 1.1053714457017412, 1.1083684117236787, 1.1113735033448175,
+    1.1143867425958924, 1.1174081515673693, 1.1204377524096067, 1.12347556733302,
+    1.1265216186082418, 1.129575928566288, 1.1326385195987192, 1.1357094141578055,
+    1.1387886347566916, 1.1418762039695616, 1.1449721444318042, 1.148076478840179,
+    1.1511892299529827, 1.154310420590216, 1.1574400736337511, 1.1605782120274988,
+    1.1637248587775775, 1.1668800369524817, 1.1700437696832502, 1.1732160801636373,
+    1.1763969916502812, 1.1795865274628758, 1.182784710984341, 1.1859915656609938,
+    1.189207115002721, 1.1924313825831512, 1.1956643920398273, 1.1989061670743806,
+    1.202156731452703, 1.2054161090051239, 1.2086843236265816, 1.2119613992768012,
+    1.215247359980469, 1.2185422298274085, 1.2218460329727576, 1.2251587936371455,
+    1.22848053610687, 1.2318112847340759, 1.2351510639369334, 1.2384998981998165,
+    1.241857812073484, 1.245224830175258, 1.2486009771892048, 1.2519862778663162,
+    1.255380757024691, 1.2587844395497165, 1.2621973503942507, 1.2656195145788063,
+    1.2690509571917332, 1.2724917033894028, 1.275941778396392, 1.2794012075056693,
+    1.2828700160787783, 1.2863482295460256, 1.2898358734066657, 1.2933329732290895,
+    1.2968395546510096, 1.3003556433796506, 1.3038812651919358, 1.3074164459346773,
+    1.3109612115247644, 1.3145155879493546, 1.318079601266064, 1.3216532776031575,
+    1.3252366431597413, 1.3288297242059544, 1.3324325470831615, 1.3360451382041458,
+    1.339667524053303, 1.3432997311868353, 1.3469417862329458, 1.3505937158920345,
+    1.3542555469368927, 1.3579273062129011, 1.3616090206382248, 1.365300717204012,
+    1.3690024229745905, 1.3727141650876684, 1.3764359707545302, 1.380167867260238,
+    1.383909881963832, 1.387662042298529, 1.3914243757719262, 1.3951969099662003,
+    1.3989796725383112, 1.4027726912202048, 1.4065759938190154, 1.4103896082172707,
+    1.4142135623730951, 1.4180478843204152, 1.4218926021691656, 1.4257477441054942,
+    1.42961333839197, 1.433489413367789, 1.4373759974489824, 1.4412731191286257,
+    1.4451808069770467, 1.449099089642035, 1.4530279958490526, 1.4569675544014438,
+    1.460917794180647, 1.4648787441464057, 1.4688504333369818, 1.4728328908693675,
+    1.4768261459394993, 1.4808302278224719, 1.4848451658727524, 1.488870989524397,
+    1.4929077282912648, 1.4969554117672355, 1.5010140696264256, 1.5050837316234065,
+    1.5091644275934228, 1.5132561874526098, 1.5173590411982147, 1.5214730189088146,
+    1.5255981507445384, 1.529734466947287, 1.533881997840956, 1.5380407738316568,
+    1.5422108254079407, 1.5463921831410214, 1.550584877685, 1.5547889397770887,
+    1.559004400237837, 1.5632312899713576, 1.567469639965553, 1.5717194812923414,
+    1.5759808451078865, 1.5802537626528246, 1.5845382652524937, 1.588834384317164,
+    1.593142151342267, 1.597461597908627, 1.6017927556826934, 1.606135656416771,
+    1.6104903319492543, 1.6148568142048607, 1.6192351351948637, 1.6236253270173289,
+    1.6280274218573478, 1.632441451987275, 1.6368674497669644, 1.6413054476440063,
+    1.645755478153965, 1.6502175739206177, 1.6546917676561943, 1.6591780921616162,
+    1.6636765803267364, 1.6681872651305825, 1.6727101796415966, 1.6772453570178785,
+    1.681792830507429, 1.6863526334483934, 1.6909247992693053, 1.6955093614893326,
+    1.7001063537185235, 1.7047158096580513, 1.709337763100463, 1.713972247929926,
+    1.718619298122478, 1.723278947746274, 1.7279512309618377, 1.732636182022311,
+    1.7373338352737062, 1.7420442251551564, 1.746767386199169, 1.7515033530318782,
+    1.7562521603732995, 1.761013843037584, 1.7657884359332727, 1.7705759740635547,
+    1.7753764925265212, 1.7801900265154245, 1.785016611318935, 1.789856282321401,
+    1.7947090750031072, 1.7995750249405351, 1.804454167806624, 1.809346539371032,
+    1.8142521755003989, 1.8191711121586085, 1.8241033854070534, 1.8290490314048973,
+    1.8340080864093424, 1.8389805867758937, 1.843966568958626, 1.8489660695104508,
+    1.8539791250833855, 1.8590057724288205, 1.864046048397789, 1.8690999899412386,
+    1.8741676341103, 1.8792490180565602, 1.8843441790323345, 1.8894531543909392,
+    1.8945759815869656, 1.8997126981765553, 1.9048633418176741, 1.9100279502703899,
+    1.9152065613971474, 1.9203992131630474, 1.925605943636125, 1.930826790987627,
+    1.9360617934922943, 1.9413109895286405, 1.9465744175792332, 1.9518521162309783,
+    1.9571441241754002, 1.9624504802089273, 1.9677712232331759, 1.9731063922552343,
+    1.978456026387951, 1.9838201648502194, 1.9891988469672663, 1.9945921121709402,
+};
 
 struct Sample {
   const float* uniform;
@@ -88,33 +142,32 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// A row's weights.  top: the largest logit's key.
+// A row's weights.
 struct Weights {
   const double* powers;  // in LDS
-  double top, rate;      // rate = log2(e) / T
+  double top, rate;      // the largest logit, log2(e) / T
   int scale;
   bool infinite;         // the largest is +inf: it shares the answer with its like alone
 
-  // w 2^scale
-  __device__ __forceinline__ double scaled(uint32_t key) const {
-    if (infinite) return key == 0xff800000u ? ldexp(1., scale) : 0.;
-    const double y = (static_cast<double>(value_of(key)) - top) * rate;
-    if (key == kLowest || !(y > -64.)) return 0.;  // below half a unit
-    const double t = y + 0x1.8p46;                 // y to the nearest 64th, its 64ths in the low bits
+  // w 2^scale; NaN and -inf weigh nothing
+  __device__ __forceinline__ double scaled(float v) const {
+    if (infinite) return v == __builtin_inff() ? ldexp(1., scale) : 0.;
+    const double y = fmax((static_cast<double>(v) - top) * rate, -64.);  // 2^-64: below half a unit
+    const double t = y + 0x1.8p44;                 // y to the nearest 256th, its 256ths in the low bits
     const int n = static_cast<int>(static_cast<uint32_t>(__double_as_longlong(t)));
-    const double r = (y - (t - 0x1.8p46)) * 0.69314718055994530942;
-    double s = 1. / 120.;
-    s = fma(s, r, 1. / 24.);
-    s = fma(s, r, 1. / 6.);
-    s = fma(s, r, 0.5);
-    s = fma(s, r, 1.);
-    const double p = powers[n & 63];
-    return ldexp(fma(p * r, s, p), (n >> 6) + scale);
+    const double f = y - (t - 0x1.8p44);           // (ln 2)^n / n!, f <= 2^-9: left out 2^-59
+    double s = 9.6181291076284771619e-3;
+    s = fma(s, f, 5.5504108664821579953e-2);
+    s = fma(s, f, 2.4022650695910071233e-1);
+    s = fma(s, f, 6.9314718055994530942e-1);
+    const double p = powers[n & 255];
+    return ldexp(fma(p * f, s, p), (n >> 8) + scale);
   }
   static __device__ __forceinline__ u64 whole(double w) {  // to nearest
     return static_cast<u64>(__double_as_longlong(w + 0x1p52)) & 0xfffffffffffffull;
   }
-  __device__ __forceinline__ u64 of(uint32_t key) const { return whole(scaled(key)); }
+  __device__ __forceinline__ u64 of(float v) const { return whole(scaled(v)); }
+  __device__ __forceinline__ u64 of(uint32_t key) const { return of(value_of(key)); }
 };
 
 // floor(f v) or, with up, the next whole number where it is none, for 0 <= f < 1.
@@ -148,32 +201,31 @@ struct Kept {
 };
 
 struct Shared {
-  double powers[64];
-  u64 wave_weight[kWavesOf];
+  double powers[256];
+  u64 wave_weight[kWavesOf], wave_more[kWavesOf];
   uint32_t wave_count[kWavesOf];
   u64 weight_before;
   uint32_t bin, count_before, listed, above, same;
   int at;
   union {
+    uint32_t bins[kBins];
     struct {
-      u64 weight[kBins];
-      uint32_t count[kBins];
+      u64 weight[kDigits];
+      uint32_t count[kDigits];
     };
-    struct {
-      u64 item[kList], item_weight[kList];
-    };
+    u64 item[kList];
     struct {
       u64 stretch[kStretches];
       uint32_t ties[kStretches];
-      uint32_t kept[kWavesOf][kStretch];
+      float kept[kWavesOf][kStretch];
     };
   };
 };
 
-// f(index, key) of every entry of the row, in any order; four vectors a thread are asked for
-// at once (one at a time a pass was bound by their latency).
+// f(first index, values) of every vector of the row, -inf behind its end; four vectors a
+// thread are asked for at once (one at a time a pass was bound by their latency).
 template <class E, class F>
-__device__ __forceinline__ void each_key(const E* row, int V, F f) {
+__device__ __forceinline__ void each_vector(const E* row, int V, F f) {
   constexpr int kAhead = 4, kStep = kThreads * kEach;
   for (int at0 = static_cast<int>(threadIdx.x) * kEach; at0 < V; at0 += kAhead * kStep) {
     Vec<E, kEach> v[kAhead];
@@ -187,9 +239,15 @@ __device__ __forceinline__ void each_key(const E* row, int V, F f) {
     for (int u = 0; u < kAhead; ++u) {
       const int at = at0 + u * kStep;
       if (at >= V) break;
+      float x[kEach];
 #pragma unroll
-      for (int k = 0; k < kEach; ++k)
-        if (at + k < V) f(at + k, key_of(v[u].get(k)));
+      for (int k = 0; k < kEach; ++k) x[k] = v[u].get(k);
+      if (at + kEach > V) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+          if (at + k >= V) x[k] = -__builtin_inff();
+      }
+      f(at, x);
     }
   }
 }
@@ -209,29 +267,29 @@ __device__ __forceinline__ void scan_threads(u64& w, uint32_t& n, Shared& s) {
   __syncthreads();
 }
 
-// The bin, from the first, at whose end `count` and `weight` before the first have grown to n or
-// w (kBins: none); what lies before it in s, the weight of all bins in *all.
-__device__ __forceinline__ uint32_t last_bin(uint32_t count, u64 weight, u64 n, u64 w, u64* all, Shared& s) {
-  constexpr int kPerBin = kBins / kThreads;
-  u64 sw = 0, mine_w[kPerBin];
-  uint32_t sn = 0, mine_n[kPerBin];
+// The digit, from the first, at whose end `count` and `weight` before the first have grown to n or
+// w (kDigits: none); what lies before it in s, the weight of all digits in *all.
+__device__ __forceinline__ uint32_t last_digit(uint32_t count, u64 weight, u64 n, u64 w, u64* all, Shared& s) {
+  constexpr int kPerDigit = kDigits / kThreads;
+  u64 sw = 0, mine_w[kPerDigit];
+  uint32_t sn = 0, mine_n[kPerDigit];
 #pragma unroll
-  for (int k = 0; k < kPerBin; ++k) {
-    mine_w[k] = s.weight[threadIdx.x * kPerBin + k];
-    mine_n[k] = s.count[threadIdx.x * kPerBin + k];
+  for (int k = 0; k < kPerDigit; ++k) {
+    mine_w[k] = s.weight[threadIdx.x * kPerDigit + k];
+    mine_n[k] = s.count[threadIdx.x * kPerDigit + k];
     sw += mine_w[k];
     sn += mine_n[k];
   }
-  if (threadIdx.x == 0) s.bin = kBins;
+  if (threadIdx.x == 0) s.bin = kDigits;
   scan_threads(sw, sn, s);
   u64 end_w = weight + sw;
   uint32_t end_n = count + sn;
 #pragma unroll
-  for (int k = kPerBin - 1; k >= 0; --k) {
+  for (int k = kPerDigit - 1; k >= 0; --k) {
     const u64 before_w = end_w - mine_w[k];
     const uint32_t before_n = end_n - mine_n[k];
     if ((end_n >= n || end_w >= w) && before_n < n && before_w < w) {  // one thread's
-      s.bin = threadIdx.x * kPerBin + k;
+      s.bin = threadIdx.x * kPerDigit + k;
       s.count_before = before_n;
       s.weight_before = before_w;
     }
@@ -254,20 +312,24 @@ __device__ Kept select(const E* row, int V, const Weights& wt, uint32_t top, uin
   uint32_t count = 0;
   for (;;) {
     int shift = 0;
-    while (((hi - lo) >> shift) >= kBins) ++shift;
-    for (int b = threadIdx.x; b < kBins; b += kThreads) s.weight[b] = 0, s.count[b] = 0;
+    while (((hi - lo) >> shift) >= kDigits) ++shift;
     __syncthreads();
-    each_key(row, V, [&](int, uint32_t key) {
-      if (key <= hi && key >= lo) {
+    for (int b = threadIdx.x; b < kDigits; b += kThreads) s.weight[b] = 0, s.count[b] = 0;
+    __syncthreads();
+    each_vector(row, V, [&](int, const float (&x)[kEach]) {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) {
+        const uint32_t key = key_of(x[q]);
+        if (key > hi || key < lo) continue;
         const uint32_t b = (hi - key) >> shift;
         atomicAdd(&s.count[b], 1u);
-        atomicAdd(&s.weight[b], wt.of(key));
+        atomicAdd(&s.weight[b], wt.of(x[q]));
       }
     });
     __syncthreads();
     u64 all_w;
-    const uint32_t bin = last_bin(count, weight, n, w, &all_w, s);
-    if (bin == kBins) {  // everything
+    const uint32_t bin = last_digit(count, weight, n, w, &all_w, s);
+    if (bin == kDigits) {  // everything
       __syncthreads();
       return {lowest, UINT_MAX, UINT_MAX, weight + all_w};
     }
@@ -291,49 +353,138 @@ __device__ Kept select(const E* row, int V, const Weights& wt, uint32_t top, uin
 // nothing or the row ends.
 struct Bins {
   float top, scale;
-  __device__ __forceinline__ uint32_t of(uint32_t key) const {  // kBins and more: weighs nothing
-    const float b = (top - value_of(key)) * scale;
+  __device__ __forceinline__ uint32_t of(float v) const {  // kBins: weighs nothing
+    const float b = (top - v) * scale;
     return b < static_cast<float>(kBins) ? static_cast<uint32_t>(b) : kBins;
   }
 };
 
-// s.item[0 .. n - 1] in falling order, n up to kList.
+__device__ __forceinline__ void clear_bins(Shared& s) {
+  __syncthreads();
+  for (int b = threadIdx.x * 4; b < kBins; b += kThreads * 4) *reinterpret_cast<uint4*>(s.bins + b) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+
+// The bin in which the n-th entry lies (kBins: there are fewer), s.count_before what lies before it.
+__device__ __forceinline__ uint32_t bin_of_count(uint32_t n, Shared& s) {
+  uint32_t mine[kPerBins], sum = 0;
+  u64 none = 0;
+#pragma unroll
+  for (int k = 0; k < kPerBins; ++k) {
+    mine[k] = s.bins[threadIdx.x * kPerBins + k];
+    sum += mine[k];
+  }
+  if (threadIdx.x == 0) s.bin = kBins;
+  scan_threads(none, sum, s);
+#pragma unroll
+  for (int k = kPerBins - 1; k >= 0; --k) {
+    const uint32_t before = sum - mine[k];
+    if (sum >= n && before < n) {
+      s.bin = threadIdx.x * kPerBins + k;
+      s.count_before = before;
+    }
+    sum = before;
+  }
+  __syncthreads();
+  return s.bin;
+}
+
+// The bins between which the p-th part of the weight is reached, as far as the bins' counts and
+// the weights of their middles tell.
+__device__ __forceinline__ void bins_of_part(const Weights& wt, const Bins& bins, float p, uint32_t& first, uint32_t& last, Shared& s) {
+  constexpr float kUnit = 16777216.f;  // 2^24
+  // a middle's weight may be off by half a bin, 0.2 percent; most bins' errors cancel
+  constexpr float kMargin = 0.0025f;
+  u64 mine[kPerBins], sum = 0;
+  uint32_t none = 0;
+  const float step = bins.scale > 0.f ? static_cast<float>(wt.rate) / bins.scale : 0.f;
+#pragma unroll
+  for (int k = 0; k < kPerBins; ++k) {
+    const uint32_t b = threadIdx.x * kPerBins + k;
+    mine[k] = static_cast<u64>(static_cast<float>(s.bins[b]) * kUnit * __builtin_amdgcn_exp2f(-(static_cast<float>(b) + 0.5f) * step));
+    sum += mine[k];
+  }
+  if (threadIdx.x == 0) s.count_before = kBins - 1, s.bin = kBins - 1;
+  scan_threads(sum, none, s);
+  u64 all = 0;
+  for (int v = 0; v < kWavesOf; ++v) all += s.wave_weight[v];
+  const float part = p * static_cast<float>(all);
+  const u64 least = static_cast<u64>(fmaxf(part - kMargin * static_cast<float>(all), 0.f)) + 1;
+  const u64 most = static_cast<u64>(part + kMargin * static_cast<float>(all)) + 1;
+#pragma unroll
+  for (int k = kPerBins - 1; k >= 0; --k) {
+    const u64 before = sum - mine[k];
+    if (sum >= least && before < least) s.count_before = threadIdx.x * kPerBins + k;
+    if (sum >= most && before < most) s.bin = threadIdx.x * kPerBins + k;
+    sum = before;
+  }
+  __syncthreads();
+  first = s.count_before;
+  last = s.bin;
+}
+
+// The least key, of those from `lo` to `hi`, that is `in` with all above it (hi is): 64 are
+// tried at once, by every wave alike.
+template <class F>
+__device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F in) {
+  const uint32_t lane = threadIdx.x & 63;
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 63) / 64, k = hi - lo > lane * step ? lo + lane * step : hi;
+    const u64 reach = __ballot(in(value_of(k)));
+    if (reach == 0) {
+      lo = min(hi, lo + 63 * step + 1);
+      continue;
+    }
+    const int first = __builtin_ctzll(reach);
+    hi = min(hi, lo + first * step);
+    if (first > 0) lo += (first - 1) * step + 1;
+  }
+  return hi;
+}
+
+// s.item[0 .. n - 1] in falling order, n up to kList.  A wave's pairs lie in 128 neighbouring items
+// while they are up to 64 apart, and need no other wave.
 __device__ void sort_items(uint32_t n, Shared& s) {
   uint32_t size = 64;
   while (size < n) size *= 2;
   for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) s.item[i] = 0;
   __syncthreads();
-  const bool alone = size <= 128;  // one wave's pairs
-  if (!alone || threadIdx.x < 64) {
-    for (uint32_t k = 2; k <= size; k *= 2) {
-      for (uint32_t j = k / 2; j > 0; j /= 2) {
-        for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
-          const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
-          const u64 x = s.item[a], y = s.item[b];
-          if (((a & k) == 0) != (x > y)) {
-            s.item[a] = y;
-            s.item[b] = x;
-          }
+  for (uint32_t k = 2; k <= size; k *= 2) {
+    for (uint32_t j = k / 2; j > 0; j /= 2) {
+      for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
+        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+        const u64 x = s.item[a], y = s.item[b];
+        if (((a & k) == 0) != (x > y)) {
+          s.item[a] = y;
+          s.item[b] = x;
         }
-        if (alone) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        else __syncthreads();
       }
+      if (j > 64 || (j == 1 && k > 64)) __syncthreads();
+      else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
   __syncthreads();
 }
 
-// Gathers the entries that `take` takes (key, index below it in order) as items; how many there
-// are, of which at most kList are there.
+// Gathers the entries from lo to below `end` (or all above where there is no end) as items; how
+// many there are, of which at most kList are there.  f sees every vector.
 template <class E, class F>
-__device__ uint32_t gather(const E* row, int V, F take, Shared& s) {
+__device__ uint32_t gather(const E* row, int V, float lo, float end, bool no_end, Shared& s, F f) {
   __syncthreads();
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  each_key(row, V, [&](int at, uint32_t key) {
-    if (take(key)) {
-      const uint32_t i = atomicAdd(&s.listed, 1u);
-      if (i < kList) s.item[i] = static_cast<u64>(key) << 32 | ~static_cast<uint32_t>(at);
+  each_vector(row, V, [&](int at, const float (&x)[kEach]) {
+    f(x);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) bits |= (x[q] >= lo && (no_end || x[q] < end) ? 1u : 0u) << q;
+    if (bits == 0) return;
+    uint32_t i = atomicAdd(&s.listed, static_cast<uint32_t>(__popc(bits)));
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      if ((bits >> q & 1) == 0) continue;
+      if (i < kList) s.item[i] = static_cast<u64>(key_of(x[q])) << 32 | ~static_cast<uint32_t>(at + q);
+      ++i;
     }
   });
   __syncthreads();
@@ -393,25 +544,6 @@ __device__ __forceinline__ Kept kept_to(uint32_t at, uint32_t n, Shared& s) {
   return {key, at + 1 - s.above, s.same, 0};
 }
 
-// The least key whose weight is at least `floor` (of keys from `lowest` to `top`, whose is): 64
-// are tried at once.
-__device__ __forceinline__ uint32_t key_of_floor(const Weights& wt, uint32_t lowest, uint32_t top, double floor) {
-  uint32_t lo = lowest, hi = top;  // hi's weight reaches it
-  const uint32_t lane = threadIdx.x & 63;
-  while (lo < hi) {
-    const uint32_t step = (hi - lo + 63) / 64, k = hi - lo > lane * step ? lo + lane * step : hi;
-    const u64 reach = __ballot(wt.scaled(k) >= floor);
-    if (reach == 0) {
-      lo = min(hi, lo + 63 * step + 1);
-      continue;
-    }
-    const int first = __builtin_ctzll(reach);
-    hi = min(hi, lo + first * step);
-    if (first > 0) lo += (first - 1) * step + 1;
-  }
-  return hi;
-}
-
 template <class E>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sample g) {
   __shared__ Shared s;
@@ -422,35 +554,51 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   const int k_given = g.top_k != nullptr ? g.top_k[r] : g.top_k_all;
   const float p = g.top_p != nullptr ? g.top_p[r] : g.top_p_all, m = g.min_p != nullptr ? g.min_p[r] : g.min_p_all;
   const float u = g.uniform[r];
-  if (tid < 64) s.powers[tid] = kPowers[tid];  // read after the next barrier
+  if (tid < 256) s.powers[tid] = kPowers[tid];  // read after the next barrier
+  const bool by_k = k_given > 0 && k_given < g.V, by_p = p < 1.f;
 
-  // the largest logit, the first that has it, and the least but -inf
-  u64 best = 0;
-  uint32_t low = 0xffffffffu;
-  each_key(row, g.V, [&](int at, uint32_t key) {
-    const u64 b = static_cast<u64>(key) << 32 | ~static_cast<uint32_t>(at);
-    best = b > best ? b : best;
-    low = key > kLowest ? min(low, key) : low;
+  // the largest logit (of the thread's own in mine) and the least but -inf; NaN is dropped
+  float mine = -__builtin_inff(), low = __builtin_inff();
+  each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      mine = fmaxf(mine, x[q]);
+      low = fminf(low, x[q] > -__builtin_inff() ? x[q] : __builtin_inff());
+    }
   });
+  float max = mine;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const u64 b = __shfl_xor(best, o);
-    best = b > best ? b : best;
-    low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), o)));
+    max = fmaxf(max, __shfl_xor(max, o));
+    low = fminf(low, __shfl_xor(low, o));
   }
-  if (lane == 0) s.wave_weight[wave] = best, s.wave_count[wave] = low;
+  if (lane == 0) s.kept[wave][0] = max, s.kept[wave][1] = low;
   __syncthreads();
   for (int v = 0; v < kWavesOf; ++v) {
-    best = s.wave_weight[v] > best ? s.wave_weight[v] : best;
-    low = min(low, s.wave_count[v]);
+    max = fmaxf(max, s.kept[v][0]);
+    low = fminf(low, s.kept[v][1]);
   }
   __syncthreads();
-  const uint32_t top = static_cast<uint32_t>(best >> 32);
-  if (top == kLowest || !(T > 0.f)) {
-    if (tid == 0) g.tokens[r] = top == kLowest ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best));
+  max += 0.f;  // -0 is 0
+  if (max == -__builtin_inff()) {
+    if (tid == 0) g.tokens[r] = -1;
     return;
   }
-  const float max = value_of(top);
+  if (!(T > 0.f)) {  // the first that is the largest
+    if (tid == 0) s.at = INT_MAX;
+    __syncthreads();
+    int first = INT_MAX;
+    each_vector(row, g.V, [&](int at, const float (&x)[kEach]) {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        if (x[q] == max) first = min(first, at + q);
+    });
+    if (first < INT_MAX) atomicMin(&s.at, first);
+    __syncthreads();
+    if (tid == 0) g.tokens[r] = s.at;
+    return;
+  }
+  const uint32_t top = key_of(max);
   const Weights wt{s.powers, max, 1.4426950408889634074 / T, g.scale, max == __builtin_inff()};
   const double floor = m > 0.f ? ldexp(static_cast<double>(m < 1.f ? m : 1.f), g.scale) : 0.;
 
@@ -458,124 +606,149 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   const double least = static_cast<double>(max) - 45. * T;
   const uint32_t lowest = wt.infinite || !(least > -3.4028234e38) ? kLowest + 1 : key_of(static_cast<float>(least)) - 1;
   Kept kept{lowest, UINT_MAX, UINT_MAX, 0};
-  const bool by_k = k_given > 0 && k_given < g.V, by_p = p < 1.f;
-  const uint32_t k = static_cast<uint32_t>(k_given);
+  const uint32_t k = by_k ? static_cast<uint32_t>(k_given) : UINT_MAX;
   // weights are nothing from 47.5 ln 2 T on
-  const float range = fminf(max - value_of(low), 33.f * T) * 1.00001f;
+  const float range = fminf(max - low, 33.f * T) * 1.00001f;
   const bool even = !wt.infinite && range < 1e37f;  // else the bins' width is no number
   const Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
+  const auto bin_start = [&](uint32_t b) {  // the least value of bin b and those before
+    return value_of(least_key(lowest, top, [&](float v) { return bins.of(v) <= b; }));
+  };
 
-  if (by_k) {
-    bool done = false;
-    if (even) {
-      for (int b = tid; b < kBins; b += kThreads) s.weight[b] = 0, s.count[b] = 0;
+  // all that can be kept as items: the k largest and what few lie near the last, or a short row
+  uint32_t listed = UINT_MAX;
+  bool all_kept = false;  // what weighs anything is fewer than k
+  if ((by_k || by_p) && g.V <= kThreads) {
+    listed = gather(row, g.V, -3.402823466e38f, 0.f, true, s, [](const float (&)[kEach]) {});
+  } else if (by_k && even) {
+    if (k <= kThreads) {
+      clear_bins(s);
+      const uint32_t b = bins.of(mine);
+      if (b < kBins) atomicAdd(&s.bins[b], 1u);
       __syncthreads();
-      each_key(row, g.V, [&](int, uint32_t key) {
-        const uint32_t b = bins.of(key);
-        if (b < kBins) atomicAdd(&s.count[b], 1u);
+      const uint32_t bin = bin_of_count(k, s);
+      if (bin < kBins) listed = gather(row, g.V, bin_start(bin), 0.f, true, s, [](const float (&)[kEach]) {});
+    }
+    if (listed > kList) {
+      clear_bins(s);
+      each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const uint32_t b = bins.of(x[q]);
+          if (b < kBins) atomicAdd(&s.bins[b], 1u);
+        }
       });
       __syncthreads();
-      u64 all;
-      const uint32_t bin = last_bin(0, 0, k, ~0ull, &all, s);
-      done = bin == kBins;  // what weighs anything is fewer than k
-      if (!done) {
-        const uint32_t before = s.count_before, in_bin = s.count[bin];
-        if (before + in_bin <= kList) {  // everything that is kept fits: no further pass
-          const uint32_t n0 = gather(row, g.V, [&](uint32_t key) { return bins.of(key) <= bin; }, s);
-          sort_items(n0, s);
-          uint32_t n = min(k, n0);
-          u64 sum[kPer];
-          u64 total = run_items(wt, n, 0, sum, s);
-          if (by_p) {
-            const u64 part = part_of(p, total, true);
-            n = min(n, first_reaching(sum, n, part > 0 ? part : 1, s) + 1);
-          }
-          if (floor > 0.) {  // weights fall: the first that does not reach it
-            if (tid == 0) s.at = static_cast<int>(n);
-            __syncthreads();
-#pragma unroll
-            for (int q = kPer - 1; q >= 0; --q) {
-              const uint32_t i = tid * kPer + q;
-              if (i < n && wt.scaled(static_cast<uint32_t>(s.item[i] >> 32)) < floor) atomicMin(&s.at, static_cast<int>(i));
-            }
-            __syncthreads();
-            n = static_cast<uint32_t>(s.at) > 0 ? s.at : 1;
-          }
-          // the kept ones by their index
-          u64 mine[kPer];
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) {
-            const uint32_t i = tid * kPer + q;
-            mine[q] = i < n ? s.item[i] : 0;
-          }
-          __syncthreads();
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) {
-            const uint32_t i = tid * kPer + q;
-            if (i < n) s.item[i] = mine[q] << 32 | mine[q] >> 32;  // ~index above the key: falling order is rising index
-          }
-          sort_items(n, s);
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) {
-            const uint32_t i = tid * kPer + q;
-            mine[q] = i < n ? s.item[i] : 0;
-          }
-          __syncthreads();
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) {
-            const uint32_t i = tid * kPer + q;
-            if (i < n) s.item[i] = mine[q] << 32 | mine[q] >> 32;
-          }
-          __syncthreads();
-          total = run_items(wt, n, 0, sum, s);
-          const u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
-          const uint32_t at = first_reaching(sum, n, target + 1, s);
-          if (tid == 0) g.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.item[at]));
-          return;
-        }
-        if (in_bin <= kList) {
-          const uint32_t n0 = gather(row, g.V, [&](uint32_t key) { return bins.of(key) == bin; }, s);
+      const uint32_t bin = bin_of_count(k, s);
+      all_kept = bin == kBins;
+      if (!all_kept) {
+        const uint32_t before = s.count_before, in_bin = s.bins[bin];
+        if (before + in_bin <= kList) {
+          listed = gather(row, g.V, bin_start(bin), 0.f, true, s, [](const float (&)[kEach]) {});
+        } else if (in_bin <= kList) {
+          const uint32_t n0 = gather(row, g.V, bin_start(bin), bin > 0 ? bin_start(bin - 1) : 0.f, bin == 0, s,
+                                     [](const float (&)[kEach]) {});
           sort_items(n0, s);
           kept = kept_to(k - before - 1, n0, s);
+          all_kept = true;
+        }
+      }
+    }
+  }
+  if (listed <= kList) {
+    sort_items(listed, s);
+    uint32_t n = min(k, listed);
+    u64 sum[kPer];
+    u64 total = run_items(wt, n, 0, sum, s);
+    if (by_p) {
+      const u64 part = part_of(p, total, true);
+      n = min(n, first_reaching(sum, n, part > 0 ? part : 1, s) + 1);
+    }
+    if (floor > 0.) {  // weights fall: the first that does not reach it
+      __syncthreads();
+      if (tid == 0) s.at = static_cast<int>(n);
+      __syncthreads();
+#pragma unroll
+      for (int q = kPer - 1; q >= 0; --q) {
+        const uint32_t i = tid * kPer + q;
+        if (i < n && wt.scaled(value_of(static_cast<uint32_t>(s.item[i] >> 32))) < floor) atomicMin(&s.at, static_cast<int>(i));
+      }
+      __syncthreads();
+      n = s.at > 0 ? static_cast<uint32_t>(s.at) : 1u;
+    }
+    // the kept ones by their index: its complement above the key, so that falling order is rising index
+    const auto swap_halves = [&] {
+      __syncthreads();
+      for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = s.item[i] << 32 | s.item[i] >> 32;
+      __syncthreads();
+    };
+    swap_halves();
+    sort_items(n, s);
+    swap_halves();
+    total = run_items(wt, n, 0, sum, s);
+    const u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
+    const uint32_t at = first_reaching(sum, n, target + 1, s);
+    if (tid == 0) g.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.item[at]));
+    return;
+  }
+  if (by_k && !all_kept) kept = select(row, g.V, wt, top, lowest, k, ~0ull, s);
+
+  if (by_p) {
+    const bool some = kept.ties < kept.same;  // the last key's weight counts `ties` times
+    const float last = value_of(kept.key);
+    u64 part = 0;
+    bool done = false;
+    if (even) {
+      clear_bins(s);
+      each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const uint32_t b = bins.of(x[q]);
+          if (b < kBins && (x[q] > last || (x[q] == last && !some))) atomicAdd(&s.bins[b], 1u);
+        }
+      });
+      if (some && tid == 0) atomicAdd(&s.bins[min(bins.of(last), kBins - 1u)], kept.ties);
+      __syncthreads();
+      uint32_t b0, b1;
+      bins_of_part(wt, bins, p, b0, b1, s);
+      const float end = b0 > 0 ? bin_start(b0 - 1) : 0.f;
+      u64 above = 0, total = 0;
+      const uint32_t n0 = gather(row, g.V, bin_start(b1), end, b0 == 0, s, [&](const float (&x)[kEach]) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const u64 w = x[q] > last || (x[q] == last && !some) ? wt.of(x[q]) : 0;
+          total += w;
+          above += b0 > 0 && x[q] >= end ? w : 0;
+        }
+      });
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        total += __shfl_xor(total, o);
+        above += __shfl_xor(above, o);
+      }
+      if (lane == 0) s.wave_weight[wave] = total, s.wave_more[wave] = above;
+      __syncthreads();
+      total = above = 0;
+      for (int v = 0; v < kWavesOf; ++v) total += s.wave_weight[v], above += s.wave_more[v];
+      __syncthreads();
+      if (some) {  // its own bin or one behind: never above the gathered ones but where all are
+        const u64 w = wt.of(last) * kept.ties;
+        total += w;
+        above += b0 > 0 && last >= end ? w : 0;
+      }
+      part = part_of(p, total, true);
+      part = part > 0 ? part : 1;
+      if (n0 <= kList && above < part) {
+        sort_items(n0, s);
+        u64 sum[kPer];
+        run_items(wt, n0, above, sum, s);
+        const uint32_t at = first_reaching(sum, n0, part, s);
+        if (at < n0) {
+          kept = kept_to(at, n0, s);
           done = true;
         }
         __syncthreads();
       }
-    }
-    if (!done) kept = select(row, g.V, wt, top, lowest, k, ~0ull, s);
-  }
-  if (by_p) {
-    bool done = false;
-    u64 part = 0;
-    const bool some = kept.ties < kept.same;  // the last key's weight counts `ties` times
-    if (even) {
-      for (int b = tid; b < kBins; b += kThreads) s.weight[b] = 0, s.count[b] = 0;
-      __syncthreads();
-      each_key(row, g.V, [&](int, uint32_t key) {
-        if (key > kept.key || (key == kept.key && !some)) {
-          const uint32_t b = bins.of(key);
-          if (b < kBins) atomicAdd(&s.weight[b], wt.of(key));
-        }
-      });
-      if (some && tid == 0) atomicAdd(&s.weight[min(bins.of(kept.key), kBins - 1u)], wt.of(kept.key) * kept.ties);
-      __syncthreads();
-      u64 all;
-      last_bin(0, 0, ~0ull, ~0ull, &all, s);
-      __syncthreads();
-      part = part_of(p, all, true);
-      part = part > 0 ? part : 1;
-      const uint32_t bin = last_bin(0, 0, ~0ull, part, &all, s);
-      const u64 before = s.weight_before;
-      const uint32_t n0 = gather(row, g.V, [&](uint32_t key) { return bins.of(key) == bin; }, s);
-      if (n0 <= kList) {
-        sort_items(n0, s);
-        u64 sum[kPer];
-        run_items(wt, n0, before, sum, s);
-        const uint32_t at = first_reaching(sum, n0, part, s);
-        kept = kept_to(min(at, n0 - 1), n0, s);
-        done = true;
-      }
-      __syncthreads();
     } else {
       if (!by_k) kept = select(row, g.V, wt, top, lowest, UINT_MAX, ~0ull, s);
       part = part_of(p, kept.weight, true);
@@ -584,23 +757,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     if (!done) kept = select(row, g.V, wt, top, lowest, ~0ull, part, s);
   }
   if (floor > 0.) {
-    const uint32_t key = key_of_floor(wt, lowest, top, floor);
+    const uint32_t key = least_key(lowest, top, [&](float v) { return wt.scaled(v) >= floor; });
     if (key > kept.key) kept = Kept{key, UINT_MAX, UINT_MAX, 0};
   }
 
   // the kept weights of each stretch, of equal last ones the first
   const int n_stretches = (g.V + kStretch - 1) / kStretch;
   const bool some = kept.ties < kept.same;
+  const float last = value_of(kept.key);
+  const auto load = [&](int st, Vec<E, kEach>& v) {
+    const int at = st * kStretch + lane * kEach;
+    v.zero();
+    if (at < g.V) v.load(row + at, g.V - at);
+  };
+  __syncthreads();
   if (some) {
     for (int st = wave; st < n_stretches; st += kWavesOf) {
-      const int at = st * kStretch + lane * kEach;
-      uint32_t n = 0;
       Vec<E, kEach> v;
-      v.zero();
-      if (at < g.V) v.load(row + at, g.V - at);
+      load(st, v);
+      uint32_t n = 0;
 #pragma unroll
-      for (int q = 0; q < kEach; ++q)
-        if (at + q < g.V) n += key_of(v.get(q)) == kept.key;
+      for (int q = 0; q < kEach; ++q) n += st * kStretch + lane * kEach + q < g.V && v.get(q) == last;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
       if (lane == 0) s.ties[st] = n;
@@ -609,66 +786,63 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     if (wave == 0) {
       uint32_t base = 0;
       for (int s0 = 0; s0 < n_stretches; s0 += 64) {
-        const uint32_t mine = s0 + lane < n_stretches ? s.ties[s0 + lane] : 0;
-        uint32_t sum = mine;
+        const uint32_t mine_n = s0 + lane < n_stretches ? s.ties[s0 + lane] : 0;
+        uint32_t sum = mine_n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
           const uint32_t b = __shfl_up(sum, o);
           if (lane >= o) sum += b;
         }
-        if (s0 + lane < n_stretches) s.ties[s0 + lane] = base + sum - mine;
+        if (s0 + lane < n_stretches) s.ties[s0 + lane] = base + sum - mine_n;
         base += __shfl(sum, 63);
       }
     }
     __syncthreads();
   }
-  // the keys of a stretch's entries of the lane, those that are not kept as the lowest
-  const auto keys_of = [&](int st, const Vec<E, kEach>& v, uint32_t (&key)[kEach]) {
-    const int at = st * kStretch + lane * kEach;
-    uint32_t n = 0, before = 0;
+  // which of the lane's entries of a stretch are kept, as bits
+  const auto kept_of = [&](int st, const Vec<E, kEach>& v) {
+    const int left = g.V - (st * kStretch + lane * kEach);
+    uint32_t bits = 0, same = 0;
 #pragma unroll
     for (int q = 0; q < kEach; ++q) {
-      key[q] = at + q < g.V ? key_of(v.get(q)) : kLowest;
-      n += key[q] == kept.key;
+      bits |= (v.get(q) > last ? 1u : 0u) << q;
+      same |= (v.get(q) == last ? 1u : 0u) << q;
     }
+    const uint32_t in = left >= kEach ? 0xffu : left > 0 ? (1u << left) - 1 : 0u;
+    bits &= in;
+    same &= in;
     if (some) {
+      const uint32_t n = __popc(same);
       uint32_t sum = n;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const uint32_t b = __shfl_up(sum, o);
         if (lane >= o) sum += b;
       }
-      before = s.ties[st] + sum - n;
+      const uint32_t before = s.ties[st] + sum - n, room = before < kept.ties ? kept.ties - before : 0;
+      while (static_cast<uint32_t>(__popc(same)) > room) same &= ~(0x80000000u >> __clz(same));  // the first ones stay
     }
-#pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      const bool last = key[q] == kept.key;
-      if (key[q] < kept.key || (last && some && before >= kept.ties)) key[q] = kLowest;
-      before += last;
-    }
+    return bits | same;
   };
   for (int st0 = wave; st0 < n_stretches; st0 += 4 * kWavesOf) {
     Vec<E, kEach> v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = (st0 + i * kWavesOf) * kStretch + lane * kEach;
-      v[i].zero();
-      if (at < g.V) v[i].load(row + at, g.V - at);
-    }
+    for (int i = 0; i < 4; ++i) load(min(st0 + i * kWavesOf, n_stretches - 1), v[i]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int st = st0 + i * kWavesOf;
       if (st >= n_stretches) break;
-      uint32_t key[kEach], n = 0;
-      keys_of(st, v[i], key);
+      const uint32_t bits = kept_of(st, v[i]);
       u64 sum = 0;
+      uint32_t n = 0;
       // few kept ones are brought together first: a weight takes 25 operations, this six
 #pragma unroll
       for (int q = 0; q < kEach; ++q) {
-        const u64 take = __ballot(key[q] != kLowest);
-        if (key[q] != kLowest) s.kept[wave][n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(take >> 32),
-                                                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(take), 0u))] = key[q];
-        n += __popcll(take);
+        const bool take = bits >> q & 1;
+        const u64 takes = __ballot(take);
+        if (take) s.kept[wave][n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(takes >> 32),
+                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(takes), 0u))] = v[i].get(q);
+        n += __popcll(takes);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       for (uint32_t e = lane; e < n; e += 64) sum += wt.of(s.kept[wave][e]);
@@ -688,8 +862,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
   int found = n_stretches - 1;
   for (int s0 = 0; s0 < n_stretches; s0 += 64) {
-    const u64 mine = s0 + lane < n_stretches ? s.stretch[s0 + lane] : 0;
-    u64 sum = mine;
+    const u64 own = s0 + lane < n_stretches ? s.stretch[s0 + lane] : 0;
+    u64 sum = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const u64 a = __shfl_up(sum, o);
@@ -698,25 +872,22 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     const u64 past = __ballot(sum > target);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      target -= __shfl(sum - mine, at);
+      target -= __shfl(sum - own, at);
       found = s0 + at;
       break;
     }
     target -= __shfl(sum, 63);
   }
   Vec<E, kEach> v;
-  v.zero();
-  const int at = found * kStretch + lane * kEach;
-  if (at < g.V) v.load(row + at, g.V - at);
-  uint32_t key[kEach];
-  keys_of(found, v, key);
+  load(found, v);
+  const uint32_t bits = kept_of(found, v);
   u64 w[kEach], sum = 0;
 #pragma unroll
   for (int q = 0; q < kEach; ++q) {
-    w[q] = key[q] != kLowest ? wt.of(key[q]) : 0;
+    w[q] = bits >> q & 1 ? wt.of(v.get(q)) : 0;
     sum += w[q];
   }
-  const u64 mine = sum;
+  const u64 own = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const u64 a = __shfl_up(sum, o);
@@ -724,13 +895,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   }
   const u64 past = __ballot(sum > target);
   if (past == 0 || lane != __builtin_ctzll(past)) return;
-  target -= sum - mine;
+  target -= sum - own;
   int q = 0;
   u64 acc = w[0];
 #pragma unroll
   for (int t = 1; t < kEach; ++t)
     if (acc <= target) acc += w[t], q = t;
-  g.tokens[r] = at + q;
+  g.tokens[r] = found * kStretch + lane * kEach + q;
 }
 
 }  // namespace
