@@ -32,6 +32,7 @@
 #include <climits>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "../../include/ossm_lm.h"
 #include "lm_types.hpp"
@@ -47,6 +48,7 @@ constexpr int kThreads = 1024, kWavesOf = kThreads / 64;
 constexpr int kBins = 8192, kPerBins = kBins / kThreads;
 constexpr int kDigits = 2048;                         // of a round of select
 constexpr int kList = 4096, kPer = kList / kThreads;  // gathered tokens, and a thread's
+constexpr int kRanked = 256;                          // items sorted by their ranks
 constexpr int kEach = 8;                              // consecutive entries of a lane
 constexpr int kStretch = 64 * kEach;                  // entries of a wave at a time
 constexpr int kMaxVocab = 1 << 20;
@@ -144,14 +146,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // A row's weights.
 struct Weights {
-  const double* powers;  // in LDS
-  double top, rate;      // the largest logit, log2(e) / T
+  const __attribute__((address_space(3))) double* powers;  // a pointer to anywhere would make its loads slow
+  double top, rate;      // the largest logit (finite), log2(e) / T
   int scale;
-  bool infinite;         // the largest is +inf: it shares the answer with its like alone
 
-  // w 2^scale; NaN and -inf weigh nothing
+  // w 2^scale; NaN and -inf weigh nothing.  No branches: eight entries' chains of dependent
+  // operations have to overlap (one at a time a pass took ten times as long).
   __device__ __forceinline__ double scaled(float v) const {
-    if (infinite) return v == __builtin_inff() ? ldexp(1., scale) : 0.;
     const double y = fmax((static_cast<double>(v) - top) * rate, -64.);  // 2^-64: below half a unit
     const double t = y + 0x1.8p44;                 // y to the nearest 256th, its 256ths in the low bits
     const int n = static_cast<int>(static_cast<uint32_t>(__double_as_longlong(t)));
@@ -207,6 +208,7 @@ struct Shared {
   u64 weight_before;
   uint32_t bin, count_before, listed, above, same;
   int at;
+  uint32_t rank[kRanked];
   union {
     uint32_t bins[kBins];
     struct {
@@ -306,7 +308,7 @@ __device__ __forceinline__ uint32_t last_digit(uint32_t count, u64 weight, u64 n
 // The shortest run of tokens in falling order that has `n` tokens or the weight `w`
 // (at least one unit), or the whole row.
 template <class E>
-__device__ Kept select(const E* row, int V, const Weights& wt, uint32_t top, uint32_t lowest, u64 n, u64 w, Shared& s) {
+__device__ __forceinline__ Kept select(const E* row, int V, const Weights& wt, uint32_t top, uint32_t lowest, u64 n, u64 w, Shared& s) {
   uint32_t hi = top, lo = lowest;  // the key is among these
   u64 weight = 0;                  // of the keys above hi
   uint32_t count = 0;
@@ -365,22 +367,24 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
 }
 
-// The bin in which the n-th entry lies (kBins: there are fewer), s.count_before what lies before it.
+// The bin, of PER a thread, in which the n-th entry lies (kBins: there are fewer), s.count_before
+// what lies before it.
+template <int PER>
 __device__ __forceinline__ uint32_t bin_of_count(uint32_t n, Shared& s) {
-  uint32_t mine[kPerBins], sum = 0;
+  uint32_t mine[PER], sum = 0;
   u64 none = 0;
 #pragma unroll
-  for (int k = 0; k < kPerBins; ++k) {
-    mine[k] = s.bins[threadIdx.x * kPerBins + k];
+  for (int k = 0; k < PER; ++k) {
+    mine[k] = s.bins[threadIdx.x * PER + k];
     sum += mine[k];
   }
   if (threadIdx.x == 0) s.bin = kBins;
   scan_threads(none, sum, s);
 #pragma unroll
-  for (int k = kPerBins - 1; k >= 0; --k) {
+  for (int k = PER - 1; k >= 0; --k) {
     const uint32_t before = sum - mine[k];
     if (sum >= n && before < n) {
-      s.bin = threadIdx.x * kPerBins + k;
+      s.bin = threadIdx.x * PER + k;
       s.count_before = before;
     }
     sum = before;
@@ -442,9 +446,36 @@ __device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F in) {
   return hi;
 }
 
-// s.item[0 .. n - 1] in falling order, n up to kList.  A wave's pairs lie in 128 neighbouring items
-// while they are up to 64 apart, and need no other wave.
-__device__ void sort_items(uint32_t n, Shared& s) {
+// s.item[0 .. n - 1] in falling order, n up to kList, no two alike.  Up to kRanked of them by
+// counting the larger ones of each (64 items a wave, the others shared among the waves): three
+// barriers against a sorting network's 36 dependent steps, 1000 cycles against 17000 at 224 items.
+// Longer lists take the network; a wave's pairs lie in 128 neighbouring items while they are up to 64
+// apart, and need no other wave.
+__device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
+  if (n <= kRanked) {
+    const uint32_t blocks = (n + 63) / 64, wave = threadIdx.x / 64, slices = kWavesOf / blocks;
+    const uint32_t i = wave % blocks * 64 + (threadIdx.x & 63), slice = wave / blocks;
+    const u64 own = i < n ? s.item[i] : 0;
+    if (threadIdx.x < kRanked) s.rank[threadIdx.x] = 0;
+    __syncthreads();
+    if (slice < slices) {
+      uint32_t larger = 0;
+      for (uint32_t j = slice; j < n; j += 4 * slices) {
+        u64 other[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) other[q] = j + q * slices < n ? s.item[j + q * slices] : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) larger += other[q] > own;
+      }
+      if (i < n) atomicAdd(&s.rank[i], larger);
+    }
+    __syncthreads();
+    const u64 mine = threadIdx.x < n ? s.item[threadIdx.x] : 0;
+    __syncthreads();
+    if (threadIdx.x < n) s.item[s.rank[threadIdx.x]] = mine;
+    __syncthreads();
+    return;
+  }
   uint32_t size = 64;
   while (size < n) size *= 2;
   for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) s.item[i] = 0;
@@ -469,7 +500,7 @@ __device__ void sort_items(uint32_t n, Shared& s) {
 // Gathers the entries from lo to below `end` (or all above where there is no end) as items; how
 // many there are, of which at most kList are there.  f sees every vector.
 template <class E, class F>
-__device__ uint32_t gather(const E* row, int V, float lo, float end, bool no_end, Shared& s, F f) {
+__device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float end, bool no_end, Shared& s, F f) {
   __syncthreads();
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
@@ -493,14 +524,15 @@ __device__ uint32_t gather(const E* row, int V, float lo, float end, bool no_end
   return n;
 }
 
-// The weights of the first n sorted items as running sums (this thread's kPer from tid kPer on) on
+// The weights of the first n sorted items as running sums (this thread's PER from tid PER on) on
 // top of `before`; and the whole.
-__device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 before, u64 (&sum)[kPer], Shared& s) {
+template <int PER>
+__device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 before, u64 (&sum)[PER], Shared& s) {
   u64 w = 0;
   uint32_t none = 0;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const uint32_t i = threadIdx.x * kPer + k;
+  for (int k = 0; k < PER; ++k) {
+    const uint32_t i = threadIdx.x * PER + k;
     sum[k] = i < n ? wt.of(static_cast<uint32_t>(s.item[i] >> 32)) : 0;
     w += sum[k];
   }
@@ -509,18 +541,19 @@ __device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 befo
   u64 at = before + w - mine, all = before;
   for (int v = 0; v < kWavesOf; ++v) all += s.wave_weight[v];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) sum[k] = at += sum[k];
+  for (int k = 0; k < PER; ++k) sum[k] = at += sum[k];
   return all;
 }
 
 // The first of n running sums that reaches `target`, n where none does.
-__device__ __forceinline__ uint32_t first_reaching(const u64 (&sum)[kPer], uint32_t n, u64 target, Shared& s) {
+template <int PER>
+__device__ __forceinline__ uint32_t first_reaching(const u64 (&sum)[PER], uint32_t n, u64 target, Shared& s) {
   __syncthreads();
   if (threadIdx.x == 0) s.at = static_cast<int>(n);
   __syncthreads();
 #pragma unroll
-  for (int k = kPer - 1; k >= 0; --k) {
-    const uint32_t i = threadIdx.x * kPer + k;
+  for (int k = PER - 1; k >= 0; --k) {
+    const uint32_t i = threadIdx.x * PER + k;
     if (i < n && sum[k] >= target) atomicMin(&s.at, static_cast<int>(i));
   }
   __syncthreads();
@@ -557,15 +590,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   if (tid < 256) s.powers[tid] = kPowers[tid];  // read after the next barrier
   const bool by_k = k_given > 0 && k_given < g.V, by_p = p < 1.f;
 
-  // the largest logit (of the thread's own in mine) and the least but -inf; NaN is dropped
+  // the largest logit (of the thread's own in mine) and, where the bins have to reach it, the
+  // least but -inf.  The median of x, y and +inf is the larger, or y where x is NaN.
   float mine = -__builtin_inff(), low = __builtin_inff();
+  const bool by_threads = by_k && k_given <= kThreads && k_given <= (g.V + kEach - 1) / kEach;
+  const bool to_low = by_p || !by_threads;
   each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
 #pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      mine = fmaxf(mine, x[q]);
-      low = fminf(low, x[q] > -__builtin_inff() ? x[q] : __builtin_inff());
+    for (int q = 0; q < kEach; ++q) mine = __builtin_amdgcn_fmed3f(x[q], mine, __builtin_inff());
+    if (to_low) {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        low = __builtin_amdgcn_fmed3f(x[q] > -__builtin_inff() ? x[q] : __builtin_inff(), low, -__builtin_inff());
     }
   });
+  if (!to_low && mine > -__builtin_inff()) low = mine;
   float max = mine;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -599,18 +638,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     return;
   }
   const uint32_t top = key_of(max);
-  const Weights wt{s.powers, max, 1.4426950408889634074 / T, g.scale, max == __builtin_inff()};
+  const bool infinite = max == __builtin_inff();  // it shares the answer with its like alone
+  const Weights wt{(const __attribute__((address_space(3))) double*)s.powers, max, 1.4426950408889634074 / T, g.scale};
   const double floor = m > 0.f ? ldexp(static_cast<double>(m < 1.f ? m : 1.f), g.scale) : 0.;
 
   // keys below the lowest weigh nothing; those next to it may weigh nothing too
   const double least = static_cast<double>(max) - 45. * T;
-  const uint32_t lowest = wt.infinite || !(least > -3.4028234e38) ? kLowest + 1 : key_of(static_cast<float>(least)) - 1;
+  const uint32_t lowest = infinite || !(least > -3.4028234e38) ? kLowest + 1 : key_of(static_cast<float>(least)) - 1;
   Kept kept{lowest, UINT_MAX, UINT_MAX, 0};
   const uint32_t k = by_k ? static_cast<uint32_t>(k_given) : UINT_MAX;
   // weights are nothing from 47.5 ln 2 T on
   const float range = fminf(max - low, 33.f * T) * 1.00001f;
-  const bool even = !wt.infinite && range < 1e37f;  // else the bins' width is no number
-  const Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
+  const bool even = range < 1e37f;  // else the bins' width is no number
+  Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
   const auto bin_start = [&](uint32_t b) {  // the least value of bin b and those before
     return value_of(least_key(lowest, top, [&](float v) { return bins.of(v) <= b; }));
   };
@@ -618,18 +658,36 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   // all that can be kept as items: the k largest and what few lie near the last, or a short row
   uint32_t listed = UINT_MAX;
   bool all_kept = false;  // what weighs anything is fewer than k
-  if ((by_k || by_p) && g.V <= kThreads) {
+  if (infinite) {  // equal weights: the first of them, as many as k and p leave
+    if (tid == 0) s.same = 0;
+    __syncthreads();
+    uint32_t n = 0;
+    each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) n += x[q] == max;
+    });
+    atomicAdd(&s.same, n);
+    __syncthreads();
+    kept = Kept{top, min(k, s.same), s.same, 0};
+    if (by_p) kept.ties = static_cast<uint32_t>(part_of(p, kept.ties, true)) | (p > 0.f ? 0u : 1u);
+  } else if ((by_k || by_p) && g.V <= kThreads) {
     listed = gather(row, g.V, -3.402823466e38f, 0.f, true, s, [](const float (&)[kEach]) {});
   } else if (by_k && even) {
-    if (k <= kThreads) {
-      clear_bins(s);
-      const uint32_t b = bins.of(mine);
-      if (b < kBins) atomicAdd(&s.bins[b], 1u);
+    if (by_threads) {
+      // eight bins in one: a bin a thread
       __syncthreads();
-      const uint32_t bin = bin_of_count(k, s);
-      if (bin < kBins) listed = gather(row, g.V, bin_start(bin), 0.f, true, s, [](const float (&)[kEach]) {});
+      s.bins[tid] = 0;
+      __syncthreads();
+      const uint32_t b = bins.of(mine);
+      if (b < kBins) atomicAdd(&s.bins[b / kPerBins], 1u);
+      __syncthreads();
+      const uint32_t bin = bin_of_count<1>(k, s);
+      if (bin < kBins)
+        listed = gather(row, g.V, bin_start(bin * kPerBins + kPerBins - 1), 0.f, true, s, [](const float (&)[kEach]) {});
     }
-    if (listed > kList) {
+    // the bins have reached the least of the threads' largest; now all that weighs anything
+    if (listed > kList && !to_low) bins.scale = 33.f * T < 1e37f ? static_cast<float>(kBins) / (33.f * T * 1.00001f) : 0.f;
+    if (listed > kList && bins.scale > 0.f) {
       clear_bins(s);
       each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
 #pragma unroll
@@ -639,7 +697,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         }
       });
       __syncthreads();
-      const uint32_t bin = bin_of_count(k, s);
+      const uint32_t bin = bin_of_count<kPerBins>(k, s);
       all_kept = bin == kBins;
       if (!all_kept) {
         const uint32_t before = s.count_before, in_bin = s.bins[bin];
@@ -655,22 +713,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       }
     }
   }
-  if (listed <= kList) {
+  // the answer from the list, PER items a thread
+  const auto from_list = [&](auto per) {
+    constexpr int PER = decltype(per)::value;
     sort_items(listed, s);
     uint32_t n = min(k, listed);
-    u64 sum[kPer];
-    u64 total = run_items(wt, n, 0, sum, s);
+    u64 sum[PER];
+    u64 total = run_items<PER>(wt, n, 0, sum, s);
     if (by_p) {
       const u64 part = part_of(p, total, true);
-      n = min(n, first_reaching(sum, n, part > 0 ? part : 1, s) + 1);
+      n = min(n, first_reaching<PER>(sum, n, part > 0 ? part : 1, s) + 1);
     }
     if (floor > 0.) {  // weights fall: the first that does not reach it
       __syncthreads();
       if (tid == 0) s.at = static_cast<int>(n);
       __syncthreads();
 #pragma unroll
-      for (int q = kPer - 1; q >= 0; --q) {
-        const uint32_t i = tid * kPer + q;
+      for (int q = PER - 1; q >= 0; --q) {
+        const uint32_t i = tid * PER + q;
         if (i < n && wt.scaled(value_of(static_cast<uint32_t>(s.item[i] >> 32))) < floor) atomicMin(&s.at, static_cast<int>(i));
       }
       __syncthreads();
@@ -685,26 +745,34 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     swap_halves();
     sort_items(n, s);
     swap_halves();
-    total = run_items(wt, n, 0, sum, s);
+    total = run_items<PER>(wt, n, 0, sum, s);
     const u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
-    const uint32_t at = first_reaching(sum, n, target + 1, s);
+    const uint32_t at = first_reaching<PER>(sum, n, target + 1, s);
     if (tid == 0) g.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.item[at]));
+  };
+  if (listed <= kThreads) {
+    from_list(std::integral_constant<int, 1>{});
     return;
   }
-  if (by_k && !all_kept) kept = select(row, g.V, wt, top, lowest, k, ~0ull, s);
+  if (listed <= kList) {
+    from_list(std::integral_constant<int, kPer>{});
+    return;
+  }
+  if (by_k && !all_kept && !infinite) kept = select(row, g.V, wt, top, lowest, k, ~0ull, s);
 
-  if (by_p) {
+  if (by_p && !infinite) {
     const bool some = kept.ties < kept.same;  // the last key's weight counts `ties` times
     const float last = value_of(kept.key);
     u64 part = 0;
     bool done = false;
     if (even) {
       clear_bins(s);
+      const float from = some ? value_of(kept.key + 1) : last;  // the least whose like are all kept
       each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
           const uint32_t b = bins.of(x[q]);
-          if (b < kBins && (x[q] > last || (x[q] == last && !some))) atomicAdd(&s.bins[b], 1u);
+          if (b < kBins && x[q] >= from) atomicAdd(&s.bins[b], 1u);
         }
       });
       if (some && tid == 0) atomicAdd(&s.bins[min(bins.of(last), kBins - 1u)], kept.ties);
@@ -712,13 +780,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       uint32_t b0, b1;
       bins_of_part(wt, bins, p, b0, b1, s);
       const float end = b0 > 0 ? bin_start(b0 - 1) : 0.f;
+      const float over = b0 > 0 ? fmaxf(end, from) : __builtin_inff();  // kept, and past the gathered ones
       u64 above = 0, total = 0;
       const uint32_t n0 = gather(row, g.V, bin_start(b1), end, b0 == 0, s, [&](const float (&x)[kEach]) {
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
-          const u64 w = x[q] > last || (x[q] == last && !some) ? wt.of(x[q]) : 0;
-          total += w;
-          above += b0 > 0 && x[q] >= end ? w : 0;
+          u64 w = wt.of(x[q]);
+          asm volatile("" : "+v"(w));  // formed for every entry, not behind a branch for each
+          total += x[q] >= from ? w : 0;
+          above += x[q] >= over ? w : 0;
         }
       });
 #pragma unroll
@@ -741,8 +811,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       if (n0 <= kList && above < part) {
         sort_items(n0, s);
         u64 sum[kPer];
-        run_items(wt, n0, above, sum, s);
-        const uint32_t at = first_reaching(sum, n0, part, s);
+        run_items<kPer>(wt, n0, above, sum, s);
+        const uint32_t at = first_reaching<kPer>(sum, n0, part, s);
         if (at < n0) {
           kept = kept_to(at, n0, s);
           done = true;
@@ -756,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     }
     if (!done) kept = select(row, g.V, wt, top, lowest, ~0ull, part, s);
   }
-  if (floor > 0.) {
+  if (floor > 0. && !infinite) {
     const uint32_t key = least_key(lowest, top, [&](float v) { return wt.scaled(v) >= floor; });
     if (key > kept.key) kept = Kept{key, UINT_MAX, UINT_MAX, 0};
   }
@@ -832,20 +902,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     for (int i = 0; i < 4; ++i) {
       const int st = st0 + i * kWavesOf;
       if (st >= n_stretches) break;
-      const uint32_t bits = kept_of(st, v[i]);
+      const bool whole = !some && (st + 1) * kStretch <= g.V;  // no entry but by its value
+      const uint32_t bits = whole ? 0 : kept_of(st, v[i]);
       u64 sum = 0;
       uint32_t n = 0;
       // few kept ones are brought together first: a weight takes 25 operations, this six
 #pragma unroll
       for (int q = 0; q < kEach; ++q) {
-        const bool take = bits >> q & 1;
+        const bool take = whole ? v[i].get(q) >= last : bits >> q & 1;
         const u64 takes = __ballot(take);
         if (take) s.kept[wave][n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(takes >> 32),
                                       __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(takes), 0u))] = v[i].get(q);
         n += __popcll(takes);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (uint32_t e = lane; e < n; e += 64) sum += wt.of(s.kept[wave][e]);
+      if (infinite) {
+        sum = lane == 0 ? static_cast<u64>(n) << g.scale : 0;
+      } else {
+        for (uint32_t e = lane; e < n; e += 64) sum += wt.of(s.kept[wave][e]);
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -884,7 +959,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   u64 w[kEach], sum = 0;
 #pragma unroll
   for (int q = 0; q < kEach; ++q) {
-    w[q] = bits >> q & 1 ? wt.of(v.get(q)) : 0;
+    w[q] = (bits >> q & 1) == 0 ? 0 : infinite ? 1ull << g.scale : wt.of(v.get(q));
     sum += w[q];
   }
   const u64 own = sum;
