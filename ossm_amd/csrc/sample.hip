@@ -48,10 +48,11 @@ constexpr int kThreads = 1024, kWavesOf = kThreads / 64;
 constexpr int kBins = 8192, kPerBins = kBins / kThreads;
 constexpr int kDigits = 2048;                         // of a round of select
 constexpr int kList = 4096, kPer = kList / kThreads;  // gathered tokens, and a thread's
-constexpr int kRanked = 256;                          // items sorted by their ranks
+constexpr int kRanked = 256;                          // items sorted by their ranks alone
+constexpr int kBuckets = kThreads, kCrowd = 512;      // where more are, and the most of one
 constexpr int kEach = 8;                              // consecutive entries of a lane
 constexpr int kStretch = 64 * kEach;                  // entries of a wave at a time
-constexpr int kMaxVocab = 1 << 20;
+constexpr int kIndexBits = 20, kMaxVocab = 1 << kIndexBits;
 constexpr int kStretches = kMaxVocab / kStretch;
 
 __constant__ double kPowers[256] = {  // 2^(j / 256)
@@ -144,6 +145,20 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// A gathered token: its key, of which bfloat16's is 16 bits, over its index's complement, so that
+// equal ones fall in rising order of index.
+constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
+template <class E>
+__device__ __forceinline__ u64 item_of(float l, uint32_t index) {
+  return static_cast<u64>(sizeof(E) == 2 ? key_of(l) >> 16 : key_of(l)) << kIndexBits | (kIndexMask ^ index);
+}
+template <class E>
+__device__ __forceinline__ uint32_t item_key(u64 item) {
+  const uint32_t k = static_cast<uint32_t>(item >> kIndexBits);
+  return sizeof(E) == 4 ? k : k << 16 | (k & 0x8000u ? 0u : 0xffffu);
+}
+__device__ __forceinline__ uint32_t item_index(u64 item) { return ~static_cast<uint32_t>(item) & kIndexMask; }
+
 // A row's weights.
 struct Weights {
   const __attribute__((address_space(3))) double* powers;  // a pointer to anywhere would make its loads slow
@@ -208,7 +223,8 @@ struct Shared {
   u64 weight_before;
   uint32_t bin, count_before, listed, above, same;
   int at;
-  uint32_t rank[kRanked];
+  uint32_t bucket[kBuckets];
+  u64 stretch[kStretches];
   union {
     uint32_t bins[kBins];
     struct {
@@ -217,30 +233,31 @@ struct Shared {
     };
     u64 item[kList];
     struct {
-      u64 stretch[kStretches];
       uint32_t ties[kStretches];
       float kept[kWavesOf][kStretch];
     };
   };
 };
 
-// f(first index, values) of every vector of the row, -inf behind its end; four vectors a
-// thread are asked for at once (one at a time a pass was bound by their latency).
+// f(first index, values) of every vector of the row, by whole waves (a stretch each), -inf behind
+// its end; four vectors a thread are asked for at once (one at a time a pass was bound by their
+// latency).
 template <class E, class F>
 __device__ __forceinline__ void each_vector(const E* row, int V, F f) {
   constexpr int kAhead = 4, kStep = kThreads * kEach;
-  for (int at0 = static_cast<int>(threadIdx.x) * kEach; at0 < V; at0 += kAhead * kStep) {
+  const int lane_at = static_cast<int>(threadIdx.x & 63) * kEach;
+  for (int st0 = static_cast<int>(threadIdx.x / 64) * kStretch; st0 < V; st0 += kAhead * kStep) {
     Vec<E, kEach> v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int at = at0 + u * kStep;
+      const int at = st0 + u * kStep + lane_at;
       v[u].zero();
       if (at < V) v[u].load(row + at, V - at);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int at = at0 + u * kStep;
-      if (at >= V) break;
+      const int at = st0 + u * kStep + lane_at;
+      if (st0 + u * kStep >= V) break;
       float x[kEach];
 #pragma unroll
       for (int k = 0; k < kEach; ++k) x[k] = v[u].get(k);
@@ -252,6 +269,24 @@ __device__ __forceinline__ void each_vector(const E* row, int V, F f) {
       f(at, x);
     }
   }
+}
+
+// The sum over a wave, in its last lane, without a way through LDS.
+__device__ __forceinline__ u64 sum_to_last(u64 v) {
+#define OSSM_ADD(CTRL, ROWS)                                                                              \
+  {                                                                                                       \
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);       \
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false); \
+    v += static_cast<u64>(hi) << 32 | lo;                                                                 \
+  }
+  OSSM_ADD(0x111, 0xf)  // a row's lanes on by 1, 2, 4, 8
+  OSSM_ADD(0x112, 0xf)
+  OSSM_ADD(0x114, 0xf)
+  OSSM_ADD(0x118, 0xf)
+  OSSM_ADD(0x142, 0xa)  // the last of rows 0 and 2 to the next row
+  OSSM_ADD(0x143, 0xc)  // the last of row 1 to rows 2 and 3
+#undef OSSM_ADD
+  return v;
 }
 
 // Inclusive sums over a workgroup's threads.
@@ -351,13 +386,13 @@ __device__ __forceinline__ Kept select(const E* row, int V, const Weights& wt, u
   }
 }
 
-// The row's bins: of equal width in the logits from the largest down, to where weights are
-// nothing or the row ends.
+// The row's bins: of equal width in the logits from the largest down, to about where weights are
+// nothing or the row ends; the last takes all below it.
 struct Bins {
   float top, scale;
-  __device__ __forceinline__ uint32_t of(float v) const {  // kBins: weighs nothing
+  __device__ __forceinline__ uint32_t of(float v) const {  // kBins: -inf and NaN
     const float b = (top - v) * scale;
-    return b < static_cast<float>(kBins) ? static_cast<uint32_t>(b) : kBins;
+    return b < 3e38f ? min(static_cast<uint32_t>(b), kBins - 1u) : kBins;
   }
 };
 
@@ -397,8 +432,10 @@ __device__ __forceinline__ uint32_t bin_of_count(uint32_t n, Shared& s) {
 // the weights of their middles tell.
 __device__ __forceinline__ void bins_of_part(const Weights& wt, const Bins& bins, float p, uint32_t& first, uint32_t& last, Shared& s) {
   constexpr float kUnit = 16777216.f;  // 2^24
-  // a middle's weight may be off by half a bin, 0.2 percent; most bins' errors cancel
-  constexpr float kMargin = 0.0025f;
+  // a middle's weight may be off by half a bin, 0.2 percent, but most bins' errors cancel; where
+  // they do not, the border is found by bits.  Four times this gathered 4200 tokens at p = 0.98 of
+  // 131072 normal logits, more than a list holds
+  constexpr float kMargin = 0.0006f;
   u64 mine[kPerBins], sum = 0;
   uint32_t none = 0;
   const float step = bins.scale > 0.f ? static_cast<float>(wt.rate) / bins.scale : 0.f;
@@ -448,15 +485,17 @@ __device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F in) {
 
 // s.item[0 .. n - 1] in falling order, n up to kList, no two alike.  Up to kRanked of them by
 // counting the larger ones of each (64 items a wave, the others shared among the waves): three
-// barriers against a sorting network's 36 dependent steps, 1000 cycles against 17000 at 224 items.
-// Longer lists take the network; a wave's pairs lie in 128 neighbouring items while they are up to 64
-// apart, and need no other wave.
+// barriers, 1000 cycles at 224 items.  More of them first go to 1024 buckets of equal width between
+// the largest and the least, and are ranked in their own.  Where many share one, they take a sorting
+// network (17000 cycles at 224 items, 43000 at 1123); a wave's pairs lie in 128 neighbouring items while
+// they are up to 64 apart, and need no other wave.
 __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
+  const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid & 63;
   if (n <= kRanked) {
-    const uint32_t blocks = (n + 63) / 64, wave = threadIdx.x / 64, slices = kWavesOf / blocks;
-    const uint32_t i = wave % blocks * 64 + (threadIdx.x & 63), slice = wave / blocks;
+    const uint32_t blocks = (n + 63) / 64, slices = kWavesOf / blocks;
+    const uint32_t i = wave % blocks * 64 + lane, slice = wave / blocks;
     const u64 own = i < n ? s.item[i] : 0;
-    if (threadIdx.x < kRanked) s.rank[threadIdx.x] = 0;
+    if (tid < kRanked) s.bucket[tid] = 0;
     __syncthreads();
     if (slice < slices) {
       uint32_t larger = 0;
@@ -467,12 +506,71 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) larger += other[q] > own;
       }
-      if (i < n) atomicAdd(&s.rank[i], larger);
+      if (i < n) atomicAdd(&s.bucket[i], larger);
     }
     __syncthreads();
-    const u64 mine = threadIdx.x < n ? s.item[threadIdx.x] : 0;
+    const u64 mine = tid < n ? s.item[tid] : 0;
     __syncthreads();
-    if (threadIdx.x < n) s.item[s.rank[threadIdx.x]] = mine;
+    if (tid < n) s.item[s.bucket[tid]] = mine;
+    __syncthreads();
+    return;
+  }
+  u64 mine[kPer], hi = 0, lo = ~0ull;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const uint32_t i = tid + q * kThreads;
+    mine[q] = i < n ? s.item[i] : 0;
+    if (i >= n) continue;
+    hi = hi > mine[q] ? hi : mine[q];
+    lo = lo < mine[q] ? lo : mine[q];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 a = __shfl_xor(hi, o), b = __shfl_xor(lo, o);
+    hi = hi > a ? hi : a;
+    lo = lo < b ? lo : b;
+  }
+  if (lane == 0) s.wave_weight[wave] = hi, s.wave_more[wave] = lo;
+  s.bucket[tid] = 0;
+  __syncthreads();
+  for (int v = 0; v < kWavesOf; ++v) {
+    hi = hi > s.wave_weight[v] ? hi : s.wave_weight[v];
+    lo = lo < s.wave_more[v] ? lo : s.wave_more[v];
+  }
+  const int shift = max(54 - __clzll(static_cast<long long>(hi - lo)), 0);  // hi > lo: ten bits stay
+  uint32_t place[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q)
+    if (tid + q * kThreads < n) place[q] = atomicAdd(&s.bucket[(hi - mine[q]) >> shift], 1u);
+  __syncthreads();
+  uint32_t own = s.bucket[tid], end = own;
+  if (!__syncthreads_or(own > kCrowd)) {
+    u64 none = 0;
+    scan_threads(none, end, s);
+    s.bucket[tid] = end - own;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      if (tid + q * kThreads < n) s.item[s.bucket[(hi - mine[q]) >> shift] + place[q]] = mine[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      if (tid + q * kThreads >= n) continue;
+      const uint32_t b = static_cast<uint32_t>((hi - mine[q]) >> shift);
+      const uint32_t from = s.bucket[b], to = b + 1 < kBuckets ? s.bucket[b + 1] : n;
+      place[q] = from;
+      for (uint32_t j = from; j < to; j += 4) {
+        u64 other[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) other[t] = j + t < to ? s.item[j + t] : 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) place[q] += other[t] > mine[q];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      if (tid + q * kThreads < n) s.item[place[q]] = mine[q];
     __syncthreads();
     return;
   }
@@ -498,14 +596,14 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
 }
 
 // Gathers the entries from lo to below `end` (or all above where there is no end) as items; how
-// many there are, of which at most kList are there.  f sees every vector.
+// many there are, of which at most kList are there.  f sees every vector, by whole waves.
 template <class E, class F>
 __device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float end, bool no_end, Shared& s, F f) {
   __syncthreads();
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
   each_vector(row, V, [&](int at, const float (&x)[kEach]) {
-    f(x);
+    f(at, x);
     uint32_t bits = 0;
 #pragma unroll
     for (int q = 0; q < kEach; ++q) bits |= (x[q] >= lo && (no_end || x[q] < end) ? 1u : 0u) << q;
@@ -514,7 +612,7 @@ __device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float 
 #pragma unroll
     for (int q = 0; q < kEach; ++q) {
       if ((bits >> q & 1) == 0) continue;
-      if (i < kList) s.item[i] = static_cast<u64>(key_of(x[q])) << 32 | ~static_cast<uint32_t>(at + q);
+      if (i < kList) s.item[i] = item_of<E>(x[q], static_cast<uint32_t>(at + q));
       ++i;
     }
   });
@@ -526,14 +624,14 @@ __device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float 
 
 // The weights of the first n sorted items as running sums (this thread's PER from tid PER on) on
 // top of `before`; and the whole.
-template <int PER>
+template <class E, int PER>
 __device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 before, u64 (&sum)[PER], Shared& s) {
   u64 w = 0;
   uint32_t none = 0;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const uint32_t i = threadIdx.x * PER + k;
-    sum[k] = i < n ? wt.of(static_cast<uint32_t>(s.item[i] >> 32)) : 0;
+    sum[k] = i < n ? wt.of(item_key<E>(s.item[i])) : 0;
     w += sum[k];
   }
   const u64 mine = w;
@@ -561,13 +659,14 @@ __device__ __forceinline__ uint32_t first_reaching(const u64 (&sum)[PER], uint32
 }
 
 // What is kept where sorted item `at` of n is the last: a key that others share is kept up to it.
+template <class E>
 __device__ __forceinline__ Kept kept_to(uint32_t at, uint32_t n, Shared& s) {
-  const uint32_t key = static_cast<uint32_t>(s.item[at] >> 32);
+  const uint32_t key = item_key<E>(s.item[at]);
   if (threadIdx.x == 0) s.above = s.same = 0;
   __syncthreads();
   uint32_t above = 0, same = 0;
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t k = static_cast<uint32_t>(s.item[i] >> 32);
+    const uint32_t k = item_key<E>(s.item[i]);
     above += k > key;
     same += k == key;
   }
@@ -590,21 +689,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   if (tid < 256) s.powers[tid] = kPowers[tid];  // read after the next barrier
   const bool by_k = k_given > 0 && k_given < g.V, by_p = p < 1.f;
 
-  // the largest logit (of the thread's own in mine) and, where the bins have to reach it, the
-  // least but -inf.  The median of x, y and +inf is the larger, or y where x is NaN.
+  // the largest logit (of the thread's own in mine) and about the least but -inf, of every
+  // eighth.  The median of x, y and +inf is the larger, or y where x is NaN.
   float mine = -__builtin_inff(), low = __builtin_inff();
   const bool by_threads = by_k && k_given <= kThreads && k_given <= (g.V + kEach - 1) / kEach;
-  const bool to_low = by_p || !by_threads;
   each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
 #pragma unroll
     for (int q = 0; q < kEach; ++q) mine = __builtin_amdgcn_fmed3f(x[q], mine, __builtin_inff());
-    if (to_low) {
-#pragma unroll
-      for (int q = 0; q < kEach; ++q)
-        low = __builtin_amdgcn_fmed3f(x[q] > -__builtin_inff() ? x[q] : __builtin_inff(), low, -__builtin_inff());
-    }
+    low = __builtin_amdgcn_fmed3f(x[0] > -__builtin_inff() ? x[0] : __builtin_inff(), low, -__builtin_inff());
   });
-  if (!to_low && mine > -__builtin_inff()) low = mine;
   float max = mine;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -648,9 +741,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   Kept kept{lowest, UINT_MAX, UINT_MAX, 0};
   const uint32_t k = by_k ? static_cast<uint32_t>(k_given) : UINT_MAX;
   // weights are nothing from 47.5 ln 2 T on
-  const float range = fminf(max - low, 33.f * T) * 1.00001f;
+  const float range = fminf(low < max ? max - low : __builtin_inff(), 33.f * T) * 1.00001f;
   const bool even = range < 1e37f;  // else the bins' width is no number
-  Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
+  const Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
   const auto bin_start = [&](uint32_t b) {  // the least value of bin b and those before
     return value_of(least_key(lowest, top, [&](float v) { return bins.of(v) <= b; }));
   };
@@ -671,7 +764,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     kept = Kept{top, min(k, s.same), s.same, 0};
     if (by_p) kept.ties = static_cast<uint32_t>(part_of(p, kept.ties, true)) | (p > 0.f ? 0u : 1u);
   } else if ((by_k || by_p) && g.V <= kThreads) {
-    listed = gather(row, g.V, -3.402823466e38f, 0.f, true, s, [](const float (&)[kEach]) {});
+    listed = gather(row, g.V, -3.402823466e38f, 0.f, true, s, [](int, const float (&)[kEach]) {});
   } else if (by_k && even) {
     if (by_threads) {
       // eight bins in one: a bin a thread
@@ -683,11 +776,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       __syncthreads();
       const uint32_t bin = bin_of_count<1>(k, s);
       if (bin < kBins)
-        listed = gather(row, g.V, bin_start(bin * kPerBins + kPerBins - 1), 0.f, true, s, [](const float (&)[kEach]) {});
+        listed = gather(row, g.V, bin_start(bin * kPerBins + kPerBins - 1), 0.f, true, s, [](int, const float (&)[kEach]) {});
     }
-    // the bins have reached the least of the threads' largest; now all that weighs anything
-    if (listed > kList && !to_low) bins.scale = 33.f * T < 1e37f ? static_cast<float>(kBins) / (33.f * T * 1.00001f) : 0.f;
-    if (listed > kList && bins.scale > 0.f) {
+    if (listed > kList) {
       clear_bins(s);
       each_vector(row, g.V, [&](int, const float (&x)[kEach]) {
 #pragma unroll
@@ -702,12 +793,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       if (!all_kept) {
         const uint32_t before = s.count_before, in_bin = s.bins[bin];
         if (before + in_bin <= kList) {
-          listed = gather(row, g.V, bin_start(bin), 0.f, true, s, [](const float (&)[kEach]) {});
+          listed = gather(row, g.V, bin_start(bin), 0.f, true, s, [](int, const float (&)[kEach]) {});
         } else if (in_bin <= kList) {
           const uint32_t n0 = gather(row, g.V, bin_start(bin), bin > 0 ? bin_start(bin - 1) : 0.f, bin == 0, s,
-                                     [](const float (&)[kEach]) {});
+                                     [](int, const float (&)[kEach]) {});
           sort_items(n0, s);
-          kept = kept_to(k - before - 1, n0, s);
+          kept = kept_to<E>(k - before - 1, n0, s);
           all_kept = true;
         }
       }
@@ -719,7 +810,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     sort_items(listed, s);
     uint32_t n = min(k, listed);
     u64 sum[PER];
-    u64 total = run_items<PER>(wt, n, 0, sum, s);
+    u64 total = run_items<E, PER>(wt, n, 0, sum, s);
     if (by_p) {
       const u64 part = part_of(p, total, true);
       n = min(n, first_reaching<PER>(sum, n, part > 0 ? part : 1, s) + 1);
@@ -731,24 +822,22 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
 #pragma unroll
       for (int q = PER - 1; q >= 0; --q) {
         const uint32_t i = tid * PER + q;
-        if (i < n && wt.scaled(value_of(static_cast<uint32_t>(s.item[i] >> 32))) < floor) atomicMin(&s.at, static_cast<int>(i));
+        if (i < n && wt.scaled(value_of(item_key<E>(s.item[i]))) < floor) atomicMin(&s.at, static_cast<int>(i));
       }
       __syncthreads();
       n = s.at > 0 ? static_cast<uint32_t>(s.at) : 1u;
     }
     // the kept ones by their index: its complement above the key, so that falling order is rising index
-    const auto swap_halves = [&] {
-      __syncthreads();
-      for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = s.item[i] << 32 | s.item[i] >> 32;
-      __syncthreads();
-    };
-    swap_halves();
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = (s.item[i] & kIndexMask) << 32 | s.item[i] >> kIndexBits;
+    __syncthreads();
     sort_items(n, s);
-    swap_halves();
-    total = run_items<PER>(wt, n, 0, sum, s);
+    for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = s.item[i] << 32 >> (32 - kIndexBits) | s.item[i] >> 32;
+    __syncthreads();
+    total = run_items<E, PER>(wt, n, 0, sum, s);
     const u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
     const uint32_t at = first_reaching<PER>(sum, n, target + 1, s);
-    if (tid == 0) g.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.item[at]));
+    if (tid == 0) g.tokens[r] = item_index(s.item[at]);
   };
   if (listed <= kThreads) {
     from_list(std::integral_constant<int, 1>{});
@@ -760,6 +849,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   }
   if (by_k && !all_kept && !infinite) kept = select(row, g.V, wt, top, lowest, k, ~0ull, s);
 
+  const uint32_t floor_key =
+      floor > 0. && !infinite ? least_key(lowest, top, [&](float v) { return wt.scaled(v) >= floor; }) : 0;
+  uint32_t summed = 0;  // so many tokens are gathered, and the stretches' kept weights known
   if (by_p && !infinite) {
     const bool some = kept.ties < kept.same;  // the last key's weight counts `ties` times
     const float last = value_of(kept.key);
@@ -780,16 +872,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       uint32_t b0, b1;
       bins_of_part(wt, bins, p, b0, b1, s);
       const float end = b0 > 0 ? bin_start(b0 - 1) : 0.f;
-      const float over = b0 > 0 ? fmaxf(end, from) : __builtin_inff();  // kept, and past the gathered ones
+      // Sure to be kept: past the gathered ones.  Where min-p keeps fewer, what it keeps, and p's
+      // border is not looked for if that is below p's part.
+      const bool fewer = b0 > 0 && floor_key > 0 && value_of(floor_key) >= fmaxf(end, from);
+      const float over = fewer ? value_of(floor_key) : b0 > 0 ? fmaxf(end, from) : __builtin_inff();
       u64 above = 0, total = 0;
-      const uint32_t n0 = gather(row, g.V, bin_start(b1), end, b0 == 0, s, [&](const float (&x)[kEach]) {
+      const uint32_t n0 = gather(row, g.V, fewer ? __builtin_inff() : bin_start(b1), end, b0 == 0, s, [&](int at, const float (&x)[kEach]) {
+        u64 high = 0;
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
           u64 w = wt.of(x[q]);
           asm volatile("" : "+v"(w));  // formed for every entry, not behind a branch for each
           total += x[q] >= from ? w : 0;
-          above += x[q] >= over ? w : 0;
+          high += x[q] >= over ? w : 0;
         }
+        above += high;
+        if (__ballot(high != 0) != 0) high = sum_to_last(high);
+        if (lane == 63) s.stretch[at / kStretch] = high;
       });
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) {
@@ -804,17 +903,30 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       if (some) {  // its own bin or one behind: never above the gathered ones but where all are
         const u64 w = wt.of(last) * kept.ties;
         total += w;
-        above += b0 > 0 && last >= end ? w : 0;
+        above += b0 > 0 && !fewer && last >= end ? w : 0;
       }
       part = part_of(p, total, true);
       part = part > 0 ? part : 1;
-      if (n0 <= kList && above < part) {
+      if (fewer) {
+        done = above < part;
+        if (done) {
+          kept = Kept{floor_key, UINT_MAX, UINT_MAX, 0};
+          summed = 1;  // no last one is left out
+        }
+      } else if (n0 <= kList && above < part) {
         sort_items(n0, s);
         u64 sum[kPer];
-        run_items<kPer>(wt, n0, above, sum, s);
+        run_items<E, kPer>(wt, n0, above, sum, s);
         const uint32_t at = first_reaching<kPer>(sum, n0, part, s);
         if (at < n0) {
-          kept = kept_to(at, n0, s);
+          if (!some) {  // the gathered tokens' weights join those above them
+            for (uint32_t i = tid; i <= at; i += kThreads) {
+              const uint32_t key = item_key<E>(s.item[i]);
+              if (key >= floor_key) atomicAdd(&s.stretch[item_index(s.item[i]) / kStretch], wt.of(key));
+            }
+            summed = n0;
+          }
+          kept = kept_to<E>(at, n0, s);
           done = true;
         }
         __syncthreads();
@@ -826,12 +938,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     }
     if (!done) kept = select(row, g.V, wt, top, lowest, ~0ull, part, s);
   }
-  if (floor > 0. && !infinite) {
-    const uint32_t key = least_key(lowest, top, [&](float v) { return wt.scaled(v) >= floor; });
-    if (key > kept.key) kept = Kept{key, UINT_MAX, UINT_MAX, 0};
-  }
+  if (floor_key > kept.key) kept = Kept{floor_key, UINT_MAX, UINT_MAX, 0};
 
-  // the kept weights of each stretch, of equal last ones the first
+  // the kept weights of each stretch, of equal last ones the first; the latter's numbers before each
   const int n_stretches = (g.V + kStretch - 1) / kStretch;
   const bool some = kept.ties < kept.same;
   const float last = value_of(kept.key);
@@ -841,7 +950,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     if (at < g.V) v.load(row + at, g.V - at);
   };
   __syncthreads();
-  if (some) {
+  if (some && summed == 0) {
     for (int st = wave; st < n_stretches; st += kWavesOf) {
       Vec<E, kEach> v;
       load(st, v);
@@ -869,8 +978,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     }
     __syncthreads();
   }
-  // which of the lane's entries of a stretch are kept, as bits
-  const auto kept_of = [&](int st, const Vec<E, kEach>& v) {
+  // which of the lane's entries of a stretch are kept, as bits, with so many of the last before it
+  const auto kept_of = [&](int st, const Vec<E, kEach>& v, uint32_t ties) {
     const int left = g.V - (st * kStretch + lane * kEach);
     uint32_t bits = 0, same = 0;
 #pragma unroll
@@ -889,12 +998,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         const uint32_t b = __shfl_up(sum, o);
         if (lane >= o) sum += b;
       }
-      const uint32_t before = s.ties[st] + sum - n, room = before < kept.ties ? kept.ties - before : 0;
+      const uint32_t before = ties + sum - n, room = before < kept.ties ? kept.ties - before : 0;
       while (static_cast<uint32_t>(__popc(same)) > room) same &= ~(0x80000000u >> __clz(same));  // the first ones stay
     }
     return bits | same;
   };
-  for (int st0 = wave; st0 < n_stretches; st0 += 4 * kWavesOf) {
+  for (int st0 = summed > 0 ? n_stretches : wave; st0 < n_stretches; st0 += 4 * kWavesOf) {
     Vec<E, kEach> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) load(min(st0 + i * kWavesOf, n_stretches - 1), v[i]);
@@ -903,7 +1012,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
       const int st = st0 + i * kWavesOf;
       if (st >= n_stretches) break;
       const bool whole = !some && (st + 1) * kStretch <= g.V;  // no entry but by its value
-      const uint32_t bits = whole ? 0 : kept_of(st, v[i]);
+      if (whole) {
+        float most = -__builtin_inff();
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) most = __builtin_amdgcn_fmed3f(v[i].get(q), most, __builtin_inff());
+        if (__ballot(most >= last) == 0) {  // most stretches, where few tokens are kept
+          if (lane == 0) s.stretch[st] = 0;
+          continue;
+        }
+      }
+      const uint32_t bits = whole ? 0 : kept_of(st, v[i], some ? s.ties[st] : 0);
       u64 sum = 0;
       uint32_t n = 0;
       // few kept ones are brought together first: a weight takes 25 operations, this six
@@ -922,9 +1040,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         for (uint32_t e = lane; e < n; e += 64) sum += wt.of(s.kept[wave][e]);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-      if (lane == 0) s.stretch[st] = sum;
+      sum = sum_to_last(sum);
+      if (lane == 63) s.stretch[st] = sum;
     }
   }
   __syncthreads();
@@ -955,7 +1072,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   }
   Vec<E, kEach> v;
   load(found, v);
-  const uint32_t bits = kept_of(found, v);
+  uint32_t ties = 0;
+  if (some && summed > 0) {
+    for (uint32_t i = lane; i < summed; i += 64)
+      ties += item_key<E>(s.item[i]) == kept.key && item_index(s.item[i]) < static_cast<uint32_t>(found) * kStretch;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ties += __shfl_xor(ties, o);
+  } else if (some) {
+    ties = s.ties[found];
+  }
+  const uint32_t bits = kept_of(found, v, ties);
   u64 w[kEach], sum = 0;
 #pragma unroll
   for (int q = 0; q < kEach; ++q) {
