@@ -118,6 +118,44 @@ def test_ties_go_to_the_lowest_index(S, dtype):
     assert got.tolist() == [0, 0, 1, 1]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_borders_of_p_and_min_p_next_to_each_other(S, dtype):
+    announce(dtype)
+    V, rng = 40000, np.random.default_rng(91)
+    x = torch.tensor(rng.normal(size=(1, V)), dtype=dtype)
+    w = np.sort(np.exp(x.double().numpy()[0] - float(x.max())))[::-1]
+    rows = []
+    for part in (0.05, 0.3, 0.7, 0.97):
+        border = w[int((np.cumsum(w) < part * w.sum()).sum())]
+        for near in (0.5, 0.999, 0.99999, 1.0, 1.00001, 1.001, 2.0):
+            for k in (0, 900, 20000):
+                rows.append((part, border * near, k))
+    part, floor, k = (np.array(c) for c in zip(*rows))
+    u = rng.uniform(size=len(rows))
+    check(S, x.expand(len(rows), V).contiguous().cuda(), u, 1.0, k, part, floor)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_crowded_and_sparse_rows(S, dtype):
+    announce(dtype)
+    V, rng = 30000, np.random.default_rng(92)
+    crowd = np.full(V, -9.0)
+    crowd[rng.permutation(V)[:3000]] = 2.0
+    crowd[[77, 29999]] = 2.015625, 2.0078125  # one bin's width of the row's, far apart in bits
+    coarse = np.round(rng.normal(size=V) * 8) / 8
+    masked = np.where(np.arange(V) % 8 == 1, rng.normal(size=V), -INF)  # none of every eighth is left
+    deep = rng.normal(size=V)
+    deep[::8] = 4.0
+    deep[1::2] -= 300.0  # far below what every eighth reaches
+    for row in (crowd, coarse, masked, deep):
+        x = torch.tensor(np.stack([row] * 24), dtype=dtype).cuda()
+        u = rng.uniform(size=24)
+        part = np.array([0.02, 0.4, 0.8, 0.99] * 6)
+        for kw in ({"top_p": part}, {"top_k": 600}, {"top_k": 2500}, {"top_k": 9000, "top_p": part},
+                   {"top_p": part, "min_p": 0.3}, {"temperature": 7.0, "top_p": part}):
+            check(S, x, u, **kw)
+
+
 def test_special_values(S):
     V = 700
     rng = np.random.default_rng(0)
