@@ -149,7 +149,8 @@ int ossm_layer_norm_backward(int dtype, int weight_dtype, const void* grad_y, in
  *   a_t = exp(-scale softplus(decay[d]) sigmoid(decay_gate_t))
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t
  *   y_t = h_t, or h_t silu(output_gate_t) where output_gate is given
- * x and the gates E, rows of dim with row strides ld_*; decay f32 [dim]; y E dense.
+ * x and the gates E, rows of dim with row strides ld_*; decay f32 [dim]; scale positive and
+ * finite; y E dense.
  *
  * ossm_recurrence_forward: [batch, length] rows of each tensor; start f32 [batch, dim] or
  * null (zeros); last f32 [batch, dim] takes h of the last step.  saved: f32, of

@@ -787,9 +787,12 @@ int backward(Backward<E> g, float* gdecay, StreamCall& call) {
   return backward_tile<E, 1, 8, 16, 16>(g, gdecay, call);
 }
 
-int check_sizes(const char* what, int dtype, int64_t B, int64_t L, int64_t D) {
+int check_sizes(const char* what, int dtype, float scale, int64_t B, int64_t L, int64_t D) {
   if (dtype != OSSM_F32 && dtype != OSSM_BF16)
     return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": unknown dtype");
+  // the root of 1 - a^2 is none where a passes one
+  if (!(scale > 0.f && scale < __builtin_inff()))
+    return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": scale must be positive and finite");
   if (B < 0 || L < 0 || D < 0) return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": negative size");
   if (B > (1 << 24) || L > (1 << 30) || D > (1 << 24))
     return set_error(OSSM_ERR_UNSUPPORTED, std::string(what) + ": size exceeds launch limits");
@@ -819,7 +822,7 @@ int ossm_recurrence_forward(int dtype, const void* x, int64_t ld_x, const void* 
                             int64_t batch, int64_t length, int64_t dim, ossm_stream_t stream_v) {
   clear_error();
   const char* what = "recurrence_forward";
-  if (int rc = check_sizes(what, dtype, batch, length, dim)) return rc;
+  if (int rc = check_sizes(what, dtype, scale, batch, length, dim)) return rc;
   if (batch == 0 || length == 0 || dim == 0) return OSSM_OK;
   if (!x || !input_gate || !decay_gate || !decay || !y || !last) return null_pointer(what);
   if (batch * length > 1 && (ld_x < dim || ld_input_gate < dim || ld_decay_gate < dim || (output_gate && ld_output_gate < dim)))
@@ -850,7 +853,7 @@ int ossm_recurrence_backward(int dtype, const void* grad_y, int64_t ld_grad, con
                              int64_t length, int64_t dim, ossm_stream_t stream_v) {
   clear_error();
   const char* what = "recurrence_backward";
-  if (int rc = check_sizes(what, dtype, batch, length, dim)) return rc;
+  if (int rc = check_sizes(what, dtype, scale, batch, length, dim)) return rc;
   if (batch == 0 || length == 0 || dim == 0) return OSSM_OK;
   if (!grad_y || !x || !input_gate || !decay_gate || !decay || !saved || !grad_x || !grad_input_gate || !grad_decay_gate ||
       (output_gate != nullptr) != (grad_output_gate != nullptr))
@@ -885,7 +888,7 @@ int ossm_recurrence_prompt(int dtype, const void* x, int64_t ld_x, const void* i
                            int64_t n_slots, int64_t dim, ossm_stream_t stream_v) {
   clear_error();
   const char* what = "recurrence_prompt";
-  if (int rc = check_sizes(what, dtype, n_seqs, rows, dim)) return rc;
+  if (int rc = check_sizes(what, dtype, scale, n_seqs, rows, dim)) return rc;
   if (n_slots < 0 || n_slots > INT_MAX) return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": bad pool size");
   if (n_seqs > 65535) return set_error(OSSM_ERR_UNSUPPORTED, std::string(what) + ": more than 65535 prompts");
   if (dim == 0 || (rows == 0 && n_seqs == 0)) return OSSM_OK;
@@ -919,7 +922,7 @@ int ossm_recurrence_step(int dtype, const void* x, int64_t ld_x, const void* inp
                          void* y, int64_t rows, int64_t n_slots, int64_t dim, ossm_stream_t stream_v) {
   clear_error();
   const char* what = "recurrence_step";
-  if (int rc = check_sizes(what, dtype, 1, rows, dim)) return rc;
+  if (int rc = check_sizes(what, dtype, scale, 1, rows, dim)) return rc;
   if (n_slots < 0 || n_slots > INT_MAX) return set_error(OSSM_ERR_INVALID_ARGUMENT, std::string(what) + ": bad pool size");
   if (dim == 0 || rows == 0) return OSSM_OK;
   if (!x || !input_gate || !decay_gate || !y || !decay || !in_slots || (n_slots > 0 && !state)) return null_pointer(what);

@@ -184,7 +184,7 @@ def gated_recurrence(x: Tensor, input_gate: Tensor, decay_gate: Tensor, decay: T
                      state: Optional[Tensor] = None, *, scale: float = 8.0) -> Tuple[Tensor, Tensor]:
     """(y [B, L, D], the states after the last step [B, D]) of the recurrence over x
     [B, L, D] and its gates (of x's dtype and shape, any strides) with decay float32 [D], from
-    state float32 [B, D] (default zeros).  Differentiable in every tensor (in reverse mode; a
+    state float32 [B, D] (default zeros); scale is positive and finite.  Differentiable in every tensor (in reverse mode; a
     forward-mode tangent raises), twice as torch's separate steps."""
     what = "gated_recurrence"
     _check(what, x, input_gate, decay_gate, output_gate, decay, 3)
@@ -279,6 +279,8 @@ class RecurrentMixer(nn.Module):
 
     def __init__(self, d_model: int, *, expand: int = 2, scale: float = 8.0, bias: bool = False) -> None:
         super().__init__()
+        if not 0.0 < scale < math.inf:
+            raise ValueError(f"scale must be positive and finite, not {scale!r}")
         self.d_model, self.d_inner, self.scale = d_model, expand * d_model, scale
         self.in_proj = nn.Linear(d_model, 4 * self.d_inner, bias=bias)
         self.out_proj = nn.Linear(self.d_inner, d_model, bias=bias)

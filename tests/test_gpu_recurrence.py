@@ -578,6 +578,15 @@ def test_refusals(R):
                         ("resume must be", (x, x, x, d, pool, s[:1], s[:2], torch.zeros(2, dtype=torch.bool).cuda()))):
         with pytest.raises(RuntimeError, match=match):
             R.recurrence_prompt(*args)
+    for scale in (-8.0, 0.0, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="scale must be positive"):
+            R.gated_recurrence(x[None], x[None], x[None], d, scale=scale)
+        with pytest.raises(RuntimeError, match="scale must be positive"):
+            R.recurrence_step(x, x, x, d, pool, s, scale=scale)
+        with pytest.raises(RuntimeError, match="scale must be positive"):
+            R.recurrence_prompt(x, x, x, d, pool, s[:1], torch.tensor([0, 6], dtype=torch.int32).cuda(), scale=scale)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            R.RecurrentMixer(8, scale=scale)
     leaf = x.clone().requires_grad_(True)
     with pytest.raises(RuntimeError, match="inference"):
         R.recurrence_step(leaf, x, x, d, pool, s)

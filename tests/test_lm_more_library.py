@@ -53,6 +53,12 @@ def test_recurrence_serving_checks_before_any_hip_call(name):
         assert _call(name, offsets=None) == (1, "recurrence_prompt: null pointer")
 
 
+@pytest.mark.parametrize("name", [f"ossm_recurrence_{w}" for w in ("forward", "backward", "prompt", "step")])
+def test_recurrence_needs_a_positive_scale(name):
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        assert _call(name, scale=scale) == (1, f"{name[5:]}: scale must be positive and finite")
+
+
 def test_sampler_checks_before_any_hip_call():
     name = "ossm_sample_logits"
     assert _call(name, dtype=2) == (1, "sample_logits: unknown dtype")
