@@ -13,9 +13,11 @@
 //   q = l dL/dl = a G l (h_{t-1} - a b / (1 - a^2)),   gr = q (1 - sigmoid(r)),   b = m g x
 //   gdecay = sigmoid(decay) / softplus(decay) sum of q
 //
-// It is bound by memory (a few bytes and some fifty operations an element), so each tensor is
-// read once: time is cut into chunks of T W steps, a workgroup of W waves takes a chunk of
-// 64 V channels (V a lane), wave w its steps from w T on.  Each wave folds its steps into
+// It is bound by memory, with the operations close behind: [4, 8192, 2048] in bf16 with a gate takes
+// 165 us forward, of which 134 are its bytes' at a copy's rate and 93 (57 percent of the cycles) VALU
+// issue; 301 backward, 242 and 160.  So each tensor is read once: time is cut into chunks
+// of T W steps, a workgroup of W waves takes a chunk of 64 V channels (V a lane),
+// wave w its steps from w T on.  Each wave folds its steps into
 // one (sum of l, state from zero), the waves are joined through LDS, and the chunk's start comes
 // from the chunks before it by records in the stream's scratch.  A chunk's place among P
 // neighbours is fixed: it waits for the aggregates of its neighbours before it and for the state
@@ -118,6 +120,7 @@ __device__ __forceinline__ float decay_rate(float decay, float scale) {
   return kLog2e * scale * (greatest(decay, 0.f) + 2.f * z * s);
 }
 
+// gdecay from the chunks' sums of q; 7 us at [4, 8192, 2048], 1024 sums a channel.
 __global__ __launch_bounds__(kSumThreads) void decay_grad_kernel(const float* partial, int n, int D, const float* decay, float* out) {
   const double t = column_sum(partial, n, D, D);
   const int i = static_cast<int>(blockIdx.x) * kSumColumns + threadIdx.x;
@@ -383,19 +386,22 @@ __global__ __launch_bounds__(W * 64) void recurrence_forward_kernel(Forward<E> g
   float rate[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) rate[k] = g.decay[ch + k];
-  Lane<E, V> x[T] = {}, in[T] = {}, r[T] = {}, z[T] = {};
-  if (!PACKED || g.L > 0) {
+  Lane<E, V> x[T], in[T], r[T], z[T];
+  // Without a condition, also for prompts of no rows, which load some row and use nothing of it:
+  // behind one, 16-bit elements are held one a register (168 of them against 120, 3 waves a SIMD).
+  const auto row_of = [&](int k) {
+    const int t = min(t0 + k, g.L - 1);
+    return row0 + (PACKED ? max(t, 0) : t);
+  };
 #pragma unroll
-    for (int k = 0; k < T; ++k) {
-      const long long row = row0 + min(t0 + k, g.L - 1);
-      r[k] = lane_load<E, V>(g.r + row * g.ld_r, ch);
-      in[k] = lane_load<E, V>(g.i + row * g.ld_i, ch);
-      x[k] = lane_load<E, V>(g.x + row * g.ld_x, ch);
-    }
-#pragma unroll
-    for (int k = 0; k < T; ++k)
-      if (GATE) z[k] = lane_load<E, V>(g.z + (row0 + min(t0 + k, g.L - 1)) * g.ld_z, ch);
+  for (int k = 0; k < T; ++k) {
+    r[k] = lane_load<E, V>(g.r + row_of(k) * g.ld_r, ch);
+    in[k] = lane_load<E, V>(g.i + row_of(k) * g.ld_i, ch);
+    x[k] = lane_load<E, V>(g.x + row_of(k) * g.ld_x, ch);
   }
+#pragma unroll
+  for (int k = 0; k < T; ++k)
+    if (GATE) z[k] = lane_load<E, V>(g.z + row_of(k) * g.ld_z, ch);
   const int lo = PACKED && g.n_seqs > 0 ? g.offsets[0] : 0, hi = PACKED && g.n_seqs > 0 ? g.offsets[g.n_seqs] : 0;
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (PACKED) {
@@ -429,9 +435,6 @@ __global__ __launch_bounds__(W * 64) void recurrence_forward_kernel(Forward<E> g
   }
 #pragma unroll
   for (int k = 0; k < T; ++k) {
-    const int first = PACKED ? __builtin_amdgcn_readfirstlane(s_first[w * T + k]) : 0;
-    float init[V];
-    if (PACKED && first != 0) prompt_start<E, V>(g, first - 1, ch, init);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       // past the end l is zero, and the state stays
@@ -439,14 +442,29 @@ __global__ __launch_bounds__(W * 64) void recurrence_forward_kernel(Forward<E> g
       float rest;
       decay_of<kFull>(l, a[k][v], rest);
       b[k][v] = __builtin_amdgcn_sqrtf(rest) * (sigmoid_of<kFull>(to_f(in[k].v[v])) * to_f(x[k].v[v]));
-      if (PACKED && first != 0) {
-        b[k][v] = fmaf(a[k][v], init[v], b[k][v]);
-        a[k][v] = -1.f;  // nothing before counts
-        sum[v] = -__builtin_inff();
-        h[v] = b[k][v];
+      sum[v] += l;
+      h[v] = fmaf(a[k][v], h[v], b[k][v]);
+    }
+  }
+  // which of the wave's tokens start and end a prompt
+  const unsigned long long firsts = PACKED ? __ballot(lane < T && s_first[w * T + lane % T] != 0) : 0;
+  const unsigned long long finals = PACKED ? __ballot(lane < T && s_final[w * T + lane % T] != 0) : 0;
+  if (firsts != 0) {
+    // apart from the loop above: a branch at each of its steps cost 4 percent of a long batch
+#pragma unroll
+    for (int k = 0; k < T; ++k) {
+      if (firsts >> k & 1) {
+        float init[V];
+        prompt_start<E, V>(g, __builtin_amdgcn_readfirstlane(s_first[w * T + k]) - 1, ch, init);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h[v] = b[k][v] = fmaf(a[k][v], init[v], b[k][v]);
+          a[k][v] = -1.f;  // nothing before counts
+          sum[v] = -__builtin_inff();
+        }
       } else {
-        sum[v] = sum[v] == -__builtin_inff() ? sum[v] : sum[v] + l;
-        h[v] = fmaf(a[k][v], h[v], b[k][v]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][v], h[v], b[k][v]);
       }
     }
   }
@@ -479,8 +497,7 @@ __global__ __launch_bounds__(W * 64) void recurrence_forward_kernel(Forward<E> g
     }
     if (active) lane_store<E, V>(g.y + (row0 + t0 + k) * g.D, ch, out);
     if constexpr (PACKED) {
-      const int final = __builtin_amdgcn_readfirstlane(s_final[w * T + k]);
-      if (final != 0) prompt_end<E, V>(g, final - 1, ch, active, carry);
+      if (finals >> k & 1) prompt_end<E, V>(g, __builtin_amdgcn_readfirstlane(s_final[w * T + k]) - 1, ch, active, carry);
     } else if (t0 + k == g.L - 1 && active) {
 #pragma unroll
       for (int v = 0; v < V; ++v) g.last[static_cast<size_t>(seq) * g.D + ch + v] = carry[v];
@@ -659,6 +676,8 @@ __global__ __launch_bounds__(W * 64) void recurrence_backward_kernel(Backward<E>
 }
 
 // ---- single tokens ------------------------------------------------------------------------
+// A channel or two a lane and no loop: the latency of three dependent loads (slot, state) is all there
+// is, 3.4 us at [32, 2048]; every lane forms its own decay's rate.
 template <class E, int V, bool GATE>
 __global__ __launch_bounds__(256) void recurrence_step_kernel(Forward<E> g) {
   constexpr bool kFull = sizeof(E) == 4;
@@ -731,16 +750,19 @@ int forward_tile(Forward<E> g, StreamCall& call) {
 // Steps a wave, waves and neighbours by how many groups of 64 V channels there are.  Few: the
 // chunks' chain is what takes time, so chunks are long and many are joined at once.  Many: workgroups
 // are small, so that some load while others compute or wait.  us, forward with a gate:
-//   bf16, T W P    8 16 16   16 4 4  |  f32          8 16 16   16 8 16   16 4 4
-//   16384 x 512       37.8     83.2  |  25600 x 128     24.7      27.9     93.6
-//   16384 x 2048     111      112    |  8192 x 1024     43.0      44.6     58.3
-//   4 x 8192 x 2048  208      165    |  2 x 8192 x 2048  155      136      151
+//   bf16, T W P    8 16 16   16 4 8   16 4 4  |  f32          8 16 16   16 8 16   16 4 4
+//   16384 x 512       37.8              83.2  |  25600 x 128     24.7      27.9     93.6
+//   16384 x 2048     111      108      114    |  8192 x 1024     43.0      44.6     58.3
+//   65536 x 2048              344      385    |  2 x 8192 x 2048  155      136      151
+//   2 x 8192 x 2048           101       99    |
+//   4 x 8192 x 2048  208      166      163    |
 template <class E, bool PACKED>
 int forward(Forward<E> g, StreamCall& call) {
   if constexpr (sizeof(E) == 2) {
     const bool pairs = in_pairs<E>(g.D, {g.ld_x, g.ld_i, g.ld_r, g.z ? g.ld_z : 0}, {g.x, g.i, g.r, g.z, g.y});
     const int64_t groups = int64_t(g.B) * ((g.D + 127) / 128);
-    if (pairs && groups >= 16) return forward_tile<E, 2, 16, 4, 4, PACKED>(g, call);
+    if (pairs && groups >= 32) return forward_tile<E, 2, 16, 4, 4, PACKED>(g, call);
+    if (pairs && groups >= 16) return forward_tile<E, 2, 16, 4, 8, PACKED>(g, call);
     if (pairs) return forward_tile<E, 2, 8, 16, 16, PACKED>(g, call);
   }
   return forward_tile<E, 1, 16, 8, 16, PACKED>(g, call);
@@ -911,6 +933,10 @@ int ossm_recurrence_prompt(int dtype, const void* x, int64_t ld_x, const void* i
     g.offsets = offsets, g.resume = resume;
     g.n_seqs = static_cast<int>(n_seqs), g.n_slots = static_cast<int>(n_slots);
     g.B = 1, g.L = static_cast<int>(rows), g.D = static_cast<int>(dim);
+    if (rows == 0) {  // the kernel loads before it looks at the length: from a row that is there
+      g.x = g.i = g.r = reinterpret_cast<const E*>(decay);
+      if (g.z != nullptr) g.z = g.x;
+    }
     return forward<E, true>(g, call);
   };
   return dtype == OSSM_BF16 ? go(bf16_t{}) : go(0.f);
