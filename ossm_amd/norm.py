@@ -32,19 +32,25 @@ def _separate(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], b
     return y if residual is None else (y, s)
 
 
+def _dense_like(t: Tensor) -> Tensor:
+    """An empty dense tensor as ``t``; a call with sizes, type and device takes a microsecond longer."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _forward(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float, save: bool):
     T, D = x.shape
     x, residual = _matrix(x), None if residual is None else _matrix(residual)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    y = torch.empty((T, D), dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     s = None if residual is None else torch.empty_like(y)
-    mean, rstd = (torch.empty(T, dtype=torch.float32, device=x.device) if save else None for _ in range(2))
+    stats = torch.empty((2, T), dtype=torch.float32, device=x.device) if save else None  # mean, rstd
+    mean = _lib.ptr(stats)
     if y.numel() > 0:
         wt = weight if weight is not None else bias
         _lib.run(_lib.load().ossm_layer_norm_forward, x, _lib.LM_DTYPES[x.dtype], _lib.LM_DTYPES[(x if wt is None else wt).dtype],
                  x.data_ptr(), _ld(x), _lib.ptr(residual), 0 if residual is None else _ld(residual), _lib.ptr(weight),
-                 _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(s), _lib.ptr(mean), _lib.ptr(rstd), T, D)
-    return y, s, mean, rstd
+                 _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(s), mean, None if mean is None else mean + 4 * T, T, D)
+    return y, s, stats
 
 
 class LayerNormFn(torch.autograd.Function):
@@ -53,15 +59,15 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor],  # type: ignore[override]
                 eps: float):
-        y, s, mean, rstd = _forward(x, residual, weight, bias, eps, True)
+        y, s, stats = _forward(x, residual, weight, bias, eps, True)
         ctx.eps, ctx.has_residual = eps, residual is not None
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if s is None else s, weight, bias, mean, rstd)
+        ctx.save_for_backward(x if s is None else s, weight, bias, stats)
         return y if s is None else (y, s)
 
     @staticmethod
     def backward(ctx, gy: Optional[Tensor], gs: Optional[Tensor] = None):  # type: ignore[override]
-        s, weight, bias, mean, rstd = ctx.saved_tensors
+        s, weight, bias, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():
             # create_graph: differentiable again, as separate steps on the sum
@@ -80,14 +86,18 @@ class LayerNormFn(torch.autograd.Function):
         s, gy = _matrix(s), _matrix(gy)
         gs = None if gs is None else _matrix(gs)
         weight = None if weight is None else weight.contiguous()
-        make = torch.empty if s.numel() > 0 else torch.zeros
-        ds = make((T, D), dtype=s.dtype, device=s.device) if need[0] or need[1] else None
         wt = weight if weight is not None else bias
-        dw, db = (make((D,), dtype=wt.dtype, device=s.device) if n else None for n in need[2:4])
-        if s.numel() > 0:
+        ds = _dense_like(s) if need[0] or need[1] else None
+        dw, db = (_dense_like(wt) if n else None for n in need[2:4])
+        if s.numel() == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        else:
+            mean = stats.data_ptr()
             _lib.run(_lib.load().ossm_layer_norm_backward, s, _lib.LM_DTYPES[s.dtype],
                      _lib.LM_DTYPES[(s if wt is None else wt).dtype], gy.data_ptr(), _ld(gy), _lib.ptr(gs),
-                     0 if gs is None else _ld(gs), s.data_ptr(), _ld(s), _lib.ptr(weight), mean.data_ptr(), rstd.data_ptr(),
+                     0 if gs is None else _ld(gs), s.data_ptr(), _ld(s), _lib.ptr(weight), mean, mean + 4 * T,
                      _lib.ptr(ds), _lib.ptr(dw), _lib.ptr(db), T, D)
         return ds if need[0] else None, ds if need[1] else None, dw, db, None
 
@@ -119,7 +129,7 @@ def _apply(what: str, x: Tensor, residual: Optional[Tensor], weight: Optional[Te
         out = LayerNormFn.apply(*two, weight, bias, float(eps))
         y, s = (out, None) if residual is None else out
     else:
-        y, s, _, _ = _forward(*two, weight, bias, float(eps), False)
+        y, s, _ = _forward(*two, weight, bias, float(eps), False)
     return (y, s) if x.dim() == 2 else (y.view(x.shape), None if s is None else s.view(x.shape))
 
 

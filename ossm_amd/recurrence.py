@@ -81,7 +81,7 @@ def _forward(x, i, r, z, decay, start, scale: float, save: bool):
     lib = _lib.load()
     keep, args = _pairs(x, i, r, z)
     decay, start = decay.contiguous(), None if start is None else start.contiguous()
-    y = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     last = torch.empty((B, D), dtype=torch.float32, device=x.device)
     saved = torch.empty(lib.ossm_recurrence_saved(B, L, D), dtype=torch.float32, device=x.device) if save else None
     if y.numel() > 0:
@@ -133,7 +133,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
             return (*(next(got) if n else None for n in need[:6]), None)
         if gy is None:
             gy = torch.zeros_like(x)
-        grads = [None if t is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for t in (x, i, r, z)]
+        grads = [None if t is None else torch.empty_like(x, memory_format=torch.contiguous_format) for t in (x, i, r, z)]
         gdecay, gstart = _backward(x, i, r, z, decay, gy, glast, saved, grads, ctx.scale, need[4], need[5])
         return (*(g if n else None for g, n in zip(grads, need)), gdecay, gstart, None)
 
