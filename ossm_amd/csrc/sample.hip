@@ -15,9 +15,9 @@
 // twenty operations, at the rate of float32's.
 //
 // A workgroup takes a row, in passes over it (from the caches after the first) that are bound by
-// the operations an entry takes, not by memory: [256, 131072] in bf16 is 100 us, 14 at a copy's
+// the operations an entry takes, not by memory: [256, 131072] in bf16 is 92 us, 14 at a copy's
 // rate, and its slowest row's cycles are 20 thousand for the largest logit, 27 for the counts, 90 for
-// the weights, 20 for the rest.  One row of 50001 takes 23 us.
+// the weights, 20 for the rest.  One row of 50001 takes 20 us.
 //   top-k: of 1024 threads' own largest, the k-th is at least k logits' lower bound, and few more than
 //     k reach it: those are gathered in LDS, sorted, and hold all that is kept; the row is not
 //     looked at again.  For larger k (or where too many reach it) the row is counted in 8192 bins of equal
@@ -304,7 +304,12 @@ __device__ __forceinline__ void scan_threads(u64& w, uint32_t& n, Shared& s) {
   }
   if (lane == 63) s.wave_weight[wave] = w, s.wave_count[wave] = n;
   __syncthreads();
-  for (int v = 0; v < wave; ++v) w += s.wave_weight[v], n += s.wave_count[v];
+#pragma unroll
+  for (int v = 0; v < kWavesOf; ++v) {  // all are read, so that one does not wait for another
+    const u64 a = s.wave_weight[v];
+    const uint32_t b = s.wave_count[v];
+    if (v < wave) w += a, n += b;
+  }
   __syncthreads();
 }
 
@@ -487,14 +492,16 @@ __device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F in) {
   return hi;
 }
 
-// s.item[0 .. n - 1] in falling order, n up to kList, no two alike.  Up to kRanked of them by
-// counting the larger ones of each (64 items a wave, the others shared among the waves): three
-// barriers, 1000 cycles at 224 items.  More of them first go to 1024 buckets of equal width between
-// the largest and the least, and are ranked in their own.  Where many share one, they take a sorting
-// network (17000 cycles at 224 items, 43000 at 1123); a wave's pairs lie in 128 neighbouring items while
-// they are up to 64 apart, and need no other wave.
+// s.item[0 .. n - 1] in falling order, n up to PER a thread, no two alike.  Up to kRanked of them by
+// counting the larger ones of each (64 items a wave, the others shared among the waves): few barriers,
+// 2000 cycles at 5 items, 10000 at 226.  More of them first go to 1024 buckets of equal width between
+// the largest and the least (12000 at 5, 13000 at 226), and are ranked in their own.  Where many share
+// one, they take a sorting network (17000 at 224, 43000 at 1123); a wave's pairs lie in 128
+// neighbouring items while they are up to 64 apart, and need no other wave.
+template <int PER>
 __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
   const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid & 63;
+  if (n <= 1) return;
   if (n <= kRanked) {
     const uint32_t blocks = (n + 63) / 64, slices = kWavesOf / blocks;
     const uint32_t i = wave % blocks * 64 + lane, slice = wave / blocks;
@@ -519,9 +526,9 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
     __syncthreads();
     return;
   }
-  u64 mine[kPer], hi = 0, lo = ~0ull;
+  u64 mine[PER], hi = 0, lo = ~0ull;
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
+  for (int q = 0; q < PER; ++q) {
     const uint32_t i = tid + q * kThreads;
     mine[q] = i < n ? s.item[i] : 0;
     if (i >= n) continue;
@@ -542,9 +549,9 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
     lo = lo < s.wave_more[v] ? lo : s.wave_more[v];
   }
   const int shift = max(54 - __clzll(static_cast<long long>(hi - lo)), 0);  // hi > lo: ten bits stay
-  uint32_t place[kPer];
+  uint32_t place[PER];
 #pragma unroll
-  for (int q = 0; q < kPer; ++q)
+  for (int q = 0; q < PER; ++q)
     if (tid + q * kThreads < n) place[q] = atomicAdd(&s.bucket[(hi - mine[q]) >> shift], 1u);
   __syncthreads();
   uint32_t own = s.bucket[tid], end = own;
@@ -554,11 +561,11 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
     s.bucket[tid] = end - own;
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kPer; ++q)
+    for (int q = 0; q < PER; ++q)
       if (tid + q * kThreads < n) s.item[s.bucket[(hi - mine[q]) >> shift] + place[q]] = mine[q];
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
+    for (int q = 0; q < PER; ++q) {
       if (tid + q * kThreads >= n) continue;
       const uint32_t b = static_cast<uint32_t>((hi - mine[q]) >> shift);
       const uint32_t from = s.bucket[b], to = b + 1 < kBuckets ? s.bucket[b + 1] : n;
@@ -573,7 +580,7 @@ __device__ __forceinline__ void sort_items(uint32_t n, Shared& s) {
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kPer; ++q)
+    for (int q = 0; q < PER; ++q)
       if (tid + q * kThreads < n) s.item[place[q]] = mine[q];
     __syncthreads();
     return;
@@ -613,11 +620,14 @@ __device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float 
     for (int q = 0; q < kEach; ++q) bits |= (x[q] >= lo && (no_end || x[q] < end) ? 1u : 0u) << q;
     if (bits == 0) return;
     uint32_t i = atomicAdd(&s.listed, static_cast<uint32_t>(__popc(bits)));
+    while (bits != 0) {  // seldom more than one a lane
+      const int t = __builtin_ctz(bits);
+      float v = x[0];
 #pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      if ((bits >> q & 1) == 0) continue;
-      if (i < kList) s.item[i] = item_of<E>(x[q], static_cast<uint32_t>(at + q));
+      for (int q = 1; q < kEach; ++q) v = t == q ? x[q] : v;
+      if (i < kList) s.item[i] = item_of<E>(v, static_cast<uint32_t>(at + t));
       ++i;
+      bits &= bits - 1;
     }
   });
   __syncthreads();
@@ -626,10 +636,10 @@ __device__ __forceinline__ uint32_t gather(const E* row, int V, float lo, float 
   return n;
 }
 
-// The weights of the first n sorted items as running sums (this thread's PER from tid PER on) on
-// top of `before`; and the whole.
+// The weights of the first n sorted items as running sums (this thread's PER from tid PER on, `first`
+// the one before them) on top of `before`; and the whole.
 template <class E, int PER>
-__device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 before, u64 (&sum)[PER], Shared& s) {
+__device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 before, u64 (&sum)[PER], u64& first, Shared& s) {
   u64 w = 0;
   uint32_t none = 0;
 #pragma unroll
@@ -640,23 +650,25 @@ __device__ __forceinline__ u64 run_items(const Weights& wt, uint32_t n, u64 befo
   }
   const u64 mine = w;
   scan_threads(w, none, s);
-  u64 at = before + w - mine, all = before;
+  u64 at = first = before + w - mine, all = before;
   for (int v = 0; v < kWavesOf; ++v) all += s.wave_weight[v];
 #pragma unroll
   for (int k = 0; k < PER; ++k) sum[k] = at += sum[k];
   return all;
 }
 
-// The first of n running sums that reaches `target`, n where none does.
+// The first of n running sums that reaches `target`, which lies above what the first starts from;
+// n where none does.
 template <int PER>
-__device__ __forceinline__ uint32_t first_reaching(const u64 (&sum)[PER], uint32_t n, u64 target, Shared& s) {
+__device__ __forceinline__ uint32_t first_reaching(const u64 (&sum)[PER], u64 first, uint32_t n, u64 target, Shared& s) {
   __syncthreads();
   if (threadIdx.x == 0) s.at = static_cast<int>(n);
   __syncthreads();
 #pragma unroll
-  for (int k = PER - 1; k >= 0; --k) {
+  for (int k = 0; k < PER; ++k) {
     const uint32_t i = threadIdx.x * PER + k;
-    if (i < n && sum[k] >= target) atomicMin(&s.at, static_cast<int>(i));
+    if (i < n && sum[k] >= target && first < target) s.at = static_cast<int>(i);  // one thread's
+    first = sum[k];
   }
   __syncthreads();
   return static_cast<uint32_t>(s.at);
@@ -734,6 +746,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     if (tid == 0) g.tokens[r] = s.at;
     return;
   }
+  asm volatile("" ::"v"(u));  // here already: where it is used it would be waited for
   const uint32_t top = key_of(max);
   const bool infinite = max == __builtin_inff();  // it shares the answer with its like alone
   const Weights wt{(const __attribute__((address_space(3))) double*)s.powers, max, 1.4426950408889634074 / T, g.scale};
@@ -801,7 +814,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         } else if (in_bin <= kList) {
           const uint32_t n0 = gather(row, g.V, bin_start(bin), bin > 0 ? bin_start(bin - 1) : 0.f, bin == 0, s,
                                      [](int, const float (&)[kEach]) {});
-          sort_items(n0, s);
+          sort_items<kPer>(n0, s);
           kept = kept_to<E>(k - before - 1, n0, s);
           all_kept = true;
         }
@@ -811,13 +824,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   // the answer from the list, PER items a thread
   const auto from_list = [&](auto per) {
     constexpr int PER = decltype(per)::value;
-    sort_items(listed, s);
+    sort_items<PER>(listed, s);
     uint32_t n = min(k, listed);
-    u64 sum[PER];
-    u64 total = run_items<E, PER>(wt, n, 0, sum, s);
+    u64 sum[PER], first;
+    u64 total = run_items<E, PER>(wt, n, 0, sum, first, s);
     if (by_p) {
       const u64 part = part_of(p, total, true);
-      n = min(n, first_reaching<PER>(sum, n, part > 0 ? part : 1, s) + 1);
+      n = min(n, first_reaching<PER>(sum, first, n, part > 0 ? part : 1, s) + 1);
     }
     if (floor > 0.) {  // weights fall: the first that does not reach it
       __syncthreads();
@@ -835,12 +848,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     __syncthreads();
     for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = (s.item[i] & kIndexMask) << 32 | s.item[i] >> kIndexBits;
     __syncthreads();
-    sort_items(n, s);
+    sort_items<PER>(n, s);
     for (uint32_t i = tid; i < n; i += kThreads) s.item[i] = s.item[i] << 32 >> (32 - kIndexBits) | s.item[i] >> 32;
     __syncthreads();
-    total = run_items<E, PER>(wt, n, 0, sum, s);
+    total = run_items<E, PER>(wt, n, 0, sum, first, s);
     const u64 target = u < 1.f ? part_of(u, total, false) : total - 1;
-    const uint32_t at = first_reaching<PER>(sum, n, target + 1, s);
+    const uint32_t at = first_reaching<PER>(sum, first, n, target + 1, s);
     if (tid == 0) g.tokens[r] = item_index(s.item[at]);
   };
   if (listed <= kThreads) {
@@ -918,10 +931,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
           summed = 1;  // no last one is left out
         }
       } else if (n0 <= kList && above < part) {
-        sort_items(n0, s);
-        u64 sum[kPer];
-        run_items<E, kPer>(wt, n0, above, sum, s);
-        const uint32_t at = first_reaching<kPer>(sum, n0, part, s);
+        if (n0 <= kThreads) sort_items<1>(n0, s);
+        else sort_items<kPer>(n0, s);
+        u64 sum[kPer], first;
+        run_items<E, kPer>(wt, n0, above, sum, first, s);
+        const uint32_t at = first_reaching<kPer>(sum, first, n0, part, s);
         if (at < n0) {
           if (!some) {  // the gathered tokens' weights join those above them
             for (uint32_t i = tid; i <= at; i += kThreads) {
