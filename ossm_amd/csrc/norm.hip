@@ -103,6 +103,14 @@ __device__ __forceinline__ Row row_of(float2 sums, float inv, float eps) {
   return {rest, 1.f / sqrtf(fmaf(-rest, rest, sums.x * inv) + eps)};
 }
 
+// a b, rounded: the mean of gy w is taken off the same numbers that it is of.  Fused into the
+// difference, the product's rounding would stay behind, times rstd, which in a row of (nearly)
+// equal elements is eps^-1/2.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // RAGGED: D is no multiple of a vector, and rows share lines.
 template <class E, class WT, int G, int NV, bool RAGGED>
 __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g) {
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> 
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float n = (s[j].get(k) - mean) * rstd, o = gy[j].get(k), q = o * w[j][k];
+        const float n = (s[j].get(k) - mean) * rstd, o = gy[j].get(k), q = product(o, w[j][k]);
         dw[j][k] = fmaf(o, n, dw[j][k]);
         db[j][k] += o;
         m1 += q;
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_backward_kernel(Norm<E, WT> 
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           const float n = (s[j].get(k) - mean) * rstd;
-          t[k] = fmaf(rstd, fmaf(-n, m2, gy[j].get(k) * w[j][k] - m1), gs[j].get(k));  // no gs: zeros
+          t[k] = fmaf(rstd, fmaf(-n, m2, product(gy[j].get(k), w[j][k]) - m1), gs[j].get(k));  // no gs: zeros
         }
         out.set(t);
         out.template store<!RAGGED>(g.gx + r * g.D + at, left_of(at));
@@ -401,7 +409,7 @@ __global__ __launch_bounds__(kMaxThreads) void long_backward_kernel(Norm<E, WT> 
       load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float q = v[1].get(k) * w[0][k];
+        const float q = product(v[1].get(k), w[0][k]);
         m1 += q;
         m2 = fmaf(q, (v[0].get(k) - mean) * rstd, m2);
       }
@@ -414,7 +422,7 @@ __global__ __launch_bounds__(kMaxThreads) void long_backward_kernel(Norm<E, WT> 
       load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
 #pragma unroll
       for (int k = 0; k < W; ++k)
-        t[k] = fmaf(rstd, fmaf(-(v[0].get(k) - mean) * rstd, m2, v[1].get(k) * w[0][k] - m1), v[2].get(k));
+        t[k] = fmaf(rstd, fmaf(-(v[0].get(k) - mean) * rstd, m2, product(v[1].get(k), w[0][k]) - m1), v[2].get(k));
       v[0].set(t);
       v[0].template store<false>(g.gx + r * g.D + at, n);
     });

@@ -149,6 +149,27 @@ def test_far_from_zero_and_constant_rows(N):
     assert torch.equal(y[2], b)
 
 
+def test_gradients_of_equal_elements(N):
+    """With every element equal, nothing but the sum's own gradient is left of a row where the
+    gradients times the weights are equal too: their mean is exact at 1, 2 and 64 columns (sums of equal
+    numbers by pairs), and at 3 off by at most 2 U of it, which rstd = eps^-1/2 carries."""
+    for D in (1, 2, 3, 64):
+        for dtype in (torch.float32, torch.bfloat16):
+            announce(f"norm of equal elements {D} {dtype}")
+            rng = np.random.default_rng(D)
+            one = lambda *shape: torch.tensor(rng.normal(size=shape)).to(dtype).cuda()  # noqa: E731
+            x, gy, gs = one(500, 1).repeat(1, D), one(500, 1).repeat(1, D), one(500, D)
+            res = torch.zeros_like(x)
+            w, b = one(1).float().repeat(D), one(D).float()
+            leaves = [t.requires_grad_(True) for t in (x, res, w, b)]
+            y, s = N.add_layer_norm(*leaves)
+            got = torch.autograd.grad([y, s], leaves[:2], [gy, gs])
+            most = 0.0 if D != 3 else 2 * U * EPS ** -0.5 * float((gy.float() * w.detach()).abs().max())
+            for g in got:
+                off = (g.double() - gs.double()).abs()
+                assert bool((off <= most * (1 + 2 * U) + (0 if D != 3 else torch.finfo(dtype).eps / 2) * (gs.double().abs() + most)).all()), (D, dtype, float(off.max()))
+
+
 def test_rows_do_not_reach_one_another(N):
     """A row with NaN or infinities gives NaN, the others what they give alone."""
     for D in (24, 128, 2048, 5000, 20000):
