@@ -60,7 +60,7 @@ class LayerNormFn(torch.autograd.Function):
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor],  # type: ignore[override]
                 eps: float):
         y, s, stats = _forward(x, residual, weight, bias, eps, True)
-        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x if s is None else s, weight, bias, stats)
         return y if s is None else (y, s)
