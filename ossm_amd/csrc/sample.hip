@@ -814,8 +814,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         } else if (in_bin <= kList) {
           const uint32_t n0 = gather(row, g.V, bin_start(bin), bin > 0 ? bin_start(bin - 1) : 0.f, bin == 0, s,
                                      [](int, const float (&)[kEach]) {});
-          sort_items<kPer>(n0, s);
-          kept = kept_to<E>(k - before - 1, n0, s);
+          // the last bin counts entries below `lowest` too, which are not gathered: where the k-th is one
+          // of those, all that weighs anything is kept
+          if (k - before <= n0) {
+            sort_items<kPer>(n0, s);
+            kept = kept_to<E>(k - before - 1, n0, s);
+          }
           all_kept = true;
         }
       }
@@ -1113,7 +1117,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
     if (lane >= o) sum += a;
   }
   const u64 past = __ballot(sum > target);
-  if (past == 0 || lane != __builtin_ctzll(past)) return;
+  if (past == 0) {  // nothing is kept: never, but a token is written on every path
+    if (lane == 0) g.tokens[r] = -1;
+    return;
+  }
+  if (lane != __builtin_ctzll(past)) return;
   target -= sum - own;
   int q = 0;
   u64 acc = w[0];

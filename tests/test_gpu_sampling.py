@@ -304,3 +304,33 @@ def test_refusals(S):
         with pytest.raises(RuntimeError, match=match):
             S.sample_logits(**{"logits": x, "uniform": u, **kw})
     assert S.sample_logits(x[:0], u[:0]).shape == (0,)
+
+
+def below_the_bins():
+    """Rows of which a large top-k reaches entries that weigh nothing: masked with finite values, or
+    far below at a low temperature.  (name, row, temperature, k)"""
+    rng = np.random.default_rng(93)
+
+    def masked(allowed, others, value):
+        row = np.full(allowed + others, value)
+        row[rng.permutation(allowed + others)[:allowed]] = rng.normal(size=allowed)
+        return row
+
+    return [("masked -1e9", masked(900, 3600, -1e9), 1.0, 1000), ("masked -1e4", masked(5000, 3000, -1e4), 1.0, 6000),
+            ("masked -1e9, most allowed", masked(5000, 1000, -1e9), 1.0, 5500), ("masked lowest", masked(5000, 1000, -3.38e38), 1.0, 5001),
+            ("masked, k the last", masked(4200, 400, -1e9), 2.0, 4599), ("low temperature", rng.normal(size=5000) * 3, 0.3, 4500),
+            ("lower temperature", rng.normal(size=8000), 0.13, 7990)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", range(7))
+def test_top_k_past_what_weighs_anything(S, case, dtype):
+    name, row, t, k = below_the_bins()[case]
+    announce(f"sample_logits {name} {dtype}")
+    n = 20
+    x = torch.tensor(np.stack([row] * n)).to(dtype).cuda()
+    u = (np.arange(n) + 0.5) / n
+    part = np.array([0.05, 0.5, 0.9, 0.999] * 5)
+    for kw in ({}, {"top_p": part}, {"min_p": 0.2}, {"top_p": part, "min_p": 0.01}):
+        out = torch.full((n,), -77, dtype=torch.int64, device="cuda")
+        check(S, x, u, t, k, out=out, **kw)
