@@ -396,12 +396,13 @@ __device__ __forceinline__ Kept select(const E* row, int V, const Weights& wt, u
 }
 
 // The row's bins: of equal width in the logits from the largest down, to about where weights are
-// nothing or the row ends; the last takes all below it.
+// nothing or the row ends; the last takes all below it down to `lowest`.  What lies lower weighs
+// nothing and is in none, so that a bin's count is the number of entries from its start on.
 struct Bins {
-  float top, scale;
-  __device__ __forceinline__ uint32_t of(float v) const {  // kBins: -inf and NaN
-    const float b = (top - v) * scale;
-    return b < 3e38f ? min(static_cast<uint32_t>(b), kBins - 1u) : kBins;
+  float top, scale, lowest;
+  __device__ __forceinline__ uint32_t of(float v) const {  // kBins: below `lowest`, -inf and NaN
+    // the least of two is the number where the other is NaN: an infinite difference at scale 0
+    return v >= lowest ? static_cast<uint32_t>(fminf((top - v) * scale, kBins - 1.f)) : kBins;
   }
 };
 
@@ -760,7 +761,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
   // weights are nothing from 47.5 ln 2 T on
   const float range = fminf(low < max ? max - low : __builtin_inff(), 33.f * T) * 1.00001f;
   const bool even = range < 1e37f;  // else the bins' width is no number
-  const Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f};
+  const Bins bins{max, range > 1e-30f ? static_cast<float>(kBins) / range : 0.f, value_of(lowest)};
   const auto bin_start = [&](uint32_t b) {  // the least value of bin b and those before
     return value_of(least_key(lowest, top, [&](float v) { return bins.of(v) <= b; }));
   };
@@ -814,12 +815,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const E* logits, Sampl
         } else if (in_bin <= kList) {
           const uint32_t n0 = gather(row, g.V, bin_start(bin), bin > 0 ? bin_start(bin - 1) : 0.f, bin == 0, s,
                                      [](int, const float (&)[kEach]) {});
-          // the last bin counts entries below `lowest` too, which are not gathered: where the k-th is one
-          // of those, all that weighs anything is kept
-          if (k - before <= n0) {
-            sort_items<kPer>(n0, s);
-            kept = kept_to<E>(k - before - 1, n0, s);
-          }
+          sort_items<kPer>(n0, s);
+          kept = kept_to<E>(k - before - 1, n0, s);
           all_kept = true;
         }
       }

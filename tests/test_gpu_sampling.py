@@ -334,3 +334,19 @@ def test_top_k_past_what_weighs_anything(S, case, dtype):
     for kw in ({}, {"top_p": part}, {"min_p": 0.2}, {"top_p": part, "min_p": 0.01}):
         out = torch.full((n,), -77, dtype=torch.int64, device="cuda")
         check(S, x, u, t, k, out=out, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_rows_whose_every_eighth_entry_is_alike(S, dtype):
+    """Every eighth entry within 1e-27 of the largest and the others 1e13 below, at a temperature at which they
+    weigh as much: top-k counts them all."""
+    V, n = 8000, 16
+    row = np.full(V, -1e13)
+    row[::8] = 0.0
+    row[0] = 1e-27
+    x = torch.tensor(np.stack([row] * n)).to(dtype).cuda()
+    u = np.append((np.arange(n - 1) + 0.5) / n, 1 - 2.0 ** -24)
+    announce(f"sample_logits every eighth alike {dtype}")
+    for k in (1000, 1001, 5000, 7999):
+        check(S, x, u, 1e13, k)
+        check(S, x, u, 1e14, k, 0.9)
