@@ -350,3 +350,35 @@ def test_rows_whose_every_eighth_entry_is_alike(S, dtype):
     for k in (1000, 1001, 5000, 7999):
         check(S, x, u, 1e13, k)
         check(S, x, u, 1e14, k, 0.9)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_parts_next_to_one(S, dtype):
+    """A top-p whose border lies in the tail of a large vocabulary, past what a list holds."""
+    announce(f"sample_logits p next to one {dtype}")
+    rng = np.random.default_rng(94)
+    part = np.array([0.9995, 0.99999, 1 - 2.0 ** -24, 0.9994, 0.9996, 0.999])
+    for V in (50001, 131072):
+        x = torch.tensor(rng.normal(size=(6, V)) * 1.5).to(dtype).cuda()
+        for u in (rng.random(6), np.full(6, 1 - 2.0 ** -24)):
+            check(S, x, u, 1.0, 0, part)
+            check(S, x, u, 1.3, V - 100, part)
+            check(S, x, u, 1.0, 0, part, 1e-5)
+
+
+def test_random_numbers_at_the_borders_of_unequal_weights(S):
+    """u next to each running sum of unequal weights, below and above: the token before and the one
+    after.  The kernel's sums are off by less than 4 units of 2^-46 of the largest weight; no u is that
+    near a sum, which is checked in extended precision first."""
+    for values in ([1.0, 2.0, 4.0, 1.0], [3.0, 5.0, 7.0, 0.01, 11.0, 1e-4], [0.3, 0.2, 0.1]):
+        row = np.log(np.array(values)).astype(np.float32).astype(np.longdouble)
+        w = np.exp(row - row.max())
+        cum = np.cumsum(w) / w.sum()
+        below = np.array([np.float32(c) if np.float32(c) < c else np.nextafter(np.float32(c), np.float32(0)) for c in cum[:-1]])
+        u = np.stack([below, np.nextafter(below, np.float32(1))], 1).reshape(-1)
+        assert np.abs(u[:, None].astype(np.longdouble) - cum[None]).min() > 2.0 ** -40
+        want = [i // 2 + i % 2 for i in range(2 * len(below))]
+        x = torch.tensor(np.stack([row] * len(u)).astype(np.float32)).cuda()
+        announce(f"sample_logits at the borders of {values}")
+        assert check(S, x, u).tolist() == want
+        assert check(S, x, u, 1.0, len(values)).tolist() == want
