@@ -93,14 +93,23 @@ __device__ __forceinline__ void load_weights(const WT* p, int D, int lane, float
   }
 }
 
-// A row's mean is rounded to its own size, which the deviations of a row far from zero
-// would all carry: their own mean, `rest`, is taken off again.
+// Sums are of the elements less the row's first one, the pivot: in a row far from zero, whose elements
+// differ little, those differences are exact, and zero where all are equal.  (With the rounding of a mean
+// of the elements themselves in every deviation, its square could pass the variance and eps: NaN
+// at equal elements of 2e8.)  The mean of the differences is rounded too, which the deviations from it
+// all carry: their own mean, `rest`, is taken off again.
 struct Row {
   float rest, rstd;
 };
 __device__ __forceinline__ Row row_of(float2 sums, float inv, float eps) {
   const float rest = sums.y * inv;
   return {rest, 1.f / sqrtf(fmaf(-rest, rest, sums.x * inv) + eps)};
+}
+
+// The first element of row r, of the sum where there is a residual.
+template <class E, class WT>
+__device__ __forceinline__ float pivot_of(const Norm<E, WT>& g, E x, E residual) {
+  return g.residual != nullptr ? to_f(from_f<E>(to_f(x) + to_f(residual))) : to_f(x);
 }
 
 // a b, rounded: the mean of gy w is taken off the same numbers that it is of.  Fused into the
@@ -127,8 +136,13 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
   Vec<E, W> raw[NV], res[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) raw[j].zero(), res[j].zero();
+  E first{}, res_first{};
   const auto fetch = [&](long long row) {
     if (row >= g.rows) return;
+    if constexpr (G >= 64) {  // fewer lanes hand on the first one's
+      first = g.x[row * g.ld_x];
+      if (g.residual != nullptr) res_first = g.residual[row * g.ld_res];
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * G + lane) * W;
@@ -154,9 +168,16 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
         raw[j].set(t);
         raw[j].template store<!RAGGED>(g.sum + r * g.D + at, left_of(at));
       }
+    }
+    float pivot;
+    if constexpr (G >= 64) pivot = pivot_of(g, first, res_first);
+    else pivot = __shfl(raw[0].get(0), 0, G);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = (j * G + lane) * W;
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        v[j][k] = raw[j].get(k);
+        v[j][k] = at + k < g.D ? raw[j].get(k) - pivot : 0.f;
         total += v[j][k];
       }
     }
@@ -174,7 +195,7 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
       }
     const Row row = row_of(row_sums<G>(square, rest, s_sum), inv, g.eps);
     if (lane == 0 && g.mean != nullptr) {
-      g.mean[r] = mean + row.rest;
+      g.mean[r] = pivot + (mean + row.rest);
       g.rstd[r] = row.rstd;
     }
 #pragma unroll
@@ -348,6 +369,7 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
   const float inv = 1.f / static_cast<float>(g.D);
   for (long long r = blockIdx.x; r < g.rows; r += gridDim.x) {
     const E* in[1] = {g.x + r * g.ld_x};
+    const float pivot = pivot_of(g, *in[0], g.residual != nullptr ? g.residual[r * g.ld_res] : E{});
     float total = 0.f;
     if (g.residual != nullptr) {
       const E* const both[2] = {in[0], g.residual + r * g.ld_res};
@@ -357,14 +379,14 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
         for (int k = 0; k < W; ++k) t[k] = v[0].get(k) + v[1].get(k);
         v[0].set(t);
 #pragma unroll
-        for (int k = 0; k < W; ++k) total += v[0].get(k);
+        for (int k = 0; k < W; ++k) total += k < n ? v[0].get(k) - pivot : 0.f;
         v[0].template store<false>(g.sum + r * g.D + at, n);
       });
       in[0] = g.sum + r * g.D;  // a thread reads back its own elements
     } else {
-      each_vector(in, g.D, [&](int, int, Vec<E, W>(&v)[1]) {
+      each_vector(in, g.D, [&](int, int n, Vec<E, W>(&v)[1]) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) total += v[0].get(k);
+        for (int k = 0; k < W; ++k) total += k < n ? v[0].get(k) - pivot : 0.f;
       });
     }
     const float mean = row_sums<kMaxThreads>(total, 0.f, s_sum).x / static_cast<float>(g.D);
@@ -372,14 +394,14 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
     each_vector(in, g.D, [&](int, int n, Vec<E, W>(&v)[1]) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float c = k < n ? v[0].get(k) - mean : 0.f;
+        const float c = k < n ? v[0].get(k) - pivot - mean : 0.f;
         square = fmaf(c, c, square);
         rest += c;
       }
     });
     const Row row = row_of(row_sums<kMaxThreads>(square, rest, s_sum), inv, g.eps);
     if (threadIdx.x == 0 && g.mean != nullptr) {
-      g.mean[r] = mean + row.rest;
+      g.mean[r] = pivot + (mean + row.rest);
       g.rstd[r] = row.rstd;
     }
     each_vector(in, g.D, [&](int at, int n, Vec<E, W>(&v)[1]) {
@@ -387,7 +409,7 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
       load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
       load_weights<WT, 1, W, kMaxThreads>(g.bias, g.D, at / W, 0.f, b);
 #pragma unroll
-      for (int k = 0; k < W; ++k) t[k] = fmaf((v[0].get(k) - mean - row.rest) * row.rstd, w[0][k], b[0][k]);
+      for (int k = 0; k < W; ++k) t[k] = fmaf((v[0].get(k) - pivot - mean - row.rest) * row.rstd, w[0][k], b[0][k]);
       v[0].set(t);
       v[0].template store<false>(g.y + r * g.D + at, n);
     });

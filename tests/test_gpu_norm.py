@@ -386,3 +386,49 @@ def test_refusals(N):
     announce("layer norm with tangents")
     with torch.no_grad(), forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangent"):
         N.layer_norm(forward_ad.make_dual(x, torch.ones_like(x)), w, w)
+
+
+def test_float32_rows_of_equal_large_elements(N):
+    """A constant row's deviations are all zero, whatever its value and length: y is the bias and
+    the gradient's factor is eps^-1/2.  ds = rstd (g - mean(g)) then, each term's roundings 16 U of it and
+    the mean's 64 U of the mean of |g|, as in `reference`."""
+    rng = np.random.default_rng(20)
+    for D in (3, 23, 100, 701, 7879, 15237, 40001):
+        T = 64
+        value = torch.tensor(np.exp(rng.uniform(np.log(1e3), np.log(1e11), size=(T, 1)))).float()
+        x = value.repeat(1, D).cuda()
+        half = (value / 2).repeat(1, D).cuda()  # exact: its double is the value
+        _, _, w, b, gy, gs = inputs(T, D, torch.float32, torch.float32, True, seed=D)
+        for eps in (1e-5, 1e-12):
+            announce(f"layer norm of equal large elements {D} {eps}")
+            y, _, (dx, _, dw, db) = run(N, x, None, w, b, gy, None, eps)
+            assert torch.equal(y, b.expand(T, D)), (D, eps, float((y - b).abs().max()))
+            g = f64(gy) * f64(w)
+            m1, a1 = g.mean(1, keepdims=True), np.abs(g).mean(1, keepdims=True)
+            root = np.float32(eps) ** np.float64(-0.5)
+            check(dx, (root * (g - m1), root * U * (16 * (np.abs(g) + np.abs(m1)) + 64 * a1)), "dx")
+            assert not dw.any()
+            y, s, _ = run(N, half, half, w, b, gy, gs, eps)
+            assert torch.equal(y, b.expand(T, D)) and torch.equal(s, x)
+
+
+def test_float32_rows_of_nearly_equal_large_elements(N):
+    """Elements a few units in the last place apart: their differences are exact, so the deviations
+    keep their digits.  A mean of differences of up to 5 units is off by 48 U of 5 units, and a
+    deviation's own rounding and the root's are 16 U of n, as in the module's derivation with the largest
+    difference in place of the largest element."""
+    rng = np.random.default_rng(21)
+    for D in (33, 701, 7879, 15237, 40001):
+        T = 24
+        base = np.float32(2.0) ** rng.integers(10, 36, size=(T, 1))
+        unit = base * 2.0 ** -23
+        x = torch.tensor(base * 1.5 + unit * rng.integers(-2, 4, size=(T, D))).float().cuda()
+        _, _, w, b, _, _ = inputs(T, D, torch.float32, torch.float32, False, seed=D)
+        announce(f"layer norm of nearly equal large elements {D}")
+        y = N.layer_norm(x, w, b, 1e-12)
+        s, w64, b64 = f64(x), f64(w), f64(b)
+        c = s - s.mean(1, keepdims=True)
+        rstd = 1 / np.sqrt((c ** 2).mean(1, keepdims=True) + float(np.float32(1e-12)))
+        n = c * rstd
+        dn = U * (48 * 5 * unit * rstd + 16 * np.abs(n))
+        check(y, (n * w64 + b64, dn * np.abs(w64) + 4 * U * (np.abs(n * w64) + np.abs(b64))), "y")
