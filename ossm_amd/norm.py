@@ -69,10 +69,10 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, gy: Optional[Tensor], gs: Optional[Tensor] = None):  # type: ignore[override]
         s, weight, bias, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
+        if gy is None:  # nothing reaches the norm, whose rows may be NaN
+            return gs if need[0] else None, gs if need[1] else None, None, None, None
         if torch.is_grad_enabled():
             # create_graph: differentiable again, as separate steps on the sum
-            if gy is None:
-                return gs if need[0] else None, gs if need[1] else None, None, None, None
             inputs = aliases(s, weight, bias)
             wanted = [t for t, n in zip(inputs, (need[0] or need[1], *need[2:4])) if n]
             got = iter(torch.autograd.grad(_separate(inputs[0], None, *inputs[1:], ctx.eps), wanted, gy, create_graph=True))
@@ -80,8 +80,6 @@ class LayerNormFn(torch.autograd.Function):
             if ds is not None and gs is not None:
                 ds = ds + gs
             return (ds if need[0] else None, ds if need[1] else None, *(next(got) if n else None for n in need[2:4]), None)
-        if gy is None:
-            gy = torch.zeros_like(s)
         T, D = s.shape
         s, gy = _matrix(s), _matrix(gy)
         gs = None if gs is None else _matrix(gs)

@@ -432,3 +432,16 @@ def test_float32_rows_of_nearly_equal_large_elements(N):
         n = c * rstd
         dn = U * (48 * 5 * unit * rstd + 16 * np.abs(n))
         check(y, (n * w64 + b64, dn * np.abs(w64) + 4 * U * (np.abs(n * w64) + np.abs(b64))), "y")
+
+
+def test_the_sum_alone_is_not_reached_by_the_norm(N):
+    """A loss of the sum alone: its gradient is the sum's own, also in rows whose norm is NaN, and
+    the weights get none."""
+    x, res, w, b, _, gs = inputs(4, 40, torch.float32, torch.float32, True, seed=22)
+    x[1, 3], x[2, 0] = float("inf"), float("nan")
+    announce("layer norm, the sum alone")
+    for graph in (False, True):
+        leaves = [t.clone().requires_grad_(True) for t in (x, res, w, b)]
+        _, s = N.add_layer_norm(*leaves)
+        dx, dres, dw, db = torch.autograd.grad(s, leaves, gs, allow_unused=True, create_graph=graph)
+        assert torch.equal(dx, gs) and torch.equal(dres, gs) and dw is None and db is None
