@@ -23,7 +23,7 @@ from . import decode
 from .gated import GatedFeedForward
 from .logits import control_logits, pack_allowed
 from .mamba import MambaMixer
-from .norm import LayerNorm
+from .norm import LayerNorm, norm_of_sum
 from .recurrence import RecurrentMixer, RecurrentState
 from .sampling import sample_logits
 
@@ -42,8 +42,8 @@ class _Block(nn.Module):
     def forward(self, x: Tensor, added: Optional[Tensor], mix=None) -> Tuple[Tensor, Tensor]:
         """The residual stream and what the block adds to it, from those of the block before
         (nothing added yet: None); each sum is taken with the norm that follows it."""
-        h, x = (self.norm1(x), x) if added is None else self.norm1(added, x)
-        h, x = self.norm2((mix or self.mixer)(h), x)
+        h, x = (self.norm1(x), x) if added is None else norm_of_sum(self.norm1, added, x)
+        h, x = norm_of_sum(self.norm2, (mix or self.mixer)(h), x)
         return x, self.feed_forward(h)
 
 
@@ -66,7 +66,7 @@ class MambaDecoder(nn.Module):
         self.norm = LayerNorm(d_model)
 
     def _logits(self, x: Tensor, added: Optional[Tensor]) -> Tensor:
-        h = self.norm(x) if added is None else self.norm(added, x)[0]
+        h = self.norm(x) if added is None else norm_of_sum(self.norm, added, x)[0]
         return F.linear(h, self.embedding.weight)
 
     def forward(self, tokens: Tensor) -> Tensor:

@@ -16,9 +16,9 @@ from torch import Tensor, nn
 
 from . import _lib
 from .gated import _ld, _matrix
-from .linear import aliases
+from .linear import aliases, calls_only
 
-__all__ = ["LayerNorm", "LayerNormFn", "add_layer_norm", "layer_norm"]
+__all__ = ["LayerNorm", "LayerNormFn", "add_layer_norm", "layer_norm", "norm_of_sum"]
 
 
 def _separate(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
@@ -156,3 +156,12 @@ class LayerNorm(nn.LayerNorm):
             raise RuntimeError(f"LayerNorm norms a last dimension of {tuple(self.normalized_shape)}, got {tuple(x.shape)}")
         y, s = _apply("LayerNorm", x, residual, self.weight, self.bias, self.eps)
         return y if residual is None else (y, s)
+
+
+def norm_of_sum(norm: nn.Module, x: Tensor, residual: Tensor) -> Tuple[Tensor, Tensor]:
+    """``(norm(s), s)`` with ``s = x + residual``: in one pass where ``norm`` is a ``LayerNorm``; a replaced
+    or hooked one is called as it is, on the sum."""
+    if calls_only(norm, LayerNorm):
+        return norm(x, residual)
+    s = x + residual
+    return norm(s), s

@@ -130,3 +130,64 @@ def test_refuses_unknown_mixers():
     for mixer in ("attention", ("mamba",), ("mamba", "recurrent", "mamba")):
         with pytest.raises(ValueError, match="mixer must be"):
             MambaDecoder(10, 16, 2, mixer=mixer)
+
+
+def small(mixer="mamba"):
+    from ossm_amd.decoder import MambaDecoder
+
+    torch.manual_seed(0)
+    return MambaDecoder(97, 64, 2, d_hidden=120, mixer=mixer).cuda()
+
+
+def stepwise(m, tokens):
+    """The model from its modules as they are, every sum on its own."""
+    x = m.embedding(tokens)
+    for b in m.blocks:
+        x = x + b.mixer(b.norm1(x))
+        x = x + b.feed_forward(b.norm2(x))
+    return torch.nn.functional.linear(m.norm(x), m.embedding.weight)
+
+
+class Halved(torch.nn.Module):
+    """A norm of a user's own."""
+
+    def forward(self, x):
+        return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-5) / 2
+
+
+@torch.random.fork_rng()
+def test_replaced_norms_are_called_as_they_are():
+    tokens = torch.randint(0, 97, (3, 20)).cuda()
+    for make in (lambda: torch.nn.LayerNorm(64).cuda(), lambda: torch.nn.RMSNorm(64).cuda(), Halved):
+        m = small()
+        m.blocks[0].norm1, m.blocks[0].norm2, m.blocks[1].norm1, m.norm = make(), make(), make(), make()
+        announce(f"decoder with {make().__class__.__name__}")
+        got, want = m(tokens), stepwise(m, tokens)
+        close(got, want)
+        params = [p for p in m.parameters() if p.requires_grad]
+        for p, q in zip(torch.autograd.grad(got.square().mean(), params), torch.autograd.grad(want.square().mean(), params)):
+            assert (p - q).abs().max() <= 1e-3 * q.abs().max()
+        states, slots = m.states(3), torch.arange(3).cuda()
+        close(m.prompt(tokens[:, :19].flatten(), 19 * torch.arange(4).cuda(), states, slots), want[:, 18])
+        close(m.step(tokens[:, 19], states, slots), want[:, 19])
+
+
+@torch.random.fork_rng()
+def test_hooks_on_norms_see_one_tensor():
+    """Hooks on norms are called with, and may replace, a tensor: what goes in and what comes out."""
+    tokens = torch.randint(0, 97, (2, 9)).cuda()
+    m = small()
+    seen = []
+
+    def hook(module, args, out):
+        assert len(args) == 1 and isinstance(args[0], torch.Tensor) and isinstance(out, torch.Tensor)
+        seen.append(module)
+        return out * 0.5
+
+    hooked = [m.blocks[0].norm2, m.blocks[1].norm1, m.norm]
+    for h in hooked:
+        h.register_forward_hook(hook)
+    announce("decoder with hooked norms")
+    got = m(tokens)
+    assert seen == hooked
+    close(got, stepwise(m, tokens))
