@@ -21,6 +21,7 @@ from torch import Tensor, nn
 
 from . import decode
 from .gated import GatedFeedForward
+from .linear import calls_only
 from .logits import control_logits, pack_allowed
 from .mamba import MambaMixer
 from .norm import LayerNorm, norm_of_sum
@@ -39,12 +40,23 @@ class _Block(nn.Module):
         self.mixer = mixer
         self.feed_forward = GatedFeedForward(d_model, d_hidden, activation=activation)
 
-    def forward(self, x: Tensor, added: Optional[Tensor], mix=None) -> Tuple[Tensor, Tensor]:
+    def forward(self, x: Tensor, mix=None) -> Tensor:
+        x, added = self.parts(x, None, mix)
+        return x + added
+
+    def parts(self, x: Tensor, added: Optional[Tensor], mix=None) -> Tuple[Tensor, Tensor]:
         """The residual stream and what the block adds to it, from those of the block before
         (nothing added yet: None); each sum is taken with the norm that follows it."""
         h, x = (self.norm1(x), x) if added is None else norm_of_sum(self.norm1, added, x)
         h, x = norm_of_sum(self.norm2, (mix or self.mixer)(h), x)
         return x, self.feed_forward(h)
+
+
+def _through(block: nn.Module, x: Tensor, added: Optional[Tensor], *mix) -> Tuple[Tensor, Optional[Tensor]]:
+    """``block`` on ``x + added``, as such a pair; a replaced or hooked one is called as it is."""
+    if calls_only(block, _Block):
+        return block.parts(x, added, *mix)
+    return block(x if added is None else x + added, *mix), None
 
 
 class MambaDecoder(nn.Module):
@@ -73,7 +85,7 @@ class MambaDecoder(nn.Module):
         """Logits [batch, length, vocab] of tokens [batch, length], differentiable."""
         x, added = self.embedding(tokens), None
         for block in self.blocks:
-            x, added = block(x, added)
+            x, added = _through(block, x, added)
         return self._logits(x, added)
 
     def states(self, slots: int) -> List[_State]:
@@ -93,7 +105,7 @@ class MambaDecoder(nn.Module):
                 mix = lambda h, b=block, s=state: b.mixer.prompt(h, s, slots, offsets, resume)  # noqa: E731
             else:
                 mix = lambda h, b=block, s=state: decode.prompt(b.mixer, h, s, slots, offsets, resume)  # noqa: E731
-            x, added = block(x, added, mix)
+            x, added = _through(block, x, added, mix)
         last = (offsets[1:] - 1).clamp(min=0).long()
         return self._logits(x[last], None if added is None else added[last])
 
@@ -106,7 +118,7 @@ class MambaDecoder(nn.Module):
                 mix = lambda h, b=block, s=state: b.mixer.step(h, s, slots)  # noqa: E731
             else:
                 mix = lambda h, b=block, s=state: decode.step(b.mixer, h, s, slots)  # noqa: E731
-            x, added = block(x, added, mix)
+            x, added = _through(block, x, added, mix)
         return self._logits(x, added)
 
     @torch.no_grad()

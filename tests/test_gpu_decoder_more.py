@@ -191,3 +191,37 @@ def test_hooks_on_norms_see_one_tensor():
     got = m(tokens)
     assert seen == hooked
     close(got, stepwise(m, tokens))
+
+
+class Twice(torch.nn.Module):
+    """A user's block without a mixer."""
+
+    def forward(self, x):
+        return 2 * x
+
+
+@torch.random.fork_rng()
+def test_blocks_take_and_give_the_residual_stream():
+    """A block by itself, hooked or replaced: one tensor in, one out."""
+    tokens = torch.randint(0, 97, (2, 9)).cuda()
+    m = small()
+    a, b = m.blocks
+    x = torch.randn(2, 9, 64).cuda()
+    announce("decoder's blocks")
+    y = x + a.mixer(a.norm1(x))
+    close(a(x), y + a.feed_forward(a.norm2(y)))
+    seen = []
+
+    def hook(module, args, out):
+        assert len(args) == 1 and isinstance(args[0], torch.Tensor) and isinstance(out, torch.Tensor)
+        seen.append(out)
+        return 0.5 * out
+
+    handle = a.register_forward_hook(hook)
+    head = lambda v: torch.nn.functional.linear(m.norm(v), m.embedding.weight)  # noqa: E731
+    got = m(tokens)
+    close(got, head(b(a(m.embedding(tokens)))))
+    close(seen[0], seen[1])
+    handle.remove()
+    m.blocks[0] = Twice()
+    close(m(tokens), head(b(2 * m.embedding(tokens))))
