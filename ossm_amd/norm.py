@@ -159,9 +159,12 @@ class LayerNorm(nn.LayerNorm):
 
 
 def norm_of_sum(norm: nn.Module, x: Tensor, residual: Tensor) -> Tuple[Tensor, Tensor]:
-    """``(norm(s), s)`` with ``s = x + residual``: in one pass where ``norm`` is a ``LayerNorm``; a replaced
-    or hooked one is called as it is, on the sum."""
-    if calls_only(norm, LayerNorm):
+    """``(norm(s), s)`` with ``s = x + residual``: in one pass where ``norm`` is a ``LayerNorm`` and both
+    are of one shape and type; a replaced or hooked one is called as it is, on torch's sum."""
+    # LayerNorm sums in its terms' type, under autocast in float32
+    alike = torch.promote_types(x.dtype, residual.dtype) == torch.float32 if torch.is_autocast_enabled("cuda") \
+        else x.dtype == residual.dtype
+    if alike and x.shape == residual.shape and calls_only(norm, LayerNorm):
         return norm(x, residual)
     s = x + residual
     return norm(s), s
