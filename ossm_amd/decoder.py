@@ -90,7 +90,7 @@ class MambaDecoder(nn.Module):
 
     def states(self, slots: int) -> List[_State]:
         """A pool of ``slots`` sequences' states, a ``MixerState`` or ``RecurrentState`` a block."""
-        return [(decode.MixerState if isinstance(b.mixer, MambaMixer) else RecurrentState).of(b.mixer, slots)
+        return [(RecurrentState if isinstance(b.mixer, RecurrentMixer) else decode.MixerState).of(b.mixer, slots)
                 for b in self.blocks]
 
     @torch.no_grad()

@@ -263,3 +263,14 @@ def test_mixers_that_answer_in_another_type():
                 assert torch.equal(total, a + b) and torch.equal(y, want) and y.dtype == want.dtype
     y, total = norm_of_sum(norm, torch.ones(5, 64).cuda(), torch.ones(64).cuda())  # broadcast
     assert torch.equal(total, torch.full((5, 64), 2.0).cuda()) and y.shape == (5, 64)
+
+
+@torch.random.fork_rng()
+def test_wrapped_mamba_mixers_have_their_states():
+    tokens = torch.randint(0, 97, (2, 9)).cuda()
+    m = small()
+    whole = m(tokens)
+    m.blocks[1].mixer = Wrapped(m.blocks[1].mixer)
+    announce("decoder with a wrapped mixer, served")
+    states, slots = m.states(2), torch.arange(2).cuda()
+    close(m.prompt(tokens.flatten(), 9 * torch.arange(3).cuda(), states, slots), whole[:, 8])
