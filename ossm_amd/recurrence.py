@@ -101,7 +101,7 @@ def _backward(x, i, r, z, decay, gy, glast, saved, grads, scale: float, need_dec
         glast = glast.contiguous()
     gdecay = torch.empty(D, dtype=torch.float32, device=x.device) if need_decay else None
     gstart = torch.empty((B, D), dtype=torch.float32, device=x.device) if need_start else None
-    ld = grads[0].stride(1) if B * L > 1 else D
+    _, ld = _flat(grads[0])  # a dimension of one may have any stride
     _lib.run(_lib.load().ossm_recurrence_backward, x, _lib.LM_DTYPES[x.dtype], *gargs, _lib.ptr(glast), *args,
              decay.data_ptr(), scale, saved.data_ptr(), *(_lib.ptr(g) for g in grads), ld, _lib.ptr(gdecay), _lib.ptr(gstart),
              B, L, D)

@@ -105,3 +105,24 @@ def test_separate_steps_match_a_loop():
         h = a * h + torch.sqrt(1 - a * a) * torch.sigmoid(i[:, t].double()) * x[:, t].double()
         assert (y[:, t] - h * torch.nn.functional.silu(z[:, t].double())).abs().max() < 1e-5
     assert (last - h).abs().max() < 1e-5
+
+
+def test_recurrence_gradients_stay_in_their_tensor(monkeypatch):
+    """A projection of one step whose step's stride is any number (such a tensor is contiguous): every
+    row of the gradients, at the row stride that the library is given, lies in the tensor."""
+    from ossm_amd import recurrence
+
+    calls = []
+    monkeypatch.setattr(_lib, "run", lambda fn, t, *args: calls.append((fn.__name__, args)))
+    B, D = 5, 4
+    for packed in (torch.zeros(1, B, 4 * D).transpose(0, 1), torch.zeros(B, 1, 4 * D),
+                   torch.zeros(4 * D * B).as_strided((B, 1, 4 * D), (4 * D, 10 ** 6, 1))):
+        assert packed.is_contiguous()
+        packed.requires_grad_(True)
+        y = recurrence.PackedRecurrenceFn.apply(packed, torch.zeros(D), 8.0)
+        grad, = torch.autograd.grad(y, packed, torch.zeros_like(y))
+        assert grad.shape == packed.shape
+        name, args = calls[-1]
+        assert name == "ossm_recurrence_backward"
+        # dtype, grad_y, its stride, grad_last, x and gates with strides, decay, scale, saved, four gradients, their stride
+        assert args[4 + 8 + 3 + 4] == 4 * D
