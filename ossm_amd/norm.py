@@ -37,24 +37,34 @@ def _dense_like(t: Tensor) -> Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _rows(t: Tensor, D: int) -> Tuple[Tensor, int]:
+    """``t`` [..., D], not empty, as rows and their stride: itself where it is dense (a reshape is a node of
+    its own in training), else as a matrix."""
+    if t.is_contiguous():
+        return t, D
+    t = _matrix(t.reshape(-1, D))
+    return t, _ld(t)
+
+
 def _forward(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float, save: bool):
-    T, D = x.shape
-    x, residual = _matrix(x), None if residual is None else _matrix(residual)
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    dtype, D = x.dtype, x.size(-1)
+    T = x.numel() // D if D > 0 else 0
     y = _dense_like(x)
-    s = None if residual is None else torch.empty_like(y)
+    s = None if residual is None else _dense_like(x)
     stats = torch.empty((2, T), dtype=torch.float32, device=x.device) if save else None  # mean, rstd
-    mean = _lib.ptr(stats)
-    if y.numel() > 0:
+    if T > 0:
+        (x, ld), (residual, ld_res) = _rows(x, D), (None, 0) if residual is None else _rows(residual, D)
+        weight, bias = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
         wt = weight if weight is not None else bias
-        _lib.run(_lib.load().ossm_layer_norm_forward, x, _lib.LM_DTYPES[x.dtype], _lib.LM_DTYPES[(x if wt is None else wt).dtype],
-                 x.data_ptr(), _ld(x), _lib.ptr(residual), 0 if residual is None else _ld(residual), _lib.ptr(weight),
-                 _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(s), mean, None if mean is None else mean + 4 * T, T, D)
+        mean = _lib.ptr(stats)
+        _lib.run(_lib.load().ossm_layer_norm_forward, x, _lib.LM_DTYPES[dtype], _lib.LM_DTYPES[dtype if wt is None else wt.dtype],
+                 x.data_ptr(), ld, _lib.ptr(residual), ld_res, _lib.ptr(weight), _lib.ptr(bias), eps, y.data_ptr(),
+                 _lib.ptr(s), mean, None if mean is None else mean + 4 * T, T, D)
     return y, s, stats
 
 
 class LayerNormFn(torch.autograd.Function):
-    """``layer_norm`` and ``add_layer_norm`` on matrices; saves the sum and two numbers a row."""
+    """``layer_norm`` and ``add_layer_norm``; saves the sum and two numbers a row."""
 
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor],  # type: ignore[override]
@@ -80,31 +90,29 @@ class LayerNormFn(torch.autograd.Function):
             if ds is not None and gs is not None:
                 ds = ds + gs
             return (ds if need[0] else None, ds if need[1] else None, *(next(got) if n else None for n in need[2:4]), None)
-        T, D = s.shape
-        s, gy = _matrix(s), _matrix(gy)
-        gs = None if gs is None else _matrix(gs)
-        weight = None if weight is None else weight.contiguous()
         wt = weight if weight is not None else bias
         ds = _dense_like(s) if need[0] or need[1] else None
-        dw, db = (_dense_like(wt) if n else None for n in need[2:4])
+        dw, db = _dense_like(wt) if need[2] else None, _dense_like(wt) if need[3] else None
         if s.numel() == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
         else:
+            D = s.size(-1)
+            T = s.numel() // D
+            (s, ld), (gy, ld_gy), (gs, ld_gs) = _rows(s, D), _rows(gy, D), (None, 0) if gs is None else _rows(gs, D)
+            weight = None if weight is None else weight.contiguous()
             mean = stats.data_ptr()
             _lib.run(_lib.load().ossm_layer_norm_backward, s, _lib.LM_DTYPES[s.dtype],
-                     _lib.LM_DTYPES[(s if wt is None else wt).dtype], gy.data_ptr(), _ld(gy), _lib.ptr(gs),
-                     0 if gs is None else _ld(gs), s.data_ptr(), _ld(s), _lib.ptr(weight), mean, mean + 4 * T,
-                     _lib.ptr(ds), _lib.ptr(dw), _lib.ptr(db), T, D)
+                     _lib.LM_DTYPES[(s if wt is None else wt).dtype], gy.data_ptr(), ld_gy, _lib.ptr(gs), ld_gs,
+                     s.data_ptr(), ld, _lib.ptr(weight), mean, mean + 4 * T, _lib.ptr(ds), _lib.ptr(dw), _lib.ptr(db), T, D)
         return ds if need[0] else None, ds if need[1] else None, dw, db, None
 
 
 def _apply(what: str, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor], eps: float):
-    args = [x, residual, weight, bias]
     if torch.is_autocast_enabled("cuda"):  # as F.layer_norm: in float32
-        args = [t if t is None or t.dtype not in (torch.bfloat16, torch.float16) else t.float() for t in args]
-        x, residual, weight, bias = args
+        x, residual, weight, bias = (t if t is None or t.dtype not in (torch.bfloat16, torch.float16) else t.float()
+                                     for t in (x, residual, weight, bias))
     index, dtype = x.get_device(), x.dtype
     if dtype not in _lib.LM_DTYPES or index < 0 or x.dim() == 0:
         raise RuntimeError(f"{what}: x must be a float32 or bfloat16 GPU tensor of at least one dimension, got {dtype} "
@@ -113,22 +121,20 @@ def _apply(what: str, x: Tensor, residual: Optional[Tensor], weight: Optional[Te
         raise RuntimeError(f"{what}: residual must be as x, {dtype} {tuple(x.shape)}, got {residual.dtype} "
                            f"{tuple(residual.shape)} on {residual.device}")
     D = x.size(-1)
-    types = {t.dtype for t in (weight, bias) if t is not None}
+    kind = bias.dtype if bias is not None else dtype
+    kind = weight.dtype if weight is not None and bias is None else kind
     for t in (weight, bias):
-        if t is not None and (t.shape != (D,) or t.get_device() != index or len(types) > 1
-                              or t.dtype not in (dtype, torch.float32)):
+        if t is not None and (t.dtype != kind or kind != dtype and kind != torch.float32 or t.dim() != 1 or t.size(0) != D
+                              or t.get_device() != index):
             raise RuntimeError(f"{what}: weight and bias must be of shape ({D},), both of x's dtype or both float32, on x's GPU, "
                                f"got {[None if t is None else (t.dtype, tuple(t.shape), str(t.device)) for t in (weight, bias)]}")
-    if _lib.has_tangent(args):
+    if _lib.has_tangent((x, residual, weight, bias)):
         raise RuntimeError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
-    two = [t if t is None or t.dim() == 2 else t.reshape(-1, D) if D > 0 else t.reshape(t.shape[:-1].numel(), 0)
-           for t in (x, residual)]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        out = LayerNormFn.apply(*two, weight, bias, float(eps))
-        y, s = (out, None) if residual is None else out
-    else:
-        y, s, _ = _forward(*two, weight, bias, float(eps), False)
-    return (y, s) if x.dim() == 2 else (y.view(x.shape), None if s is None else s.view(x.shape))
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad
+                                    or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad):
+        out = LayerNormFn.apply(x, residual, weight, bias, float(eps))
+        return (out, None) if residual is None else out
+    return _forward(x, residual, weight, bias, float(eps), False)[:2]
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
@@ -152,7 +158,7 @@ class LayerNorm(nn.LayerNorm):
     it returns the norm of the sum and the sum."""
 
     def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
-        if len(self.normalized_shape) != 1 or x.shape[-1:] != torch.Size(self.normalized_shape):
+        if x.dim() == 0 or self.normalized_shape != (x.size(-1),):
             raise RuntimeError(f"LayerNorm norms a last dimension of {tuple(self.normalized_shape)}, got {tuple(x.shape)}")
         y, s = _apply("LayerNorm", x, residual, self.weight, self.bias, self.eps)
         return y if residual is None else (y, s)
@@ -165,6 +171,6 @@ def norm_of_sum(norm: nn.Module, x: Tensor, residual: Tensor) -> Tuple[Tensor, T
     alike = torch.promote_types(x.dtype, residual.dtype) == torch.float32 if torch.is_autocast_enabled("cuda") \
         else x.dtype == residual.dtype
     if alike and x.shape == residual.shape and calls_only(norm, LayerNorm):
-        return norm(x, residual)
+        return norm.forward(x, residual)
     s = x + residual
     return norm(s), s
