@@ -136,7 +136,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 
 // ---- records ------------------------------------------------------------------------
 // Per chunk and channel: the aggregate's sum of l and state, and the state at the
-// chunk's end (written by the last chunk of W neighbours only).
+// chunk's end (written by the last chunk of P neighbours only).
 enum { kSumL = 0, kState = 1, kEnd = 2, kRecords = 3 };
 
 struct Rec {
