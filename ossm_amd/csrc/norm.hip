@@ -93,11 +93,12 @@ __device__ __forceinline__ void load_weights(const WT* p, int D, int lane, float
   }
 }
 
-// Sums are of the elements less the row's first one, the pivot: in a row far from zero, whose elements
-// differ little, those differences are exact, and zero where all are equal.  (With the rounding of a mean
-// of the elements themselves in every deviation, its square could pass the variance and eps: NaN
-// at equal elements of 2e8.)  The mean of the differences is rounded too, which the deviations from it
-// all carry: their own mean, `rest`, is taken off again.
+// The mean is the row's first element, the pivot, and the mean of the differences from it: in a row far
+// from zero, whose elements differ little, those are exact, and zero where all are equal.  (A mean of
+// the elements' own sum is off by many roundings of its size, which every deviation would carry: its square
+// could pass the variance and eps, NaN at equal elements of 2e8.)  The mean is still rounded to its own
+// size, by no more than the elements differ, which the deviations all carry: their own mean, `rest`, is
+// taken off again.
 struct Row {
   float rest, rstd;
 };
@@ -177,13 +178,13 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
       const int at = (j * G + lane) * W;
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        v[j][k] = at + k < g.D ? raw[j].get(k) - pivot : 0.f;
-        total += v[j][k];
+        v[j][k] = raw[j].get(k);
+        total += at + k < g.D ? v[j][k] - pivot : 0.f;
       }
     }
     fetch(r + step);  // the next row comes in while this one is summed
     __builtin_amdgcn_sched_barrier(0);
-    const float mean = row_sums<G>(total, 0.f, s_sum).x / static_cast<float>(g.D);
+    const float mean = pivot + row_sums<G>(total, 0.f, s_sum).x / static_cast<float>(g.D);
     float square = 0.f, rest = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(kBlockOf<G>) void norm_forward_kernel(Norm<E, WT> g
       }
     const Row row = row_of(row_sums<G>(square, rest, s_sum), inv, g.eps);
     if (lane == 0 && g.mean != nullptr) {
-      g.mean[r] = pivot + (mean + row.rest);
+      g.mean[r] = mean + row.rest;
       g.rstd[r] = row.rstd;
     }
 #pragma unroll
@@ -389,19 +390,19 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
         for (int k = 0; k < W; ++k) total += k < n ? v[0].get(k) - pivot : 0.f;
       });
     }
-    const float mean = row_sums<kMaxThreads>(total, 0.f, s_sum).x / static_cast<float>(g.D);
+    const float mean = pivot + row_sums<kMaxThreads>(total, 0.f, s_sum).x / static_cast<float>(g.D);
     float square = 0.f, rest = 0.f;
     each_vector(in, g.D, [&](int, int n, Vec<E, W>(&v)[1]) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float c = k < n ? v[0].get(k) - pivot - mean : 0.f;
+        const float c = k < n ? v[0].get(k) - mean : 0.f;
         square = fmaf(c, c, square);
         rest += c;
       }
     });
     const Row row = row_of(row_sums<kMaxThreads>(square, rest, s_sum), inv, g.eps);
     if (threadIdx.x == 0 && g.mean != nullptr) {
-      g.mean[r] = pivot + (mean + row.rest);
+      g.mean[r] = mean + row.rest;
       g.rstd[r] = row.rstd;
     }
     each_vector(in, g.D, [&](int at, int n, Vec<E, W>(&v)[1]) {
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kMaxThreads) void long_forward_kernel(Norm<E, WT> g
       load_weights<WT, 1, W, kMaxThreads>(g.weight, g.D, at / W, 1.f, w);
       load_weights<WT, 1, W, kMaxThreads>(g.bias, g.D, at / W, 0.f, b);
 #pragma unroll
-      for (int k = 0; k < W; ++k) t[k] = fmaf((v[0].get(k) - pivot - mean - row.rest) * row.rstd, w[0][k], b[0][k]);
+      for (int k = 0; k < W; ++k) t[k] = fmaf((v[0].get(k) - mean - row.rest) * row.rstd, w[0][k], b[0][k]);
       v[0].set(t);
       v[0].template store<false>(g.y + r * g.D + at, n);
     });
