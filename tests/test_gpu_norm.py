@@ -445,3 +445,36 @@ def test_the_sum_alone_is_not_reached_by_the_norm(N):
         _, s = N.add_layer_norm(*leaves)
         dx, dres, dw, db = torch.autograd.grad(s, leaves, gs, allow_unused=True, create_graph=graph)
         assert torch.equal(dx, gs) and torch.equal(dres, gs) and dw is None and db is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_training_on_tensors_of_any_shape(N, dtype):
+    """Dense, transposed, cut out and broadcast tensors and gradients of one to four dimensions: what
+    their matrices give, outputs dense."""
+    D = 37
+    _, _, w, b, _, _ = inputs(1, D, dtype, torch.float32, False, seed=23)
+    rand = lambda *s: torch.randn(*s, device="cuda").to(dtype)  # noqa: E731
+    with torch.random.fork_rng():
+        torch.manual_seed(5)
+        cases = [[rand(D) for _ in range(4)], [rand(2, 3, D) for _ in range(4)], [rand(2, 1, 3, D) for _ in range(4)],
+                 [rand(3, 2, D).transpose(0, 1) for _ in range(4)], [rand(2, 5, D)[:, 1:4] for _ in range(4)],
+                 [rand(2, D, 3).transpose(1, 2) for _ in range(4)], [rand(2, 3, 2 * D)[..., ::2] for _ in range(4)],
+                 [rand(1, 1, D).expand(2, 3, D) for _ in range(4)], [rand(2, 3, 1).expand(2, 3, D) for _ in range(4)],
+                 [rand(2, 0, D) for _ in range(4)], [rand(5, 1, D).as_strided((5, 1, D), (D, 10 ** 6, 1)) for _ in range(4)]]
+    for x, res, gy, gs in cases:
+        announce(f"layer norm training {tuple(x.shape)} {x.stride()}")
+        flat = [t.reshape(-1, D).contiguous() for t in (x, res, gy, gs)]
+        for two in (False, True):
+            y, s, grads = run(N, x, res if two else None, w, b, gy, gs)
+            wy, ws, want = run(N, flat[0], flat[1] if two else None, w, b, *flat[2:])
+            assert y.shape == x.shape and y.is_contiguous() and torch.equal(y.view(-1, D), wy)
+            assert not two or s.shape == x.shape and torch.equal(s.view(-1, D), ws)
+            for p, q in zip(grads, want):
+                assert (p is None and q is None) or torch.equal(p.reshape(q.shape), q)
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, res)]
+        y, s = N.add_layer_norm(*leaves, w, b)
+        g1 = torch.autograd.grad([y, s], leaves, [gy, gs], create_graph=True)
+        g2 = torch.autograd.grad([y, s], leaves, [gy, gs])
+        for p, q in zip(g1, g2):
+            assert p.shape == q.shape == x.shape
+            assert x.numel() == 0 or (p - q).abs().max() <= (1e-4 if dtype == torch.float32 else 0.05) * q.abs().max()
