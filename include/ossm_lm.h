@@ -146,7 +146,7 @@ int ossm_layer_norm_backward(int dtype, int weight_dtype, const void* grad_y, in
 
 /*
  * The gated linear recurrence, per channel d of dim:
- *   a_t = exp(-scale softplus(decay[d]) sigmoid(decay_gate_t))
+ *   a_t = exp(-scale softplus(decay[d]) sigmoid(decay_gate_t)), 2^-126 where that is less
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t
  *   y_t = h_t, or h_t silu(output_gate_t) where output_gate is given
  * x and the gates E, rows of dim with row strides ld_*; decay f32 [dim]; scale positive and

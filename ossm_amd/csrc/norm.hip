@@ -6,7 +6,7 @@
 //   g = gy w;  ds = rstd (g - mean(g) - n mean(g n)) + gs,  n = c rstd
 //   dw = sum over rows of gy n,  db = sum over rows of gy
 //
-// All of it is bound by memory: [32768, 2048] in bf16 with a residual takes 92 to 102 us forward (5.3
+// All of it is bound by memory: [32768, 2048] in bf16 with a residual takes 92 to 103 us forward (5.2
 // to 5.8 TB/s) and 103 to 117 backward (4.6 to 5.2), a copy runs at 4.9; short calls by their
 // latency, 4 us at [4, 2048].  A group of G lanes holds a whole row in registers, in
 // vectors of 16 bytes, so that every tensor is read once and the squares are summed about
