@@ -90,9 +90,10 @@ class LinearFn(torch.autograd.Function):
 
 def calls_only(module: nn.Module, cls: type) -> bool:
     """Whether calling ``module`` is ``cls.forward`` and nothing else (no hooks, its own or
-    global, no replaced forward)."""
+    global, no replaced or compiled forward)."""
     glob = nn.modules.module
     return (isinstance(module, cls) and type(module).forward is cls.forward and "forward" not in module.__dict__
+            and module._compiled_call_impl is None
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
                      or module._backward_pre_hooks or glob._global_forward_hooks
                      or glob._global_forward_pre_hooks or glob._global_backward_hooks

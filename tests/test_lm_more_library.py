@@ -126,3 +126,31 @@ def test_recurrence_gradients_stay_in_their_tensor(monkeypatch):
         assert name == "ossm_recurrence_backward"
         # dtype, grad_y, its stride, grad_last, x and gates with strides, decay, scale, saved, four gradients, their stride
         assert args[4 + 8 + 3 + 4] == 4 * D
+
+
+def test_only_bare_modules_are_passed_by():
+    """What a caller may do in a module's place: nothing where anything else is called with it."""
+    from torch import nn
+
+    from ossm_amd.linear import calls_only
+    from ossm_amd.norm import LayerNorm
+
+    assert calls_only(LayerNorm(8), LayerNorm) and not calls_only(nn.LayerNorm(8), LayerNorm)
+    none = lambda *a: None  # noqa: E731
+    for change in (lambda m: m.register_forward_hook(none), lambda m: m.register_forward_pre_hook(none),
+                   lambda m: m.register_full_backward_hook(none), lambda m: m.register_full_backward_pre_hook(none),
+                   lambda m: setattr(m, "forward", none), lambda m: m.compile()):
+        m = LayerNorm(8)
+        change(m)
+        assert not calls_only(m, LayerNorm)
+
+    class Own(LayerNorm):
+        def forward(self, x, residual=None):
+            return x
+
+    assert not calls_only(Own(8), LayerNorm) and calls_only(type("Same", (LayerNorm,), {})(8), LayerNorm)
+    handle = nn.modules.module.register_module_forward_hook(none)
+    try:
+        assert not calls_only(LayerNorm(8), LayerNorm)
+    finally:
+        handle.remove()
