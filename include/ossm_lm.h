@@ -129,6 +129,7 @@ int ossm_gated_backward(int dtype, const void* grad_y, int64_t ld_grad, const vo
  * x, residual E [rows, dim] with row strides ld_*; weight, bias [dim] of weight_dtype (the
  * same as dtype, or OSSM_F32), or null for ones and zeros; y, sum E [rows, dim] dense, sum
  * given exactly where residual is.  mean, rstd f32 [rows], written for the backward, or both null.
+ * y and sum overlap no input: a row's first element is read by all of its lanes.
  *
  * ossm_layer_norm_backward: with grad_y, grad_sum (null where nothing reaches the sum) E
  * [rows, dim] and s, the forward's sum (or x), the gradients of x (and of the residual,

@@ -72,9 +72,10 @@ __device__ __forceinline__ float sigmoid_of(float x) {
 }
 
 // a = 2^l and 1 - a^2 of a log-decay l <= 0 (to base 2).  a is no less than the smallest normal
-// number, by which an infinite state stays infinite: a step leaves at least 2^-126 of a state.  Near zero 1 - a^2 is the series of
-// -expm1 (what is left out is below 2^-24 of it); from where a^2 is far enough from one
-// it is 1 - a a, at 0.67 with three times a's rounding, in 16 bits at 0.88 with eight.
+// number, by which an infinite state stays infinite: a step leaves at least 2^-126 of a state.
+// Near zero 1 - a^2 is the series of -expm1 (what is left out is below 2^-24 of it); from where
+// a^2 is far enough from one it is 1 - a a, at 0.67 with three times a's rounding, in 16 bits at
+// 0.88 with eight.
 template <bool kFull>
 __device__ __forceinline__ void decay_of(float l, float& a, float& rest) {
   a = greatest(__builtin_amdgcn_exp2f(l), kTiny);
